@@ -66,6 +66,10 @@ extern "C" {
 #define IT_OP_PAGED_PREFILL 5
 #define IT_OP_FLASH_ATTENTION 6 /* CoreOperator::FlashAttention, src/types.rs:202-208 */
 #define IT_OP_KV_COPY_BLOCKS 7
+#define IT_OP_KV_APPEND_ROTARY 8 /* dtype: the cache's */
+#define IT_OP_ROTARY 9           /* dtype: the tensor's */
+#define IT_OP_KV_MOVE 10         /* dtype: the cache's */
+#define IT_OP_SAMPLE 11          /* dtype: the logits' */
 
 /* Thread-local message for the last non-OK status on this thread. */
 const char* it_last_error(void);
@@ -186,6 +190,25 @@ int32_t it_kv_manager_append_cow(it_kv_manager* mgr, const int32_t* seqs, const 
                                  int32_t n, int64_t* slots_out, int32_t* evicted_out,
                                  int32_t evicted_cap, int32_t* n_evicted, int32_t* cow_src,
                                  int32_t* cow_dst, int32_t cow_cap, int32_t* n_cow);
+/* Compact sequence `seq` to the tokens at the positions keep[0..n_keep)
+ * (ascending, each below the sequence's next position): keep[i] becomes
+ * position i and n_keep the next position.  Leading blocks whose tokens all
+ * keep their positions stay as they are (dropping only a tail, as after a
+ * rejected draft, moves nothing); from the first other block on, kept rows go
+ * to fresh blocks, so that forks of the sequence are untouched and no row is
+ * overwritten before it is read.  The caller then runs, in this order:
+ * it_kv_move(src, dst, delta), it_kv_evict(evicted), it_kv_sync_tables(seq,
+ * pos, dst).
+ *   src, dst: int64[moves_cap] slots of the moved rows; delta: new - old
+ *     position of each (NULL = not wanted); pos: new position (NULL likewise);
+ *     *n_moves of them (at most n_keep)
+ *   evicted: blocks that returned to the pool (refcount 0), *n_evicted of them
+ * IT_INVALID_INPUT, and nothing changes, where a capacity does not suffice,
+ * the pool holds too few free blocks, or a kept position is not held; for a
+ * manager with a window IT_NOT_IMPLEMENTED: its blocks go by position. */
+int32_t it_kv_manager_compact(it_kv_manager* mgr, int32_t seq, const int32_t* keep, int32_t n_keep,
+                              int64_t* src, int64_t* dst, int32_t* delta, int32_t* pos, int32_t moves_cap,
+                              int32_t* n_moves, int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted);
 /* Export tables [max_seqs][max_blocks] (-1 = not held), ctx_lens[max_seqs]
  * (= next position) and start_pos[max_seqs] (window start, else 0).  Any
  * output pointer may be NULL. */
@@ -306,6 +329,72 @@ int32_t it_kv_append_rope(it_kv_cache* cache, const it_rope_table* rope, const f
                           const int32_t* positions, int32_t n_tokens, void* q_out, int32_t q_out_dtype,
                           void* stream);
 
+/* ---- rotary positions ---------------------------------------------------
+ * The rotation models train with, in either pair layout, over all or part of
+ * a head, with frequencies scaled for contexts longer than those trained on:
+ *   (a', b') = magnitude * (a cos t - b sin t, a sin t + b cos t),
+ *   t = position * f_p   (pair p < n_dims / 2, f_p = freq_base^(-2 p / n_dims))
+ * it_kv_append_rope beside it reproduces rope_f32 (src/backend/arm/rope.rs:
+ * 6-44) bit for bit from a table; this one holds no table, takes any int32
+ * position, and rounds once: the angle is taken in 64 bits, its cosine and sine
+ * are each within about one fp32 unit in the last place.  No counterpart in
+ * the reference beyond rope_f32's interleaved, unscaled pairs. */
+#define IT_ROTARY_INTERLEAVED 0 /* pair p: elements 2p, 2p + 1 (rope_f32) */
+#define IT_ROTARY_HALF 1        /* pair p: elements p, p + n_dims / 2 */
+#define IT_ROTARY_SCALE_NONE 0
+#define IT_ROTARY_SCALE_LINEAR 1 /* position interpolation: f / factor */
+#define IT_ROTARY_SCALE_BASE 2   /* freq_base * factor^(n_dims / (n_dims - 2)) */
+#define IT_ROTARY_SCALE_PARTS 3  /* by parts: with r = original_ctx * f / (2 pi) turns over the trained
+                                    context and g = (r - low) / (high - low) clamped to [0, 1],
+                                    f * (g + (1 - g) / factor) */
+typedef struct {
+  int32_t n_dims;        /* rotated elements of a head, the first ones: even, 2 .. 1024 */
+  int32_t layout;        /* IT_ROTARY_INTERLEAVED, IT_ROTARY_HALF */
+  int32_t scaling;       /* IT_ROTARY_SCALE_* */
+  int32_t original_ctx;  /* PARTS: positions trained on */
+  double freq_base;
+  double factor;         /* LINEAR, BASE, PARTS: > 0 */
+  double low, high;      /* PARTS: turns below which f / factor, above which f */
+  double magnitude;      /* > 0; 1 for a plain rotation (YaRN: 0.1 ln factor + 1) */
+  const double* inv_freq; /* NULL, or host double[n_dims / 2]: the f_p themselves, radians per
+                             position (freq_base, scaling and what goes with it unused) */
+} it_rotary_desc;
+typedef struct it_rotary it_rotary;
+/* f_p of every pair (host arithmetic, no device): freqs[n_dims / 2]. */
+int32_t it_rotary_frequencies(const it_rotary_desc* desc, double* freqs);
+/* Device memory: 8 bytes per pair. */
+int32_t it_rotary_new(int32_t device, const it_rotary_desc* desc, it_rotary** out);
+int32_t it_rotary_destroy(it_rotary* rotary);
+/* out = R(position) x for every head of every token; transpose != 0: the
+ * transposed rotation, magnitude * R(-position) -- the gradient of the forward
+ * one, and with magnitude 1 its inverse.
+ *   x, out: [n_tokens][n_heads][head_dim] of dtype F32, F16 or BF16, with
+ *     token_stride / out_stride elements between tokens (at least a token's
+ *     own; not read for one token); out may be x itself with its stride, and
+ *     must not overlap it otherwise
+ *   positions: int32[n_tokens], device; any value, negative ones too
+ * Products in fp32, rounded once to dtype; elements past n_dims pass through.
+ * 16-byte aligned rows run fastest; others are taken too. */
+int32_t it_rotary_apply(const it_rotary* rotary, const void* x, int32_t dtype, int64_t token_stride,
+                        const int32_t* positions, int32_t n_tokens, int32_t n_heads, int32_t head_dim,
+                        int32_t transpose, void* out, int64_t out_stride, void* stream);
+/* Rotation then append: rotated q to q_out, rotated k and v as it is into the
+ * cache's pages in its format (each rounded or quantised once, from fp32).
+ *   q: [n_tokens][n_heads][head_dim], k, v: [n_tokens][n_kv_heads][head_dim] of
+ *     src_dtype F32, F16 or BF16, q_stride / k_stride / v_stride elements
+ *     between tokens (a fused projection's rows: all three the same)
+ *   n_heads: a multiple of n_kv_heads; 0: no q (q, q_out NULL)
+ *   slot_mapping: int64[n_tokens] (slot < 0 = padding: q still rotated)
+ *   positions: int32[n_tokens]; a negative one is latched
+ *     (it_kv_cache_check) and its token writes nothing
+ *   q_out: [n_tokens][n_heads][head_dim] contiguous, of q_out_dtype F32, F16 or
+ *     BF16; may be q itself where that is contiguous and of that dtype */
+int32_t it_kv_append_rotary(it_kv_cache* cache, const it_rotary* rotary, const void* q, const void* k,
+                            const void* v, int32_t src_dtype, int64_t q_stride, int64_t k_stride,
+                            int64_t v_stride, int32_t n_heads, const int64_t* slot_mapping,
+                            const int32_t* positions, int32_t n_tokens, void* q_out, int32_t q_out_dtype,
+                            void* stream);
+
 /* Block-table gather: materialise the contiguous slices that
  * forward.rs:233-243 reads, through a block table.
  *   block_tables: int32[n_seqs][max_blocks] (absolute logical block index)
@@ -339,6 +428,22 @@ int32_t it_kv_sync_tables(it_kv_cache* cache, int32_t* tables, int32_t max_block
  * every layer). */
 int32_t it_kv_copy_blocks(it_kv_cache* cache, const int32_t* src, const int32_t* dst, int32_t n,
                           void* stream);
+
+/* Move token rows between slots: for each i, in every layer and head, the K
+ * and V row of slot src[i] becomes that of slot dst[i].  With `rotary`, K rows
+ * are also turned by delta[i] positions (new position - old position; K is
+ * cached rotated), without its magnitude, which they already carry: F32, F16
+ * and BF16 rows are turned in fp32 and rounded once, quantised rows are
+ * dequantised, turned and quantised again; a row with delta 0 keeps its bytes.
+ *   src, dst: int64[n], device; a pair with a negative slot is skipped; slots
+ *     out of range are latched and skipped
+ *   rotary: NULL = copy as it is; delta: int32[n], device, NULL only without it
+ * dst slots must be distinct and none may be another pair's src (fresh blocks,
+ * as it_kv_manager_compact hands out); src[i] == dst[i] is allowed: the row
+ * is turned in place (a shift of a sequence's positions).  Takes a multi-layer
+ * cache or a layer's view. */
+int32_t it_kv_move(it_kv_cache* cache, const int64_t* src, const int64_t* dst, int32_t n,
+                   const it_rotary* rotary, const int32_t* delta, void* stream);
 
 /* ======================================================================== */
 /* Device: attention over the cache.                                         */
@@ -463,6 +568,44 @@ size_t it_flash_attention_workspace(int32_t n_heads, int32_t head_dim, int32_t n
 int32_t it_flash_attention(const float* q, const float* k, const float* v, const float* mask,
                            float* out, int32_t n_heads, int32_t head_dim, int32_t n_kv, void* ws,
                            size_t ws_bytes, void* stream);
+
+/* ======================================================================== */
+/* Device: the next token.  The reference's step ends with                  */
+/* ForwardExecutor::sample (src/inference/forward.rs:765-796); a batcher's   */
+/* rows each have settings of their own.                                     */
+/* ======================================================================== */
+/* One token per row of logits z from a given uniform number u:
+ *   order: z descending, equal z by the lower token first; NaN counts as -inf,
+ *     tokens at -inf are never drawn
+ *   w_i = exp((z_i - max z) / temperature)  (a maximum of +inf: the tokens at
+ *     +inf weigh 1, all others nothing)
+ *   min-p keeps w_i >= min_p (the largest weight is 1); then top-k the first k;
+ *     then top-p those whose mass before them is below top_p of the mass left;
+ *     the first of the order is always kept
+ *   token = the first kept one with cumulative mass > u * kept mass
+ *   prob = its share of the kept mass
+ * temperature <= 0 (or NaN): the first of the order, prob 1.  A row with
+ * nothing above -inf: token -1, prob 0.
+ * Masses are 64-bit integers in units of 2^-44 of the largest token's, each
+ * rounded to nearest once: sums are exact, so a result depends on neither the
+ * batch nor the order of the sums.
+ *   logits: [n_rows][vocab] of F32, F16 or BF16, row_stride elements between
+ *     rows; vocab 1 .. 262144
+ *   u: float[n_rows], device, in [0, 1) (below 0 and NaN count as 0, 1 and
+ *     above as the last kept token)
+ *   temperatures, top_ps, min_ps: float[n_rows], top_ks: int32[n_rows], device;
+ *     NULL: temperature / top_k / top_p / min_p holds for every row (finite,
+ *     temperature >= 0, min_p <= 1).  Off: top_k <= 0, top_p >= 1, min_p <= 0;
+ *     min_p above 1 counts as 1, NaN as off
+ *   tokens: int32[n_rows]; probs: float[n_rows] or NULL; device
+ *   ws: it_sample_workspace(...) bytes, device, 256-byte aligned; it need not
+ *     be cleared, and calls that overlap in time need one each
+ * Launched on the current device, to which `stream` must belong. */
+size_t it_sample_workspace(int32_t n_rows, int32_t vocab);
+int32_t it_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t n_rows, int32_t vocab,
+                  const float* u, const float* temperatures, const int32_t* top_ks, const float* top_ps,
+                  const float* min_ps, float temperature, int32_t top_k, float top_p, float min_p,
+                  int32_t* tokens, float* probs, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,6 +28,9 @@ BLOCK_Q5_0_BYTES = 22  # ggml block_q5_0 (types.rs:116 has only the id)
 BLOCK_Q5_1_BYTES = 24  # ggml block_q5_1 (types.rs:117)
 QUANT_TYPES = (Q8_0, Q4_0, Q4_1, Q5_0, Q5_1)
 OP_KV_APPEND, OP_KV_GATHER, OP_KV_EVICT, OP_PAGED_DECODE, OP_PAGED_PREFILL, OP_FLASH_ATTENTION, OP_KV_COPY_BLOCKS = range(1, 8)
+OP_KV_APPEND_ROTARY, OP_ROTARY, OP_KV_MOVE, OP_SAMPLE = range(8, 12)
+ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
+ROTARY_SCALE_NONE, ROTARY_SCALE_LINEAR, ROTARY_SCALE_BASE, ROTARY_SCALE_PARTS = range(4)
 
 
 class OpError(RuntimeError):
@@ -68,6 +71,22 @@ class CacheDesc(C.Structure):
         ("device", C.c_int32),
         ("owns_memory", C.c_int32),
         ("n_layers", C.c_int32),
+    ]
+
+
+class RotaryDesc(C.Structure):
+    """it_rotary_desc (include/it_kv.h)."""
+    _fields_ = [
+        ("n_dims", C.c_int32),
+        ("layout", C.c_int32),
+        ("scaling", C.c_int32),
+        ("original_ctx", C.c_int32),
+        ("freq_base", C.c_double),
+        ("factor", C.c_double),
+        ("low", C.c_double),
+        ("high", C.c_double),
+        ("magnitude", C.c_double),
+        ("inv_freq", C.c_void_p),
     ]
 
 
@@ -147,6 +166,15 @@ SIGNATURES = {
     "it_paged_prefill_ws": (i32, [P, P, i32, i32, P, i32, P, i32, P, i32, f32, i32, P, sz, P, i32, P]),
     "it_flash_attention_workspace": (sz, [i32, i32, i32]),
     "it_flash_attention": (i32, [P, P, P, P, P, i32, i32, i32, P, sz, P]),
+    "it_rotary_frequencies": (i32, [C.POINTER(RotaryDesc), P]),
+    "it_rotary_new": (i32, [i32, C.POINTER(RotaryDesc), PP]),
+    "it_rotary_destroy": (i32, [P]),
+    "it_rotary_apply": (i32, [P, P, i32, i64, P, i32, i32, i32, i32, P, i64, P]),
+    "it_kv_append_rotary": (i32, [P, P, P, P, P, i32, i64, i64, i64, i32, P, P, i32, P, i32, P]),
+    "it_kv_move": (i32, [P, P, P, i32, P, P, P]),
+    "it_kv_manager_compact": (i32, [P, i32, P, i32, P, P, P, P, i32, P, P, i32, P]),
+    "it_sample_workspace": (sz, [i32, i32]),
+    "it_sample": (i32, [P, i32, i64, i32, i32, P, P, P, P, P, f32, i32, f32, f32, P, P, P, sz, P]),
 }
 
 

@@ -14,7 +14,8 @@ import numpy as np
 from ._lib import StepPlanC, check, lib
 from .memory import BlockPool
 
-__all__ = ["KvManager", "ContinuousBatcher", "RequestState", "RequestContext", "StepPlan"]
+__all__ = ["KvManager", "ContinuousBatcher", "RequestState", "RequestContext", "StepPlan", "CompactPlan",
+           "SamplingParams"]
 
 
 _EMPTY = np.zeros(0, np.int32)
@@ -38,6 +39,21 @@ class StepPlan:
     token_pos: np.ndarray = field(default_factory=lambda: np.zeros(0, np.int32))
     ctx_lens: Optional[np.ndarray] = None
     start_pos: Optional[np.ndarray] = None
+
+
+@dataclass
+class CompactPlan:
+    """What dropping tokens out of a sequence hands to the device, in this
+    order: kv_move (src, dst, and delta for rotated keys), kv_evict of the
+    blocks that returned to the pool, kv_sync_tables with (token_seq,
+    token_pos, dst)."""
+
+    src: np.ndarray
+    dst: np.ndarray
+    delta: np.ndarray
+    token_seq: np.ndarray
+    token_pos: np.ndarray
+    evicted: np.ndarray
 
 
 class KvManager:
@@ -130,6 +146,22 @@ class KvManager:
                         self._cs[:nc].copy() if nc else _EMPTY, self._cd[:nc].copy() if nc else _EMPTY,
                         tsp[0], tsp[1], lens[0], lens[1])
 
+    def compact(self, seq: int, keep: Sequence[int]) -> CompactPlan:
+        """Keep only the tokens at these positions (ascending) of `seq`:
+        keep[i] becomes position i (it_kv_manager_compact).  Tokens before the
+        first dropped one stay in their blocks, the others move to fresh ones;
+        dropping a tail moves nothing."""
+        pos = np.ascontiguousarray(keep, dtype=np.int32).reshape(-1)
+        n = pos.size
+        src, dst = np.empty(n, np.int64), np.empty(n, np.int64)
+        delta, new = np.empty(n, np.int32), np.empty(n, np.int32)
+        ev = np.empty(self.max_blocks, np.int32)
+        nm, nev = C.c_int32(0), C.c_int32(0)
+        check(lib.it_kv_manager_compact(self._h, seq, pos.ctypes.data, n, src.ctypes.data, dst.ctypes.data, delta.ctypes.data,
+                                        new.ctypes.data, n, C.byref(nm), ev.ctypes.data, ev.size, C.byref(nev)))
+        m = nm.value
+        return CompactPlan(src[:m], dst[:m], delta[:m], np.full(m, seq, np.int32), new[:m], ev[:nev.value].copy())
+
     def positions(self) -> np.ndarray:
         """Next position (= context length) of every sequence slot."""
         cl = np.empty(self.max_seqs, dtype=np.int32)
@@ -163,6 +195,18 @@ class KvManager:
             self._h = None
 
 
+@dataclass(frozen=True)
+class SamplingParams:
+    """How a request's tokens are drawn (sampling.sample); the defaults draw
+    from the whole distribution.  temperature 0 takes the most likely token;
+    top_k 0, top_p 1 and min_p 0 are off."""
+
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+
+
 class RequestState(Enum):  # continuous.rs:8-15
     Running = "Running"
     Waiting = "Waiting"
@@ -177,6 +221,7 @@ class RequestContext:  # continuous.rs:17-25
     prompt_tokens: List[int]
     generated_tokens: List[int]
     max_tokens: int
+    sampling: SamplingParams = SamplingParams()
 
 
 class ContinuousBatcher:
@@ -210,8 +255,9 @@ class ContinuousBatcher:
         self.preempted: deque = deque()  # preemption order
         self.needs_prefill: set = set()  # released by preemption: prefill again on resume
 
-    def add_request(self, request_id: int, prompt: Sequence[int], max_tokens: int) -> None:  # :45-60
-        self.requests[request_id] = RequestContext(request_id, RequestState.Waiting, list(prompt), [], max_tokens)
+    def add_request(self, request_id: int, prompt: Sequence[int], max_tokens: int,
+                    sampling: SamplingParams = SamplingParams()) -> None:  # :45-60
+        self.requests[request_id] = RequestContext(request_id, RequestState.Waiting, list(prompt), [], max_tokens, sampling)
         self.waiting.append(request_id)
 
     def schedule(self) -> List[int]:  # :62-73
@@ -284,6 +330,36 @@ class ContinuousBatcher:
 
     def plan_decode(self) -> StepPlan:
         return self.manager.append([self.seq_of[r] for r in self.running], 1)
+
+    def sample(self, logits, u) -> List[int]:
+        """Draw the running requests' next tokens, each with its own settings,
+        from logits [len(running), vocab] in plan_decode's order and uniform
+        numbers u [len(running)] (device tensors, as sampling.sample takes
+        them); they join the requests' generated_tokens, and the caller
+        finishes those that reached max_tokens.  A row with nothing above -inf
+        raises before any request changes."""
+        import torch
+
+        from .sampling import sample
+
+        n = len(self.running)
+        if logits.dim() != 2 or logits.shape[0] != n:
+            raise ValueError(f"logits must be [{n}, vocab], a row per running request")
+        if n == 0:
+            return []
+        host = np.empty((4, n), np.float32)  # one copy to the device
+        for i, rid in enumerate(self.running):
+            p = self.requests[rid].sampling
+            host[0, i], host[2, i], host[3, i] = p.temperature, p.top_p, p.min_p
+            host[1].view(np.int32)[i] = p.top_k
+        dev = torch.from_numpy(host).to(logits.device)
+        drawn, _ = sample(logits, u, temperature=dev[0], top_k=dev[1].view(torch.int32), top_p=dev[2], min_p=dev[3])
+        tokens = drawn.tolist()
+        if min(tokens) < 0:
+            raise ValueError(f"request {self.running[tokens.index(-1)]}: no token above -inf")
+        for rid, token in zip(self.running, tokens):
+            self.requests[rid].generated_tokens.append(token)
+        return tokens
 
     def finish(self, request_id: int) -> np.ndarray:
         """Running or Preempted -> Finished; the request's blocks (if it

@@ -970,7 +970,11 @@ extern "C" int32_t it_supports(int32_t op, int32_t dtype) {
     case IT_OP_KV_GATHER:
     case IT_OP_KV_EVICT:
     case IT_OP_KV_COPY_BLOCKS:
+    case IT_OP_KV_APPEND_ROTARY:
+    case IT_OP_KV_MOVE:
     case IT_OP_PAGED_DECODE: return kv ? 1 : 0;
+    case IT_OP_ROTARY:
+    case IT_OP_SAMPLE: return kv && !is_quant(dtype) ? 1 : 0;
     case IT_OP_PAGED_PREFILL: return (dtype == IT_BF16 || dtype == IT_F16) ? 1 : 0;
     case IT_OP_FLASH_ATTENTION: return dtype == IT_F32 ? 1 : 0;
     default: return 0;

@@ -153,6 +153,7 @@ struct it_kv_manager {
   std::vector<int32_t> pending;    // blocks the step returned to the pool, in free order
   std::vector<uint32_t> blk_step;  // [pool capacity] step number of a block's first write...
   std::vector<int32_t> blk_first;  // ...and the output index of that write
+  std::vector<int32_t> old_row;    // [max_blocks] a sequence's blocks before its compaction
   uint32_t step = 0;
 };
 
@@ -175,6 +176,7 @@ extern "C" int32_t it_kv_manager_new(it_block_pool* pool, int32_t block_size, in
   m->table.assign(size_t(max_seqs) * size_t(max_blocks_per_seq), -1);
   m->pos.assign(size_t(max_seqs), 0);
   m->first.assign(size_t(max_seqs), 0);
+  m->old_row.assign(size_t(max_blocks_per_seq), -1);
   m->blk_step.assign(size_t(it_block_pool_capacity(pool)), 0u);
   m->blk_first.assign(size_t(it_block_pool_capacity(pool)), 0);
   *out = m;
@@ -436,6 +438,63 @@ extern "C" int32_t it_kv_manager_fork(it_kv_manager* m, int32_t src, int32_t dst
   }
   m->pos[size_t(dst)] = m->pos[size_t(src)];
   m->first[size_t(dst)] = m->first[size_t(src)];
+  return IT_OK;
+}
+
+extern "C" int32_t it_kv_manager_compact(it_kv_manager* m, int32_t seq, const int32_t* keep, int32_t n_keep, int64_t* src,
+                                         int64_t* dst, int32_t* delta, int32_t* pos, int32_t moves_cap, int32_t* n_moves,
+                                         int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted) {
+  const char* who = "it_kv_manager_compact";
+  if (!m || !n_moves || !n_evicted || (n_keep > 0 && !keep)) return fail(IT_INVALID_INPUT, "%s: NULL argument", who);
+  if (seq < 0 || seq >= m->max_seqs || n_keep < 0) return fail(IT_INVALID_INPUT, "%s: seq %d, n_keep %d", who, seq, n_keep);
+  if (m->window > 0) return fail(IT_NOT_IMPLEMENTED, "%s: the manager's window drops blocks by position", who);
+  const int64_t bs = m->bs, next = m->pos[size_t(seq)];
+  int32_t* const row = &m->table[size_t(seq) * size_t(m->max_blocks)];
+  // Every check before any change.
+  int64_t same = 0;  // tokens before the first that changes its position
+  for (int32_t i = 0; i < n_keep; ++i) {
+    if (keep[i] < 0 || keep[i] >= next || (i && keep[i] <= keep[i - 1]) || keep[i] / bs >= m->max_blocks || row[keep[i] / bs] < 0)
+      return fail(IT_INVALID_INPUT, "%s: keep[%d] = %d is not held, or not above the one before", who, i, keep[i]);
+    if (keep[i] == i && same == i) same = i + 1;
+  }
+  // Blocks that stay: all of what is kept, where no token changes its
+  // position; else the whole ones before the first that does.
+  const int64_t total = (n_keep + bs - 1) / bs, stay = same == n_keep ? total : same / bs;
+  const int64_t moves = n_keep - stay * bs > 0 ? n_keep - stay * bs : 0, fresh = total - stay;
+  if (moves > moves_cap || (moves > 0 && (!src || !dst)))
+    return fail(IT_INVALID_INPUT, "%s: %lld rows to move, capacity %d", who, (long long)moves, moves_cap);
+  if (it_block_pool_num_free(m->pool) < fresh)
+    return fail(IT_INVALID_INPUT, "%s: %lld fresh blocks, the pool has %lld", who, (long long)fresh,
+                (long long)it_block_pool_num_free(m->pool));
+  int64_t returned = 0;
+  for (int64_t j = stay; j < m->max_blocks; ++j) {
+    if (row[j] < 0) continue;
+    const int64_t rc = it_block_pool_ref_count(m->pool, row[j]);
+    if (rc <= 0) return fail(IT_INVALID_INPUT, "%s: block %d is already free", who, row[j]);
+    returned += rc == 1;
+  }
+  if (returned > 0 && (!evicted || returned > evicted_cap))
+    return fail(IT_INVALID_INPUT, "%s: %lld blocks return to the pool, capacity %d", who, (long long)returned, evicted_cap);
+  std::copy(row, row + m->max_blocks, m->old_row.begin());
+  // Fresh blocks first: none of them is one that this call gives back.
+  for (int64_t j = stay; j < m->max_blocks; ++j) row[j] = j < total ? int32_t(it_block_pool_allocate(m->pool)) : -1;
+  for (int64_t i = stay * bs, t = 0; i < n_keep; ++i, ++t) {
+    src[t] = int64_t(m->old_row[size_t(keep[i] / bs)]) * bs + keep[i] % bs;
+    dst[t] = int64_t(row[i / bs]) * bs + i % bs;
+    if (delta) delta[t] = int32_t(i - keep[i]);
+    if (pos) pos[t] = int32_t(i);
+  }
+  int32_t ne = 0;
+  for (int64_t j = stay; j < m->max_blocks; ++j) {
+    const int32_t id = m->old_row[size_t(j)];
+    if (id < 0) continue;
+    if (it_block_pool_free(m->pool, id) != IT_OK) return IT_INVALID_INPUT;
+    if (it_block_pool_ref_count(m->pool, id) == 0) evicted[ne++] = id;
+  }
+  m->pos[size_t(seq)] = n_keep;
+  m->first[size_t(seq)] = 0;
+  *n_moves = int32_t(moves);
+  *n_evicted = ne;
   return IT_OK;
 }
 

@@ -99,7 +99,8 @@ struct Call<kHost, R (*)(A...)> {
   X(it_kv_sync_tables, false) X(it_kv_copy_blocks, false) X(it_paged_decode_workspace, false)                            \
   X(it_paged_decode_partition, true) X(it_paged_decode, false) X(it_paged_decode_split, false)                           \
   X(it_paged_decode_combine, false) X(it_paged_prefill_workspace, false) X(it_paged_prefill_ws, false)                   \
-  X(it_flash_attention_workspace, false) X(it_flash_attention, false)
+  X(it_flash_attention_workspace, false) X(it_flash_attention, false) X(it_rotary_apply, false)                          \
+  X(it_kv_append_rotary, false) X(it_kv_move, false) X(it_sample_workspace, false) X(it_sample, false)
 
 #define IT_WRAP(name, host)                                                         \
   decltype(&name) p_##name = nullptr;                                               \

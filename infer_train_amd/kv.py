@@ -13,9 +13,11 @@ from typing import Optional, Tuple
 import numpy as np
 import torch
 
-from ._lib import BF16, CacheDesc, F16, F32, Q4_0, Q4_1, Q5_0, Q5_1, Q8_0, call, check, lib
+from ._lib import (BF16, CacheDesc, F16, F32, Q4_0, Q4_1, Q5_0, Q5_1, Q8_0, ROTARY_HALF, ROTARY_INTERLEAVED,
+                   ROTARY_SCALE_BASE, ROTARY_SCALE_LINEAR, ROTARY_SCALE_NONE, ROTARY_SCALE_PARTS, RotaryDesc, call, check,
+                   lib)
 
-__all__ = ["PagedKvCache", "RopeTable", "flash_attention", "torch_dtype_id", "stream_handle"]
+__all__ = ["PagedKvCache", "RopeTable", "Rotary", "flash_attention", "torch_dtype_id", "stream_handle"]
 
 _TORCH_IDS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _ID_TORCH = {F32: torch.float32, F16: torch.float16, BF16: torch.bfloat16}
@@ -67,6 +69,80 @@ class RopeTable:
         self._h, self._at = h, h.value
         self.n_dims, self.max_pos, self.freq_base, self.device = n_dims, max_pos, freq_base, device
         self._destroy = lib.it_rope_table_destroy
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            self._destroy(h)
+            self._h = None
+
+
+_LAYOUTS = {"interleaved": ROTARY_INTERLEAVED, "half": ROTARY_HALF}
+_SCALINGS = {"none": ROTARY_SCALE_NONE, "linear": ROTARY_SCALE_LINEAR, "base": ROTARY_SCALE_BASE,
+             "parts": ROTARY_SCALE_PARTS}
+
+
+def _rows(t: torch.Tensor, name: str) -> Tuple[int, int]:
+    """Address and token stride of a [tokens, heads, head_dim] tensor whose
+    tokens are each contiguous."""
+    if not t.is_cuda:
+        raise ValueError("device tensor expected")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim]")
+    s = t.stride()
+    if (s[2] != 1 and t.shape[2] != 1) or (s[1] != t.shape[2] and t.shape[1] != 1):
+        raise ValueError(f"{name}: each token's heads must be contiguous")
+    return t.data_ptr(), s[0]
+
+
+class Rotary:
+    """Rotary positions (it_rotary_new): pairs (2p, 2p + 1) ("interleaved") or
+    (p, p + n_dims/2) ("half") of a head's first n_dims elements turned by
+    position * f_p, f_p = freq_base^(-2p/n_dims).  scaling stretches the
+    frequencies for contexts longer than those trained on: "linear" (f /
+    factor), "base" (freq_base * factor^(n_dims/(n_dims-2))) or "parts" (pairs
+    that turn less than `low` times in original_ctx positions f / factor, those
+    above `high` times f, a blend between); inv_freq gives the f_p themselves.
+    magnitude multiplies the rotated elements (YaRN: 0.1 ln(factor) + 1)."""
+
+    def __init__(self, n_dims: int, layout: str = "half", freq_base: float = 10000.0, scaling: str = "none",
+                 factor: float = 1.0, original_ctx: int = 0, low: float = 1.0, high: float = 32.0, magnitude: float = 1.0,
+                 inv_freq=None, device: int = 0):
+        if layout not in _LAYOUTS or scaling not in _SCALINGS:
+            raise ValueError(f"layout {layout!r} (one of {list(_LAYOUTS)}), scaling {scaling!r} (one of {list(_SCALINGS)})")
+        freqs = None
+        if inv_freq is not None:
+            freqs = np.ascontiguousarray(inv_freq, dtype=np.float64)
+            if freqs.shape != (n_dims // 2,):
+                raise ValueError("inv_freq must hold n_dims / 2 frequencies")
+        desc = RotaryDesc(n_dims, _LAYOUTS[layout], _SCALINGS[scaling], original_ctx, freq_base, factor, low, high, magnitude,
+                          None if freqs is None else freqs.ctypes.data)
+        used = np.empty(max(n_dims // 2, 1), np.float64)
+        check(lib.it_rotary_frequencies(C.byref(desc), used.ctypes.data))
+        h = C.c_void_p()
+        check(lib.it_rotary_new(device, C.byref(desc), C.byref(h)))
+        self._h, self._at = h, h.value
+        self._destroy = lib.it_rotary_destroy
+        self.n_dims, self.layout, self.magnitude, self.device = n_dims, layout, magnitude, device
+        self.inv_freq = used  # radians per position of each pair
+
+    def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None,
+              transpose: bool = False) -> torch.Tensor:
+        """x [n_tokens, n_heads, head_dim] (any token stride) rotated to int32
+        positions [n_tokens]; transpose: the gradient of that rotation (with
+        magnitude 1 its inverse).  out may be x itself."""
+        at, stride = _rows(x, "x")
+        n, heads, d = x.shape
+        if positions.dtype != torch.int32 or positions.numel() != n:
+            raise TypeError("positions must be int32, one per token")
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif out.dtype != x.dtype or out.shape != x.shape:
+            raise TypeError("out must have x's shape and dtype")
+        to, to_stride = _rows(out, "out")
+        _check(call.it_rotary_apply(self._at, at, torch_dtype_id(x.dtype), stride, _ptr(positions), n, heads, d,
+                                    int(bool(transpose)), to, to_stride, _raw_stream(self.device)))
+        return out
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -222,6 +298,41 @@ class PagedKvCache:
                                       torch_dtype_id(q_out.dtype), _raw_stream(self._index)))
         return q_out
 
+    def append_rotary(self, rotary: Rotary, q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor,
+                      slot_mapping: torch.Tensor, positions: torch.Tensor, q_out: Optional[torch.Tensor] = None,
+                      q_out_dtype: Optional[torch.dtype] = None) -> Optional[torch.Tensor]:
+        """Rotary positions then append (it_kv_append_rotary): q [n_tokens,
+        n_heads, D], k, v [n_tokens, n_kv_heads, D] of one float dtype, each
+        token contiguous (views of a fused projection's rows too); positions
+        int32 [n_tokens].  Returns the rotated q (q's dtype, or q_out_dtype);
+        q None: k and v only."""
+        if slot_mapping.dtype != torch.int64 or positions.dtype != torch.int32:
+            raise TypeError("slot_mapping must be int64 and positions int32")
+        n = slot_mapping.numel()
+        row = (n, self.n_kv_heads, self.head_dim)
+        if positions.numel() != n or k.shape != row or v.shape != row:
+            raise ValueError("k, v must be [n_tokens, n_kv_heads, head_dim], with a slot and a position per token")
+        if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+            raise TypeError("q, k, v must have one dtype")
+        (ka, ks), (va, vs) = _rows(k, "k"), _rows(v, "v")
+        qa = oa = None
+        qs = heads = out_id = 0
+        if q is not None:
+            if q.shape[0] != n or q.shape[-1] != self.head_dim:
+                raise ValueError("q must be [n_tokens, n_heads, head_dim]")
+            qa, qs = _rows(q, "q")
+            heads = q.shape[1]
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q_out_dtype or q.dtype, device=q.device)
+            elif q_out.shape != q.shape:
+                raise ValueError("q_out must have q's shape")
+            oa, out_id = _ptr(q_out), torch_dtype_id(q_out.dtype)
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        _check(call.it_kv_append_rotary(self._at, rotary._at, qa, ka, va, torch_dtype_id(k.dtype), qs, ks, vs, heads,
+                                        _ptr(slot_mapping), _ptr(positions), n, oa, out_id, _raw_stream(self._index)))
+        return q_out
+
     def gather(self, block_tables: torch.Tensor, ctx_lens: torch.Tensor, start_pos: Optional[torch.Tensor],
                cu_out: torch.Tensor, max_tokens: int, k_out: torch.Tensor, v_out: torch.Tensor) -> None:
         _check(call.it_kv_gather(self._at, _ptr(block_tables), block_tables.shape[1], _ptr(ctx_lens), _ptr(start_pos),
@@ -238,6 +349,20 @@ class PagedKvCache:
 
     def copy_blocks(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         _check(call.it_kv_copy_blocks(self._at, _ptr(src), _ptr(dst), src.numel(), _raw_stream(self._index)))
+
+    def move(self, src: torch.Tensor, dst: torch.Tensor, rotary: Optional[Rotary] = None,
+             delta: Optional[torch.Tensor] = None) -> None:
+        """Rows of slots src to slots dst (int64 [n]) in every layer and head
+        (it_kv_move); with rotary, keys are turned by delta positions (int32
+        [n], new - old), as KvManager.compact plans it."""
+        if src.dtype != torch.int64 or dst.dtype != torch.int64 or src.numel() != dst.numel():
+            raise TypeError("src and dst must be int64, one slot each per row")
+        if (rotary is None) != (delta is None):
+            raise TypeError("rotary and delta go together")
+        if delta is not None and (delta.dtype != torch.int32 or delta.numel() != src.numel()):
+            raise TypeError("delta must be int32, one per row")
+        _check(call.it_kv_move(self._at, _ptr(src), _ptr(dst), src.numel(), None if rotary is None else rotary._at,
+                               _ptr(delta), _raw_stream(self._index)))
 
     # ---- attention --------------------------------------------------------
     def decode_workspace(self, n_seqs: int, n_heads: int, max_tokens: int, partition: int = 512) -> torch.Tensor:
