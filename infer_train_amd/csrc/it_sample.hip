@@ -12,14 +12,15 @@
 // exact, so any number of workgroups may add them in any order, and the same
 // row gives the same token in any batch.
 //
-// Two launches.  The first reads the logits from HBM and takes each slice's
+// Three launches.  The first reads the logits from HBM and takes each slice's
 // maximum.  The second reads them again (from the last-level cache where the
 // call's logits fit its 256 MB), weighs them in fp64 against the row's maximum
-// and adds counts and masses of 1024 bins, linear in z, in LDS and then per row;
-// the row's last workgroup to finish answers the questions.  Where top-k or
-// min-p bound the tokens that matter, those alone are weighed, and listed, so
-// that the last workgroup need not read the row a third time: of the maxima of
-// groups of tokens the k-th largest is a lower bound of the k-th largest token.
+// and adds counts and masses of 2048 bins, linear in z, in LDS and then per row.
+// The third finds the few bins that a row's answers lie in, gathers their tokens
+// and answers from those.  Where top-k or min-p bound the
+// tokens that matter, those alone are weighed, and listed, so that the third need
+// not read the row again: of the maxima of groups of tokens the k-th largest is a
+// lower bound of the k-th largest token.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -29,21 +30,27 @@
 using namespace itkv;
 
 namespace {
-constexpr int kThreads = 512;
+constexpr int kSliceThreads = 512;   // of a slice's workgroup
+constexpr int kSliceWaves = kSliceThreads / 64;
+constexpr int kThreads = 512;        // of a row's
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2 * kThreads;  // locate(): two per thread
-constexpr int kList = 2048;          // tokens listed per row, and held in LDS
+constexpr int kBins = 2048;          // of a row, linear in z
+constexpr int kList = 2048;          // tokens listed per row, and gathered in LDS
+constexpr int kSliceList = kList - 1;  // of a slice: its workgroup's LDS is a quarter of a CU's
+constexpr int kFew = 256;            // tokens compared all with all
+constexpr int kFineBits = 10, kFine = 1 << kFineBits;
+constexpr uint32_t kGathered = 1u << 31;  // of a bin's count
 constexpr int kMaxSlices = 32;
-constexpr int kGroups = 2 * kWaves;  // group maxima per slice: half waves
+constexpr int kGroups = 2 * kSliceWaves;  // group maxima per slice: half waves
 constexpr int kMaxVocab = 1 << 18;   // a sum of weights stays below 2^62
 constexpr int kIndexBits = 18;
 constexpr double kUnit = 0x1p44;      // weight of the largest token
-constexpr double kBinsPerBit = 22.0;  // of log2 weight; 45.x bits weigh at all
+constexpr double kLeast = 0x1.0000000000001p-45;  // smaller weights round to nothing
+constexpr double kBinsPerBit = 44.0;  // of log2 weight, of which 45 weigh at all
 constexpr uint32_t kDeadKey = 0x007FFFFFu;  // order_key(-inf)
 
 struct RowState {
-  uint32_t ticket, n_list;
-  uint64_t pad[31];
+  uint32_t n_list, n_gathered, ticket, pad[61];
   uint64_t best[kMaxSlices];               // order of each slice's first token, 0: nothing above -inf
   uint32_t group_max[kMaxSlices * kGroups];
   uint32_t count[kBins];
@@ -78,39 +85,53 @@ __device__ __forceinline__ uint64_t order_of(float z, int index) {
 __device__ __forceinline__ float order_value(uint64_t o) { return key_value(uint32_t(o >> kIndexBits)); }
 __device__ __forceinline__ int order_index(uint64_t o) { return kMaxVocab - 1 - int(o & (kMaxVocab - 1)); }
 
-// 2^x for x in [-46, 0] within 2^-51 of its value: the Taylor sum of exp(f ln 2)
-// around the nearest integer, |f| <= 1/2, to f^12 (the next term is below 2^-58).
-__device__ __forceinline__ double exp2_neg(double x) {
-  const double n = __builtin_rint(x), f = (x - n) * 0.6931471805599453;
-  double p = 1.0 / 479001600.0;
-  constexpr double kInv[12] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320,
-                               1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800};
-#pragma unroll
-  for (int i = 11; i >= 0; --i) p = fma(p, f, kInv[i]);
-  return __builtin_amdgcn_ldexp(p, int(n));
+// 2^x = 2^n (1 + f h(f)) with n the nearest integer, |f| <= 1/2, and h the
+// polynomial through (2^f - 1) / f at the ten Chebyshev nodes of [-1/2, 1/2]: off by
+// less than 2^-50 of 2^x, and exactly 1 at x = 0.
+constexpr double kExp2[10] = {0x1.62e42fefa39f7p-1,  0x1.ebfbdff82c590p-3,  0x1.c6b08d7044119p-5, 0x1.3b2ab6fba385fp-7, 0x1.5d87fe908f88ap-10,
+                              0x1.4309130378460p-13, 0x1.ffcb76789860fp-17, 0x1.62bfe46117445p-20, 0x1.b6571de2f2351p-24, 0x1.e5e9f548e5726p-28};
+
+// An fp64 constant kept in scalar registers: as a literal it would be moved
+// into vector registers before each use, twice as much work as the products.
+__device__ __forceinline__ double scalar(double x) {
+  asm("" : "+s"(x));
+  return x;
 }
 
-// A row's settings, the same in all its threads.
+// A row's weights, the same in all its threads.
 struct Weigher {
   float top;      // max z
   float floor;    // tokens below weigh nothing, fail min-p or cannot be among the first k
   double bits;    // log2(e) / T
-  double min_p;
-  // Weight and bin of a token with z >= floor; false: not kept.
+  double least;   // min-p, or the smallest weight that does not round to nothing
+  double exp2[10], unit, magic, bins;  // kExp2, kUnit, 2^52, -kBinsPerBit in scalar registers
+  __device__ __forceinline__ void constants() {
+#pragma unroll
+    for (int i = 0; i < 10; ++i) exp2[i] = scalar(kExp2[i]);
+    unit = scalar(kUnit);
+    magic = scalar(0x1p52);
+    bins = scalar(-kBinsPerBit);
+  }
+  // Weight and bin of a token with floor <= z <= top; false: not kept.
   __device__ __forceinline__ bool operator()(float z, uint64_t& w, int& bin) const {
-    const double x = z == top ? 0.0 : (double(z) - double(top)) * bits;
-    if (!(x > -46.0)) return false;
-    const double e = exp2_neg(x);
+    // inf - inf is NaN, of which fmin makes 0: tokens at a top of +inf weigh 1.
+    const double x = fmin((double(z) - double(top)) * bits, 0.0);
+    const double n = __builtin_rint(x), f = x - n;
+    double h = exp2[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) h = fma(h, f, exp2[i]);
+    const double e = __builtin_amdgcn_ldexp(fma(h, f, 1.0), int(n));
     // Rounded to a whole number of units by the sum with 2^52.
-    w = __builtin_bit_cast(uint64_t, fma(e, kUnit, 0x1p52)) & ((uint64_t(1) << 52) - 1);
-    bin = int(x * -kBinsPerBit);
-    return w != 0 && e >= min_p;
+    w = __builtin_bit_cast(uint64_t, fma(e, unit, magic)) & ((uint64_t(1) << 52) - 1);
+    bin = min(int(x * bins), kBins - 1);
+    return e >= least;
   }
 };
 
-// f(index, z) for tokens of a row, 16-byte vectors `lo` .. `hi` of its aligned
-// part, with `head` also the tokens before it and with `tail` those behind.
-template <int DT, class F>
+// f(index, z) for the tokens of a slice of a row: its share of the 16-byte vectors
+// of the row's aligned part, the first slice also the tokens before that part,
+// the last those behind it.  A thread's tokens come in ascending order.
+template <int DT, int kBlock, class F>
 __device__ __forceinline__ void each_token(const char* row, int vocab, int slice, int slices, F&& f) {
   constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es, U = 4;
   using In = RowVec<DT, V>;
@@ -120,13 +141,13 @@ __device__ __forceinline__ void each_token(const char* row, int vocab, int slice
   const int per = (vecs + slices - 1) / slices, lo = min(vecs, slice * per), hi = min(vecs, lo + per);
   if (slice == 0 && tid < head) f(tid, load_element(row, tid, DT));
   const auto* const v = reinterpret_cast<const typename In::raw*>(row + head * es);
-  for (int x0 = lo + tid; x0 < hi; x0 += kThreads * U) {
+  for (int x0 = lo + tid; x0 < hi; x0 += kBlock * U) {
     typename In::raw w[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) w[j] = v[min(x0 + j * kThreads, hi - 1)];
+    for (int j = 0; j < U; ++j) w[j] = v[min(x0 + j * kBlock, hi - 1)];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int x = x0 + j * kThreads;
+      const int x = x0 + j * kBlock;
       if (x >= hi) break;
       float z[V];
       In::widen(w[j], z);
@@ -148,17 +169,17 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void sample_maxima(SampleArgs a) {
-  __shared__ uint64_t best_of[kWaves];
+__global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
+  __shared__ uint64_t best_of[kSliceWaves];
   const int slice = int(blockIdx.x), lane = int(threadIdx.x & 63), wave = int(threadIdx.x >> 6);
   RowState& rs = a.rows[blockIdx.y];
-  // Clear what the second launch adds to.
-  if (slice == 0 && threadIdx.x == 0) rs.ticket = rs.n_list = 0u;
-  for (int b = slice * kThreads + int(threadIdx.x); b < kBins; b += a.slices * kThreads) rs.count[b] = 0u, rs.mass[b] = 0u;
+  if (slice == 0 && threadIdx.x == 0)  // what the second launch adds to
+    rs.n_list = rs.n_gathered = rs.ticket = 0u;
+  for (int b = slice * kSliceThreads + int(threadIdx.x); b < kBins; b += a.slices * kSliceThreads) rs.count[b] = 0u, rs.mass[b] = 0u;
   float top = -INFINITY;
   int at = -1;
-  each_token<DT>(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices, [&](int i, float z) {
-    if (z > top) top = z, at = i;  // the first of equals: a thread's tokens come in ascending order
+  each_token<DT, kSliceThreads>(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices, [&](int i, float z) {
+    if (z > top) top = z, at = i;  // of equals the first
   });
   uint64_t best = at < 0 ? 0u : order_of(top, at);
   uint32_t group = order_key(top);
@@ -169,148 +190,373 @@ __global__ __launch_bounds__(kThreads) void sample_maxima(SampleArgs a) {
   if (lane == 0) best_of[wave] = best;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < kWaves; ++i) best = best_of[i] > best ? best_of[i] : best;
+    for (int i = 1; i < kSliceWaves; ++i) best = best_of[i] > best ? best_of[i] : best;
     rs.best[slice] = best;
   }
 }
 
+// A row's settings, as all its workgroups derive them from the first launch's
+// maxima; false where there is nothing to weigh: an empty row, or one that takes
+// the first of the order (best is its place).
+struct Settings {
+  Weigher weigh;
+  uint64_t best;
+  int top_k;
+  bool listed;  // few tokens can be kept: they are listed
+  __device__ __forceinline__ bool derive(const SampleArgs& a, int row) {
+    const RowState& rs = a.rows[row];
+    const int lane = int(threadIdx.x & 63), groups = a.slices * kGroups;
+    const float temp = a.temperatures ? a.temperatures[row] : a.temperature;
+    const float min_p = a.min_ps ? a.min_ps[row] : a.min_p;
+    top_k = a.top_ks ? a.top_ks[row] : a.top_k;
+    best = wave_max64(lane < a.slices ? rs.best[lane] : 0u);
+    best = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(best >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(best)));
+    if (best == 0u || !(temp > 0.0f)) return false;  // uniform
+    weigh.top = order_value(best);
+    weigh.bits = 1.4426950408889634 / double(temp);
+    const double share = min_p > 0.0f ? fmin(double(min_p), 1.0) : 0.0;  // NaN: off
+    weigh.least = fmax(share, kLeast);
+    // Below floor a weight is below `least`: z - top < T ln(least), widened by
+    // fp32's rounding.
+    weigh.floor = weigh.top;
+    if (weigh.top < INFINITY) {
+      const double low = double(weigh.top) + (share > kLeast ? log2(share) : -45.0) / weigh.bits;
+      weigh.floor = float(low - fabs(low) * 0x1p-20);
+    }
+    // Whatever the floor, a token at -inf is never kept.
+    weigh.floor = fmaxf(weigh.floor, -3.402823466e38f);
+    listed = share > 0.0 || (top_k > 0 && top_k <= groups);
+    return true;
+  }
+  // The floor raised to the first sixteen bits of the top_k-th largest group
+  // maximum: at least top_k tokens have keys that large.
+  __device__ __forceinline__ void raise_floor(const SampleArgs& a, int row) {
+    const int lane = int(threadIdx.x & 63), groups = a.slices * kGroups;
+    if (top_k <= 0 || top_k > groups) return;
+    constexpr int kLoads = kMaxSlices * kGroups / 64;
+    uint32_t g[kLoads], key = 0u;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = j * 64 + lane;
+      g[j] = i < groups ? a.rows[row].group_max[i] : 0u;
+    }
+    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
+      const uint32_t with = key | bit;
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j)
+        if (j * 64 < groups) n += __popcll(__ballot(g[j] >= with));
+      if (n >= top_k) key = with;
+    }
+    if (key > kDeadKey) weigh.floor = fmaxf(weigh.floor, key_value(key));
+  }
+};
+
+template <int DT>
+__global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
+  __shared__ uint64_t mass[kBins], list[kSliceList];
+  __shared__ uint32_t count[kBins], n, base;
+  const int t = int(threadIdx.x), slice = int(blockIdx.x), row = int(blockIdx.y);
+  RowState& rs = a.rows[row];
+  Settings set;
+  if (!set.derive(a, row)) return;
+  set.raise_floor(a, row);
+  set.weigh.constants();
+  for (int b = t; b < kBins; b += kSliceThreads) count[b] = 0u, mass[b] = 0u;
+  if (t == 0) n = 0u;
+  __syncthreads();
+  each_token<DT, kSliceThreads>(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices, [&](int i, float z) {
+    if (!(z >= set.weigh.floor)) return;
+    uint64_t w;
+    int b;
+    if (!set.weigh(z, w, b)) return;
+    atomicAdd(reinterpret_cast<unsigned long long*>(&mass[b]), (unsigned long long)(w));
+    if (set.top_k > 0) atomicAdd(&count[b], 1u);  // only top-k asks for counts
+    if (set.listed) {
+      const uint32_t at = atomicAdd(&n, 1u);
+      if (at < kSliceList) list[at] = order_of(z, i);
+    }
+  });
+  __syncthreads();
+  for (int b = t; b < kBins; b += kSliceThreads) {
+    if (mass[b] == 0u) continue;
+    atomicAdd(reinterpret_cast<unsigned long long*>(&rs.mass[b]), (unsigned long long)(mass[b]));
+    if (set.top_k > 0) atomicAdd(&rs.count[b], count[b]);
+  }
+  if (!set.listed) return;
+  if (t == 0) base = atomicAdd(&rs.n_list, n <= kSliceList ? n : uint32_t(kList + 1));
+  __syncthreads();
+  if (n <= kSliceList && base + n <= kList)
+    for (uint32_t i = t; i < n; i += kSliceThreads) rs.list[base + i] = list[i];
+}
+
 struct Shared {
-  uint64_t mass[kBins];   // the row's bins (before the last workgroup: its slice's)
-  uint64_t fine[kBins];   // masses of the bins inside one of them
-  uint64_t cand[kList];   // tokens of that bin (before: the slice's list)
-  uint64_t last[64];
+  uint64_t mass[kBins];   // the row's bins, then what lies before each but is not gathered
+  uint64_t cand[kList];   // the tokens gathered to answer from
+  struct Weighed {
+    uint64_t order, weight;
+  };
+  union {
+    uint64_t fine[kFine];          // narrow(): bins inside a bin
+    Weighed weighed[kFew];         // answer_from()
+  };
   uint32_t count[kBins];
-  uint32_t fine_count[kBins];
+  uint32_t fine_count[kFine];
+  uint64_t last[64];
   uint64_t wave_mass[kWaves];
   uint32_t wave_count[kWaves];
   unsigned long long lo, hi;
-  uint32_t n, is_last, base;
-  // locate()'s and select()'s answers
-  uint64_t before_mass, total_mass, mass_to, weight;
-  uint32_t before_count, total_count, in_bin, bin;
+  uint32_t n, base;
+  uint64_t kept;
+  struct Found {
+    uint64_t before_mass, mass;
+    uint32_t before_count, count, bin;
+  } found[5];
+  uint64_t weight, mass_to;
   int token;
 };
 
-// The bin in which the cumulative count (or mass), from before_* on, reaches
-// `goal`: s.bin, s.in_bin tokens, what is before it in s.before_*.
-__device__ __forceinline__ void locate(Shared& s, const uint32_t* count, const uint64_t* mass, bool by_count, uint64_t goal,
-                                       uint32_t before_count, uint64_t before_mass) {
-  const int t = int(threadIdx.x), lane = t & 63, wave = t >> 6;
-  const uint32_t c0 = count[2 * t], c1 = count[2 * t + 1];
-  const uint64_t m0 = mass[2 * t], m1 = mass[2 * t + 1];
-  uint32_t c = c0 + c1;
-  uint64_t m = m0 + m1;
+// Sums over the threads before this one, and over all.
+struct Scan {
+  uint64_t mass, total_mass;
+  uint32_t count, total_count;
+};
+__device__ __forceinline__ Scan block_scan(Shared& s, uint32_t count, uint64_t mass) {
+  const int lane = int(threadIdx.x & 63), wave = int(threadIdx.x >> 6);
+  uint32_t c = count;
+  uint64_t m = mass;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const uint32_t cu = uint32_t(__shfl_up(int(c), o));
     const uint64_t mu = uint64_t(__shfl_up((unsigned long long)(m), o));
     if (lane >= o) c += cu, m += mu;
   }
+  __syncthreads();  // the sums of the call before are read
   if (lane == 63) s.wave_count[wave] = c, s.wave_mass[wave] = m;
   __syncthreads();
-  uint32_t cs = before_count + c - c0 - c1;
-  uint64_t ms = before_mass + m - m0 - m1;
-  for (int w = 0; w < wave; ++w) cs += s.wave_count[w], ms += s.wave_mass[w];
-  if (t == kThreads - 1) s.total_count = cs + c0 + c1, s.total_mass = ms + m0 + m1;
+  Scan r{m - mass, 0u, c - count, 0u};
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t ci = i ? c1 : c0;
-    const uint64_t mi = i ? m1 : m0;
-    const uint64_t before = by_count ? cs : ms, after = before + (by_count ? uint64_t(ci) : mi);
-    if (before < goal && goal <= after) {
-      s.bin = uint32_t(2 * t + i);
-      s.in_bin = ci;
-      s.before_count = cs;
-      s.before_mass = ms;
-    }
-    cs += ci;
-    ms += mi;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) r.count += s.wave_count[w], r.mass += s.wave_mass[w];
+    r.total_count += s.wave_count[w];
+    r.total_mass += s.wave_mass[w];
   }
-  __syncthreads();
+  return r;
 }
+
+// A thread's N consecutive bins with what is before the first of them.
+template <int N>
+struct Bins {
+  uint64_t mass[N], before_mass, total_mass;
+  uint32_t count[N], before_count, total_count;
+  __device__ __forceinline__ Bins(Shared& s, const uint32_t* c, const uint64_t* m, uint32_t base_count, uint64_t base_mass) {
+    uint32_t cs = 0u;
+    uint64_t ms = 0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      count[i] = c[N * threadIdx.x + i];
+      mass[i] = m[N * threadIdx.x + i];
+      cs += count[i];
+      ms += mass[i];
+    }
+    const Scan scan = block_scan(s, cs, ms);
+    before_count = base_count + scan.count;
+    before_mass = base_mass + scan.mass;
+    total_count = base_count + scan.total_count;
+    total_mass = base_mass + scan.total_mass;
+  }
+  // The one bin in which the cumulative count (or mass) reaches `goal`, 1 <=
+  // goal <= the total, into `f` (a barrier later).
+  __device__ __forceinline__ void find(Shared::Found& f, bool by_count, uint64_t goal) const {
+    uint32_t cs = before_count;
+    uint64_t ms = before_mass;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint64_t before = by_count ? cs : ms, after = before + (by_count ? uint64_t(count[i]) : mass[i]);
+      if (before < goal && goal <= after) f = {ms, mass[i], cs, count[i], uint32_t(N * threadIdx.x + i)};
+      cs += count[i];
+      ms += mass[i];
+    }
+  }
+};
 
 template <int DT>
 struct Row {
   const char* data;
   int vocab;
-  const uint64_t* list;  // or NULL: too many tokens to list
-  uint32_t n_list;
   Weigher weigh;
-  // f(order, z) for the row's tokens with lo <= z <= hi that may be kept.
+  // f(order, z) for the row's tokens with lo <= z <= hi.
   template <class F>
   __device__ __forceinline__ void each(float lo, float hi, F&& f) const {
-    if (list) {
-      for (uint32_t i = threadIdx.x; i < n_list; i += kThreads) {
-        const uint64_t o = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const float z = order_value(o);
-        if (z >= lo && z <= hi) f(o, z);
-      }
-    } else {
-      each_token<DT>(data, vocab, 0, 1, [&](int i, float z) {
-        if (z >= lo && z <= hi) f(order_of(z, i), z);
-      });
+    each_token<DT, kThreads>(data, vocab, 0, 1, [&](int i, float z) {
+      if (z >= lo && z <= hi) f(order_of(z, i), z);
+    });
+  }
+  // The z of bins first .. last, widened by what rounding can move an edge.
+  __device__ __forceinline__ void span(int first, int last, float& lo, float& hi) const {
+    lo = weigh.floor;
+    hi = INFINITY;
+    if (weigh.top < INFINITY && weigh.bits > 0.0) {
+      const double edge = 1.0 / (kBinsPerBit * weigh.bits), top = double(weigh.top);
+      const double begin = top - double(first) * edge, end = top - double(last + 1) * edge;
+      hi = float(begin + (fabs(begin) + edge) * 0x1p-20);
+      lo = fmaxf(lo, float(end - (fabs(end) + edge) * 0x1p-20));
     }
   }
 };
 
-// The token at which the cumulative count (or mass) along the order reaches
-// `goal`: s.token, its weight, and the mass up to and with it in s.mass_to.
-// All threads of the workgroup; 1 <= goal <= the row's total.
-template <int DT>
-__device__ void select(Shared& s, const Row<DT>& row, bool by_count, uint64_t goal) {
-  const int t = int(threadIdx.x);
-  locate(s, s.count, s.mass, by_count, goal, 0u, 0u);
-  const int bin = int(s.bin);
-  uint32_t n = s.in_bin, bc = s.before_count;
-  uint64_t bm = s.before_mass;
-  // The bin's z, widened by what fp32 and fp64 rounding can move an edge.
-  float zlo = row.weigh.floor, zhi = INFINITY;
-  if (row.weigh.top < INFINITY && row.weigh.bits > 0.0) {
-    const double edge = 1.0 / (kBinsPerBit * row.weigh.bits), top = double(row.weigh.top);
-    const double first = top - double(bin) * edge, end = top - double(bin + 1) * edge;
-    zhi = float(first + (fabs(first) + edge) * 0x1p-20);
-    zlo = fmaxf(zlo, float(end - (fabs(end) + edge) * 0x1p-20));
+// Where top-k ends, where top-p ends (each leaves the mass kept), the draw: the
+// goal of each as a function of the mass kept so far, which none decreases with.
+struct Questions {
+  uint64_t top_k;  // 0: off
+  float top_p, u;
+  __device__ __forceinline__ bool cuts() const { return top_p < 1.0f; }  // NaN: off
+  __device__ __forceinline__ uint64_t cut(uint64_t kept) const {
+    // before < top_p kept  <=>  before < ceil(top_p kept), before being whole.
+    const double part = top_p > 0.0f ? ceil(double(top_p) * double(kept)) : 0.0;
+    const uint64_t goal = part < 1.0 ? 1u : uint64_t(part);
+    return goal < kept ? goal : kept;
   }
-  bool held = n <= kList;  // in s.cand
+  __device__ __forceinline__ uint64_t draw(uint64_t kept) const {
+    const uint64_t goal = u > 0.0f ? uint64_t(fmin(double(u), 1.0) * double(kept)) : 0u;  // kept <= 2^62
+    return (goal < kept ? goal : kept - 1) + 1;
+  }
+};
+
+// Answers from the tokens in s.cand (n <= kFew of them), each after those of
+// s.mass and s.count of its bin that are not among them (`gaps`; else there are
+// no others).  kept, tokens: the row's mass and number, with gaps.  Each token's
+// place is found by comparing it with all others, a power of two of threads
+// sharing them: no step waits for the one before, but the work grows with n^2
+// (n = 128: 1 us, 256: 4, 512: 28).
+template <int DT>
+__device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, bool gaps, uint64_t kept,
+                                            uint32_t tokens, const SampleArgs& a, int out) {
+  const int t = int(threadIdx.x);
+  int log2_parts = 0;
+  while (log2_parts < 6 && uint32_t(kThreads >> (log2_parts + 1)) >= n) ++log2_parts;
+  const uint32_t parts = 1u << log2_parts;
+  __syncthreads();
+  Shared::Weighed* const all = s.weighed;
+  uint64_t own = 0u, w = 0u;
+  int bin = 0;
+  if (t < int(n)) {
+    own = s.cand[t];
+    row.weigh(order_value(own), w, bin);
+    all[t] = {own, w};
+  }
+  __syncthreads();
+  const uint32_t i = uint32_t(t) >> log2_parts, part = uint32_t(t) & (parts - 1);
+  own = i < n ? all[i].order : ~0ull;
+  uint32_t before_count = 0u;
+  uint64_t before_mass = 0u;
+#pragma unroll 4
+  for (uint32_t j = part; j < n; j += parts) {
+    const Shared::Weighed x = all[j];
+    if (x.order > own) before_count += 1u, before_mass += x.weight;
+  }
+  for (uint32_t o = 1; o < parts; o <<= 1) {
+    before_count += uint32_t(__shfl_xor(int(before_count), int(o)));
+    before_mass += uint64_t(__shfl_xor((unsigned long long)(before_mass), int(o)));
+  }
+  w = i < n ? all[i].weight : 0u;
+  if (!gaps) {  // the last of them all knows the totals
+    if (i < n && before_count == n - 1 && part == 0) s.kept = before_mass + w;
+    __syncthreads();
+    kept = s.kept;
+    tokens = n;
+    __syncthreads();
+  } else if (i < n) {
+    row.weigh(order_value(own), w, bin);
+    before_count += s.count[bin] & ~kGathered;
+    before_mass += s.mass[bin];
+  }
+  const bool one = i < n && part == 0;
+  // f() for the token at which the count, or the mass, reaches the goal.
+  const auto at = [&](bool by_count, uint64_t goal, auto&& f) {
+    const uint64_t before = by_count ? uint64_t(before_count) : before_mass, after = before + (by_count ? 1u : w);
+    if (one && before < goal && goal <= after) f();
+  };
+  if (ask.top_k > 0 && ask.top_k < tokens) {
+    at(true, ask.top_k, [&] { s.kept = before_mass + w; });
+    __syncthreads();
+    kept = s.kept;
+    __syncthreads();
+  }
+  if (ask.cuts()) {
+    at(false, ask.cut(kept), [&] { s.kept = before_mass + w; });
+    __syncthreads();
+    kept = s.kept;
+  }
+  at(false, ask.draw(kept), [&] {
+    a.tokens[out] = order_index(own);
+    if (a.probs) a.probs[out] = float(double(w) / double(kept));
+  });
+}
+
+// One question over any number of tokens (many equal logits, a flat row): bins
+// inside the bin f, by order, until 64 tokens are left.  gathered: s.cand holds
+// that many tokens, all of the bin's among them; past kList they are read from
+// the row, again each time until they fit.  The answer is s.token, its weight, and
+// the mass up to and with it in s.mass_to.
+template <int DT>
+__device__ __forceinline__ void narrow(Shared& s, const Row<DT>& row, const Shared::Found& f, bool by_count, uint64_t goal,
+                                       uint32_t gathered) {
+  const int t = int(threadIdx.x), bin = int(f.bin);
+  uint32_t n, bc = f.before_count;
+  uint64_t bm = f.before_mass;
+  __syncthreads();
   if (t == 0) s.n = 0u, s.lo = ~0ull, s.hi = 0ull;
   __syncthreads();
   unsigned long long tlo = ~0ull, thi = 0ull;
-  row.each(zlo, zhi, [&](uint64_t o, float z) {
+  const auto member = [&](uint64_t o, float z) {
     uint64_t w;
     int b;
-    if (!row.weigh(z, w, b) || b != bin) return;
+    if (!row.weigh(z, w, b) || b != bin) return false;
     tlo = o < tlo ? o : tlo;
     thi = o > thi ? o : thi;
-    if (held) {
+    return true;
+  };
+  if (gathered <= kList) {
+    uint32_t own = 0u;
+    for (uint32_t i = t; i < gathered; i += kThreads) own += member(s.cand[i], order_value(s.cand[i]));
+    if (own) atomicAdd(&s.n, own);
+  } else {
+    float zlo, zhi;
+    row.span(bin, bin, zlo, zhi);
+    row.each(zlo, zhi, [&](uint64_t o, float z) {
+      if (!member(o, z)) return;
       const uint32_t at = atomicAdd(&s.n, 1u);
       if (at < kList) s.cand[at] = o;
-    }
-  });
+    });
+  }
   if (thi) {
     atomicMin(&s.lo, tlo);
     atomicMax(&s.hi, thi);
   }
   __syncthreads();
   uint64_t lo = s.lo, hi = s.hi;
-  uint32_t cands = min(s.n, uint32_t(kList));
+  n = s.n;
+  bool held = gathered <= kList || n <= kList;  // all of them in s.cand
+  uint32_t cands = gathered <= kList ? gathered : n;
   // f(order) for the tokens with lo <= order <= hi.
-  const auto each_in = [&](auto&& f) {
+  const auto each_in = [&](auto&& g) {
     if (held) {
       for (uint32_t i = t; i < cands; i += kThreads) {
         const uint64_t o = s.cand[i];
-        if (o >= lo && o <= hi) f(o);
+        if (o >= lo && o <= hi) g(o);
       }
     } else {
       row.each(order_value(lo), order_value(hi), [&](uint64_t o, float) {
-        if (o >= lo && o <= hi) f(o);
+        if (o >= lo && o <= hi) g(o);
       });
     }
   };
-  // 1024 bins of a power of two of orders each: nine bits of hi - lo < 2^50 a
+  // kFine bins of a power of two of orders each: nine bits of hi - lo < 2^50 a
   // turn or more, orders are unique.
   for (int turn = 0; n > 64 && turn < 6; ++turn) {
-    const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
-    for (int b = t; b < kBins; b += kThreads) s.fine_count[b] = 0u, s.fine[b] = 0u;
+    const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - kFineBits);
+    for (int b = t; b < kFine; b += kThreads) s.fine_count[b] = 0u, s.fine[b] = 0u;
     __syncthreads();
     each_in([&](uint64_t o) {
       uint64_t w = 0;
@@ -321,11 +567,13 @@ __device__ void select(Shared& s, const Row<DT>& row, bool by_count, uint64_t go
       atomicAdd(reinterpret_cast<unsigned long long*>(&s.fine[x]), (unsigned long long)(w));
     });
     __syncthreads();
-    locate(s, s.fine_count, s.fine, by_count, goal, bc, bm);
-    n = s.in_bin;
-    bc = s.before_count;
-    bm = s.before_mass;
-    hi -= uint64_t(s.bin) << shift;
+    const Bins<kFine / kThreads> fine(s, s.fine_count, s.fine, bc, bm);
+    fine.find(s.found[4], by_count, goal);
+    __syncthreads();
+    n = s.found[4].count;
+    bc = s.found[4].before_count;
+    bm = s.found[4].before_mass;
+    hi -= uint64_t(s.found[4].bin) << shift;
     const uint64_t width = uint64_t(1) << shift;
     lo = hi >= width && hi - width + 1 > lo ? hi - width + 1 : lo;
     if (!held && n <= kList) {
@@ -371,123 +619,148 @@ __device__ void select(Shared& s, const Row<DT>& row, bool by_count, uint64_t go
 }
 
 template <int DT>
-__global__ __launch_bounds__(kThreads) void sample_draw(SampleArgs a) {
+__global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
   __shared__ Shared s;
-  const int t = int(threadIdx.x), lane = t & 63, slice = int(blockIdx.x), row = int(blockIdx.y);
+  const int t = int(threadIdx.x), part = int(blockIdx.x), parts = int(gridDim.x), row = int(blockIdx.y);
   RowState& rs = a.rows[row];
-  const uint64_t best = wave_max64(lane < a.slices ? rs.best[lane] : 0u);
-  const float temp = a.temperatures ? a.temperatures[row] : a.temperature;
-  if (best == 0u || !(temp > 0.0f)) {  // uniform: an empty row, or the first of the order
-    if (slice == 0 && t == 0) {
-      a.tokens[row] = best ? order_index(best) : -1;
-      if (a.probs) a.probs[row] = best ? 1.0f : 0.0f;
+  // Read before they are known to be needed: one wait for all of them.
+  uint32_t counts[kBins / kThreads];
+  uint64_t masses[kBins / kThreads];
+#pragma unroll
+  for (int i = 0; i < kBins / kThreads; ++i) counts[i] = rs.count[i * kThreads + t], masses[i] = rs.mass[i * kThreads + t];
+  const uint32_t n_list = rs.n_list;
+  Settings set;
+  if (!set.derive(a, row)) {  // uniform: an empty row, or the first of the order
+    if (t == 0 && part == 0) {
+      a.tokens[row] = set.best ? order_index(set.best) : -1;
+      if (a.probs) a.probs[row] = set.best ? 1.0f : 0.0f;
     }
     return;
   }
-  const int top_k = a.top_ks ? a.top_ks[row] : a.top_k;
-  const float top_p = a.top_ps ? a.top_ps[row] : a.top_p, min_p = a.min_ps ? a.min_ps[row] : a.min_p;
-  Weigher weigh;
-  weigh.top = order_value(best);
-  weigh.bits = 1.4426950408889634 / double(temp);
-  weigh.min_p = min_p > 0.0f ? fmin(double(min_p), 1.0) : 0.0;
-  // Below floor a weight rounds to nothing or fails min-p: z - top < T ln(max(min_p, 2^-46)),
-  // widened by fp32's rounding.
-  weigh.floor = weigh.top;
-  if (weigh.top < INFINITY) {
-    const double low = double(weigh.top) + fmax(log2(fmax(weigh.min_p, 0x1p-46)), -46.0) / weigh.bits;
-    weigh.floor = float(low - fabs(low) * 0x1p-20);
+  const Questions ask{set.top_k > 0 ? uint64_t(set.top_k) : 0u, a.top_ps ? a.top_ps[row] : a.top_p, a.u[row]};
+  set.weigh.constants();
+  Row<DT> r{a.logits + int64_t(row) * a.row_bytes, a.vocab, set.weigh};
+  const bool from_list = set.listed && n_list <= kList;  // every token that may be kept
+  if (from_list && part) return;
+  if (from_list && n_list <= kFew / 2) {
+    for (uint32_t i = t; i < n_list; i += kThreads) s.cand[i] = rs.list[i];
+    answer_from(s, r, ask, n_list, false, 0u, 0u, a, row);
+    return;
   }
-  bool listed = weigh.min_p > 0.0;
-  const int groups = a.slices * kGroups;
-  if (top_k > 0 && top_k <= groups) {
-    // The first sixteen bits of the top_k-th largest group maximum: at least
-    // top_k tokens have keys that large.
-    uint32_t g[kMaxSlices * kGroups / 64], key = 0u;
+  set.raise_floor(a, row);
+  const Weigher weigh = r.weigh = set.weigh;
 #pragma unroll
-    for (int j = 0; j < kMaxSlices * kGroups / 64; ++j) {
-      const int i = j * 64 + lane;
-      g[j] = i < groups ? rs.group_max[i] : 0u;
-    }
-    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
-      const uint32_t with = key | bit;
-      int n = 0;
-#pragma unroll
-      for (int j = 0; j < kMaxSlices * kGroups / 64; ++j) n += __popcll(__ballot(g[j] >= with));
-      if (n >= top_k) key = with;
-    }
-    if (key > kDeadKey) weigh.floor = fmaxf(weigh.floor, key_value(key));
-    listed = true;
+  for (int i = 0; i < kBins / kThreads; ++i) s.count[i * kThreads + t] = counts[i], s.mass[i * kThreads + t] = masses[i];
+  __syncthreads();
+  const Bins<kBins / kThreads> bins(s, s.count, s.mass, 0u, 0u);
+  // The bins that the answers lie in: a question's goal is known within the
+  // mass of the bin that the one before it ends in.
+  uint64_t low = bins.total_mass, high = low;  // bounds of the mass kept
+  const bool by_k = ask.top_k > 0 && ask.top_k < bins.total_count;  // counts are there with top-k alone
+  uint32_t k_bin = kBins, p_first = kBins, p_last = 0u;
+  if (by_k) {
+    bins.find(s.found[0], true, ask.top_k);
+    __syncthreads();
+    k_bin = s.found[0].bin;
+    low = s.found[0].before_mass + 1;
+    high = s.found[0].before_mass + s.found[0].mass;
   }
-  // Whatever the floor, a token at -inf is never kept.
-  weigh.floor = fmaxf(weigh.floor, -3.402823466e38f);
-
-  for (int b = t; b < kBins; b += kThreads) s.count[b] = 0u, s.mass[b] = 0u;
+  if (ask.cuts()) {
+    bins.find(s.found[1], false, ask.cut(low));
+    bins.find(s.found[2], false, ask.cut(high));
+    __syncthreads();
+    p_first = s.found[1].bin;
+    p_last = s.found[2].bin;
+    low = ask.cut(low);
+    const uint64_t to = s.found[2].before_mass + s.found[2].mass;
+    high = to < high ? to : high;
+  }
+  bins.find(s.found[3], false, ask.draw(low));
+  bins.find(s.found[4], false, ask.draw(high));
+  __syncthreads();
+  const uint32_t d_first = s.found[3].bin, d_last = s.found[4].bin;
+  // What is before each bin and not in one of them.
+  uint32_t skip_count = 0u;
+  uint64_t skip_mass = 0u;
+  const auto taken = [&](uint32_t b) { return b == k_bin || (b >= p_first && b <= p_last) || (b >= d_first && b <= d_last); };
+#pragma unroll
+  for (int i = 0; i < kBins / kThreads; ++i)
+    if (!taken(uint32_t(t * (kBins / kThreads) + i))) skip_count += bins.count[i], skip_mass += bins.mass[i];
+  const Scan skip = block_scan(s, skip_count, skip_mass);
+  skip_count = skip.count;
+  skip_mass = skip.mass;
+#pragma unroll
+  for (int i = 0; i < kBins / kThreads; ++i) {
+    const uint32_t b = uint32_t(t * (kBins / kThreads) + i);
+    const bool take = taken(b);
+    s.count[b] = skip_count | (take ? kGathered : 0u);
+    s.mass[b] = skip_mass;
+    if (!take) skip_count += bins.count[i], skip_mass += bins.mass[i];
+  }
   if (t == 0) s.n = 0u;
   __syncthreads();
-  const char* const data = a.logits + int64_t(row) * a.row_bytes;
-  each_token<DT>(data, a.vocab, slice, a.slices, [&](int i, float z) {
-    if (!(z >= weigh.floor)) return;
+  // Only tokens in the z of those bins are weighed again.
+  // A row's workgroups have all come here alike; each gathers its part.
+  const int shares = from_list ? 1 : parts;
+  float lo[3], hi[3];
+  r.span(int(by_k ? k_bin : d_first), int(by_k ? k_bin : d_last), lo[0], hi[0]);
+  r.span(int(ask.cuts() ? p_first : d_first), int(ask.cuts() ? p_last : d_last), lo[1], hi[1]);
+  r.span(int(d_first), int(d_last), lo[2], hi[2]);
+  const float any_lo = fminf(fminf(lo[0], lo[1]), lo[2]), any_hi = fmaxf(fmaxf(hi[0], hi[1]), hi[2]);
+  const auto gather = [&](float z, auto&& order) {
+    if (!(z >= any_lo && z <= any_hi)) return;
+    if (!((z >= lo[0] && z <= hi[0]) || (z >= lo[1] && z <= hi[1]) || (z >= lo[2] && z <= hi[2]))) return;
     uint64_t w;
     int b;
-    if (!weigh(z, w, b)) return;
-    atomicAdd(&s.count[b], 1u);
-    atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)(w));
-    if (listed) {
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < kList) s.cand[at] = order_of(z, i);
+    if (!weigh(z, w, b) || !(s.count[b] & kGathered)) return;
+    const uint32_t at = atomicAdd(&s.n, 1u);
+    if (at < kList) s.cand[at] = order();
+  };
+  if (from_list) {
+    for (uint32_t i = t; i < n_list; i += kThreads) {
+      const uint64_t o = rs.list[i];
+      gather(order_value(o), [&] { return o; });
     }
-  });
-  __syncthreads();
-  for (int b = t; b < kBins; b += kThreads) {
-    if (s.count[b] == 0u) continue;
-    atomicAdd(&rs.count[b], s.count[b]);
-    atomicAdd(reinterpret_cast<unsigned long long*>(&rs.mass[b]), (unsigned long long)(s.mass[b]));
+  } else {
+    each_token<DT, kThreads>(r.data, a.vocab, part, parts, [&](int i, float z) { gather(z, [&] { return order_of(z, i); }); });
   }
-  if (listed) {
-    if (t == 0) s.base = atomicAdd(&rs.n_list, min(s.n, uint32_t(kList + 1)));
+  __syncthreads();
+  uint32_t n = s.n;
+  if (shares > 1) {
+    // The row's last workgroup answers, from what all of them gathered.  What
+    // passes between them goes through device-scope atomics, which meet behind the
+    // XCDs' caches: each wave waits for its own to be acknowledged before the
+    // ticket is taken, and the last one's loads follow its ticket.  A device-scope
+    // fence would do the same by writing back and dropping the XCD's L2, for 20 to
+    // 35 us in each workgroup of a large call.
+    if (t == 0) s.base = atomicAdd(&rs.n_gathered, n <= kList ? n : uint32_t(kList + 1));
     __syncthreads();
-    if (s.n <= kList && s.base + s.n <= kList)
-      for (uint32_t i = t; i < s.n; i += kThreads) rs.list[s.base + i] = s.cand[i];
+    if (n <= kList && s.base + n <= kList)
+      for (uint32_t i = t; i < n; i += kThreads)
+        __hip_atomic_store(&rs.list[s.base + i], s.cand[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (t == 0) s.base = atomicAdd(&rs.ticket, 1u);
+    __syncthreads();
+    if (s.base != uint32_t(shares - 1)) return;  // uniform
+    n = __hip_atomic_load(&rs.n_gathered, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (n <= kList)
+      for (uint32_t i = t; i < n; i += kThreads)
+        s.cand[i] = __hip_atomic_load(&rs.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  // The row's last workgroup: every other one's additions are visible to it.
-  __threadfence();
-  __syncthreads();
-  if (t == 0) s.is_last = atomicAdd(&rs.ticket, 1u) == uint32_t(a.slices - 1);
-  __syncthreads();
-  if (!s.is_last) return;  // uniform
-  __threadfence();
-  for (int b = t; b < kBins; b += kThreads) {
-    s.count[b] = __hip_atomic_load(&rs.count[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s.mass[b] = __hip_atomic_load(&rs.mass[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (n <= kFew) {
+    answer_from(s, r, ask, n, true, bins.total_mass, bins.total_count, a, row);
+    return;
   }
-  const uint32_t n_list = __hip_atomic_load(&rs.n_list, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  const Row<DT> r{data, a.vocab, listed && n_list <= kList ? rs.list : nullptr, n_list, weigh};
-  __syncthreads();
-  locate(s, s.count, s.mass, true, 1u, 0u, 0u);  // for the totals
-  uint64_t kept = s.total_mass;
-  const uint32_t tokens = s.total_count;
-  __syncthreads();
-  // Where top-k ends, where top-p ends (each leaves the mass kept), the draw.
-  for (int question = 0; question < 3; ++question) {
-    uint64_t goal;
-    if (question == 0) {
-      if (top_k <= 0 || uint32_t(top_k) >= tokens) continue;
-      goal = uint64_t(top_k);
-    } else if (question == 1) {
-      if (!(top_p < 1.0f)) continue;  // NaN: off
-      // before < top_p kept  <=>  before < ceil(top_p kept), before being whole.
-      const double part = top_p > 0.0f ? ceil(double(top_p) * double(kept)) : 0.0;
-      goal = part < 1.0 ? 1u : uint64_t(part);
-      if (goal >= kept) continue;
-    } else {
-      const float u = a.u[row];
-      const double at = u > 0.0f ? fmin(double(u), 1.0) * double(kept) : 0.0;  // kept <= 2^62
-      goal = uint64_t(at);
-      goal = (goal < kept ? goal : kept - 1) + 1;
-    }
-    select(s, r, question == 0, goal);
+  uint64_t kept = bins.total_mass;
+  for (int question = by_k ? 0 : 1; question < 3; ++question) {
+    if (question == 1 && !ask.cuts()) continue;
+    const uint64_t goal = question == 0 ? ask.top_k : question == 1 ? ask.cut(kept) : ask.draw(kept);
+    __syncthreads();
+    bins.find(s.found[question], question == 0, goal);
+    __syncthreads();
+    narrow(s, r, s.found[question], question == 0, goal, n);
     if (question < 2) kept = s.mass_to;
-    __syncthreads();
   }
   if (t == 0) {
     a.tokens[row] = s.token;
@@ -495,20 +768,27 @@ __global__ __launch_bounds__(kThreads) void sample_draw(SampleArgs a) {
   }
 }
 
-// Slices of a row: of 4096 tokens or more, as many as leave 2048 workgroups
-// (four resident on each of 256 CUs, twice).  The result does not depend on it.
+// Slices of a row in the first two launches: of 2048 tokens or more, as many as
+// leave 2048 workgroups (eight for each of 256 CUs).  The result does not depend
+// on it, nor on the workgroups that gather in the third.
 int slice_count(int32_t rows, int32_t vocab) {
-  int s = (vocab + 4095) / 4096;
+  int s = (vocab + 2047) / 2048;
   const int fill = 2048 / rows > 0 ? 2048 / rows : 1;
   s = s < fill ? s : fill;
   return s < kMaxSlices ? s : kMaxSlices;
+}
+// Workgroups of a row in the third: of 8192 tokens or more, 512 in all.
+int part_count(int32_t rows, int32_t vocab) {
+  const int p = (vocab + 8191) / 8192, fill = 512 / rows > 0 ? 512 / rows : 1;
+  return p < fill ? p : fill;
 }
 
 template <int DT>
 void launch_sample(const SampleArgs& a, int32_t rows, hipStream_t s) {
   const dim3 grid(unsigned(a.slices), unsigned(rows));
-  hipLaunchKernelGGL(sample_maxima<DT>, grid, dim3(kThreads), 0, s, a);
-  hipLaunchKernelGGL(sample_draw<DT>, grid, dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(sample_maxima<DT>, grid, dim3(kSliceThreads), 0, s, a);
+  hipLaunchKernelGGL(sample_weigh<DT>, grid, dim3(kSliceThreads), 0, s, a);
+  hipLaunchKernelGGL(sample_draw<DT>, dim3(unsigned(part_count(rows, a.vocab)), unsigned(rows)), dim3(kThreads), 0, s, a);
 }
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 }  // namespace
