@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kThreads) void kv_move_rows(MoveArgs a) {
   constexpr int V = DT == IT_F32 ? 4 : 8;
   constexpr int kBytes = DT == IT_F32 ? 4 : 2;
   using Row = RowVec<DT, V>;
-  extern __shared__ float2 angles[];
+  extern __shared__ __attribute__((aligned(16))) float2 angles[];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = int(threadIdx.x & 63);
   const int64_t i = int64_t(blockIdx.x) * kWaves + wave;
   if (i >= a.n) return;  // uniform
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(kThreads) void kv_move_rows(MoveArgs a) {
   if (s == d && delta == 0) return;
   const RowSplit& sp = a.split;
   const int pairs = sp.n_dims >> 1;
-  float2* const own = angles + wave * pairs;
+  float2* const own = angles + wave * angle_room<V>(sp.n_dims);
   const int sub = int((uint32_t(lane) * sp.inv) >> 16), c = lane - sub * sp.lanes;
   const bool used = sub < sp.rows;
   const int64_t bs = int64_t(1) << a.log2_bs, so = s & (bs - 1), dof = d & (bs - 1);
@@ -219,7 +219,7 @@ __device__ __forceinline__ float4 dequant4(const char* page, int64_t off, int64_
 // any of it is written (src may be dst).
 template <int DT>
 __global__ __launch_bounds__(kThreads) void kv_move_quant(MoveArgs a) {
-  extern __shared__ float2 angles[];
+  extern __shared__ __attribute__((aligned(16))) float2 angles[];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = int(threadIdx.x & 63);
   const int64_t i = int64_t(blockIdx.x) * kWaves + wave;
   if (i >= a.n) return;  // uniform
@@ -297,7 +297,7 @@ void launch_rows(const MoveArgs& a, bool split, hipStream_t s) {
     hipLaunchKernelGGL(kv_move_general<DT>, dim3(unsigned(blocks)), dim3(kThreads), 0, s, a);
     return;
   }
-  const size_t lds = size_t(kWaves) * (a.split.n_dims / 2) * sizeof(float2);
+  const size_t lds = size_t(kWaves) * angle_room<DT == IT_F32 ? 4 : 8>(a.split.n_dims) * sizeof(float2);
   const auto chunks = [&](int g) { return (int64_t(a.rows) + a.split.rows * g - 1) / (a.split.rows * g); };
   const unsigned bx = unsigned((a.n + kWaves - 1) / kWaves);
   if (a.n * chunks(1) <= kResident)

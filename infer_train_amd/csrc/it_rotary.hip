@@ -47,13 +47,13 @@ struct RotaryArgs {
 template <int SRC, int DT, int V, int G>
 __global__ __launch_bounds__(kThreads) void rotary_rows(RotaryArgs a) {
   using In = RowVec<SRC, V>;
-  extern __shared__ float2 angles[];
+  extern __shared__ __attribute__((aligned(16))) float2 angles[];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = int(threadIdx.x & 63);
   const int64_t t = int64_t(blockIdx.x) * kWaves + wave;
   if (t >= a.n_tokens) return;  // uniform
   const RowSplit& s = a.split;
   const int pairs = s.n_dims >> 1;
-  float2* const own = angles + wave * pairs;
+  float2* const own = angles + wave * angle_room<V>(s.n_dims);
   const int sub = int((uint32_t(lane) * s.inv) >> 16), c = lane - sub * s.lanes;
   const bool used = sub < s.rows;  // lanes past the wave's last whole row idle
   const int rows = a.hq + 2 * a.hkv;
@@ -196,7 +196,7 @@ constexpr int64_t kResident = 256 * 32;
 template <int SRC, int DT, int V, int G>
 void launch_rows(const RotaryArgs& a, int64_t chunks, hipStream_t s) {
   const dim3 grid(unsigned((a.n_tokens + kWaves - 1) / kWaves), unsigned(chunks));
-  hipLaunchKernelGGL((rotary_rows<SRC, DT, V, G>), grid, dim3(kThreads), size_t(kWaves) * (a.split.n_dims / 2) * sizeof(float2), s, a);
+  hipLaunchKernelGGL((rotary_rows<SRC, DT, V, G>), grid, dim3(kThreads), size_t(kWaves) * angle_room<V>(a.split.n_dims) * sizeof(float2), s, a);
 }
 template <int SRC, int DT>
 void launch_split(const RotaryArgs& a, hipStream_t s) {

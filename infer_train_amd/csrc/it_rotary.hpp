@@ -44,6 +44,13 @@ __device__ __forceinline__ float2 rotary_angle(double turns, int pos) {
 __device__ __forceinline__ float turn_first(float2 cs, float a, float b) { return fmaf(a, cs.x, -(b * cs.y)); }
 __device__ __forceinline__ float turn_second(float2 cs, float a, float b) { return fmaf(a, cs.y, b * cs.x); }
 
+// Two floats as bf16, each rounded to nearest even (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  const pair p = {static_cast<__bf16>(lo), static_cast<__bf16>(hi)};
+  return __builtin_bit_cast(uint32_t, p);
+}
+
 // ---- rows as float vectors -------------------------------------------------
 // V elements of dtype DT at an address aligned to their size, 16 bytes at most <-> floats.
 template <int DT, int V>
@@ -74,7 +81,7 @@ struct RowVec {
       if constexpr (DT == IT_F32) {
         w[i] = __float_as_uint(x[i]);
       } else if constexpr (DT == IT_BF16) {
-        w[i] = f32_to_bf16_bits(x[2 * i]) | (f32_to_bf16_bits(x[2 * i + 1]) << 16);
+        w[i] = bf16_pair(x[2 * i], x[2 * i + 1]);
       } else {
         w[i] = f16_bits_rne(x[2 * i]) | (f16_bits_rne(x[2 * i + 1]) << 16);
       }
@@ -99,7 +106,7 @@ __device__ __forceinline__ float load_element(const void* base, int64_t element,
 }
 __device__ __forceinline__ void store_element(void* base, int64_t element, int dtype, float x) {
   if (dtype == IT_F32) static_cast<float*>(base)[element] = x;
-  else static_cast<uint16_t*>(base)[element] = uint16_t(dtype == IT_BF16 ? f32_to_bf16_bits(x) : f16_bits_rne(x));
+  else static_cast<uint16_t*>(base)[element] = uint16_t(dtype == IT_BF16 ? bf16_pair(x, x) & 0xFFFFu : f16_bits_rne(x));
 }
 
 // ---- how a row is shared out among lanes ----------------------------------
@@ -131,6 +138,12 @@ inline bool row_split(int head_dim, int n_dims, int layout, int v, int group, Ro
   return true;
 }
 
+// Entries of a wave's LDS array of (cos, sin): whole runs of V / 2 pairs.
+template <int V>
+__host__ __device__ constexpr int angle_room(int n_dims) {
+  return (n_dims / 2 + V / 2 - 1) / (V / 2) * (V / 2);
+}
+
 // A lane's vectors of its row, and its pairs' (cos, sin) from the wave's LDS
 // array of them.
 template <int V>
@@ -148,13 +161,15 @@ struct LanePairs {
       eb = ea + (s.head_dim >> 1);
     }
   }
-  // pairs = n_dims / 2 entries at `all`; pairs past them do not turn.
+  // From angle_room<V>(n_dims) entries; those of pairs that do not turn are not used.
   __device__ __forceinline__ void load(const RowSplit& s, const float2* all) {
-    const int half = s.n_dims >> 1;
+    const int most = angle_room<V>(s.n_dims) - V / 2;
+    const int p0 = min(s.layout == IT_ROTARY_HALF ? ea : ea >> 1, most);
+    const int p1 = min(s.layout == IT_ROTARY_HALF ? ea + V / 2 : eb >> 1, most);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int p = s.layout == IT_ROTARY_HALF ? ea + j : (j < V / 2 ? (ea >> 1) + j : (eb >> 1) + j - V / 2);
-      cs[j] = p < half ? all[p] : make_float2(1.0f, 0.0f);
+    for (int j = 0; j < V / 2; ++j) {
+      cs[j] = all[p0 + j];
+      cs[V / 2 + j] = all[p1 + j];
     }
   }
   __device__ __forceinline__ void turn(const RowSplit& s, float (&a)[V], float (&b)[V]) const {

@@ -36,7 +36,8 @@ constexpr int kThreads = 512;        // of a row's
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;          // of a row, linear in z
 constexpr int kList = 2048;          // tokens listed per row, and gathered in LDS
-constexpr int kSliceList = kList - 1;  // of a slice: its workgroup's LDS is a quarter of a CU's
+constexpr int kRowList = 8192;       // room for a row's slices' lists: a slice may hold most of the likely tokens
+constexpr int kSliceList = kList - 1;  // of a slice at most: its workgroup's LDS is a quarter of a CU's
 constexpr int kFew = 256;            // tokens compared all with all
 constexpr int kFineBits = 10, kFine = 1 << kFineBits;
 constexpr uint32_t kGathered = 1u << 31;  // of a bin's count
@@ -50,14 +51,17 @@ constexpr double kBinsPerBit = 44.0;  // of log2 weight, of which 45 weigh at al
 constexpr uint32_t kDeadKey = 0x007FFFFFu;  // order_key(-inf)
 
 struct RowState {
-  uint32_t n_list, n_gathered, ticket, pad[61];
+  uint32_t n_gathered, ticket, pad[30];
+  uint32_t n_list[kMaxSlices];              // tokens of each slice that are listed, or more than its room
   uint64_t best[kMaxSlices];               // order of each slice's first token, 0: nothing above -inf
   uint32_t group_max[kMaxSlices * kGroups];
   uint32_t count[kBins];
   uint64_t mass[kBins];
-  uint64_t list[kList];
+  uint64_t list[kRowList];                  // by slice; then what the third launch's workgroups gather
 };
 static_assert(sizeof(RowState) % 256 == 0, "rows of the workspace stay aligned");
+
+__host__ __device__ constexpr int slice_list(int slices) { return kRowList / slices < kSliceList ? kRowList / slices : kSliceList; }
 
 struct SampleArgs {
   const char* logits;
@@ -128,35 +132,54 @@ struct Weigher {
   }
 };
 
-// f(index, z) for the tokens of a slice of a row: its share of the 16-byte vectors
-// of the row's aligned part, the first slice also the tokens before that part,
-// the last those behind it.  A thread's tokens come in ascending order.
-template <int DT, int kBlock, class F>
-__device__ __forceinline__ void each_token(const char* row, int vocab, int slice, int slices, F&& f) {
-  constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es, U = 4;
+// The tokens of a slice of a row: its share of the 16-byte vectors of the row's
+// aligned part, the first slice also the tokens before that part, the last those
+// behind it.  The first vectors are loaded when the walk is made, so that what
+// a kernel does before each() runs in their shadow.
+template <int DT, int kBlock>
+struct Walk {
+  static constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es, U = 4;
   using In = RowVec<DT, V>;
-  const int tid = int(threadIdx.x);
-  const int head = min(vocab, int((16 - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / es);
-  const int vecs = (vocab - head) / V, done = head + vecs * V;
-  const int per = (vecs + slices - 1) / slices, lo = min(vecs, slice * per), hi = min(vecs, lo + per);
-  if (slice == 0 && tid < head) f(tid, load_element(row, tid, DT));
-  const auto* const v = reinterpret_cast<const typename In::raw*>(row + head * es);
-  for (int x0 = lo + tid; x0 < hi; x0 += kBlock * U) {
-    typename In::raw w[U];
+  const char* row;
+  const typename In::raw* v;
+  int vocab, head, done, lo, hi;
+  bool first, last;
+  typename In::raw w[U];
+  __device__ __forceinline__ Walk(const char* row_, int vocab_, int slice, int slices) : row(row_), vocab(vocab_) {
+    head = min(vocab, int((16 - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / es);
+    const int vecs = (vocab - head) / V, per = (vecs + slices - 1) / slices;
+    done = head + vecs * V;
+    lo = min(vecs, slice * per);
+    hi = min(vecs, lo + per);
+    first = slice == 0;
+    last = slice == slices - 1;
+    v = reinterpret_cast<const typename In::raw*>(row + head * es);
+    if (lo < hi) load(lo + int(threadIdx.x));
+  }
+  __device__ __forceinline__ void load(int x0) {
 #pragma unroll
     for (int j = 0; j < U; ++j) w[j] = v[min(x0 + j * kBlock, hi - 1)];
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int x = x0 + j * kBlock;
-      if (x >= hi) break;
-      float z[V];
-      In::widen(w[j], z);
-#pragma unroll
-      for (int e = 0; e < V; ++e) f(head + x * V + e, z[e]);
-    }
   }
-  if (slice == slices - 1 && tid < vocab - done) f(done + tid, load_element(row, done + tid, DT));
-}
+  // f(index, z); a thread's tokens come in ascending order.
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) {
+    const int tid = int(threadIdx.x);
+    if (first && tid < head) f(tid, load_element(row, tid, DT));
+    for (int x0 = lo + tid; x0 < hi; x0 += kBlock * U) {
+      if (x0 != lo + tid) load(x0);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int x = x0 + j * kBlock;
+        if (x >= hi) break;
+        float z[V];
+        In::widen(w[j], z);
+#pragma unroll
+        for (int e = 0; e < V; ++e) f(head + x * V + e, z[e]);
+      }
+    }
+    if (last && tid < vocab - done) f(done + tid, load_element(row, done + tid, DT));
+  }
+};
 
 __device__ __forceinline__ uint64_t shfl64(uint64_t x, int lane) { return uint64_t(__shfl((unsigned long long)(x), lane)); }
 __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
@@ -168,17 +191,24 @@ __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
   return x;
 }
 
+// x summed over the wave's lanes up to and with each; returns the sum of all.
+__device__ __forceinline__ uint32_t wave_sums(uint32_t& x) {
+  x = uint32_t(wave_inclusive_sum(int(x)));
+  return uint32_t(__builtin_amdgcn_readlane(int(x), 63));
+}
+
 template <int DT>
 __global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
   __shared__ uint64_t best_of[kSliceWaves];
   const int slice = int(blockIdx.x), lane = int(threadIdx.x & 63), wave = int(threadIdx.x >> 6);
   RowState& rs = a.rows[blockIdx.y];
   if (slice == 0 && threadIdx.x == 0)  // what the second launch adds to
-    rs.n_list = rs.n_gathered = rs.ticket = 0u;
+    rs.n_gathered = rs.ticket = 0u;
   for (int b = slice * kSliceThreads + int(threadIdx.x); b < kBins; b += a.slices * kSliceThreads) rs.count[b] = 0u, rs.mass[b] = 0u;
   float top = -INFINITY;
   int at = -1;
-  each_token<DT, kSliceThreads>(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices, [&](int i, float z) {
+  Walk<DT, kSliceThreads> walk(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices);
+  walk.each([&](int i, float z) {
     if (z > top) top = z, at = i;  // of equals the first
   });
   uint64_t best = at < 0 ? 0u : order_of(top, at);
@@ -203,6 +233,18 @@ struct Settings {
   uint64_t best;
   int top_k;
   bool listed;  // few tokens can be kept: they are listed
+  static constexpr int kLoads = kMaxSlices * kGroups / 64;
+  uint32_t group[kLoads];
+  // The group maxima, 64 to a register, before it is known whether they count.
+  __device__ __forceinline__ void load_groups(const SampleArgs& a, int row) {
+    const int lane = int(threadIdx.x & 63), groups = a.slices * kGroups;
+    if (!a.top_ks && a.top_k <= 0) return;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = j * 64 + lane;
+      group[j] = i < groups ? a.rows[row].group_max[i] : 0u;
+    }
+  }
   __device__ __forceinline__ bool derive(const SampleArgs& a, int row) {
     const RowState& rs = a.rows[row];
     const int lane = int(threadIdx.x & 63), groups = a.slices * kGroups;
@@ -230,22 +272,16 @@ struct Settings {
   }
   // The floor raised to the first sixteen bits of the top_k-th largest group
   // maximum: at least top_k tokens have keys that large.
-  __device__ __forceinline__ void raise_floor(const SampleArgs& a, int row) {
-    const int lane = int(threadIdx.x & 63), groups = a.slices * kGroups;
+  __device__ __forceinline__ void raise_floor(const SampleArgs& a) {
+    const int groups = a.slices * kGroups;
     if (top_k <= 0 || top_k > groups) return;
-    constexpr int kLoads = kMaxSlices * kGroups / 64;
-    uint32_t g[kLoads], key = 0u;
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int i = j * 64 + lane;
-      g[j] = i < groups ? a.rows[row].group_max[i] : 0u;
-    }
+    uint32_t key = 0u;
     for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
       const uint32_t with = key | bit;
       int n = 0;
 #pragma unroll
       for (int j = 0; j < kLoads; ++j)
-        if (j * 64 < groups) n += __popcll(__ballot(g[j] >= with));
+        if (j * 64 < groups) n += __popcll(__ballot(group[j] >= with));
       if (n >= top_k) key = with;
     }
     if (key > kDeadKey) weigh.floor = fmaxf(weigh.floor, key_value(key));
@@ -255,17 +291,20 @@ struct Settings {
 template <int DT>
 __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
   __shared__ uint64_t mass[kBins], list[kSliceList];
-  __shared__ uint32_t count[kBins], n, base;
+  __shared__ uint32_t count[kBins], n;
   const int t = int(threadIdx.x), slice = int(blockIdx.x), row = int(blockIdx.y);
   RowState& rs = a.rows[row];
+  Walk<DT, kSliceThreads> walk(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices);
   Settings set;
+  set.load_groups(a, row);
   if (!set.derive(a, row)) return;
-  set.raise_floor(a, row);
+  set.raise_floor(a);
   set.weigh.constants();
   for (int b = t; b < kBins; b += kSliceThreads) count[b] = 0u, mass[b] = 0u;
   if (t == 0) n = 0u;
   __syncthreads();
-  each_token<DT, kSliceThreads>(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices, [&](int i, float z) {
+  const uint32_t room = slice_list(a.slices);
+  walk.each([&](int i, float z) {
     if (!(z >= set.weigh.floor)) return;
     uint64_t w;
     int b;
@@ -274,24 +313,25 @@ __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
     if (set.top_k > 0) atomicAdd(&count[b], 1u);  // only top-k asks for counts
     if (set.listed) {
       const uint32_t at = atomicAdd(&n, 1u);
-      if (at < kSliceList) list[at] = order_of(z, i);
+      if (at < room) list[at] = order_of(z, i);
     }
   });
   __syncthreads();
+  if (set.listed) {  // each slice in its own part of the row's list
+    if (t == 0) rs.n_list[slice] = n;
+    if (n <= room)
+      for (uint32_t i = t; i < n; i += kSliceThreads) rs.list[slice * room + i] = list[i];
+  }
   for (int b = t; b < kBins; b += kSliceThreads) {
     if (mass[b] == 0u) continue;
     atomicAdd(reinterpret_cast<unsigned long long*>(&rs.mass[b]), (unsigned long long)(mass[b]));
     if (set.top_k > 0) atomicAdd(&rs.count[b], count[b]);
   }
-  if (!set.listed) return;
-  if (t == 0) base = atomicAdd(&rs.n_list, n <= kSliceList ? n : uint32_t(kList + 1));
-  __syncthreads();
-  if (n <= kSliceList && base + n <= kList)
-    for (uint32_t i = t; i < n; i += kSliceThreads) rs.list[base + i] = list[i];
 }
 
 struct Shared {
-  uint64_t mass[kBins];   // the row's bins, then what lies before each but is not gathered
+  uint64_t mass[kBins];   // the row's bins
+  uint64_t skip_mass[kBins];  // what lies before each but is not gathered
   uint64_t cand[kList];   // the tokens gathered to answer from
   struct Weighed {
     uint64_t order, weight;
@@ -301,6 +341,7 @@ struct Shared {
     Weighed weighed[kFew];         // answer_from()
   };
   uint32_t count[kBins];
+  uint32_t skip_count[kBins];
   uint32_t fine_count[kFine];
   uint64_t last[64];
   uint64_t wave_mass[kWaves];
@@ -344,21 +385,16 @@ __device__ __forceinline__ Scan block_scan(Shared& s, uint32_t count, uint64_t m
   return r;
 }
 
-// A thread's N consecutive bins with what is before the first of them.
+// What is before a thread's N consecutive bins of LDS, which stay there.
 template <int N>
 struct Bins {
-  uint64_t mass[N], before_mass, total_mass;
-  uint32_t count[N], before_count, total_count;
+  uint64_t before_mass, total_mass;
+  uint32_t before_count, total_count;
   __device__ __forceinline__ Bins(Shared& s, const uint32_t* c, const uint64_t* m, uint32_t base_count, uint64_t base_mass) {
     uint32_t cs = 0u;
     uint64_t ms = 0u;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      count[i] = c[N * threadIdx.x + i];
-      mass[i] = m[N * threadIdx.x + i];
-      cs += count[i];
-      ms += mass[i];
-    }
+    for (int i = 0; i < N; ++i) cs += c[N * threadIdx.x + i], ms += m[N * threadIdx.x + i];
     const Scan scan = block_scan(s, cs, ms);
     before_count = base_count + scan.count;
     before_mass = base_mass + scan.mass;
@@ -367,15 +403,17 @@ struct Bins {
   }
   // The one bin in which the cumulative count (or mass) reaches `goal`, 1 <=
   // goal <= the total, into `f` (a barrier later).
-  __device__ __forceinline__ void find(Shared::Found& f, bool by_count, uint64_t goal) const {
+  __device__ __forceinline__ void find(const uint32_t* c, const uint64_t* m, Shared::Found& f, bool by_count, uint64_t goal) const {
     uint32_t cs = before_count;
     uint64_t ms = before_mass;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const uint64_t before = by_count ? cs : ms, after = before + (by_count ? uint64_t(count[i]) : mass[i]);
-      if (before < goal && goal <= after) f = {ms, mass[i], cs, count[i], uint32_t(N * threadIdx.x + i)};
-      cs += count[i];
-      ms += mass[i];
+      const uint32_t ci = c[N * threadIdx.x + i];
+      const uint64_t mi = m[N * threadIdx.x + i];
+      const uint64_t before = by_count ? cs : ms, after = before + (by_count ? uint64_t(ci) : mi);
+      if (before < goal && goal <= after) f = {ms, mi, cs, ci, uint32_t(N * threadIdx.x + i)};
+      cs += ci;
+      ms += mi;
     }
   }
 };
@@ -388,7 +426,8 @@ struct Row {
   // f(order, z) for the row's tokens with lo <= z <= hi.
   template <class F>
   __device__ __forceinline__ void each(float lo, float hi, F&& f) const {
-    each_token<DT, kThreads>(data, vocab, 0, 1, [&](int i, float z) {
+    Walk<DT, kThreads> walk(data, vocab, 0, 1);
+    walk.each([&](int i, float z) {
       if (z >= lo && z <= hi) f(order_of(z, i), z);
     });
   }
@@ -424,7 +463,7 @@ struct Questions {
 };
 
 // Answers from the tokens in s.cand (n <= kFew of them), each after those of
-// s.mass and s.count of its bin that are not among them (`gaps`; else there are
+// s.skip_mass and s.skip_count of its bin that are not among them (`gaps`; else there are
 // no others).  kept, tokens: the row's mass and number, with gaps.  Each token's
 // place is found by comparing it with all others, a power of two of threads
 // sharing them: no step waits for the one before, but the work grows with n^2
@@ -468,8 +507,8 @@ __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const
     __syncthreads();
   } else if (i < n) {
     row.weigh(order_value(own), w, bin);
-    before_count += s.count[bin] & ~kGathered;
-    before_mass += s.mass[bin];
+    before_count += s.skip_count[bin] & ~kGathered;
+    before_mass += s.skip_mass[bin];
   }
   const bool one = i < n && part == 0;
   // f() for the token at which the count, or the mass, reaches the goal.
@@ -499,12 +538,15 @@ __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const
 // that many tokens, all of the bin's among them; past kList they are read from
 // the row, again each time until they fit.  The answer is s.token, its weight, and
 // the mass up to and with it in s.mass_to.
+// A function of its own, called with values: rows that need it are few, and what
+// it holds would take registers from those that do not.
 template <int DT>
-__device__ __forceinline__ void narrow(Shared& s, const Row<DT>& row, const Shared::Found& f, bool by_count, uint64_t goal,
-                                       uint32_t gathered) {
-  const int t = int(threadIdx.x), bin = int(f.bin);
-  uint32_t n, bc = f.before_count;
-  uint64_t bm = f.before_mass;
+__device__ __noinline__ void narrow(Shared& s, const char* data, int vocab, float top, float floor, double bits, double least, int bin,
+                                    uint32_t bc, uint64_t bm, bool by_count, uint64_t goal, uint32_t gathered) {
+  const int t = int(threadIdx.x);
+  Row<DT> row{data, vocab, {top, floor, bits, least}};
+  row.weigh.constants();
+  uint32_t n;
   __syncthreads();
   if (t == 0) s.n = 0u, s.lo = ~0ull, s.hi = 0ull;
   __syncthreads();
@@ -568,7 +610,7 @@ __device__ __forceinline__ void narrow(Shared& s, const Row<DT>& row, const Shar
     });
     __syncthreads();
     const Bins<kFine / kThreads> fine(s, s.fine_count, s.fine, bc, bm);
-    fine.find(s.found[4], by_count, goal);
+    fine.find(s.fine_count, s.fine, s.found[4], by_count, goal);
     __syncthreads();
     n = s.found[4].count;
     bc = s.found[4].before_count;
@@ -628,7 +670,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
   uint64_t masses[kBins / kThreads];
 #pragma unroll
   for (int i = 0; i < kBins / kThreads; ++i) counts[i] = rs.count[i * kThreads + t], masses[i] = rs.mass[i * kThreads + t];
-  const uint32_t n_list = rs.n_list;
+  const uint32_t listed_here = rs.n_list[t & (kMaxSlices - 1)];  // lane i: of slice i (not written where nothing is listed)
   Settings set;
   if (!set.derive(a, row)) {  // uniform: an empty row, or the first of the order
     if (t == 0 && part == 0) {
@@ -640,14 +682,27 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
   const Questions ask{set.top_k > 0 ? uint64_t(set.top_k) : 0u, a.top_ps ? a.top_ps[row] : a.top_p, a.u[row]};
   set.weigh.constants();
   Row<DT> r{a.logits + int64_t(row) * a.row_bytes, a.vocab, set.weigh};
-  const bool from_list = set.listed && n_list <= kList;  // every token that may be kept
+  // Every token that may be kept is listed, unless there are too many.
+  const uint32_t room = slice_list(a.slices);
+  uint32_t n_list = (t & 63) < a.slices && set.listed ? listed_here : 0u, list_at = n_list;
+  const bool fits = !__any(n_list > room);
+  const uint32_t n_listed = wave_sums(list_at);
+  const bool from_list = set.listed && fits && n_listed <= kList;
   if (from_list && part) return;
-  if (from_list && n_list <= kFew / 2) {
-    for (uint32_t i = t; i < n_list; i += kThreads) s.cand[i] = rs.list[i];
-    answer_from(s, r, ask, n_list, false, 0u, 0u, a, row);
+  // f(order, place) for them.
+  const auto each_listed = [&](auto&& f) {
+    for (int i = t >> 6; i < a.slices; i += kWaves) {
+      const uint32_t n = uint32_t(__shfl(int(n_list), i)), at = uint32_t(__shfl(int(list_at), i)) - n;
+      for (uint32_t j = t & 63; j < n; j += 64) f(rs.list[i * room + j], at + j);
+    }
+  };
+  if (from_list && n_listed <= kFew / 2) {
+    each_listed([&](uint64_t o, uint32_t at) { s.cand[at] = o; });
+    answer_from(s, r, ask, n_listed, false, 0u, 0u, a, row);
     return;
   }
-  set.raise_floor(a, row);
+  set.load_groups(a, row);
+  set.raise_floor(a);
   const Weigher weigh = r.weigh = set.weigh;
 #pragma unroll
   for (int i = 0; i < kBins / kThreads; ++i) s.count[i * kThreads + t] = counts[i], s.mass[i * kThreads + t] = masses[i];
@@ -659,15 +714,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
   const bool by_k = ask.top_k > 0 && ask.top_k < bins.total_count;  // counts are there with top-k alone
   uint32_t k_bin = kBins, p_first = kBins, p_last = 0u;
   if (by_k) {
-    bins.find(s.found[0], true, ask.top_k);
+    bins.find(s.count, s.mass, s.found[0], true, ask.top_k);
     __syncthreads();
     k_bin = s.found[0].bin;
     low = s.found[0].before_mass + 1;
     high = s.found[0].before_mass + s.found[0].mass;
   }
   if (ask.cuts()) {
-    bins.find(s.found[1], false, ask.cut(low));
-    bins.find(s.found[2], false, ask.cut(high));
+    bins.find(s.count, s.mass, s.found[1], false, ask.cut(low));
+    bins.find(s.count, s.mass, s.found[2], false, ask.cut(high));
     __syncthreads();
     p_first = s.found[1].bin;
     p_last = s.found[2].bin;
@@ -675,8 +730,8 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
     const uint64_t to = s.found[2].before_mass + s.found[2].mass;
     high = to < high ? to : high;
   }
-  bins.find(s.found[3], false, ask.draw(low));
-  bins.find(s.found[4], false, ask.draw(high));
+  bins.find(s.count, s.mass, s.found[3], false, ask.draw(low));
+  bins.find(s.count, s.mass, s.found[4], false, ask.draw(high));
   __syncthreads();
   const uint32_t d_first = s.found[3].bin, d_last = s.found[4].bin;
   // What is before each bin and not in one of them.
@@ -684,8 +739,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
   uint64_t skip_mass = 0u;
   const auto taken = [&](uint32_t b) { return b == k_bin || (b >= p_first && b <= p_last) || (b >= d_first && b <= d_last); };
 #pragma unroll
-  for (int i = 0; i < kBins / kThreads; ++i)
-    if (!taken(uint32_t(t * (kBins / kThreads) + i))) skip_count += bins.count[i], skip_mass += bins.mass[i];
+  for (int i = 0; i < kBins / kThreads; ++i) {
+    const uint32_t b = uint32_t(t * (kBins / kThreads) + i);
+    if (!taken(b)) skip_count += s.count[b], skip_mass += s.mass[b];
+  }
   const Scan skip = block_scan(s, skip_count, skip_mass);
   skip_count = skip.count;
   skip_mass = skip.mass;
@@ -693,9 +750,9 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
   for (int i = 0; i < kBins / kThreads; ++i) {
     const uint32_t b = uint32_t(t * (kBins / kThreads) + i);
     const bool take = taken(b);
-    s.count[b] = skip_count | (take ? kGathered : 0u);
-    s.mass[b] = skip_mass;
-    if (!take) skip_count += bins.count[i], skip_mass += bins.mass[i];
+    s.skip_count[b] = skip_count | (take ? kGathered : 0u);
+    s.skip_mass[b] = skip_mass;
+    if (!take) skip_count += s.count[b], skip_mass += s.mass[b];
   }
   if (t == 0) s.n = 0u;
   __syncthreads();
@@ -712,17 +769,15 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
     if (!((z >= lo[0] && z <= hi[0]) || (z >= lo[1] && z <= hi[1]) || (z >= lo[2] && z <= hi[2]))) return;
     uint64_t w;
     int b;
-    if (!weigh(z, w, b) || !(s.count[b] & kGathered)) return;
+    if (!weigh(z, w, b) || !(s.skip_count[b] & kGathered)) return;
     const uint32_t at = atomicAdd(&s.n, 1u);
     if (at < kList) s.cand[at] = order();
   };
   if (from_list) {
-    for (uint32_t i = t; i < n_list; i += kThreads) {
-      const uint64_t o = rs.list[i];
-      gather(order_value(o), [&] { return o; });
-    }
+    each_listed([&](uint64_t o, uint32_t) { gather(order_value(o), [&] { return o; }); });
   } else {
-    each_token<DT, kThreads>(r.data, a.vocab, part, parts, [&](int i, float z) { gather(z, [&] { return order_of(z, i); }); });
+    Walk<DT, kThreads> walk(r.data, a.vocab, part, parts);
+    walk.each([&](int i, float z) { gather(z, [&] { return order_of(z, i); }); });
   }
   __syncthreads();
   uint32_t n = s.n;
@@ -757,9 +812,10 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
     if (question == 1 && !ask.cuts()) continue;
     const uint64_t goal = question == 0 ? ask.top_k : question == 1 ? ask.cut(kept) : ask.draw(kept);
     __syncthreads();
-    bins.find(s.found[question], question == 0, goal);
+    bins.find(s.count, s.mass, s.found[question], question == 0, goal);
     __syncthreads();
-    narrow(s, r, s.found[question], question == 0, goal, n);
+    narrow<DT>(s, r.data, a.vocab, weigh.top, weigh.floor, weigh.bits, weigh.least, int(s.found[question].bin),
+               s.found[question].before_count, s.found[question].before_mass, question == 0, goal, n);
     if (question < 2) kept = s.mass_to;
   }
   if (t == 0) {
@@ -769,11 +825,11 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
 }
 
 // Slices of a row in the first two launches: of 2048 tokens or more, as many as
-// leave 2048 workgroups (eight for each of 256 CUs).  The result does not depend
-// on it, nor on the workgroups that gather in the third.
+// are resident at once (four workgroups on each of 256 CUs).  The result does not
+// depend on it, nor on the workgroups that gather in the third.
 int slice_count(int32_t rows, int32_t vocab) {
   int s = (vocab + 2047) / 2048;
-  const int fill = 2048 / rows > 0 ? 2048 / rows : 1;
+  const int fill = 1024 / rows > 0 ? 1024 / rows : 1;
   s = s < fill ? s : fill;
   return s < kMaxSlices ? s : kMaxSlices;
 }
