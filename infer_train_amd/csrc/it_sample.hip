@@ -38,9 +38,8 @@ constexpr int kBins = 2048;          // of a row, linear in z
 constexpr int kList = 2048;          // tokens listed per row, and gathered in LDS
 constexpr int kRowList = 8192;       // room for a row's slices' lists: a slice may hold most of the likely tokens
 constexpr int kSliceList = kList - 1;  // of a slice at most: its workgroup's LDS is a quarter of a CU's
-constexpr int kFew = 256;            // tokens compared all with all
+constexpr int kFew = 128;            // tokens compared all with all
 constexpr int kFineBits = 10, kFine = 1 << kFineBits;
-constexpr uint32_t kGathered = 1u << 31;  // of a bin's count
 constexpr int kMaxSlices = 32;
 constexpr int kGroups = 2 * kSliceWaves;  // group maxima per slice: half waves
 constexpr int kMaxVocab = 1 << 18;   // a sum of weights stays below 2^62
@@ -136,9 +135,9 @@ struct Weigher {
 // aligned part, the first slice also the tokens before that part, the last those
 // behind it.  The first vectors are loaded when the walk is made, so that what
 // a kernel does before each() runs in their shadow.
-template <int DT, int kBlock>
+template <int DT, int kBlock, int U>
 struct Walk {
-  static constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es, U = 4;
+  static constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es;
   using In = RowVec<DT, V>;
   const char* row;
   const typename In::raw* v;
@@ -181,7 +180,10 @@ struct Walk {
   }
 };
 
-__device__ __forceinline__ uint64_t shfl64(uint64_t x, int lane) { return uint64_t(__shfl((unsigned long long)(x), lane)); }
+// x of one lane, the same for all.
+__device__ __forceinline__ uint64_t lane64(uint64_t x, int lane) {
+  return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(x >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(x), lane));
+}
 __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
 #pragma unroll
   for (int o = 32; o; o >>= 1) {
@@ -207,7 +209,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
   for (int b = slice * kSliceThreads + int(threadIdx.x); b < kBins; b += a.slices * kSliceThreads) rs.count[b] = 0u, rs.mass[b] = 0u;
   float top = -INFINITY;
   int at = -1;
-  Walk<DT, kSliceThreads> walk(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices);
+  Walk<DT, kSliceThreads, 4> walk(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices);
   walk.each([&](int i, float z) {
     if (z > top) top = z, at = i;  // of equals the first
   });
@@ -252,7 +254,7 @@ struct Settings {
     const float min_p = a.min_ps ? a.min_ps[row] : a.min_p;
     top_k = a.top_ks ? a.top_ks[row] : a.top_k;
     best = wave_max64(lane < a.slices ? rs.best[lane] : 0u);
-    best = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(best >> 32)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(best)));
+    best = lane64(best, 0);
     if (best == 0u || !(temp > 0.0f)) return false;  // uniform
     weigh.top = order_value(best);
     weigh.bits = 1.4426950408889634 / double(temp);
@@ -294,7 +296,7 @@ __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
   __shared__ uint32_t count[kBins], n;
   const int t = int(threadIdx.x), slice = int(blockIdx.x), row = int(blockIdx.y);
   RowState& rs = a.rows[row];
-  Walk<DT, kSliceThreads> walk(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices);
+  Walk<DT, kSliceThreads, 4> walk(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices);
   Settings set;
   set.load_groups(a, row);
   if (!set.derive(a, row)) return;
@@ -331,7 +333,6 @@ __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
 
 struct Shared {
   uint64_t mass[kBins];   // the row's bins
-  uint64_t skip_mass[kBins];  // what lies before each but is not gathered
   uint64_t cand[kList];   // the tokens gathered to answer from
   struct Weighed {
     uint64_t order, weight;
@@ -341,12 +342,10 @@ struct Shared {
     Weighed weighed[kFew];         // answer_from()
   };
   uint32_t count[kBins];
-  uint32_t skip_count[kBins];
   uint32_t fine_count[kFine];
-  uint64_t last[64];
+  Weighed last[64];
   uint64_t wave_mass[kWaves];
   uint32_t wave_count[kWaves];
-  unsigned long long lo, hi;
   uint32_t n, base;
   uint64_t kept;
   struct Found {
@@ -426,7 +425,7 @@ struct Row {
   // f(order, z) for the row's tokens with lo <= z <= hi.
   template <class F>
   __device__ __forceinline__ void each(float lo, float hi, F&& f) const {
-    Walk<DT, kThreads> walk(data, vocab, 0, 1);
+    Walk<DT, kThreads, 1> walk(data, vocab, 0, 1);
     walk.each([&](int i, float z) {
       if (z >= lo && z <= hi) f(order_of(z, i), z);
     });
@@ -462,15 +461,13 @@ struct Questions {
   }
 };
 
-// Answers from the tokens in s.cand (n <= kFew of them), each after those of
-// s.skip_mass and s.skip_count of its bin that are not among them (`gaps`; else there are
-// no others).  kept, tokens: the row's mass and number, with gaps.  Each token's
-// place is found by comparing it with all others, a power of two of threads
-// sharing them: no step waits for the one before, but the work grows with n^2
-// (n = 128: 1 us, 256: 4, 512: 28).
+// All answers from the n <= kFew tokens in s.cand, which are all that may be kept.
+// Each one's place is found by comparing it with all others, a power of two of
+// threads sharing them: no step waits for the one before, but the work grows with n^2
+// (n = 128: 1 us, 256: 8, 512: 28).
 template <int DT>
-__device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, bool gaps, uint64_t kept,
-                                            uint32_t tokens, const SampleArgs& a, int out) {
+__device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, const SampleArgs& a,
+                                            int out) {
   const int t = int(threadIdx.x);
   int log2_parts = 0;
   while (log2_parts < 6 && uint32_t(kThreads >> (log2_parts + 1)) >= n) ++log2_parts;
@@ -499,24 +496,17 @@ __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const
     before_mass += uint64_t(__shfl_xor((unsigned long long)(before_mass), int(o)));
   }
   w = i < n ? all[i].weight : 0u;
-  if (!gaps) {  // the last of them all knows the totals
-    if (i < n && before_count == n - 1 && part == 0) s.kept = before_mass + w;
-    __syncthreads();
-    kept = s.kept;
-    tokens = n;
-    __syncthreads();
-  } else if (i < n) {
-    row.weigh(order_value(own), w, bin);
-    before_count += s.skip_count[bin] & ~kGathered;
-    before_mass += s.skip_mass[bin];
-  }
   const bool one = i < n && part == 0;
+  if (one && before_count == n - 1) s.kept = before_mass + w;  // the last of them all knows the total
+  __syncthreads();
+  uint64_t kept = s.kept;
+  __syncthreads();
   // f() for the token at which the count, or the mass, reaches the goal.
   const auto at = [&](bool by_count, uint64_t goal, auto&& f) {
     const uint64_t before = by_count ? uint64_t(before_count) : before_mass, after = before + (by_count ? 1u : w);
     if (one && before < goal && goal <= after) f();
   };
-  if (ask.top_k > 0 && ask.top_k < tokens) {
+  if (ask.top_k > 0 && ask.top_k < n) {
     at(true, ask.top_k, [&] { s.kept = before_mass + w; });
     __syncthreads();
     kept = s.kept;
@@ -534,76 +524,54 @@ __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const
 }
 
 // One question over any number of tokens (many equal logits, a flat row): bins
-// inside the bin f, by order, until 64 tokens are left.  gathered: s.cand holds
-// that many tokens, all of the bin's among them; past kList they are read from
-// the row, again each time until they fit.  The answer is s.token, its weight, and
-// the mass up to and with it in s.mass_to.
-// A function of its own, called with values: rows that need it are few, and what
-// it holds would take registers from those that do not.
+// inside the bin f, a power of two of orders each, until 64 tokens are left.
+// gathered: s.cand holds that many tokens, all of the bin's among them; past kList
+// they are read from the row, again each time until they fit.  The answer is
+// s.token, its weight, and the mass up to and with it in s.mass_to.
 template <int DT>
-__device__ __noinline__ void narrow(Shared& s, const char* data, int vocab, float top, float floor, double bits, double least, int bin,
-                                    uint32_t bc, uint64_t bm, bool by_count, uint64_t goal, uint32_t gathered) {
-  const int t = int(threadIdx.x);
-  Row<DT> row{data, vocab, {top, floor, bits, least}};
-  row.weigh.constants();
-  uint32_t n;
-  __syncthreads();
-  if (t == 0) s.n = 0u, s.lo = ~0ull, s.hi = 0ull;
-  __syncthreads();
-  unsigned long long tlo = ~0ull, thi = 0ull;
-  const auto member = [&](uint64_t o, float z) {
-    uint64_t w;
-    int b;
-    if (!row.weigh(z, w, b) || b != bin) return false;
-    tlo = o < tlo ? o : tlo;
-    thi = o > thi ? o : thi;
-    return true;
-  };
-  if (gathered <= kList) {
-    uint32_t own = 0u;
-    for (uint32_t i = t; i < gathered; i += kThreads) own += member(s.cand[i], order_value(s.cand[i]));
-    if (own) atomicAdd(&s.n, own);
-  } else {
-    float zlo, zhi;
-    row.span(bin, bin, zlo, zhi);
-    row.each(zlo, zhi, [&](uint64_t o, float z) {
-      if (!member(o, z)) return;
-      const uint32_t at = atomicAdd(&s.n, 1u);
-      if (at < kList) s.cand[at] = o;
-    });
-  }
-  if (thi) {
-    atomicMin(&s.lo, tlo);
-    atomicMax(&s.hi, thi);
-  }
-  __syncthreads();
-  uint64_t lo = s.lo, hi = s.hi;
-  n = s.n;
-  bool held = gathered <= kList || n <= kList;  // all of them in s.cand
-  uint32_t cands = gathered <= kList ? gathered : n;
-  // f(order) for the tokens with lo <= order <= hi.
+__device__ __forceinline__ void narrow(Shared& s, const Row<DT>& row, const Shared::Found& f, bool by_count, uint64_t goal,
+                                       uint32_t gathered) {
+  const int t = int(threadIdx.x), bin = int(f.bin);
+  uint32_t n, bc = f.before_count;
+  uint64_t bm = f.before_mass;
+  float zlo, zhi;
+  row.span(bin, bin, zlo, zhi);
+  uint64_t lo = order_of(zlo, kMaxVocab - 1), hi = order_of(fminf(zhi, row.weigh.top), 0);
+  bool held = gathered <= kList;  // in s.cand
+  uint32_t cands = gathered;
+  // g(order, weight) for the bin's tokens with lo <= order <= hi.
   const auto each_in = [&](auto&& g) {
+    const auto member = [&](uint64_t o, float z) {
+      uint64_t w;
+      int b;
+      if (o >= lo && o <= hi && row.weigh(z, w, b) && b == bin) g(o, w);
+    };
     if (held) {
-      for (uint32_t i = t; i < cands; i += kThreads) {
-        const uint64_t o = s.cand[i];
-        if (o >= lo && o <= hi) g(o);
-      }
+      for (uint32_t i = t; i < cands; i += kThreads) member(s.cand[i], order_value(s.cand[i]));
     } else {
-      row.each(order_value(lo), order_value(hi), [&](uint64_t o, float) {
-        if (o >= lo && o <= hi) g(o);
-      });
+      row.each(order_value(lo), order_value(hi), member);
     }
   };
-  // kFine bins of a power of two of orders each: nine bits of hi - lo < 2^50 a
-  // turn or more, orders are unique.
+  // Their number; the first 64 of them in s.last.
+  const auto collect = [&] {
+    __syncthreads();
+    if (t == 0) s.n = 0u;
+    __syncthreads();
+    each_in([&](uint64_t o, uint64_t w) {
+      const uint32_t at = atomicAdd(&s.n, 1u);
+      if (at < 64) s.last[at] = {o, w};
+    });
+    __syncthreads();
+    return s.n;
+  };
+  n = gathered <= kFew ? collect() : kFew;
+  // Nine bits of hi - lo < 2^50 a turn or more; orders are unique.
   for (int turn = 0; n > 64 && turn < 6; ++turn) {
     const int shift = max(0, 64 - __clzll((long long)(hi - lo)) - kFineBits);
+    __syncthreads();
     for (int b = t; b < kFine; b += kThreads) s.fine_count[b] = 0u, s.fine[b] = 0u;
     __syncthreads();
-    each_in([&](uint64_t o) {
-      uint64_t w = 0;
-      int b;
-      row.weigh(order_value(o), w, b);
+    each_in([&](uint64_t o, uint64_t w) {
       const uint32_t x = uint32_t((hi - o) >> shift);
       atomicAdd(&s.fine_count[x], 1u);
       atomicAdd(reinterpret_cast<unsigned long long*>(&s.fine[x]), (unsigned long long)(w));
@@ -611,6 +579,7 @@ __device__ __noinline__ void narrow(Shared& s, const char* data, int vocab, floa
     __syncthreads();
     const Bins<kFine / kThreads> fine(s, s.fine_count, s.fine, bc, bm);
     fine.find(s.fine_count, s.fine, s.found[4], by_count, goal);
+    if (t == 0) s.n = 0u;
     __syncthreads();
     n = s.found[4].count;
     bc = s.found[4].before_count;
@@ -618,42 +587,32 @@ __device__ __noinline__ void narrow(Shared& s, const char* data, int vocab, floa
     hi -= uint64_t(s.found[4].bin) << shift;
     const uint64_t width = uint64_t(1) << shift;
     lo = hi >= width && hi - width + 1 > lo ? hi - width + 1 : lo;
+    if (n <= 64) {  // uniform
+      n = collect();
+      break;
+    }
     if (!held && n <= kList) {
-      if (t == 0) s.n = 0u;
-      __syncthreads();
-      each_in([&](uint64_t o) {
+      each_in([&](uint64_t o, uint64_t) {
         const uint32_t at = atomicAdd(&s.n, 1u);
         if (at < kList) s.cand[at] = o;
       });
-      __syncthreads();
       held = true;
-      cands = min(s.n, uint32_t(kList));
+      cands = n;
     }
-    __syncthreads();
   }
-  if (t == 0) s.n = 0u;
-  __syncthreads();
-  each_in([&](uint64_t o) {
-    const uint32_t at = atomicAdd(&s.n, 1u);
-    if (at < 64) s.last[at] = o;
-  });
-  __syncthreads();
   if (t < 64) {  // one wave: a token a lane, each with the mass of those before it
-    n = min(n, 64u);
-    const uint64_t own = t < int(n) ? s.last[t] : 0u;
-    uint64_t w = 0;
-    int b;
-    if (t < int(n)) row.weigh(order_value(own), w, b);
+    n = min(uint32_t(__builtin_amdgcn_readfirstlane(int(n))), 64u);
+    const Shared::Weighed own = t < int(n) ? s.last[t] : Shared::Weighed{0u, 0u};
     uint32_t ci = 0u;
     uint64_t mi = 0u;
     for (uint32_t j = 0; j < n; ++j) {
-      const uint64_t o = shfl64(own, int(j)), wj = shfl64(w, int(j));
-      if (o >= own) ci += 1u, mi += wj;
+      const uint64_t o = lane64(own.order, int(j)), w = lane64(own.weight, int(j));
+      if (o >= own.order) ci += 1u, mi += w;
     }
-    const uint64_t after = by_count ? uint64_t(bc + ci) : bm + mi, before = by_count ? after - 1 : after - w;
+    const uint64_t after = by_count ? uint64_t(bc + ci) : bm + mi, before = by_count ? after - 1 : after - own.weight;
     if (t < int(n) && before < goal && goal <= after) {
-      s.token = order_index(own);
-      s.weight = w;
+      s.token = order_index(own.order);
+      s.weight = own.weight;
       s.mass_to = bm + mi;
     }
   }
@@ -696,9 +655,9 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
       for (uint32_t j = t & 63; j < n; j += 64) f(rs.list[i * room + j], at + j);
     }
   };
-  if (from_list && n_listed <= kFew / 2) {
+  if (from_list && n_listed <= kFew) {
     each_listed([&](uint64_t o, uint32_t at) { s.cand[at] = o; });
-    answer_from(s, r, ask, n_listed, false, 0u, 0u, a, row);
+    answer_from(s, r, ask, n_listed, a, row);
     return;
   }
   set.load_groups(a, row);
@@ -734,49 +693,28 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
   bins.find(s.count, s.mass, s.found[4], false, ask.draw(high));
   __syncthreads();
   const uint32_t d_first = s.found[3].bin, d_last = s.found[4].bin;
-  // What is before each bin and not in one of them.
-  uint32_t skip_count = 0u;
-  uint64_t skip_mass = 0u;
-  const auto taken = [&](uint32_t b) { return b == k_bin || (b >= p_first && b <= p_last) || (b >= d_first && b <= d_last); };
-#pragma unroll
-  for (int i = 0; i < kBins / kThreads; ++i) {
-    const uint32_t b = uint32_t(t * (kBins / kThreads) + i);
-    if (!taken(b)) skip_count += s.count[b], skip_mass += s.mass[b];
-  }
-  const Scan skip = block_scan(s, skip_count, skip_mass);
-  skip_count = skip.count;
-  skip_mass = skip.mass;
-#pragma unroll
-  for (int i = 0; i < kBins / kThreads; ++i) {
-    const uint32_t b = uint32_t(t * (kBins / kThreads) + i);
-    const bool take = taken(b);
-    s.skip_count[b] = skip_count | (take ? kGathered : 0u);
-    s.skip_mass[b] = skip_mass;
-    if (!take) skip_count += s.count[b], skip_mass += s.mass[b];
-  }
   if (t == 0) s.n = 0u;
   __syncthreads();
-  // Only tokens in the z of those bins are weighed again.
-  // A row's workgroups have all come here alike; each gathers its part.
+  // A row's workgroups have all come here alike; each gathers its part of the
+  // tokens in the z of those bins.
   const int shares = from_list ? 1 : parts;
   float lo[3], hi[3];
-  r.span(int(by_k ? k_bin : d_first), int(by_k ? k_bin : d_last), lo[0], hi[0]);
+  r.span(int(d_first), int(d_last), lo[0], hi[0]);
   r.span(int(ask.cuts() ? p_first : d_first), int(ask.cuts() ? p_last : d_last), lo[1], hi[1]);
-  r.span(int(d_first), int(d_last), lo[2], hi[2]);
-  const float any_lo = fminf(fminf(lo[0], lo[1]), lo[2]), any_hi = fmaxf(fmaxf(hi[0], hi[1]), hi[2]);
+  r.span(int(by_k ? k_bin : d_first), int(by_k ? k_bin : d_last), lo[2], hi[2]);
+  const float lowest = fminf(fminf(lo[0], lo[1]), lo[2]);
   const auto gather = [&](float z, auto&& order) {
-    if (!(z >= any_lo && z <= any_hi)) return;
-    if (!((z >= lo[0] && z <= hi[0]) || (z >= lo[1] && z <= hi[1]) || (z >= lo[2] && z <= hi[2]))) return;
-    uint64_t w;
-    int b;
-    if (!weigh(z, w, b) || !(s.skip_count[b] & kGathered)) return;
+    if (!(z >= lowest)) return;  // most tokens
+    bool in = (z >= lo[0] && z <= hi[0]) || (z >= lo[1] && z <= hi[1]);
+    if (by_k) in = in || (z >= lo[2] && z <= hi[2]);  // uniform
+    if (!in) return;
     const uint32_t at = atomicAdd(&s.n, 1u);
     if (at < kList) s.cand[at] = order();
   };
   if (from_list) {
     each_listed([&](uint64_t o, uint32_t) { gather(order_value(o), [&] { return o; }); });
   } else {
-    Walk<DT, kThreads> walk(r.data, a.vocab, part, parts);
+    Walk<DT, kThreads, 4> walk(r.data, a.vocab, part, parts);
     walk.each([&](int i, float z) { gather(z, [&] { return order_of(z, i); }); });
   }
   __syncthreads();
@@ -803,10 +741,6 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
       for (uint32_t i = t; i < n; i += kThreads)
         s.cand[i] = __hip_atomic_load(&rs.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  if (n <= kFew) {
-    answer_from(s, r, ask, n, true, bins.total_mass, bins.total_count, a, row);
-    return;
-  }
   uint64_t kept = bins.total_mass;
   for (int question = by_k ? 0 : 1; question < 3; ++question) {
     if (question == 1 && !ask.cuts()) continue;
@@ -814,8 +748,7 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
     __syncthreads();
     bins.find(s.count, s.mass, s.found[question], question == 0, goal);
     __syncthreads();
-    narrow<DT>(s, r.data, a.vocab, weigh.top, weigh.floor, weigh.bits, weigh.least, int(s.found[question].bin),
-               s.found[question].before_count, s.found[question].before_mass, question == 0, goal, n);
+    narrow(s, r, s.found[question], question == 0, goal, n);
     if (question < 2) kept = s.mass_to;
   }
   if (t == 0) {
