@@ -599,7 +599,8 @@ int32_t it_flash_attention(const float* q, const float* k, const float* v, const
  *     min_p above 1 counts as 1, NaN as off
  *   tokens: int32[n_rows]; probs: float[n_rows] or NULL; device
  *   ws: it_sample_workspace(...) bytes, device, 256-byte aligned; it need not
- *     be cleared, and calls that overlap in time need one each
+ *     be cleared, and calls that overlap in time need one each; short rows and
+ *     large batches need none (0 bytes: ws may be NULL)
  * Launched on the current device, to which `stream` must belong. */
 size_t it_sample_workspace(int32_t n_rows, int32_t vocab);
 int32_t it_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t n_rows, int32_t vocab,

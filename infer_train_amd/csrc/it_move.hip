@@ -137,8 +137,8 @@ __global__ __launch_bounds__(kThreads) void kv_move_rows(MoveArgs a) {
       xa[j] = Row::narrow(fa);
       xb[j] = Row::narrow(fb);
     }
-    *reinterpret_cast<typename Row::raw*>(row + lp.ea * kBytes) = xa[j];
-    *reinterpret_cast<typename Row::raw*>(row + lp.eb * kBytes) = xb[j];
+    __builtin_nontemporal_store(xa[j], reinterpret_cast<typename Row::raw*>(row + lp.ea * kBytes));
+    __builtin_nontemporal_store(xb[j], reinterpret_cast<typename Row::raw*>(row + lp.eb * kBytes));
   }
 }
 

@@ -12,15 +12,15 @@
 // exact, so any number of workgroups may add them in any order, and the same
 // row gives the same token in any batch.
 //
-// Three launches.  The first reads the logits from HBM and takes each slice's
-// maximum.  The second reads them again (from the last-level cache where the
-// call's logits fit its 256 MB), weighs them in fp64 against the row's maximum
-// and adds counts and masses of 2048 bins, linear in z, in LDS and then per row.
-// The third finds the few bins that a row's answers lie in, gathers their tokens
-// and answers from those.  Where top-k or min-p bound the
-// tokens that matter, those alone are weighed, and listed, so that the third need
-// not read the row again: of the maxima of groups of tokens the k-th largest is a
-// lower bound of the k-th largest token.
+// The logits are read from HBM for their maximum and again, from a cache where the
+// call's logits fit it, to be weighed in fp64 against that: counts and masses are
+// added into 2048 bins, linear in z, in LDS.  Then the few bins that the answers lie
+// in are found, their tokens gathered, and the answers taken from those.  Where
+// top-k or min-p bound the tokens that matter, those alone are weighed, and listed,
+// so that the row need not be read a third time: of the maxima of groups of tokens
+// the k-th largest is a lower bound of the k-th largest token.  A workgroup per row
+// does all this in one launch; a few long rows are divided among many workgroups,
+// in three.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -32,17 +32,18 @@ using namespace itkv;
 namespace {
 constexpr int kSliceThreads = 512;   // of a slice's workgroup
 constexpr int kSliceWaves = kSliceThreads / 64;
-constexpr int kThreads = 512;        // of a row's
+constexpr int kThreads = 1024;       // of a row's
 constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 2048;          // of a row, linear in z
 constexpr int kList = 2048;          // tokens listed per row, and gathered in LDS
 constexpr int kRowList = 8192;       // room for a row's slices' lists: a slice may hold most of the likely tokens
 constexpr int kSliceList = kList - 1;  // of a slice at most: its workgroup's LDS is a quarter of a CU's
-constexpr int kFew = 128;            // tokens compared all with all
+constexpr int kFew = 256;            // tokens compared all with all
 constexpr int kFineBits = 10, kFine = 1 << kFineBits;
 constexpr int kMaxSlices = 32;
 constexpr int kGroups = 2 * kSliceWaves;  // group maxima per slice: half waves
 constexpr int kMaxVocab = 1 << 18;   // a sum of weights stays below 2^62
+constexpr int kRowGroups = kThreads / 2;  // group maxima of such a row, at most
 constexpr int kIndexBits = 18;
 constexpr double kUnit = 0x1p44;      // weight of the largest token
 constexpr double kLeast = 0x1.0000000000001p-45;  // smaller weights round to nothing
@@ -233,28 +234,27 @@ __global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
 struct Settings {
   Weigher weigh;
   uint64_t best;
-  int top_k;
+  int top_k, groups;
   bool listed;  // few tokens can be kept: they are listed
   static constexpr int kLoads = kMaxSlices * kGroups / 64;
   uint32_t group[kLoads];
   // The group maxima, 64 to a register, before it is known whether they count.
-  __device__ __forceinline__ void load_groups(const SampleArgs& a, int row) {
-    const int lane = int(threadIdx.x & 63), groups = a.slices * kGroups;
+  __device__ __forceinline__ void load_groups(const SampleArgs& a, const uint32_t* maxima, int n) {
+    const int lane = int(threadIdx.x & 63);
+    groups = n;
     if (!a.top_ks && a.top_k <= 0) return;
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int i = j * 64 + lane;
-      group[j] = i < groups ? a.rows[row].group_max[i] : 0u;
+      group[j] = i < groups ? maxima[i] : 0u;
     }
   }
-  __device__ __forceinline__ bool derive(const SampleArgs& a, int row) {
-    const RowState& rs = a.rows[row];
-    const int lane = int(threadIdx.x & 63), groups = a.slices * kGroups;
+  // first: the place of the row's first token, 0 where nothing is above -inf.
+  __device__ __forceinline__ bool derive(const SampleArgs& a, int row, uint64_t first) {
     const float temp = a.temperatures ? a.temperatures[row] : a.temperature;
     const float min_p = a.min_ps ? a.min_ps[row] : a.min_p;
     top_k = a.top_ks ? a.top_ks[row] : a.top_k;
-    best = wave_max64(lane < a.slices ? rs.best[lane] : 0u);
-    best = lane64(best, 0);
+    best = lane64(first, 0);
     if (best == 0u || !(temp > 0.0f)) return false;  // uniform
     weigh.top = order_value(best);
     weigh.bits = 1.4426950408889634 / double(temp);
@@ -274,8 +274,7 @@ struct Settings {
   }
   // The floor raised to the first sixteen bits of the top_k-th largest group
   // maximum: at least top_k tokens have keys that large.
-  __device__ __forceinline__ void raise_floor(const SampleArgs& a) {
-    const int groups = a.slices * kGroups;
+  __device__ __forceinline__ void raise_floor() {
     if (top_k <= 0 || top_k > groups) return;
     uint32_t key = 0u;
     for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
@@ -288,7 +287,28 @@ struct Settings {
     }
     if (key > kDeadKey) weigh.floor = fmaxf(weigh.floor, key_value(key));
   }
+  // What a row without anything to weigh answers.
+  __device__ __forceinline__ void trivial(const SampleArgs& a, int row) const {
+    a.tokens[row] = best ? order_index(best) : -1;
+    if (a.probs) a.probs[row] = best ? 1.0f : 0.0f;
+  }
 };
+
+// Adds a token to a workgroup's bins, and to its list of `room` places where
+// few tokens can be kept.
+__device__ __forceinline__ void weigh_token(const Settings& set, float z, int index, uint64_t* mass, uint32_t* count, uint64_t* list,
+                                            uint32_t* n, uint32_t room) {
+  if (!(z >= set.weigh.floor)) return;
+  uint64_t w;
+  int b;
+  if (!set.weigh(z, w, b)) return;
+  atomicAdd(reinterpret_cast<unsigned long long*>(&mass[b]), (unsigned long long)(w));
+  if (set.top_k > 0) atomicAdd(&count[b], 1u);  // only top-k asks for counts
+  if (set.listed) {
+    const uint32_t at = atomicAdd(n, 1u);
+    if (at < room) list[at] = order_of(z, index);
+  }
+}
 
 template <int DT>
 __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
@@ -298,26 +318,15 @@ __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
   RowState& rs = a.rows[row];
   Walk<DT, kSliceThreads, 4> walk(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices);
   Settings set;
-  set.load_groups(a, row);
-  if (!set.derive(a, row)) return;
-  set.raise_floor(a);
+  set.load_groups(a, rs.group_max, a.slices * kGroups);
+  if (!set.derive(a, row, wave_max64((t & 63) < a.slices ? rs.best[t & 63] : 0u))) return;
+  set.raise_floor();
   set.weigh.constants();
   for (int b = t; b < kBins; b += kSliceThreads) count[b] = 0u, mass[b] = 0u;
   if (t == 0) n = 0u;
   __syncthreads();
   const uint32_t room = slice_list(a.slices);
-  walk.each([&](int i, float z) {
-    if (!(z >= set.weigh.floor)) return;
-    uint64_t w;
-    int b;
-    if (!set.weigh(z, w, b)) return;
-    atomicAdd(reinterpret_cast<unsigned long long*>(&mass[b]), (unsigned long long)(w));
-    if (set.top_k > 0) atomicAdd(&count[b], 1u);  // only top-k asks for counts
-    if (set.listed) {
-      const uint32_t at = atomicAdd(&n, 1u);
-      if (at < room) list[at] = order_of(z, i);
-    }
-  });
+  walk.each([&](int i, float z) { weigh_token(set, z, i, mass, count, list, &n, room); });
   __syncthreads();
   if (set.listed) {  // each slice in its own part of the row's list
     if (t == 0) rs.n_list[slice] = n;
@@ -464,7 +473,7 @@ struct Questions {
 // All answers from the n <= kFew tokens in s.cand, which are all that may be kept.
 // Each one's place is found by comparing it with all others, a power of two of
 // threads sharing them: no step waits for the one before, but the work grows with n^2
-// (n = 128: 1 us, 256: 8, 512: 28).
+// (n = 128: 1 us, 256: 4, 512: 15).
 template <int DT>
 __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, const SampleArgs& a,
                                             int out) {
@@ -619,8 +628,80 @@ __device__ __forceinline__ void narrow(Shared& s, const Row<DT>& row, const Shar
   __syncthreads();
 }
 
+// The z of the tokens to answer from, once a row's bins are in s.count and s.mass.
 template <int DT>
-__global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
+struct Plan {
+  Bins<kBins / kThreads> bins;
+  bool by_k;
+  float lo[3], hi[3], lowest;
+  // The bins that the answers lie in: a question's goal is known within the mass
+  // of the bin that the one before it ends in.
+  __device__ __forceinline__ Plan(Shared& s, const Row<DT>& row, const Questions& ask) : bins(s, s.count, s.mass, 0u, 0u) {
+    uint64_t low = bins.total_mass, high = low;  // bounds of the mass kept
+    by_k = ask.top_k > 0 && ask.top_k < bins.total_count;  // counts are there with top-k alone
+    uint32_t k_bin = 0u, p_first = 0u, p_last = 0u;
+    if (by_k) {
+      bins.find(s.count, s.mass, s.found[0], true, ask.top_k);
+      __syncthreads();
+      k_bin = s.found[0].bin;
+      low = s.found[0].before_mass + 1;
+      high = s.found[0].before_mass + s.found[0].mass;
+    }
+    if (ask.cuts()) {
+      bins.find(s.count, s.mass, s.found[1], false, ask.cut(low));
+      bins.find(s.count, s.mass, s.found[2], false, ask.cut(high));
+      __syncthreads();
+      p_first = s.found[1].bin;
+      p_last = s.found[2].bin;
+      low = ask.cut(low);
+      const uint64_t to = s.found[2].before_mass + s.found[2].mass;
+      high = to < high ? to : high;
+    }
+    bins.find(s.count, s.mass, s.found[3], false, ask.draw(low));
+    bins.find(s.count, s.mass, s.found[4], false, ask.draw(high));
+    if (threadIdx.x == 0) s.n = 0u;
+    __syncthreads();
+    const uint32_t d_first = s.found[3].bin, d_last = s.found[4].bin;
+    row.span(int(d_first), int(d_last), lo[0], hi[0]);
+    row.span(int(ask.cuts() ? p_first : d_first), int(ask.cuts() ? p_last : d_last), lo[1], hi[1]);
+    row.span(int(by_k ? k_bin : d_first), int(by_k ? k_bin : d_last), lo[2], hi[2]);
+    lowest = fminf(fminf(lo[0], lo[1]), lo[2]);
+  }
+  // A token of the row into s.cand, if it is one of them; their number in s.n.
+  template <class F>
+  __device__ __forceinline__ void gather(Shared& s, float z, F&& order) const {
+    if (!(z >= lowest)) return;  // most tokens
+    bool in = (z >= lo[0] && z <= hi[0]) || (z >= lo[1] && z <= hi[1]);
+    if (by_k) in = in || (z >= lo[2] && z <= hi[2]);  // uniform
+    if (!in) return;
+    const uint32_t at = atomicAdd(&s.n, 1u);
+    if (at < kList) s.cand[at] = order();
+  }
+  // The answers, from the n tokens gathered (from the row where they are too many).
+  __device__ __forceinline__ void answer(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, const SampleArgs& a,
+                                         int out) const {
+    uint64_t kept = bins.total_mass;
+    for (int question = by_k ? 0 : 1; question < 3; ++question) {
+      if (question == 1 && !ask.cuts()) continue;
+      const uint64_t goal = question == 0 ? ask.top_k : question == 1 ? ask.cut(kept) : ask.draw(kept);
+      __syncthreads();
+      bins.find(s.count, s.mass, s.found[question], question == 0, goal);
+      __syncthreads();
+      narrow(s, row, s.found[question], question == 0, goal, n);
+      if (question < 2) kept = s.mass_to;
+    }
+    if (threadIdx.x == 0) {
+      a.tokens[out] = s.token;
+      if (a.probs) a.probs[out] = float(double(s.weight) / double(kept));
+    }
+  }
+};
+__device__ __forceinline__ Questions questions(const SampleArgs& a, const Settings& set, int row) {
+  return {set.top_k > 0 ? uint64_t(set.top_k) : 0u, a.top_ps ? a.top_ps[row] : a.top_p, a.u[row]};
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void sample_draw(SampleArgs a) {
   __shared__ Shared s;
   const int t = int(threadIdx.x), part = int(blockIdx.x), parts = int(gridDim.x), row = int(blockIdx.y);
   RowState& rs = a.rows[row];
@@ -631,14 +712,12 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
   for (int i = 0; i < kBins / kThreads; ++i) counts[i] = rs.count[i * kThreads + t], masses[i] = rs.mass[i * kThreads + t];
   const uint32_t listed_here = rs.n_list[t & (kMaxSlices - 1)];  // lane i: of slice i (not written where nothing is listed)
   Settings set;
-  if (!set.derive(a, row)) {  // uniform: an empty row, or the first of the order
-    if (t == 0 && part == 0) {
-      a.tokens[row] = set.best ? order_index(set.best) : -1;
-      if (a.probs) a.probs[row] = set.best ? 1.0f : 0.0f;
-    }
+  set.groups = a.slices * kGroups;
+  if (!set.derive(a, row, wave_max64((t & 63) < a.slices ? rs.best[t & 63] : 0u))) {  // uniform
+    if (t == 0 && part == 0) set.trivial(a, row);
     return;
   }
-  const Questions ask{set.top_k > 0 ? uint64_t(set.top_k) : 0u, a.top_ps ? a.top_ps[row] : a.top_p, a.u[row]};
+  const Questions ask = questions(a, set, row);
   set.weigh.constants();
   Row<DT> r{a.logits + int64_t(row) * a.row_bytes, a.vocab, set.weigh};
   // Every token that may be kept is listed, unless there are too many.
@@ -660,66 +739,23 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
     answer_from(s, r, ask, n_listed, a, row);
     return;
   }
-  set.load_groups(a, row);
-  set.raise_floor(a);
-  const Weigher weigh = r.weigh = set.weigh;
+  set.load_groups(a, rs.group_max, a.slices * kGroups);
+  set.raise_floor();
+  r.weigh.floor = set.weigh.floor;
 #pragma unroll
   for (int i = 0; i < kBins / kThreads; ++i) s.count[i * kThreads + t] = counts[i], s.mass[i * kThreads + t] = masses[i];
   __syncthreads();
-  const Bins<kBins / kThreads> bins(s, s.count, s.mass, 0u, 0u);
-  // The bins that the answers lie in: a question's goal is known within the
-  // mass of the bin that the one before it ends in.
-  uint64_t low = bins.total_mass, high = low;  // bounds of the mass kept
-  const bool by_k = ask.top_k > 0 && ask.top_k < bins.total_count;  // counts are there with top-k alone
-  uint32_t k_bin = kBins, p_first = kBins, p_last = 0u;
-  if (by_k) {
-    bins.find(s.count, s.mass, s.found[0], true, ask.top_k);
-    __syncthreads();
-    k_bin = s.found[0].bin;
-    low = s.found[0].before_mass + 1;
-    high = s.found[0].before_mass + s.found[0].mass;
-  }
-  if (ask.cuts()) {
-    bins.find(s.count, s.mass, s.found[1], false, ask.cut(low));
-    bins.find(s.count, s.mass, s.found[2], false, ask.cut(high));
-    __syncthreads();
-    p_first = s.found[1].bin;
-    p_last = s.found[2].bin;
-    low = ask.cut(low);
-    const uint64_t to = s.found[2].before_mass + s.found[2].mass;
-    high = to < high ? to : high;
-  }
-  bins.find(s.count, s.mass, s.found[3], false, ask.draw(low));
-  bins.find(s.count, s.mass, s.found[4], false, ask.draw(high));
-  __syncthreads();
-  const uint32_t d_first = s.found[3].bin, d_last = s.found[4].bin;
-  if (t == 0) s.n = 0u;
-  __syncthreads();
-  // A row's workgroups have all come here alike; each gathers its part of the
-  // tokens in the z of those bins.
-  const int shares = from_list ? 1 : parts;
-  float lo[3], hi[3];
-  r.span(int(d_first), int(d_last), lo[0], hi[0]);
-  r.span(int(ask.cuts() ? p_first : d_first), int(ask.cuts() ? p_last : d_last), lo[1], hi[1]);
-  r.span(int(by_k ? k_bin : d_first), int(by_k ? k_bin : d_last), lo[2], hi[2]);
-  const float lowest = fminf(fminf(lo[0], lo[1]), lo[2]);
-  const auto gather = [&](float z, auto&& order) {
-    if (!(z >= lowest)) return;  // most tokens
-    bool in = (z >= lo[0] && z <= hi[0]) || (z >= lo[1] && z <= hi[1]);
-    if (by_k) in = in || (z >= lo[2] && z <= hi[2]);  // uniform
-    if (!in) return;
-    const uint32_t at = atomicAdd(&s.n, 1u);
-    if (at < kList) s.cand[at] = order();
-  };
+  const Plan<DT> plan(s, r, ask);
+  // A row's workgroups have all come here alike; each gathers its part.
   if (from_list) {
-    each_listed([&](uint64_t o, uint32_t) { gather(order_value(o), [&] { return o; }); });
+    each_listed([&](uint64_t o, uint32_t) { plan.gather(s, order_value(o), [&] { return o; }); });
   } else {
     Walk<DT, kThreads, 4> walk(r.data, a.vocab, part, parts);
-    walk.each([&](int i, float z) { gather(z, [&] { return order_of(z, i); }); });
+    walk.each([&](int i, float z) { plan.gather(s, z, [&] { return order_of(z, i); }); });
   }
   __syncthreads();
   uint32_t n = s.n;
-  if (shares > 1) {
+  if (parts > 1 && !from_list) {
     // The row's last workgroup answers, from what all of them gathered.  What
     // passes between them goes through device-scope atomics, which meet behind the
     // XCDs' caches: each wave waits for its own to be acknowledged before the
@@ -735,27 +771,81 @@ __global__ __launch_bounds__(kThreads, 4) void sample_draw(SampleArgs a) {
     __syncthreads();
     if (t == 0) s.base = atomicAdd(&rs.ticket, 1u);
     __syncthreads();
-    if (s.base != uint32_t(shares - 1)) return;  // uniform
+    if (s.base != uint32_t(parts - 1)) return;  // uniform
     n = __hip_atomic_load(&rs.n_gathered, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (n <= kList)
       for (uint32_t i = t; i < n; i += kThreads)
         s.cand[i] = __hip_atomic_load(&rs.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  uint64_t kept = bins.total_mass;
-  for (int question = by_k ? 0 : 1; question < 3; ++question) {
-    if (question == 1 && !ask.cuts()) continue;
-    const uint64_t goal = question == 0 ? ask.top_k : question == 1 ? ask.cut(kept) : ask.draw(kept);
-    __syncthreads();
-    bins.find(s.count, s.mass, s.found[question], question == 0, goal);
-    __syncthreads();
-    narrow(s, r, s.found[question], question == 0, goal, n);
-    if (question < 2) kept = s.mass_to;
-  }
-  if (t == 0) {
-    a.tokens[row] = s.token;
-    if (a.probs) a.probs[row] = float(double(s.weight) / double(kept));
-  }
+  plan.answer(s, r, ask, n, a, row);
 }
+
+// All three launches' work by one workgroup per row, whose bins and list stay in
+// its LDS: for rows that one CU weighs in the time that two more launches would
+// take, and for batches that fill the device so (see row_per_workgroup).
+template <int DT>
+__global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
+  __shared__ Shared s;
+  __shared__ uint32_t maxima[kRowGroups];
+  const int t = int(threadIdx.x), lane = t & 63, row = int(blockIdx.x);
+  const char* const data = a.logits + int64_t(row) * a.row_bytes;
+  float top = -INFINITY;
+  int at = -1;
+  {
+    Walk<DT, kThreads, 4> walk(data, a.vocab, 0, 1);
+    for (int b = t; b < kBins; b += kThreads) s.count[b] = 0u, s.mass[b] = 0u;
+    walk.each([&](int i, float z) {
+      if (z > top) top = z, at = i;  // of equals the first
+    });
+  }
+  // Groups of eight lanes; of two where many threads may have no tokens.
+  const int log2_lanes = a.vocab >= 8 * kThreads ? 3 : 1;
+  uint32_t group = order_key(top);
+  for (int o = 1 << log2_lanes >> 1; o; o >>= 1) group = max(group, uint32_t(__shfl_xor(int(group), o)));
+  if ((lane & ((1 << log2_lanes) - 1)) == 0) maxima[t >> log2_lanes] = group;
+  const uint64_t best = wave_max64(at < 0 ? 0u : order_of(top, at));
+  if (lane == 0) s.wave_mass[t >> 6] = best;
+  if (t == 0) s.n = 0u;
+  __syncthreads();
+  Settings set;
+  set.load_groups(a, maxima, kThreads >> log2_lanes);
+  if (!set.derive(a, row, wave_max64(lane < kWaves ? s.wave_mass[lane] : 0u))) {  // uniform
+    if (t == 0) set.trivial(a, row);
+    return;
+  }
+  set.raise_floor();
+  set.weigh.constants();
+  const Questions ask = questions(a, set, row);
+  const Row<DT> r{data, a.vocab, set.weigh};
+  {
+    Walk<DT, kThreads, 4> walk(data, a.vocab, 0, 1);  // from the XCD's L2
+    walk.each([&](int i, float z) { weigh_token(set, z, i, s.mass, s.count, s.cand, &s.n, kList); });
+  }
+  __syncthreads();
+  const uint32_t n_listed = s.n;
+  if (set.listed && n_listed <= kFew) {
+    answer_from(s, r, ask, n_listed, a, row);
+    return;
+  }
+  __syncthreads();
+  const Plan<DT> plan(s, r, ask);
+  uint32_t n = n_listed;  // a list holds all that can be asked for
+  if (!set.listed || n_listed > kList) {
+    Walk<DT, kThreads, 4> walk(data, a.vocab, 0, 1);
+    walk.each([&](int i, float z) { plan.gather(s, z, [&] { return order_of(z, i); }); });
+    __syncthreads();
+    n = s.n;
+  }
+  plan.answer(s, r, ask, n, a, row);
+}
+
+// One launch of a workgroup per row, or three of many per row.  us, f32, T 1 whole
+// / top-k 50 and top-p 0.95 / top-p 0.9, one launch then three: 1 x 4096 12.2 /
+// 12.0 / 14.3 and 17.4 / 22.5 / 19.5; 1 x 32768 21.7 / 12.3 / 25.6 and 19.2 / 15.9 /
+// 22.5; 64 x 65536 46.1 / 16.8 / 38.7 and 35.9 / 25.5 / 34.3; 128 x 65536 46.6 /
+// 17.6 / 39.3 and 44.4 / 27.4 / 41.7; 128 x 100000 66.6 / 26.8 / 59.0 and 55.1 /
+// 33.5 / 53.2; 256 x 131072, a row for each CU, 94 / 45 / 84 and 104 / 63 / 95.
+bool row_per_workgroup(int32_t rows, int32_t vocab) { return vocab <= 32768 || vocab <= 512 * int64_t(rows); }
 
 // Slices of a row in the first two launches: of 2048 tokens or more, as many as
 // are resident at once (four workgroups on each of 256 CUs).  The result does not
@@ -768,12 +858,16 @@ int slice_count(int32_t rows, int32_t vocab) {
 }
 // Workgroups of a row in the third: of 8192 tokens or more, 512 in all.
 int part_count(int32_t rows, int32_t vocab) {
-  const int p = (vocab + 8191) / 8192, fill = 512 / rows > 0 ? 512 / rows : 1;
+  const int p = (vocab + 8191) / 8192, fill = 256 / rows > 0 ? 256 / rows : 1;
   return p < fill ? p : fill;
 }
 
 template <int DT>
 void launch_sample(const SampleArgs& a, int32_t rows, hipStream_t s) {
+  if (row_per_workgroup(rows, a.vocab)) {
+    hipLaunchKernelGGL(sample_row<DT>, dim3(unsigned(rows)), dim3(kThreads), 0, s, a);
+    return;
+  }
   const dim3 grid(unsigned(a.slices), unsigned(rows));
   hipLaunchKernelGGL(sample_maxima<DT>, grid, dim3(kSliceThreads), 0, s, a);
   hipLaunchKernelGGL(sample_weigh<DT>, grid, dim3(kSliceThreads), 0, s, a);
@@ -783,7 +877,7 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 }  // namespace
 
 extern "C" size_t it_sample_workspace(int32_t n_rows, int32_t vocab) {
-  return n_rows > 0 && vocab > 0 ? size_t(n_rows) * sizeof(RowState) : 0;
+  return n_rows > 0 && vocab > 0 && !row_per_workgroup(n_rows, vocab) ? size_t(n_rows) * sizeof(RowState) : 0;
 }
 
 extern "C" int32_t it_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t n_rows, int32_t vocab, const float* u,
@@ -805,9 +899,9 @@ extern "C" int32_t it_sample(const void* logits, int32_t dtype, int64_t row_stri
   if (!logits || !u || !tokens) return fail(IT_INVALID_INPUT, "%s: NULL tensor", who);
   const int64_t es = dtype_bytes(dtype);
   if (!aligned(logits, uintptr_t(es))) return fail(IT_INVALID_INPUT, "%s: logits must be aligned to their elements", who);
-  if (!ws || ws_bytes < it_sample_workspace(n_rows, vocab) || !aligned(ws, 256))
-    return fail(IT_INVALID_INPUT, "%s: workspace of %zu bytes, %zu needed, 256-byte aligned", who, ws ? ws_bytes : size_t(0),
-                it_sample_workspace(n_rows, vocab));
+  const size_t need = it_sample_workspace(n_rows, vocab);
+  if (need && (!ws || ws_bytes < need || !aligned(ws, 256)))
+    return fail(IT_INVALID_INPUT, "%s: workspace of %zu bytes, %zu needed, 256-byte aligned", who, ws ? ws_bytes : size_t(0), need);
   SampleArgs a{};
   a.logits = static_cast<const char*>(logits);
   a.row_bytes = (n_rows > 1 ? row_stride : int64_t(vocab)) * es;

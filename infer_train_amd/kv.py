@@ -89,10 +89,11 @@ def _rows(t: torch.Tensor, name: str) -> Tuple[int, int]:
         raise ValueError("device tensor expected")
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim]")
-    s = t.stride()
-    if (s[2] != 1 and t.shape[2] != 1) or (s[1] != t.shape[2] and t.shape[1] != 1):
+    token, head, element = t.stride()
+    _, heads, dim = t.shape
+    if (head != dim and heads != 1) or (element != 1 and dim != 1):
         raise ValueError(f"{name}: each token's heads must be contiguous")
-    return t.data_ptr(), s[0]
+    return t.data_ptr(), token
 
 
 class Rotary:
@@ -136,7 +137,7 @@ class Rotary:
         if positions.dtype != torch.int32 or positions.numel() != n:
             raise TypeError("positions must be int32, one per token")
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         elif out.dtype != x.dtype or out.shape != x.shape:
             raise TypeError("out must have x's shape and dtype")
         to, to_stride = _rows(out, "out")
@@ -308,28 +309,31 @@ class PagedKvCache:
         q None: k and v only."""
         if slot_mapping.dtype != torch.int64 or positions.dtype != torch.int32:
             raise TypeError("slot_mapping must be int64 and positions int32")
-        n = slot_mapping.numel()
+        n, kind = slot_mapping.numel(), k.dtype
         row = (n, self.n_kv_heads, self.head_dim)
         if positions.numel() != n or k.shape != row or v.shape != row:
             raise ValueError("k, v must be [n_tokens, n_kv_heads, head_dim], with a slot and a position per token")
-        if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype):
+        if v.dtype != kind or (q is not None and q.dtype != kind):
             raise TypeError("q, k, v must have one dtype")
         (ka, ks), (va, vs) = _rows(k, "k"), _rows(v, "v")
+        src_id = torch_dtype_id(kind)
         qa = oa = None
         qs = heads = out_id = 0
         if q is not None:
-            if q.shape[0] != n or q.shape[-1] != self.head_dim:
-                raise ValueError("q must be [n_tokens, n_heads, head_dim]")
             qa, qs = _rows(q, "q")
             heads = q.shape[1]
+            if q.shape != (n, heads, row[2]):
+                raise ValueError("q must be [n_tokens, n_heads, head_dim]")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q_out_dtype or q.dtype, device=q.device)
+                q_out = torch.empty_like(q, dtype=q_out_dtype, memory_format=torch.contiguous_format)
+                oa, out_id = q_out.data_ptr(), src_id if q_out_dtype is None else torch_dtype_id(q_out_dtype)
             elif q_out.shape != q.shape:
                 raise ValueError("q_out must have q's shape")
-            oa, out_id = _ptr(q_out), torch_dtype_id(q_out.dtype)
+            else:
+                oa, out_id = _ptr(q_out), torch_dtype_id(q_out.dtype)
         elif q_out is not None:
             raise ValueError("q_out without q")
-        _check(call.it_kv_append_rotary(self._at, rotary._at, qa, ka, va, torch_dtype_id(k.dtype), qs, ks, vs, heads,
+        _check(call.it_kv_append_rotary(self._at, rotary._at, qa, ka, va, src_id, qs, ks, vs, heads,
                                         _ptr(slot_mapping), _ptr(positions), n, oa, out_id, _raw_stream(self._index)))
         return q_out
 

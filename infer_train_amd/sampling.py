@@ -14,8 +14,15 @@ __all__ = ["sample", "sample_workspace"]
 
 
 def sample_workspace(n_rows: int, vocab: int, device) -> torch.Tensor:
-    """A workspace for `sample` (calls that overlap in time need one each)."""
+    """A workspace for `sample` (calls that overlap in time need one each);
+    empty for short rows and large batches, which need none."""
     return torch.empty(call.it_sample_workspace(n_rows, vocab), dtype=torch.uint8, device=device)
+
+
+def _per_row(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> int:
+    if t.dtype != dtype or t.numel() != n:
+        raise TypeError(f"{name} must be {dtype}, one per row")
+    return _ptr(t)
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torch.Tensor] = 1.0,
@@ -32,33 +39,31 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     if not logits.is_cuda:
         raise ValueError("device tensor expected")
     n, vocab = logits.shape
-    arrays, numbers = [], []
-    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if isinstance(x, torch.Tensor):
-            if x.dtype != dtype or x.numel() != n:
-                raise TypeError(f"{name} must be {dtype}, one per row")
-            arrays.append(_ptr(x))
-            numbers.append(0)
-        else:
-            arrays.append(None)
-            numbers.append(x)
-    if u.dtype != torch.float32 or u.numel() != n:
-        raise TypeError("u must be float32, one per row")
+    temperatures = top_ks = top_ps = min_ps = None
+    if isinstance(temperature, torch.Tensor):
+        temperatures, temperature = _per_row(temperature, "temperature", torch.float32, n), 1.0
+    if isinstance(top_k, torch.Tensor):
+        top_ks, top_k = _per_row(top_k, "top_k", torch.int32, n), 0
+    if isinstance(top_p, torch.Tensor):
+        top_ps, top_p = _per_row(top_p, "top_p", torch.float32, n), 1.0
+    if isinstance(min_p, torch.Tensor):
+        min_ps, min_p = _per_row(min_p, "min_p", torch.float32, n), 0.0
+    us = _per_row(u, "u", torch.float32, n)
     if tokens is None:
-        tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
-    elif tokens.dtype != torch.int32 or tokens.numel() != n:
-        raise TypeError("tokens must be int32, one per row")
+        tokens = torch.empty_like(u, dtype=torch.int32)
     if probs is None:
-        probs = torch.empty(n, dtype=torch.float32, device=logits.device)
-    elif probs.dtype != torch.float32 or probs.numel() != n:
-        raise TypeError("probs must be float32, one per row")
+        probs = torch.empty_like(u)
+    need = 0
     if ws is None:
-        ws = sample_workspace(n, vocab, logits.device)
+        need = call.it_sample_workspace(n, vocab)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    else:
+        need = ws.nbytes
     index = logits.device.index
-    args = (logits.data_ptr(), torch_dtype_id(logits.dtype), logits.stride(0), n, vocab, _ptr(u), *arrays,
-            float(numbers[0]), int(numbers[1]), float(numbers[2]), float(numbers[3]), _ptr(tokens), _ptr(probs), _ptr(ws),
-            ws.numel() * ws.element_size(), _raw_stream(index))
+    args = (logits.data_ptr(), torch_dtype_id(logits.dtype), logits.stride(0), n, vocab, us, temperatures, top_ks, top_ps, min_ps,
+            float(temperature), int(top_k), float(top_p), float(min_p), _per_row(tokens, "tokens", torch.int32, n),
+            _per_row(probs, "probs", torch.float32, n), _ptr(ws), need, _raw_stream(index))
     if torch.cuda.current_device() == index:
         _check(call.it_sample(*args))
     else:

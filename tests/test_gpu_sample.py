@@ -66,7 +66,7 @@ def logits(seed, rows, vocab, scale=2.5):
 
 
 @pytest.mark.parametrize("dtype", ("float32", "float16", "bfloat16"))
-@pytest.mark.parametrize("vocab", (1, 2, 7, 63, 64, 65, 513, 4096, 4097, 32000, 100003, 262144))
+@pytest.mark.parametrize("vocab", (1, 2, 7, 63, 64, 65, 513, 4096, 4097, 32768, 32769, 100003, 262144))
 def test_settings(vocab, dtype):
     """Every setting alone and together, rows of odd lengths (each starts at another alignment)."""
     import torch
@@ -79,12 +79,13 @@ def test_settings(vocab, dtype):
 
 @pytest.mark.parametrize("u", (0.0, 2.0 ** -24, 0.5, 1 - 2.0 ** -24, 1.0, 7.0, -1.0, math.nan))
 def test_uniform_numbers(u):
-    z = logits(1, 4, 5000)
-    run(z, [u] * 4)
-    run(z, [u] * 4, t=0.9, k=30, p=0.9, m=0.01)
+    for vocab in (5000, 50000):
+        z = logits(1, 4, vocab)
+        run(z, [u] * 4)
+        run(z, [u] * 4, t=0.9, k=30, p=0.9, m=0.01)
 
 
-@pytest.mark.parametrize("vocab", (3, 500, 70000))
+@pytest.mark.parametrize("vocab", (3, 500, 20000, 70000))
 def test_equal_tokens(vocab):
     """All tokens equal, or two values: the lower token first, at the borders of every filter, past what is listed."""
     same = np.full((6, vocab), 1.25, np.float32)
@@ -100,17 +101,18 @@ def test_equal_tokens(vocab):
     assert run(zero, [0.0] * 6, k=1)[0].tolist() == [0] * 6  # -0 equals +0
 
 
-def test_masked_rows():
+@pytest.mark.parametrize("vocab", (9001, 33001))
+def test_masked_rows(vocab):
     """Rows with -inf, the type's lowest value, NaN, +inf, and nothing left."""
     import torch
 
     rng = np.random.default_rng(3)
     for dtype in (torch.float32, torch.float16, torch.bfloat16):
-        z = torch.from_numpy(logits(4, 12, 9001)).cuda().to(dtype)
+        z = torch.from_numpy(logits(4, 12, vocab)).cuda().to(dtype)
         z[0, 1:] = -math.inf
         z[1] = -math.inf
-        z[2, rng.random(9001) < 0.9] = -math.inf
-        z[3, rng.random(9001) < 0.9] = torch.finfo(dtype).min
+        z[2, rng.random(vocab) < 0.9] = -math.inf
+        z[3, rng.random(vocab) < 0.9] = torch.finfo(dtype).min
         z[4] = torch.finfo(dtype).min
         z[5] = math.nan
         z[6, ::2] = math.nan
@@ -118,36 +120,38 @@ def test_masked_rows():
         z[8] = math.inf
         z[9, 10:] = -math.inf
         z[10] = torch.finfo(dtype).max
-        z[11, :8999] = -math.inf
+        z[11, :vocab - 2] = -math.inf
         u = rng.random(12)
         for kw in (dict(), dict(t=0.0), dict(k=20), dict(p=0.8), dict(m=0.1), dict(t=0.5, k=1500, p=0.95, m=0.001)):
             tokens, probs = run(z, u, **kw)
             assert tokens[1] == -1 and probs[1] == 0 and tokens[5] == -1 and tokens[0] == 0
 
 
-def test_extreme_settings():
-    z = logits(5, 8, 3001)
+@pytest.mark.parametrize("vocab", (3001, 40001))
+def test_extreme_settings(vocab):
+    z = logits(5, 8, vocab)
     u = np.random.default_rng(6).random(8)
     run(z, u, t=np.array([1e-30, 1e-6, 1e30, math.inf, 1e-45, -1.0, math.nan, 100.0]))
     run(z, u, p=np.array([0.0, -1.0, 1e-9, 1e-45, 0.5, 1.0, 2.0, math.nan]))
     run(z, u, m=np.array([0.0, -1.0, 1e-30, 1.0, 5.0, 1e-9, 0.999, math.nan]))
-    run(z, u, k=np.array([0, -3, 1, 3000, 3001, 3002, 2 ** 31 - 1, -2 ** 31]))
-    tiny = np.full((2, 4000), 1e-40, np.float32)
+    run(z, u, k=np.array([0, -3, 1, vocab - 1, vocab, vocab + 1, 2 ** 31 - 1, -2 ** 31]))
+    tiny = np.full((2, vocab), 1e-40, np.float32)
     tiny[:, 7] = 2e-40
     run(tiny, [0.3, 0.9])
     run(tiny * 1e38, [0.3, 0.9], t=1e-3, k=300)
-    wide = np.linspace(-3e38, 3e38, 5000, dtype=np.float32)[None]
+    wide = np.linspace(-3e38, 3e38, vocab, dtype=np.float32)[None]
     run(wide, [0.4])
     run(wide, [0.4], t=np.array([1e38]))
 
 
-@pytest.mark.parametrize("stride,offset", ((5003, 0), (5003, 3), (5008, 1), (6000, 0)))
-def test_row_strides(stride, offset):
+@pytest.mark.parametrize("vocab,stride,offset", ((5003, 5003, 0), (5003, 5003, 3), (5003, 5008, 1), (5003, 6000, 0),
+                                                 (33333, 33333, 5), (33333, 40000, 2)))
+def test_row_strides(vocab, stride, offset):
     import torch
 
     base = torch.from_numpy(logits(7, 1, offset + 9 * stride)[0]).cuda()
     for dtype in (torch.float32, torch.bfloat16):
-        z = base.to(dtype)[offset:].as_strided((9, 5003), (stride, 1), offset)
+        z = base.to(dtype)[offset:].as_strided((9, vocab), (stride, 1), offset)
         run(z, np.linspace(0.05, 0.95, 9), t=0.9, p=0.9)
     one = torch.from_numpy(logits(8, 700, 1)).cuda().t()  # [1, 700], any row stride
     run(one, [0.5])
@@ -155,19 +159,21 @@ def test_row_strides(stride, offset):
 
 @pytest.mark.parametrize("kw", (dict(), dict(k=60), dict(p=0.92), dict(t=0.6, k=400, p=0.9, m=0.003)))
 def test_a_row_does_not_depend_on_its_batch(kw):
-    """Batches of 1 to 3000 rows divide a row among 9 to 1 workgroups: the same token and the same bits."""
+    """One row is divided among many workgroups, 5 and 40 rows likewise, 3000 take one each: the same token and the same
+    bits."""
     import torch
     from infer_train_amd.sampling import sample
 
-    z, u = torch.from_numpy(logits(9, 5, 33333)).cuda(), torch.rand(5, generator=torch.Generator().manual_seed(1)).cuda()
+    z, u = torch.from_numpy(logits(9, 5, 70001)).cuda(), torch.rand(5, generator=torch.Generator().manual_seed(1)).cuda()
     names = dict(t="temperature", k="top_k", p="top_p", m="min_p")
     kw = {names[a]: b for a, b in kw.items()}
     tokens, probs = sample(z, u, **kw)
     for r in range(5):
         a, b = sample(z[r:r + 1], u[r:r + 1], **kw)
         assert a[0] == tokens[r] and b[0] == probs[r]
-    a, b = sample(z.repeat(600, 1), u.repeat(600), **kw)
-    assert torch.equal(a, tokens.repeat(600)) and torch.equal(b, probs.repeat(600))
+    for n in (8, 600):
+        a, b = sample(z.repeat(n, 1), u.repeat(n), **kw)
+        assert torch.equal(a, tokens.repeat(n)) and torch.equal(b, probs.repeat(n))
 
 
 def test_distribution():
@@ -190,9 +196,9 @@ def test_captured_with_a_shared_and_a_dirty_workspace():
     import torch
     from infer_train_amd.sampling import sample, sample_workspace
 
-    z, u = torch.from_numpy(logits(11, 6, 20011)).cuda(), torch.rand(6).cuda()
-    z2, u2 = torch.from_numpy(logits(12, 3, 5000)).cuda().half(), torch.rand(3).cuda()
-    ws = sample_workspace(6, 20011, z.device)
+    z, u = torch.from_numpy(logits(11, 6, 40011)).cuda(), torch.rand(6).cuda()
+    z2, u2 = torch.from_numpy(logits(12, 3, 50000)).cuda().half(), torch.rand(3).cuda()
+    ws = sample_workspace(6, 40011, z.device)
     ws.fill_(0xA5)
     want = sample(z, u, top_p=0.9)
     got = sample(z, u, top_p=0.9, ws=ws)
@@ -204,8 +210,8 @@ def test_captured_with_a_shared_and_a_dirty_workspace():
     with torch.cuda.graph(graphs[1]):
         sample(z2, u2, temperature=0.8, top_k=30, tokens=out2[0], probs=out2[1], ws=ws)
     for i in range(4):
-        z.copy_(torch.from_numpy(logits(20 + i, 6, 20011)))
-        z2.copy_(torch.from_numpy(logits(30 + i, 3, 5000)))
+        z.copy_(torch.from_numpy(logits(20 + i, 6, 40011)))
+        z2.copy_(torch.from_numpy(logits(30 + i, 3, 50000)))
         u.copy_(torch.rand(6))
         graphs[0].replay()
         graphs[1].replay()
@@ -239,9 +245,11 @@ def test_sample_refusals():
 
     z, u = torch.zeros(3, 50, device="cuda"), torch.zeros(3, device="cuda")
     for bad in (dict(temperature=-1.0), dict(temperature=math.inf), dict(top_p=math.nan), dict(min_p=2.0),
-                dict(ws=torch.zeros(16, dtype=torch.uint8, device="cuda"))):
+                ):
         with pytest.raises(InvalidInput):
             sample(z, u, **bad)
+    with pytest.raises(InvalidInput):
+        sample(torch.zeros(3, 40000, device="cuda"), u, ws=torch.zeros(16, dtype=torch.uint8, device="cuda"))
     with pytest.raises(NotImplementedOp):
         sample(torch.zeros(1, 262145, device="cuda"), u[:1])
     for bad in (dict(temperature=u.double()), dict(top_k=u), dict(min_p=u[:2]), dict(tokens=u), dict(probs=u.int())):

@@ -80,12 +80,12 @@ def test_supports():
 
 
 def test_sample_refusals():
-    need = L.lib.it_sample_workspace(2, 100)
-    assert need > 0 and L.lib.it_sample_workspace(0, 100) == 0
-    ok = dict(logits=SOME, dtype=L.F32, stride=100, rows=2, vocab=100, u=SOME, temps=None, ks=None, ps=None, ms=None, temp=1.0,
+    need = L.lib.it_sample_workspace(2, 40000)
+    assert need > 0 and L.lib.it_sample_workspace(0, 40000) == 0 == L.lib.it_sample_workspace(2, 32768)
+    ok = dict(logits=SOME, dtype=L.F32, stride=40000, rows=2, vocab=40000, u=SOME, temps=None, ks=None, ps=None, ms=None, temp=1.0,
               k=0, p=1.0, m=0.0, tokens=SOME, probs=None, ws=SOME, ws_bytes=need, stream=None)
     call = lambda **kw: L.lib.it_sample(*{**ok, **kw}.values())  # noqa: E731
-    for kw in (dict(rows=-1), dict(rows=65536), dict(vocab=0), dict(vocab=-5), dict(stride=99), dict(temp=-1.0), dict(temp=math.nan),
+    for kw in (dict(rows=-1), dict(rows=65536), dict(vocab=0), dict(vocab=-5), dict(stride=39999), dict(temp=-1.0), dict(temp=math.nan),
                dict(temp=math.inf), dict(p=math.nan), dict(m=1.5), dict(m=math.nan), dict(logits=None), dict(u=None),
                dict(tokens=None), dict(logits=SOME + 2), dict(ws=None), dict(ws_bytes=need - 1), dict(ws=SOME + 16)):
         assert call(**kw) == L.INVALID_INPUT, kw
