@@ -134,9 +134,11 @@ struct Weigher {
 
 // The tokens of a slice of a row: its share of the 16-byte vectors of the row's
 // aligned part, the first slice also the tokens before that part, the last those
-// behind it.  The first vectors are loaded when the walk is made, so that what
-// a kernel does before each() runs in their shadow.
-template <int DT, int kBlock, int U>
+// behind it.  Each thread's next vector is loaded while one is worked on, its
+// first when the walk is made, in the shadow of what a kernel does before each().
+// (Batches of four vectors per thread keep more loads in flight, but unroll what is
+// done with a token 16 or 32 times: small calls then wait for instructions.)
+template <int DT, int kBlock>
 struct Walk {
   static constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es;
   using In = RowVec<DT, V>;
@@ -144,7 +146,7 @@ struct Walk {
   const typename In::raw* v;
   int vocab, head, done, lo, hi;
   bool first, last;
-  typename In::raw w[U];
+  typename In::raw next;
   __device__ __forceinline__ Walk(const char* row_, int vocab_, int slice, int slices) : row(row_), vocab(vocab_) {
     head = min(vocab, int((16 - (reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / es);
     const int vecs = (vocab - head) / V, per = (vecs + slices - 1) / slices;
@@ -154,28 +156,21 @@ struct Walk {
     first = slice == 0;
     last = slice == slices - 1;
     v = reinterpret_cast<const typename In::raw*>(row + head * es);
-    if (lo < hi) load(lo + int(threadIdx.x));
+    if (lo + int(threadIdx.x) < hi) next = v[lo + int(threadIdx.x)];
   }
-  __device__ __forceinline__ void load(int x0) {
-#pragma unroll
-    for (int j = 0; j < U; ++j) w[j] = v[min(x0 + j * kBlock, hi - 1)];
-  }
-  // f(index, z); a thread's tokens come in ascending order.
+  // f(index, z); a thread's tokens come in ascending order.  Once.
   template <class F>
   __device__ __forceinline__ void each(F&& f) {
     const int tid = int(threadIdx.x);
     if (first && tid < head) f(tid, load_element(row, tid, DT));
-    for (int x0 = lo + tid; x0 < hi; x0 += kBlock * U) {
-      if (x0 != lo + tid) load(x0);
+#pragma unroll 1
+    for (int x = lo + tid; x < hi; x += kBlock) {
+      const typename In::raw w = next;
+      if (x + kBlock < hi) next = v[x + kBlock];
+      float z[V];
+      In::widen(w, z);
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int x = x0 + j * kBlock;
-        if (x >= hi) break;
-        float z[V];
-        In::widen(w[j], z);
-#pragma unroll
-        for (int e = 0; e < V; ++e) f(head + x * V + e, z[e]);
-      }
+      for (int e = 0; e < V; ++e) f(head + x * V + e, z[e]);
     }
     if (last && tid < vocab - done) f(done + tid, load_element(row, done + tid, DT));
   }
@@ -210,7 +205,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
   for (int b = slice * kSliceThreads + int(threadIdx.x); b < kBins; b += a.slices * kSliceThreads) rs.count[b] = 0u, rs.mass[b] = 0u;
   float top = -INFINITY;
   int at = -1;
-  Walk<DT, kSliceThreads, 4> walk(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices);
+  Walk<DT, kSliceThreads> walk(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices);
   walk.each([&](int i, float z) {
     if (z > top) top = z, at = i;  // of equals the first
   });
@@ -316,7 +311,7 @@ __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
   __shared__ uint32_t count[kBins], n;
   const int t = int(threadIdx.x), slice = int(blockIdx.x), row = int(blockIdx.y);
   RowState& rs = a.rows[row];
-  Walk<DT, kSliceThreads, 4> walk(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices);
+  Walk<DT, kSliceThreads> walk(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices);
   Settings set;
   set.load_groups(a, rs.group_max, a.slices * kGroups);
   if (!set.derive(a, row, wave_max64((t & 63) < a.slices ? rs.best[t & 63] : 0u))) return;
@@ -434,7 +429,7 @@ struct Row {
   // f(order, z) for the row's tokens with lo <= z <= hi.
   template <class F>
   __device__ __forceinline__ void each(float lo, float hi, F&& f) const {
-    Walk<DT, kThreads, 1> walk(data, vocab, 0, 1);
+    Walk<DT, kThreads> walk(data, vocab, 0, 1);
     walk.each([&](int i, float z) {
       if (z >= lo && z <= hi) f(order_of(z, i), z);
     });
@@ -750,7 +745,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw(SampleArgs a) {
   if (from_list) {
     each_listed([&](uint64_t o, uint32_t) { plan.gather(s, order_value(o), [&] { return o; }); });
   } else {
-    Walk<DT, kThreads, 4> walk(r.data, a.vocab, part, parts);
+    Walk<DT, kThreads> walk(r.data, a.vocab, part, parts);
     walk.each([&](int i, float z) { plan.gather(s, z, [&] { return order_of(z, i); }); });
   }
   __syncthreads();
@@ -792,7 +787,7 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   float top = -INFINITY;
   int at = -1;
   {
-    Walk<DT, kThreads, 4> walk(data, a.vocab, 0, 1);
+    Walk<DT, kThreads> walk(data, a.vocab, 0, 1);
     for (int b = t; b < kBins; b += kThreads) s.count[b] = 0u, s.mass[b] = 0u;
     walk.each([&](int i, float z) {
       if (z > top) top = z, at = i;  // of equals the first
@@ -818,7 +813,7 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   const Questions ask = questions(a, set, row);
   const Row<DT> r{data, a.vocab, set.weigh};
   {
-    Walk<DT, kThreads, 4> walk(data, a.vocab, 0, 1);  // from the XCD's L2
+    Walk<DT, kThreads> walk(data, a.vocab, 0, 1);  // from the XCD's L2
     walk.each([&](int i, float z) { weigh_token(set, z, i, s.mass, s.count, s.cand, &s.n, kList); });
   }
   __syncthreads();
@@ -831,7 +826,7 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   const Plan<DT> plan(s, r, ask);
   uint32_t n = n_listed;  // a list holds all that can be asked for
   if (!set.listed || n_listed > kList) {
-    Walk<DT, kThreads, 4> walk(data, a.vocab, 0, 1);
+    Walk<DT, kThreads> walk(data, a.vocab, 0, 1);
     walk.each([&](int i, float z) { plan.gather(s, z, [&] { return order_of(z, i); }); });
     __syncthreads();
     n = s.n;
