@@ -151,7 +151,12 @@ class KvManager:
         keep[i] becomes position i (it_kv_manager_compact).  Tokens before the
         first dropped one stay in their blocks, the others move to fresh ones;
         dropping a tail moves nothing."""
-        pos = np.ascontiguousarray(keep, dtype=np.int32).reshape(-1)
+        kept = np.asarray(keep)
+        if kept.size and kept.dtype.kind not in "iu":
+            raise TypeError("keep must hold positions (integers)")
+        if kept.size and (kept.min() < 0 or kept.max() > np.iinfo(np.int32).max):
+            raise ValueError("keep: positions outside the sequence")
+        pos = np.ascontiguousarray(kept, dtype=np.int32).reshape(-1)
         n = pos.size
         src, dst = np.empty(n, np.int64), np.empty(n, np.int64)
         delta, new = np.empty(n, np.int32), np.empty(n, np.int32)

@@ -835,11 +835,12 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
 }
 
 // One launch of a workgroup per row, or three of many per row.  us, f32, T 1 whole
-// / top-k 50 and top-p 0.95 / top-p 0.9, one launch then three: 1 x 4096 12.2 /
-// 12.0 / 14.3 and 17.4 / 22.5 / 19.5; 1 x 32768 21.7 / 12.3 / 25.6 and 19.2 / 15.9 /
-// 22.5; 64 x 65536 46.1 / 16.8 / 38.7 and 35.9 / 25.5 / 34.3; 128 x 65536 46.6 /
-// 17.6 / 39.3 and 44.4 / 27.4 / 41.7; 128 x 100000 66.6 / 26.8 / 59.0 and 55.1 /
-// 33.5 / 53.2; 256 x 131072, a row for each CU, 94 / 45 / 84 and 104 / 63 / 95.
+// / T 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096
+// 12.3 / 11.9 / 14.6 against 17.1 / 22.6 / 19.5; 1 x 32768 22.7 / 13.2 / 25.9 against
+// 19.7 / 15.8 / 22.5; 1 x 50000 27.6 / 15.1 / 31.5 against 19.4 / 16.4 / 22.2; 64 x
+// 65536 44.9 / 17.5 / 39.5 against 34.8 / 25.3 / 34.1; 128 x 65536 46.5 / 18.0 / 39.9
+// against 45.3 / 28.0 / 42.3; 128 x 100000 66.9 / 26.9 / 57.7 against 55.7 / 31.9 /
+// 51.3; 256 x 131072, a row for each CU, 91 / 43 / 81 against 100 / 56 / 91.
 bool row_per_workgroup(int32_t rows, int32_t vocab) { return vocab <= 32768 || vocab <= 512 * int64_t(rows); }
 
 // Slices of a row in the first two launches: of 2048 tokens or more, as many as

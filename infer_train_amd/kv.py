@@ -82,11 +82,20 @@ _SCALINGS = {"none": ROTARY_SCALE_NONE, "linear": ROTARY_SCALE_LINEAR, "base": R
              "parts": ROTARY_SCALE_PARTS}
 
 
-def _rows(t: torch.Tensor, name: str) -> Tuple[int, int]:
-    """Address and token stride of a [tokens, heads, head_dim] tensor whose
-    tokens are each contiguous."""
-    if not t.is_cuda:
-        raise ValueError("device tensor expected")
+def _on(t: torch.Tensor, index: int) -> int:
+    """Address of a contiguous tensor on device `index`."""
+    if t.get_device() != index:  # -1: host memory
+        raise ValueError(f"tensor on cuda:{index} expected")
+    if not t.is_contiguous():
+        raise ValueError("contiguous tensor expected")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, name: str, index: int) -> Tuple[int, int]:
+    """Address and token stride of a [tokens, heads, head_dim] tensor on
+    device `index` whose tokens are each contiguous."""
+    if t.get_device() != index:
+        raise ValueError(f"{name}: tensor on cuda:{index} expected")
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim]")
     token, head, element = t.stride()
@@ -132,7 +141,7 @@ class Rotary:
         """x [n_tokens, n_heads, head_dim] (any token stride) rotated to int32
         positions [n_tokens]; transpose: the gradient of that rotation (with
         magnitude 1 its inverse).  out may be x itself."""
-        at, stride = _rows(x, "x")
+        at, stride = _rows(x, "x", self.device)
         n, heads, d = x.shape
         if positions.dtype != torch.int32 or positions.numel() != n:
             raise TypeError("positions must be int32, one per token")
@@ -140,8 +149,8 @@ class Rotary:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
         elif out.dtype != x.dtype or out.shape != x.shape:
             raise TypeError("out must have x's shape and dtype")
-        to, to_stride = _rows(out, "out")
-        _check(call.it_rotary_apply(self._at, at, torch_dtype_id(x.dtype), stride, _ptr(positions), n, heads, d,
+        to, to_stride = _rows(out, "out", self.device)
+        _check(call.it_rotary_apply(self._at, at, torch_dtype_id(x.dtype), stride, _on(positions, self.device), n, heads, d,
                                     int(bool(transpose)), to, to_stride, _raw_stream(self.device)))
         return out
 
@@ -315,12 +324,12 @@ class PagedKvCache:
             raise ValueError("k, v must be [n_tokens, n_kv_heads, head_dim], with a slot and a position per token")
         if v.dtype != kind or (q is not None and q.dtype != kind):
             raise TypeError("q, k, v must have one dtype")
-        (ka, ks), (va, vs) = _rows(k, "k"), _rows(v, "v")
+        (ka, ks), (va, vs) = _rows(k, "k", self._index), _rows(v, "v", self._index)
         src_id = torch_dtype_id(kind)
         qa = oa = None
         qs = heads = out_id = 0
         if q is not None:
-            qa, qs = _rows(q, "q")
+            qa, qs = _rows(q, "q", self._index)
             heads = q.shape[1]
             if q.shape != (n, heads, row[2]):
                 raise ValueError("q must be [n_tokens, n_heads, head_dim]")
@@ -330,11 +339,11 @@ class PagedKvCache:
             elif q_out.shape != q.shape:
                 raise ValueError("q_out must have q's shape")
             else:
-                oa, out_id = _ptr(q_out), torch_dtype_id(q_out.dtype)
+                oa, out_id = _on(q_out, self._index), torch_dtype_id(q_out.dtype)
         elif q_out is not None:
             raise ValueError("q_out without q")
         _check(call.it_kv_append_rotary(self._at, rotary._at, qa, ka, va, src_id, qs, ks, vs, heads,
-                                        _ptr(slot_mapping), _ptr(positions), n, oa, out_id, _raw_stream(self._index)))
+                                        _on(slot_mapping, self._index), _on(positions, self._index), n, oa, out_id, _raw_stream(self._index)))
         return q_out
 
     def gather(self, block_tables: torch.Tensor, ctx_lens: torch.Tensor, start_pos: Optional[torch.Tensor],
@@ -365,8 +374,9 @@ class PagedKvCache:
             raise TypeError("rotary and delta go together")
         if delta is not None and (delta.dtype != torch.int32 or delta.numel() != src.numel()):
             raise TypeError("delta must be int32, one per row")
-        _check(call.it_kv_move(self._at, _ptr(src), _ptr(dst), src.numel(), None if rotary is None else rotary._at,
-                               _ptr(delta), _raw_stream(self._index)))
+        at = self._index
+        _check(call.it_kv_move(self._at, _on(src, at), _on(dst, at), src.numel(), None if rotary is None else rotary._at,
+                               None if delta is None else _on(delta, at), _raw_stream(at)))
 
     # ---- attention --------------------------------------------------------
     def decode_workspace(self, n_seqs: int, n_heads: int, max_tokens: int, partition: int = 512) -> torch.Tensor:

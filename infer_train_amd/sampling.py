@@ -8,7 +8,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from ._lib import call
-from .kv import _check, _ptr, _raw_stream, torch_dtype_id
+from .kv import _check, _on, _raw_stream, torch_dtype_id
 
 __all__ = ["sample", "sample_workspace"]
 
@@ -19,10 +19,10 @@ def sample_workspace(n_rows: int, vocab: int, device) -> torch.Tensor:
     return torch.empty(call.it_sample_workspace(n_rows, vocab), dtype=torch.uint8, device=device)
 
 
-def _per_row(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> int:
+def _per_row(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, index: int) -> int:
     if t.dtype != dtype or t.numel() != n:
         raise TypeError(f"{name} must be {dtype}, one per row")
-    return _ptr(t)
+    return _on(t, index)
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torch.Tensor] = 1.0,
@@ -39,16 +39,17 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     if not logits.is_cuda:
         raise ValueError("device tensor expected")
     n, vocab = logits.shape
+    index = logits.get_device()
     temperatures = top_ks = top_ps = min_ps = None
     if isinstance(temperature, torch.Tensor):
-        temperatures, temperature = _per_row(temperature, "temperature", torch.float32, n), 1.0
+        temperatures, temperature = _per_row(temperature, "temperature", torch.float32, n, index), 1.0
     if isinstance(top_k, torch.Tensor):
-        top_ks, top_k = _per_row(top_k, "top_k", torch.int32, n), 0
+        top_ks, top_k = _per_row(top_k, "top_k", torch.int32, n, index), 0
     if isinstance(top_p, torch.Tensor):
-        top_ps, top_p = _per_row(top_p, "top_p", torch.float32, n), 1.0
+        top_ps, top_p = _per_row(top_p, "top_p", torch.float32, n, index), 1.0
     if isinstance(min_p, torch.Tensor):
-        min_ps, min_p = _per_row(min_p, "min_p", torch.float32, n), 0.0
-    us = _per_row(u, "u", torch.float32, n)
+        min_ps, min_p = _per_row(min_p, "min_p", torch.float32, n, index), 0.0
+    us = _per_row(u, "u", torch.float32, n, index)
     if tokens is None:
         tokens = torch.empty_like(u, dtype=torch.int32)
     if probs is None:
@@ -60,10 +61,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
             ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
     else:
         need = ws.nbytes
-    index = logits.device.index
     args = (logits.data_ptr(), torch_dtype_id(logits.dtype), logits.stride(0), n, vocab, us, temperatures, top_ks, top_ps, min_ps,
-            float(temperature), int(top_k), float(top_p), float(min_p), _per_row(tokens, "tokens", torch.int32, n),
-            _per_row(probs, "probs", torch.float32, n), _ptr(ws), need, _raw_stream(index))
+            float(temperature), int(top_k), float(top_p), float(min_p), _per_row(tokens, "tokens", torch.int32, n, index),
+            _per_row(probs, "probs", torch.float32, n, index), None if ws is None else _on(ws, index), need, _raw_stream(index))
     if torch.cuda.current_device() == index:
         _check(call.it_sample(*args))
     else:

@@ -335,3 +335,29 @@ def test_append_rotary_captured_and_on_another_stream():
         torch.cuda.synchronize()
         want = ref.append_rotary(r, q, k, v, slots, pos)
         assert torch.equal(out, want) and torch.equal(cache.k_pool, ref.k_pool) and torch.equal(cache.v_pool, ref.v_pool), i
+
+
+def test_rows_past_four_gibibytes():
+    """The last block of pools of 4.5 GiB: appended to, moved out of, moved into; nothing else is touched."""
+    import torch
+    from infer_train_amd.kv import PagedKvCache, Rotary
+
+    h, d, bs, nb = 8, 128, 16, 150000
+    cache = PagedKvCache(nb, bs, h, d, CACHE["bf16"])
+    assert cache.k_pool.numel() > 9 << 29
+    r, n = Rotary(d), 5
+    x = torch.from_numpy(values(12, n, 3 * h, d)).cuda().bfloat16()
+    q, k, v = x[:, :h], x[:, h:2 * h], x[:, 2 * h:]
+    last = (nb - 1) * bs
+    slots, pos = to_dev(np.arange(n, dtype=np.int64) + last), to_dev(np.arange(n, dtype=np.int32))
+    cache.append_rotary(r, q, k, v, slots, pos)
+    want = r.apply(k, pos)
+    assert torch.equal(cache.view("k")[-1, :, :n].transpose(0, 1), want) and torch.equal(cache.view("v")[-1, :, :n].transpose(0, 1), v)
+    delta = to_dev(np.full(n, 100, np.int32))
+    cache.move(slots, slots - last, r, delta)
+    cache.move(slots - last, slots + 8)
+    cache.check()
+    turned = r.apply(want, delta)
+    assert torch.equal(cache.view("k")[0, :, :n].transpose(0, 1), turned) and torch.equal(cache.view("k")[-1, :, 8:8 + n].transpose(0, 1), turned)
+    assert torch.equal(cache.view("v")[-1, :, 8:8 + n].transpose(0, 1), v)
+    assert not cache.k_pool[h * bs * d * 2:-h * bs * d * 2].any() and not cache.v_pool[h * bs * d * 2:-h * bs * d * 2].any()

@@ -190,7 +190,14 @@ def test_compact_refusals_change_nothing():
         t, c, f = mgr.tables()[0], mgr.positions(), pool.num_free()
         return np.array_equal(t, before[0]) and np.array_equal(c, before[1]) and f == before[2]
 
-    for seq, keep in ((0, [1, 1]), (0, [2, 1]), (0, [-1]), (0, [22]), (0, [0, 5, 40]), (1, [0]), (2, []), (-1, []),
+    for keep in ([-1], [2 ** 40], np.array([0, -5])):
+        with pytest.raises(ValueError):
+            mgr.compact(0, keep)
+    for keep in ([0.0, 1.0], np.ones(22, bool)):
+        with pytest.raises(TypeError):
+            mgr.compact(0, keep)
+    assert unchanged()
+    for seq, keep in ((0, [1, 1]), (0, [2, 1]), (0, [22]), (0, [0, 5, 40]), (1, [0]), (2, []), (-1, []),
                       (0, list(range(1, 22)))):  # the last: six fresh blocks
         with pytest.raises(InvalidInput):
             mgr.compact(seq, keep)
