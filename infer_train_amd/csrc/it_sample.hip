@@ -48,6 +48,7 @@ constexpr int kIndexBits = 18;
 constexpr double kUnit = 0x1p44;      // weight of the largest token
 constexpr double kLeast = 0x1.0000000000001p-45;  // smaller weights round to nothing
 constexpr double kBinsPerBit = 44.0;  // of log2 weight, of which 45 weigh at all
+static_assert(45 * kBinsPerBit + 2 < kBins, "a bin for every weight");
 constexpr uint32_t kDeadKey = 0x007FFFFFu;  // order_key(-inf)
 
 struct RowState {
@@ -127,17 +128,14 @@ struct Weigher {
     const double e = __builtin_amdgcn_ldexp(fma(h, f, 1.0), int(n));
     // Rounded to a whole number of units by the sum with 2^52.
     w = __builtin_bit_cast(uint64_t, fma(e, unit, magic)) & ((uint64_t(1) << 52) - 1);
-    bin = min(int(x * bins), kBins - 1);
+    bin = int(x * bins);  // below 45 kBinsPerBit + 1 for what is kept
     return e >= least;
   }
 };
 
 // The tokens of a slice of a row: its share of the 16-byte vectors of the row's
 // aligned part, the first slice also the tokens before that part, the last those
-// behind it.  Each thread's next vector is loaded while one is worked on, its
-// first when the walk is made, in the shadow of what a kernel does before each().
-// (Batches of four vectors per thread keep more loads in flight, but unroll what is
-// done with a token 16 or 32 times: small calls then wait for instructions.)
+// behind it.
 template <int DT, int kBlock>
 struct Walk {
   static constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es;
@@ -156,23 +154,61 @@ struct Walk {
     first = slice == 0;
     last = slice == slices - 1;
     v = reinterpret_cast<const typename In::raw*>(row + head * es);
+  }
+  // Loads what each() begins with, in the shadow of what a kernel does before it.
+  __device__ __forceinline__ void start() {
     if (lo + int(threadIdx.x) < hi) next = v[lo + int(threadIdx.x)];
   }
-  // f(index, z); a thread's tokens come in ascending order.  Once.
   template <class F>
-  __device__ __forceinline__ void each(F&& f) {
+  __device__ __forceinline__ void vector(const typename In::raw& w, int x, F&& f) const {
+    float z[V];
+    In::widen(w, z);
+#pragma unroll
+    for (int e = 0; e < V; ++e) f(head + x * V + e, z[e]);
+  }
+  template <class F>
+  __device__ __forceinline__ void ends(F&& f) const {
     const int tid = int(threadIdx.x);
     if (first && tid < head) f(tid, load_element(row, tid, DT));
+    if (last && tid < vocab - done) f(done + tid, load_element(row, done + tid, DT));
+  }
+  // f(index, z), once after start(): one vector is loaded while one is worked on.
+  // (Batches of vectors in flight read no faster, 16 waves a CU keep enough; and
+  // unrolled over them the weighing is 16 to 64 times its code, which small calls
+  // wait for.)
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) {
 #pragma unroll 1
-    for (int x = lo + tid; x < hi; x += kBlock) {
+    for (int x = lo + int(threadIdx.x); x < hi; x += kBlock) {
       const typename In::raw w = next;
       if (x + kBlock < hi) next = v[x + kBlock];
-      float z[V];
-      In::widen(w, z);
-#pragma unroll
-      for (int e = 0; e < V; ++e) f(head + x * V + e, z[e]);
+      vector(w, x, f);
     }
-    if (last && tid < vocab - done) f(done + tid, load_element(row, done + tid, DT));
+    ends(f);
+  }
+  // The same of those threads' tokens alone that a thread has `wanted`: where
+  // few have, their vectors are shared out among all.  columns: LDS, kBlock
+  // places; n: an LDS word.
+  template <class F>
+  __device__ __forceinline__ void each_wanted(bool wanted, uint32_t* columns, uint32_t* n, F&& f) {
+    if (threadIdx.x == 0) *n = 0u;
+    __syncthreads();
+    if (wanted) columns[atomicAdd(n, 1u)] = threadIdx.x;
+    __syncthreads();
+    const uint32_t few = *n;
+    if (few > kBlock / 2) {
+      start();
+      each(f);
+      return;
+    }
+    const uint32_t total = few * uint32_t((hi - lo + kBlock - 1) / kBlock);
+#pragma unroll 1
+    for (uint32_t i = threadIdx.x; i < total; i += kBlock) {
+      const uint32_t turn = i / few;
+      const int x = lo + int(turn * kBlock + columns[i - turn * few]);
+      if (x < hi) vector(v[x], x, f);
+    }
+    ends(f);
   }
 };
 
@@ -204,12 +240,13 @@ __global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
     rs.n_gathered = rs.ticket = 0u;
   for (int b = slice * kSliceThreads + int(threadIdx.x); b < kBins; b += a.slices * kSliceThreads) rs.count[b] = 0u, rs.mass[b] = 0u;
   float top = -INFINITY;
-  int at = -1;
+  int at = kMaxVocab;
   Walk<DT, kSliceThreads> walk(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices);
+  walk.start();
   walk.each([&](int i, float z) {
-    if (z > top) top = z, at = i;  // of equals the first
+    if (z > top || (z == top && i < at)) top = z, at = i;
   });
-  uint64_t best = at < 0 ? 0u : order_of(top, at);
+  uint64_t best = top > -INFINITY ? order_of(top, at) : 0u;
   uint32_t group = order_key(top);
 #pragma unroll
   for (int o = 16; o; o >>= 1) group = max(group, uint32_t(__shfl_xor(int(group), o)));
@@ -271,16 +308,21 @@ struct Settings {
   // maximum: at least top_k tokens have keys that large.
   __device__ __forceinline__ void raise_floor() {
     if (top_k <= 0 || top_k > groups) return;
+    const uint32_t key = groups <= 128 ? search<2>() : search<kLoads>();
+    if (key > kDeadKey) weigh.floor = fmaxf(weigh.floor, key_value(key));
+  }
+  template <int N>
+  __device__ __forceinline__ uint32_t search() const {
     uint32_t key = 0u;
-    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1) {
-      const uint32_t with = key | bit;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+      const uint32_t with = key | 1u << bit;
       int n = 0;
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j)
-        if (j * 64 < groups) n += __popcll(__ballot(group[j] >= with));
+      for (int j = 0; j < N; ++j) n += __popcll(__ballot(group[j] >= with));
       if (n >= top_k) key = with;
     }
-    if (key > kDeadKey) weigh.floor = fmaxf(weigh.floor, key_value(key));
+    return key;
   }
   // What a row without anything to weigh answers.
   __device__ __forceinline__ void trivial(const SampleArgs& a, int row) const {
@@ -312,6 +354,7 @@ __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
   const int t = int(threadIdx.x), slice = int(blockIdx.x), row = int(blockIdx.y);
   RowState& rs = a.rows[row];
   Walk<DT, kSliceThreads> walk(a.logits + int64_t(row) * a.row_bytes, a.vocab, slice, a.slices);
+  walk.start();
   Settings set;
   set.load_groups(a, rs.group_max, a.slices * kGroups);
   if (!set.derive(a, row, wave_max64((t & 63) < a.slices ? rs.best[t & 63] : 0u))) return;
@@ -430,6 +473,7 @@ struct Row {
   template <class F>
   __device__ __forceinline__ void each(float lo, float hi, F&& f) const {
     Walk<DT, kThreads> walk(data, vocab, 0, 1);
+    walk.start();
     walk.each([&](int i, float z) {
       if (z >= lo && z <= hi) f(order_of(z, i), z);
     });
@@ -746,6 +790,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw(SampleArgs a) {
     each_listed([&](uint64_t o, uint32_t) { plan.gather(s, order_value(o), [&] { return o; }); });
   } else {
     Walk<DT, kThreads> walk(r.data, a.vocab, part, parts);
+    walk.start();
     walk.each([&](int i, float z) { plan.gather(s, z, [&] { return order_of(z, i); }); });
   }
   __syncthreads();
@@ -785,20 +830,19 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   const int t = int(threadIdx.x), lane = t & 63, row = int(blockIdx.x);
   const char* const data = a.logits + int64_t(row) * a.row_bytes;
   float top = -INFINITY;
-  int at = -1;
-  {
-    Walk<DT, kThreads> walk(data, a.vocab, 0, 1);
-    for (int b = t; b < kBins; b += kThreads) s.count[b] = 0u, s.mass[b] = 0u;
-    walk.each([&](int i, float z) {
-      if (z > top) top = z, at = i;  // of equals the first
-    });
-  }
+  int at = kMaxVocab;
+  Walk<DT, kThreads> walk(data, a.vocab, 0, 1);
+  walk.start();
+  for (int b = t; b < kBins; b += kThreads) s.count[b] = 0u, s.mass[b] = 0u;
+  walk.each([&](int i, float z) {
+    if (z > top || (z == top && i < at)) top = z, at = i;
+  });
   // Groups of eight lanes; of two where many threads may have no tokens.
   const int log2_lanes = a.vocab >= 8 * kThreads ? 3 : 1;
   uint32_t group = order_key(top);
   for (int o = 1 << log2_lanes >> 1; o; o >>= 1) group = max(group, uint32_t(__shfl_xor(int(group), o)));
   if ((lane & ((1 << log2_lanes) - 1)) == 0) maxima[t >> log2_lanes] = group;
-  const uint64_t best = wave_max64(at < 0 ? 0u : order_of(top, at));
+  const uint64_t best = wave_max64(top > -INFINITY ? order_of(top, at) : 0u);
   if (lane == 0) s.wave_mass[t >> 6] = best;
   if (t == 0) s.n = 0u;
   __syncthreads();
@@ -812,10 +856,9 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   set.weigh.constants();
   const Questions ask = questions(a, set, row);
   const Row<DT> r{data, a.vocab, set.weigh};
-  {
-    Walk<DT, kThreads> walk(data, a.vocab, 0, 1);  // from the XCD's L2
-    walk.each([&](int i, float z) { weigh_token(set, z, i, s.mass, s.count, s.cand, &s.n, kList); });
-  }
+  // A thread whose largest token is below the floor has none to weigh.
+  walk.each_wanted(top >= set.weigh.floor, s.fine_count, &s.base,
+                   [&](int i, float z) { weigh_token(set, z, i, s.mass, s.count, s.cand, &s.n, kList); });
   __syncthreads();
   const uint32_t n_listed = s.n;
   if (set.listed && n_listed <= kFew) {
@@ -826,8 +869,8 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   const Plan<DT> plan(s, r, ask);
   uint32_t n = n_listed;  // a list holds all that can be asked for
   if (!set.listed || n_listed > kList) {
-    Walk<DT, kThreads> walk(data, a.vocab, 0, 1);
-    walk.each([&](int i, float z) { plan.gather(s, z, [&] { return order_of(z, i); }); });
+    walk.each_wanted(top >= plan.lowest, s.fine_count, &s.base,
+                     [&](int i, float z) { plan.gather(s, z, [&] { return order_of(z, i); }); });
     __syncthreads();
     n = s.n;
   }
