@@ -57,7 +57,6 @@ __device__ __forceinline__ char* move_page(const MoveArgs& a, uint32_t r, int64_
 
 // Rows as they are: 16-byte pieces of the main row, then 2-byte ones of the
 // side row.
-template <int G>
 __global__ __launch_bounds__(kThreads) void kv_move_bytes(MoveArgs a) {
   const int64_t i = int64_t(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
   if (i >= a.n) return;  // uniform
@@ -66,26 +65,17 @@ __global__ __launch_bounds__(kThreads) void kv_move_bytes(MoveArgs a) {
   if (!move_slots(a, i, s, d, blockIdx.y == 0 && lane == 0) || s == d) return;  // uniform
   const uint32_t vecs = uint32_t(a.main_bytes) >> 4, items = vecs + (uint32_t(a.side_bytes) >> 1), total = a.rows * items;
   const int64_t bs = int64_t(1) << a.log2_bs, so = s & (bs - 1), dof = d & (bs - 1);
-  const uint32_t x0 = blockIdx.y * (64 * G) + lane;
-  uint4 w[G];
-#pragma unroll
-  for (int j = 0; j < G; ++j) {
-    const uint32_t x = min(x0 + 64 * j, total - 1);  // past the end: re-read, not stored
-    const uint32_t r = x / items, item = x - r * items;
-    bool key;
-    const char* const page = move_page(a, r, s, key);
-    if (item < vecs) w[j] = ld16_nt(page + so * a.main_bytes + item * 16);
-    else w[j].x = *reinterpret_cast<const uint16_t*>(page + bs * a.main_bytes + so * a.side_bytes + (item - vecs) * 2);
-  }
-#pragma unroll
-  for (int j = 0; j < G; ++j) {
-    const uint32_t x = x0 + 64 * j;
-    if (x >= total) continue;
-    const uint32_t r = x / items, item = x - r * items;
-    bool key;
-    char* const page = move_page(a, r, d, key);
-    if (item < vecs) st16(page + dof * a.main_bytes + item * 16, w[j]);
-    else *reinterpret_cast<uint16_t*>(page + bs * a.main_bytes + dof * a.side_bytes + (item - vecs) * 2) = uint16_t(w[j].x);
+  const uint32_t x = blockIdx.y * 64 + uint32_t(lane);
+  if (x >= total) return;
+  const uint32_t r = x / items, item = x - r * items;
+  bool key;
+  const char* const from = move_page(a, r, s, key);
+  char* const to = move_page(a, r, d, key);
+  if (item < vecs) {
+    st16(to + dof * a.main_bytes + item * 16, ld16_nt(from + so * a.main_bytes + item * 16));
+  } else {
+    const int64_t side = bs * a.main_bytes + (item - vecs) * 2;
+    *reinterpret_cast<uint16_t*>(to + side + dof * a.side_bytes) = *reinterpret_cast<const uint16_t*>(from + side + so * a.side_bytes);
   }
 }
 
@@ -274,21 +264,19 @@ __global__ __launch_bounds__(kThreads) void kv_move_quant(MoveArgs a) {
   }
 }
 
-// Steps per wave: as many as keep all waves resident at once (32 of 256 CUs),
-// one, two or four.
-constexpr int64_t kResident = 256 * 32;
-
 void launch_bytes(const MoveArgs& a, hipStream_t s) {
+  // One 16-byte piece per lane: two or four were slower at every size but one (28
+  // layers x 4 heads of 128 bf16: 16 tokens 2.20 us, 2.55 with two, 2000 35.2, 36.0).
   const int64_t total = int64_t(a.rows) * (a.main_bytes / 16 + a.side_bytes / 2);
-  const auto chunks = [&](int g) { return (total + 64 * g - 1) / (64 * g); };
-  const unsigned bx = unsigned((a.n + kWaves - 1) / kWaves);
-  if (a.n * chunks(1) <= kResident)
-    hipLaunchKernelGGL(kv_move_bytes<1>, dim3(bx, unsigned(chunks(1))), dim3(kThreads), 0, s, a);
-  else if (a.n * chunks(2) <= kResident)
-    hipLaunchKernelGGL(kv_move_bytes<2>, dim3(bx, unsigned(chunks(2))), dim3(kThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL(kv_move_bytes<4>, dim3(bx, unsigned(chunks(4))), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(kv_move_bytes, dim3(unsigned((a.n + kWaves - 1) / kWaves), unsigned((total + 63) / 64)), dim3(kThreads), 0, s, a);
 }
+
+// Row steps per wave: one, or two where the waves of one would come to four times
+// what is resident (32 of 256 CUs), which shares a token's angles among more rows.
+// us with one / two / four, 28 layers x 4 heads of 128 bf16: 16 tokens 2.92 / 3.40 /
+// 4.11, 260 6.4 / 6.4 / 5.9, 2000 39.2 / 38.1 / 39.5 (6 TB/s from a warm cache).
+constexpr int64_t kManyWaves = 4 * 256 * 32;
+
 template <int DT>
 void launch_rows(const MoveArgs& a, bool split, hipStream_t s) {
   if (!split) {
@@ -300,12 +288,10 @@ void launch_rows(const MoveArgs& a, bool split, hipStream_t s) {
   const size_t lds = size_t(kWaves) * angle_room<DT == IT_F32 ? 4 : 8>(a.split.n_dims) * sizeof(float2);
   const auto chunks = [&](int g) { return (int64_t(a.rows) + a.split.rows * g - 1) / (a.split.rows * g); };
   const unsigned bx = unsigned((a.n + kWaves - 1) / kWaves);
-  if (a.n * chunks(1) <= kResident)
+  if (a.n * chunks(1) <= kManyWaves)
     hipLaunchKernelGGL((kv_move_rows<DT, 1>), dim3(bx, unsigned(chunks(1))), dim3(kThreads), lds, s, a);
-  else if (a.n * chunks(2) <= kResident)
-    hipLaunchKernelGGL((kv_move_rows<DT, 2>), dim3(bx, unsigned(chunks(2))), dim3(kThreads), lds, s, a);
   else
-    hipLaunchKernelGGL((kv_move_rows<DT, 4>), dim3(bx, unsigned(chunks(4))), dim3(kThreads), lds, s, a);
+    hipLaunchKernelGGL((kv_move_rows<DT, 2>), dim3(bx, unsigned(chunks(2))), dim3(kThreads), lds, s, a);
 }
 template <int DT>
 void launch_quant(MoveArgs a, hipStream_t s) {
@@ -316,7 +302,8 @@ void launch_quant(MoveArgs a, hipStream_t s) {
   char* const v = a.vpool;
   a.vpool = a.kpool;
   const size_t lds = size_t(kWaves) * (a.split.n_dims / 2 + a.split.head_dim / 2) * sizeof(float2);
-  const int64_t want = kResident / a.n, y = want < 1 ? 1 : want > int64_t(a.rows) ? int64_t(a.rows) : want;
+  // A wave per row, rows beyond what is resident one after another.
+  const int64_t want = 256 * 32 / a.n, y = want < 1 ? 1 : want > int64_t(a.rows) ? int64_t(a.rows) : want;
   hipLaunchKernelGGL(kv_move_quant<DT>, dim3(unsigned((a.n + kWaves - 1) / kWaves), unsigned(y < 65535 ? y : 65535)),
                      dim3(kThreads), lds, s, a);
   a.vpool = v;
@@ -339,8 +326,9 @@ extern "C" int32_t it_kv_move(it_kv_cache* c, const int64_t* src, const int64_t*
   if (rotary && !delta) return fail(IT_INVALID_INPUT, "%s: delta is NULL", who);
   const int64_t rows = int64_t(c->n_layers) * c->n_kv_heads * 2, row_items = int64_t(c->head_dim) * 2;
   // A pair's rows are chunks of a grid's second direction (fewer than 65536 at
-  // this limit), pairs its first (2^32 work items).
-  if (rows * row_items >= int64_t(1) << 25 || n > 1 << 25)
+  // this limit: a chunk is 64 pieces of 16 bytes or 2), pairs its first (2^32 work
+  // items).
+  if (rows * row_items >= int64_t(1) << 24 || n > 1 << 25)
     return fail(IT_INVALID_INPUT, "%s: %d pairs of %lld rows of %d elements", who, n, (long long)rows, c->head_dim);
   MoveArgs a{};
   a.kpool = static_cast<char*>(c->k_pool);

@@ -188,10 +188,12 @@ __global__ __launch_bounds__(kThreads) void rotary_general(RotaryArgs a) {
   }
 }
 
-// Row steps per wave, the fewest with which all waves are resident at once
-// (32 of 256 CUs): small calls are a chain of waits, longer with each step,
-// large ones amortise a wave's angles over its rows.
-constexpr int64_t kResident = 256 * 32;
+// Row steps per wave: one, or two where the waves of one would come to four times
+// what is resident (32 of 256 CUs).  us with one / two / four, 32 + 2 x 8 heads of
+// 128 into a bf16 cache: f32, 1 token 2.41 / 2.81 / 3.58, 1024 8.84 / 9.40 / 9.34, 4096
+// (201 MB) 34.8 / 33.1 / 33.7; bf16, 128 tokens 3.01 / 3.50 / 4.43, 1024 5.59 / 5.76 /
+// 6.24, 4096 20.7 / 20.8 / 20.8.  Large calls move 5 to 6 TB/s, a copy's rate.
+constexpr int64_t kManyWaves = 4 * 256 * 32;
 
 template <int SRC, int DT, int V, int G>
 void launch_rows(const RotaryArgs& a, int64_t chunks, hipStream_t s) {
@@ -204,9 +206,8 @@ void launch_split(const RotaryArgs& a, hipStream_t s) {
   constexpr int V = kFloat && SRC != IT_F32 ? 8 : 4;
   const int64_t rows = int64_t(a.hq) + 2 * int64_t(a.hkv);
   const auto chunks = [&](int g) { return (rows + a.split.rows * g - 1) / (a.split.rows * g); };
-  if (a.n_tokens * chunks(1) <= kResident) launch_rows<SRC, DT, V, 1>(a, chunks(1), s);
-  else if (a.n_tokens * chunks(2) <= kResident) launch_rows<SRC, DT, V, 2>(a, chunks(2), s);
-  else launch_rows<SRC, DT, V, 4>(a, chunks(4), s);
+  if (a.n_tokens * chunks(1) <= kManyWaves) launch_rows<SRC, DT, V, 1>(a, chunks(1), s);
+  else launch_rows<SRC, DT, V, 2>(a, chunks(2), s);
 }
 template <int DT>
 void launch_general(const RotaryArgs& a, int64_t blocks, hipStream_t s) {

@@ -25,7 +25,8 @@
 
 #include <cmath>
 
-#include "it_rotary.hpp"
+#include "it_internal.hpp"
+#include "it_rows.hpp"
 
 using namespace itkv;
 
@@ -837,8 +838,10 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   walk.each([&](int i, float z) {
     if (z > top || (z == top && i < at)) top = z, at = i;
   });
-  // Groups of eight lanes; of two where many threads may have no tokens.
-  const int log2_lanes = a.vocab >= 8 * kThreads ? 3 : 1;
+  // Groups of eight lanes; of two where threads have no tokens: top-k 50 of 1000
+  // would find 31 groups, and take 22.5 us for its long list instead of 11.0
+  // (4096: 9.2 with groups of eight, 11.9 of two, a longer floor search).
+  const int log2_lanes = walk.hi - walk.lo >= kThreads ? 3 : 1;
   uint32_t group = order_key(top);
   for (int o = 1 << log2_lanes >> 1; o; o >>= 1) group = max(group, uint32_t(__shfl_xor(int(group), o)));
   if ((lane & ((1 << log2_lanes) - 1)) == 0) maxima[t >> log2_lanes] = group;
@@ -856,7 +859,8 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   set.weigh.constants();
   const Questions ask = questions(a, set, row);
   const Row<DT> r{data, a.vocab, set.weigh};
-  // A thread whose largest token is below the floor has none to weigh.
+  // A thread whose largest token is below the floor has none to weigh: with top-k
+  // 50 of 256 x 131072 the second reading takes 7 us of 33 instead of 13 of 43.
   walk.each_wanted(top >= set.weigh.floor, s.fine_count, &s.base,
                    [&](int i, float z) { weigh_token(set, z, i, s.mass, s.count, s.cand, &s.n, kList); });
   __syncthreads();
@@ -879,15 +883,16 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
 
 // One launch of a workgroup per row, or three of many per row.  us, f32, T 1 whole
 // / T 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096
-// 12.3 / 11.9 / 14.6 against 17.1 / 22.6 / 19.5; 1 x 32768 22.7 / 13.2 / 25.9 against
-// 19.7 / 15.8 / 22.5; 1 x 50000 27.6 / 15.1 / 31.5 against 19.4 / 16.4 / 22.2; 64 x
-// 65536 44.9 / 17.5 / 39.5 against 34.8 / 25.3 / 34.1; 128 x 65536 46.5 / 18.0 / 39.9
-// against 45.3 / 28.0 / 42.3; 128 x 100000 66.9 / 26.9 / 57.7 against 55.7 / 31.9 /
-// 51.3; 256 x 131072, a row for each CU, 91 / 43 / 81 against 100 / 56 / 91.
+// 13.2 / 11.0 / 15.2 against 17.6 / 22.9 / 19.8; 1 x 32768 22.6 / 12.7 / 25.1 against
+// 19.7 / 15.5 / 22.3; 1 x 50000 28.2 / 14.1 / 31.8 against 19.8 / 15.9 / 22.0; 64 x
+// 65536 48.6 / 16.1 / 39.8 against 36.2 / 25.0 / 34.5; 128 x 65536 47.1 / 16.4 / 40.0
+// against 43.1 / 25.4 / 42.0; 128 x 100000 67.3 / 20.5 / 56.2 against 55.8 / 29.5 /
+// 51.6; 256 x 131072, a row for each CU, 83 / 33 / 84 against 94 / 55 / 91.
 bool row_per_workgroup(int32_t rows, int32_t vocab) { return vocab <= 32768 || vocab <= 512 * int64_t(rows); }
 
 // Slices of a row in the first two launches: of 2048 tokens or more, as many as
-// are resident at once (four workgroups on each of 256 CUs).  The result does not
+// are resident at once (four workgroups on each of 256 CUs; twice as many took 8.6
+// and 22.0 us for 64 x 100003 bf16, instead of 6.8 and 15.0).  The result does not
 // depend on it, nor on the workgroups that gather in the third.
 int slice_count(int32_t rows, int32_t vocab) {
   int s = (vocab + 2047) / 2048;
@@ -895,7 +900,8 @@ int slice_count(int32_t rows, int32_t vocab) {
   s = s < fill ? s : fill;
   return s < kMaxSlices ? s : kMaxSlices;
 }
-// Workgroups of a row in the third: of 8192 tokens or more, 512 in all.
+// Workgroups of a row in the third: of 8192 tokens or more, 256 in all (64 x 100000,
+// whole / top-p 0.9: 40.7 / 38.6 us; one per row 54.0 / 43.2, 512 in all 50.5 / 51.9).
 int part_count(int32_t rows, int32_t vocab) {
   const int p = (vocab + 8191) / 8192, fill = 256 / rows > 0 ? 256 / rows : 1;
   return p < fill ? p : fill;
