@@ -39,7 +39,8 @@ constexpr int kBins = 2048;          // of a row, linear in z
 constexpr int kList = 2048;          // tokens listed per row, and gathered in LDS
 constexpr int kRowList = 8192;       // room for a row's slices' lists: a slice may hold most of the likely tokens
 constexpr int kSliceList = kList - 1;  // of a slice at most: its workgroup's LDS is a quarter of a CU's
-constexpr int kFew = 256;            // tokens compared all with all
+constexpr int kFew = 256;            // tokens compared all with all (below)
+static_assert(kFew > 64, "narrow() takes more than it for more than a last step's 64");
 constexpr int kFineBits = 10, kFine = 1 << kFineBits;
 constexpr int kMaxSlices = 32;
 constexpr int kGroups = 2 * kSliceWaves;  // group maxima per slice: half waves
@@ -103,33 +104,45 @@ __device__ __forceinline__ double scalar(double x) {
   asm("" : "+s"(x));
   return x;
 }
+// One kept in vector registers: an instruction reads one scalar operand.
+__device__ __forceinline__ double vector(double x) {
+  asm("" : "+v"(x));
+  return x;
+}
 
-// A row's weights, the same in all its threads.
+// A row's weights, the same in all its threads.  fp64 work bounds them (an fma of
+// every token of 256 x 131072 takes 1.4 us), so whole numbers are taken from the
+// low word of a sum with 1.5 x 2^52 and exponents are added as integers: 35 us,
+// and 38 with fp64's roundings, conversions and ldexp.
 struct Weigher {
   float top;      // max z
   float floor;    // tokens below weigh nothing, fail min-p or cannot be among the first k
   double bits;    // log2(e) / T
   double least;   // min-p, or the smallest weight that does not round to nothing
-  double exp2[10], unit, magic, bins;  // kExp2, kUnit, 2^52, -kBinsPerBit in scalar registers
+  double below;   // z - top of 2^-64; lower ones weigh no more
+  double bin_bits, exp2[10], unit, zero, whole;
   __device__ __forceinline__ void constants() {
+    // inf - inf is NaN, of which fmax makes 0: tokens at a top of +inf weigh 1.
+    below = top < INFINITY ? -64.0 / bits : 0.0;
+    bin_bits = -kBinsPerBit * bits;
 #pragma unroll
-    for (int i = 0; i < 10; ++i) exp2[i] = scalar(kExp2[i]);
+    for (int i = 0; i < 10; ++i) exp2[i] = i == 8 ? vector(kExp2[i]) : scalar(kExp2[i]);
     unit = scalar(kUnit);
-    magic = scalar(0x1p52);
-    bins = scalar(-kBinsPerBit);
+    zero = vector(0x1p52);
+    whole = vector(0x1.8p52);
   }
   // Weight and bin of a token with floor <= z <= top; false: not kept.
   __device__ __forceinline__ bool operator()(float z, uint64_t& w, int& bin) const {
-    // inf - inf is NaN, of which fmin makes 0: tokens at a top of +inf weigh 1.
-    const double x = fmin((double(z) - double(top)) * bits, 0.0);
-    const double n = __builtin_rint(x), f = x - n;
-    double h = exp2[9];
+    const double d = fmax(double(z) - double(top), below);
+    const double n = fma(d, bits, whole), f = fma(d, bits, whole - n);
+    double h = fma(exp2[9], f, exp2[8]);
 #pragma unroll
-    for (int i = 8; i >= 0; --i) h = fma(h, f, exp2[i]);
-    const double e = __builtin_amdgcn_ldexp(fma(h, f, 1.0), int(n));
+    for (int i = 7; i >= 0; --i) h = fma(h, f, exp2[i]);
+    const double m = fma(h, f, 1.0);  // 2^f, above 0.7
+    const double e = __hiloint2double(int(uint32_t(__double2hiint(m)) + (uint32_t(__double2loint(n)) << 20)), __double2loint(m));
     // Rounded to a whole number of units by the sum with 2^52.
-    w = __builtin_bit_cast(uint64_t, fma(e, unit, magic)) & ((uint64_t(1) << 52) - 1);
-    bin = int(x * bins);  // below 45 kBinsPerBit + 1 for what is kept
+    w = __builtin_bit_cast(uint64_t, fma(e, unit, zero)) & ((uint64_t(1) << 52) - 1);
+    bin = __double2loint(fma(d, bin_bits, whole));  // up to 45 kBinsPerBit for what is kept
     return e >= least;
   }
 };
@@ -217,12 +230,45 @@ struct Walk {
 __device__ __forceinline__ uint64_t lane64(uint64_t x, int lane) {
   return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(x >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(x), lane));
 }
+// The 64-bit x of the lane that a DPP pattern names; 0 for lanes it leaves out.
+template <int CTRL, int ROWS = 0xF, int BANKS = 0xF, bool kBound = true>
+__device__ __forceinline__ uint64_t dpp64(uint64_t x) {
+  const int hi = __builtin_amdgcn_update_dpp(0, int(x >> 32), CTRL, ROWS, BANKS, kBound);
+  return uint64_t(uint32_t(hi)) << 32 | uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, ROWS, BANKS, kBound));
+}
+// The largest of the wave's, in every lane.
 __device__ __forceinline__ uint64_t wave_max64(uint64_t x) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const uint64_t y = uint64_t(__shfl_xor((unsigned long long)(x), o));
-    x = y > x ? y : x;
-  }
+  x = max(x, dpp64<kDppQuadXor1>(x));
+  x = max(x, dpp64<kDppQuadXor2>(x));
+  x = max(x, dpp64<kDppHalfMirror>(x));
+  x = max(x, dpp64<kDppRowRor8>(x));
+  return max(max(lane64(x, 0), lane64(x, 16)), max(lane64(x, 32), lane64(x, 48)));
+}
+// The largest of groups of n lanes, n a power of two up to 32, in every lane of each.
+__device__ __forceinline__ uint32_t group_max32(uint32_t x, int n) {
+  if (n >= 2) x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppQuadXor1, 0xF, 0xF, true)));
+  if (n >= 4) x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppQuadXor2, 0xF, 0xF, true)));
+  if (n >= 8) x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppHalfMirror, 0xF, 0xF, true)));
+  if (n >= 16) x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppRowRor8, 0xF, 0xF, true)));
+  if (n >= 32) x = max(x, uint32_t(__shfl_xor(int(x), 16)));
+  return x;
+}
+// x summed over the lanes up to and with each.
+__device__ __forceinline__ uint64_t wave_inclusive_sum64(uint64_t x) {
+  uint64_t v = x + dpp64<0x111>(x);          // row_shr:1
+  v += dpp64<0x112>(x);                      // row_shr:2
+  v += dpp64<0x113>(x);                      // row_shr:3
+  v += dpp64<0x114, 0xF, 0xE, false>(v);     // row_shr:4, banks 1-3
+  v += dpp64<0x118, 0xF, 0xC, false>(v);     // row_shr:8, banks 2-3
+  v += dpp64<0x142, 0xA, 0xF, false>(v);     // row_bcast:15, rows 1, 3
+  return v + dpp64<0x143, 0xC, 0xF, false>(v);  // row_bcast:31, rows 2-3
+}
+// x summed over groups of n lanes, n a power of two up to 16, in every lane of each.
+__device__ __forceinline__ uint64_t group_sum64(uint64_t x, uint32_t n) {
+  if (n >= 2) x += dpp64<kDppQuadXor1>(x);
+  if (n >= 4) x += dpp64<kDppQuadXor2>(x);
+  if (n >= 8) x += dpp64<kDppHalfMirror>(x);
+  if (n >= 16) x += dpp64<kDppRowRor8>(x);
   return x;
 }
 
@@ -248,9 +294,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
     if (z > top || (z == top && i < at)) top = z, at = i;
   });
   uint64_t best = top > -INFINITY ? order_of(top, at) : 0u;
-  uint32_t group = order_key(top);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) group = max(group, uint32_t(__shfl_xor(int(group), o)));
+  const uint32_t group = group_max32(order_key(top), 32);
   if ((lane & 31) == 0) rs.group_max[slice * kGroups + wave * 2 + (lane >> 5)] = group;
   best = wave_max64(best);
   if (lane == 0) best_of[wave] = best;
@@ -411,14 +455,8 @@ struct Scan {
 };
 __device__ __forceinline__ Scan block_scan(Shared& s, uint32_t count, uint64_t mass) {
   const int lane = int(threadIdx.x & 63), wave = int(threadIdx.x >> 6);
-  uint32_t c = count;
-  uint64_t m = mass;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t cu = uint32_t(__shfl_up(int(c), o));
-    const uint64_t mu = uint64_t(__shfl_up((unsigned long long)(m), o));
-    if (lane >= o) c += cu, m += mu;
-  }
+  const uint32_t c = uint32_t(wave_inclusive_sum(int(count)));
+  const uint64_t m = wave_inclusive_sum64(mass);
   __syncthreads();  // the sums of the call before are read
   if (lane == 63) s.wave_count[wave] = c, s.wave_mass[wave] = m;
   __syncthreads();
@@ -485,7 +523,7 @@ struct Row {
     hi = INFINITY;
     if (weigh.top < INFINITY && weigh.bits > 0.0) {
       const double edge = 1.0 / (kBinsPerBit * weigh.bits), top = double(weigh.top);
-      const double begin = top - double(first) * edge, end = top - double(last + 1) * edge;
+      const double begin = top - (double(first) - 0.5) * edge, end = top - (double(last) + 0.5) * edge;
       hi = float(begin + (fabs(begin) + edge) * 0x1p-20);
       lo = fmaxf(lo, float(end - (fabs(end) + edge) * 0x1p-20));
     }
@@ -512,14 +550,15 @@ struct Questions {
 
 // All answers from the n <= kFew tokens in s.cand, which are all that may be kept.
 // Each one's place is found by comparing it with all others, a power of two of
-// threads sharing them: no step waits for the one before, but the work grows with n^2
-// (n = 128: 1 us, 256: 4, 512: 15).
+// threads sharing them: no step waits for the one before, but the work grows with
+// n^2.  1 x 32000 with top-k 100, which lists 129 to 256 tokens, takes 16.9 us, and
+// 24.9 by bins; with 120, 257 to 512 tokens, 30.9 all with all and 26.4 by bins.
 template <int DT>
 __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, const SampleArgs& a,
                                             int out) {
   const int t = int(threadIdx.x);
   int log2_parts = 0;
-  while (log2_parts < 6 && uint32_t(kThreads >> (log2_parts + 1)) >= n) ++log2_parts;
+  while (log2_parts < 4 && uint32_t(kThreads >> (log2_parts + 1)) >= n) ++log2_parts;
   const uint32_t parts = 1u << log2_parts;
   __syncthreads();
   Shared::Weighed* const all = s.weighed;
@@ -540,10 +579,8 @@ __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const
     const Shared::Weighed x = all[j];
     if (x.order > own) before_count += 1u, before_mass += x.weight;
   }
-  for (uint32_t o = 1; o < parts; o <<= 1) {
-    before_count += uint32_t(__shfl_xor(int(before_count), int(o)));
-    before_mass += uint64_t(__shfl_xor((unsigned long long)(before_mass), int(o)));
-  }
+  before_mass = group_sum64(before_mass, parts);
+  before_count = uint32_t(group_sum64(before_count, parts));
   w = i < n ? all[i].weight : 0u;
   const bool one = i < n && part == 0;
   if (one && before_count == n - 1) s.kept = before_mass + w;  // the last of them all knows the total
@@ -649,21 +686,25 @@ __device__ __forceinline__ void narrow(Shared& s, const Row<DT>& row, const Shar
       cands = n;
     }
   }
-  if (t < 64) {  // one wave: a token a lane, each with the mass of those before it
-    n = min(uint32_t(__builtin_amdgcn_readfirstlane(int(n))), 64u);
-    const Shared::Weighed own = t < int(n) ? s.last[t] : Shared::Weighed{0u, 0u};
-    uint32_t ci = 0u;
-    uint64_t mi = 0u;
-    for (uint32_t j = 0; j < n; ++j) {
-      const uint64_t o = lane64(own.order, int(j)), w = lane64(own.weight, int(j));
-      if (o >= own.order) ci += 1u, mi += w;
-    }
-    const uint64_t after = by_count ? uint64_t(bc + ci) : bm + mi, before = by_count ? after - 1 : after - own.weight;
-    if (t < int(n) && before < goal && goal <= after) {
-      s.token = order_index(own.order);
-      s.weight = own.weight;
-      s.mass_to = bm + mi;
-    }
+  // Sixteen threads a token sum the mass of those up to it.
+  n = min(n, 64u);
+  const uint32_t i = uint32_t(t) >> 4;
+  const Shared::Weighed own = i < n ? s.last[i] : Shared::Weighed{~0ull, 0u};
+  uint32_t ci = 0u;
+  uint64_t mi = 0u;
+#pragma unroll
+  for (uint32_t j = uint32_t(t) & 15u; j < 64u; j += 16u) {
+    if (j >= n) continue;
+    const Shared::Weighed x = s.last[j];
+    if (x.order >= own.order) ci += 1u, mi += x.weight;
+  }
+  ci = uint32_t(group_sum64(ci, 16));
+  mi = group_sum64(mi, 16);
+  const uint64_t after = by_count ? uint64_t(bc + ci) : bm + mi, before = by_count ? after - 1 : after - own.weight;
+  if (i < n && (t & 15) == 0 && before < goal && goal <= after) {
+    s.token = order_index(own.order);
+    s.weight = own.weight;
+    s.mass_to = bm + mi;
   }
   __syncthreads();
 }
@@ -839,11 +880,10 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
     if (z > top || (z == top && i < at)) top = z, at = i;
   });
   // Groups of eight lanes; of two where threads have no tokens: top-k 50 of 1000
-  // would find 31 groups, and take 22.5 us for its long list instead of 11.0
-  // (4096: 9.2 with groups of eight, 11.9 of two, a longer floor search).
+  // would find 31 groups, and take 20.5 us for its long list instead of 9.5
+  // (4096: 8.2 with groups of eight, 9.5 of two, a longer floor search).
   const int log2_lanes = walk.hi - walk.lo >= kThreads ? 3 : 1;
-  uint32_t group = order_key(top);
-  for (int o = 1 << log2_lanes >> 1; o; o >>= 1) group = max(group, uint32_t(__shfl_xor(int(group), o)));
+  const uint32_t group = group_max32(order_key(top), 1 << log2_lanes);
   if ((lane & ((1 << log2_lanes) - 1)) == 0) maxima[t >> log2_lanes] = group;
   const uint64_t best = wave_max64(top > -INFINITY ? order_of(top, at) : 0u);
   if (lane == 0) s.wave_mass[t >> 6] = best;
@@ -860,7 +900,7 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   const Questions ask = questions(a, set, row);
   const Row<DT> r{data, a.vocab, set.weigh};
   // A thread whose largest token is below the floor has none to weigh: with top-k
-  // 50 of 256 x 131072 the second reading takes 7 us of 33 instead of 13 of 43.
+  // 50 of 256 x 131072 the call takes 32 us instead of 41.
   walk.each_wanted(top >= set.weigh.floor, s.fine_count, &s.base,
                    [&](int i, float z) { weigh_token(set, z, i, s.mass, s.count, s.cand, &s.n, kList); });
   __syncthreads();
@@ -881,27 +921,27 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   plan.answer(s, r, ask, n, a, row);
 }
 
-// One launch of a workgroup per row, or three of many per row.  us, f32, T 1 whole
-// / T 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096
-// 13.2 / 11.0 / 15.2 against 17.6 / 22.9 / 19.8; 1 x 32768 22.6 / 12.7 / 25.1 against
-// 19.7 / 15.5 / 22.3; 1 x 50000 28.2 / 14.1 / 31.8 against 19.8 / 15.9 / 22.0; 64 x
-// 65536 48.6 / 16.1 / 39.8 against 36.2 / 25.0 / 34.5; 128 x 65536 47.1 / 16.4 / 40.0
-// against 43.1 / 25.4 / 42.0; 128 x 100000 67.3 / 20.5 / 56.2 against 55.8 / 29.5 /
-// 51.6; 256 x 131072, a row for each CU, 83 / 33 / 84 against 94 / 55 / 91.
+// One launch of a workgroup per row, or three of many per row.  us, f32, T 1 whole / T
+// 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096 11.3 /
+// 8.2 / 13.8 against 16.0 / 21.5 / 18.4; 1 x 32768 20.2 / 11.3 / 23.1 against 18.2 /
+// 14.6 / 20.9; 1 x 50000 27.1 / 13.1 / 29.3 against 18.5 / 14.5 / 21.0; 64 x 65536 40.0
+// / 15.1 / 36.4 against 31.5 / 24.6 / 32.9; 128 x 65536 42.9 / 15.3 / 36.7 against 39.8
+// / 24.8 / 39.8; 128 x 100000 64.0 / 19.7 / 52.2 against 52.2 / 28.7 / 48.5; 256 x
+// 131072, a row for each CU, 85.9 / 32.0 / 79.2 against 95.6 / 55.3 / 86.2.
 bool row_per_workgroup(int32_t rows, int32_t vocab) { return vocab <= 32768 || vocab <= 512 * int64_t(rows); }
 
 // Slices of a row in the first two launches: of 2048 tokens or more, as many as
-// are resident at once (four workgroups on each of 256 CUs; twice as many took 8.6
-// and 22.0 us for 64 x 100003 bf16, instead of 6.8 and 15.0).  The result does not
-// depend on it, nor on the workgroups that gather in the third.
+// are resident at once (four workgroups on each of 256 CUs; with twice as many 64 x
+// 100003 bf16, whole / top-p 0.9, take 41.8 / 43.3 us, instead of 34.8 / 36.0).  The
+// result does not depend on it, nor on the workgroups that gather in the third.
 int slice_count(int32_t rows, int32_t vocab) {
   int s = (vocab + 2047) / 2048;
   const int fill = 1024 / rows > 0 ? 1024 / rows : 1;
   s = s < fill ? s : fill;
   return s < kMaxSlices ? s : kMaxSlices;
 }
-// Workgroups of a row in the third: of 8192 tokens or more, 256 in all (64 x 100000,
-// whole / top-p 0.9: 40.7 / 38.6 us; one per row 54.0 / 43.2, 512 in all 50.5 / 51.9).
+// Workgroups of a row in the third: of 8192 tokens or more, 256 in all (the same
+// calls: 34.8 / 36.0 us; one per row 41.4 / 39.7, 512 in all 43.5 / 48.6).
 int part_count(int32_t rows, int32_t vocab) {
   const int p = (vocab + 8191) / 8192, fill = 256 / rows > 0 ? 256 / rows : 1;
   return p < fill ? p : fill;
