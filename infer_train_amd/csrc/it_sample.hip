@@ -118,12 +118,13 @@ struct Weigher {
   float top;      // max z
   float floor;    // tokens below weigh nothing, fail min-p or cannot be among the first k
   double bits;    // log2(e) / T
+  double per_bit; // its reciprocal: z for a factor of two
   double least;   // min-p, or the smallest weight that does not round to nothing
   double below;   // z - top of 2^-64; lower ones weigh no more
   double bin_bits, exp2[10], unit, zero, whole;
   __device__ __forceinline__ void constants() {
     // inf - inf is NaN, of which fmax makes 0: tokens at a top of +inf weigh 1.
-    below = top < INFINITY ? -64.0 / bits : 0.0;
+    below = top < INFINITY ? -64.0 * per_bit : 0.0;
     bin_bits = -kBinsPerBit * bits;
 #pragma unroll
     for (int i = 0; i < 10; ++i) exp2[i] = i == 8 ? vector(kExp2[i]) : scalar(kExp2[i]);
@@ -335,13 +336,14 @@ struct Settings {
     if (best == 0u || !(temp > 0.0f)) return false;  // uniform
     weigh.top = order_value(best);
     weigh.bits = 1.4426950408889634 / double(temp);
+    weigh.per_bit = 0.6931471805599453 * double(temp);
     const double share = min_p > 0.0f ? fmin(double(min_p), 1.0) : 0.0;  // NaN: off
     weigh.least = fmax(share, kLeast);
     // Below floor a weight is below `least`: z - top < T ln(least), widened by
     // fp32's rounding.
     weigh.floor = weigh.top;
     if (weigh.top < INFINITY) {
-      const double low = double(weigh.top) + (share > kLeast ? log2(share) : -45.0) / weigh.bits;
+      const double low = double(weigh.top) + (share > kLeast ? log2(share) : -45.0) * weigh.per_bit;
       weigh.floor = float(low - fabs(low) * 0x1p-20);
     }
     // Whatever the floor, a token at -inf is never kept.
@@ -460,14 +462,13 @@ __device__ __forceinline__ Scan block_scan(Shared& s, uint32_t count, uint64_t m
   __syncthreads();  // the sums of the call before are read
   if (lane == 63) s.wave_count[wave] = c, s.wave_mass[wave] = m;
   __syncthreads();
-  Scan r{m - mass, 0u, c - count, 0u};
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) r.count += s.wave_count[w], r.mass += s.wave_mass[w];
-    r.total_count += s.wave_count[w];
-    r.total_mass += s.wave_mass[w];
-  }
-  return r;
+  static_assert(kWaves == 16, "a wave's sums in each lane of a DPP row");
+  const uint32_t wave_c = s.wave_count[lane & 15];
+  const uint64_t wave_m = s.wave_mass[lane & 15], to_m = wave_inclusive_sum64(lane < 16 ? wave_m : 0u);
+  const uint32_t to_c = uint32_t(wave_inclusive_sum(int(lane < 16 ? wave_c : 0u)));
+  const uint64_t before_m = lane64(to_m, wave) - lane64(wave_m, wave);
+  const uint32_t before_c = uint32_t(__builtin_amdgcn_readlane(int(to_c), wave) - __builtin_amdgcn_readlane(int(wave_c), wave));
+  return {before_m + m - mass, lane64(to_m, 15), before_c + c - count, uint32_t(__builtin_amdgcn_readlane(int(to_c), 15))};
 }
 
 // What is before a thread's N consecutive bins of LDS, which stay there.
@@ -521,8 +522,8 @@ struct Row {
   __device__ __forceinline__ void span(int first, int last, float& lo, float& hi) const {
     lo = weigh.floor;
     hi = INFINITY;
-    if (weigh.top < INFINITY && weigh.bits > 0.0) {
-      const double edge = 1.0 / (kBinsPerBit * weigh.bits), top = double(weigh.top);
+    if (weigh.top < INFINITY && weigh.per_bit < double(INFINITY)) {
+      const double edge = weigh.per_bit / kBinsPerBit, top = double(weigh.top);
       const double begin = top - (double(first) - 0.5) * edge, end = top - (double(last) + 0.5) * edge;
       hi = float(begin + (fabs(begin) + edge) * 0x1p-20);
       lo = fmaxf(lo, float(end - (fabs(end) + edge) * 0x1p-20));
