@@ -168,11 +168,6 @@ def test_transpose_is_the_gradient(layout):
 
 
 # ---- with the append ---------------------------------------------------------
-def expected_pools(cache, k_rot, v, slots):
-    """Cache bytes after appending float rows with the library's own plain append (its formats are pinned elsewhere)."""
-    cache.append(k_rot, v, slots)
-
-
 APPEND = [  # cache, source, hq, hkv, D, n_dims, layout
     ("bf16", "bf16", 28, 4, 128, 128, "half"), ("f16", "f16", 6, 3, 96, 32, "half"), ("f32", "f32", 8, 2, 64, 64, "interleaved"),
     ("bf16", "f32", 4, 4, 128, 96, "interleaved"), ("f32", "bf16", 2, 1, 256, 256, "half"), ("f16", "bf16", 2, 2, 24, 10, "half"),
