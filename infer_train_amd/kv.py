@@ -91,15 +91,12 @@ def _on(t: torch.Tensor, index: int) -> int:
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, name: str, index: int) -> Tuple[int, int]:
-    """Address and token stride of a [tokens, heads, head_dim] tensor on
-    device `index` whose tokens are each contiguous."""
+def _rows(t: torch.Tensor, name: str, index: int, heads: int, dim: int) -> Tuple[int, int]:
+    """Address and token stride of a [tokens, heads, dim] tensor on device
+    `index` whose tokens are each contiguous."""
     if t.get_device() != index:
         raise ValueError(f"{name}: tensor on cuda:{index} expected")
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim]")
     token, head, element = t.stride()
-    _, heads, dim = t.shape
     if (head != dim and heads != 1) or (element != 1 and dim != 1):
         raise ValueError(f"{name}: each token's heads must be contiguous")
     return t.data_ptr(), token
@@ -141,15 +138,17 @@ class Rotary:
         """x [n_tokens, n_heads, head_dim] (any token stride) rotated to int32
         positions [n_tokens]; transpose: the gradient of that rotation (with
         magnitude 1 its inverse).  out may be x itself."""
-        at, stride = _rows(x, "x", self.device)
+        if x.dim() != 3:
+            raise ValueError("x must be [tokens, heads, head_dim]")
         n, heads, d = x.shape
+        at, stride = _rows(x, "x", self.device, heads, d)
         if positions.dtype != torch.int32 or positions.numel() != n:
             raise TypeError("positions must be int32, one per token")
         if out is None:
             out = torch.empty_like(x, memory_format=torch.contiguous_format)
         elif out.dtype != x.dtype or out.shape != x.shape:
             raise TypeError("out must have x's shape and dtype")
-        to, to_stride = _rows(out, "out", self.device)
+        to, to_stride = _rows(out, "out", self.device, heads, d)
         _check(call.it_rotary_apply(self._at, at, torch_dtype_id(x.dtype), stride, _on(positions, self.device), n, heads, d,
                                     int(bool(transpose)), to, to_stride, _raw_stream(self.device)))
         return out
@@ -318,32 +317,33 @@ class PagedKvCache:
         q None: k and v only."""
         if slot_mapping.dtype != torch.int64 or positions.dtype != torch.int32:
             raise TypeError("slot_mapping must be int64 and positions int32")
-        n, kind = slot_mapping.numel(), k.dtype
-        row = (n, self.n_kv_heads, self.head_dim)
+        n, kind, index = slot_mapping.numel(), k.dtype, self._index
+        row = n, kv_heads, dim = n, self.n_kv_heads, self.head_dim
         if positions.numel() != n or k.shape != row or v.shape != row:
             raise ValueError("k, v must be [n_tokens, n_kv_heads, head_dim], with a slot and a position per token")
         if v.dtype != kind or (q is not None and q.dtype != kind):
             raise TypeError("q, k, v must have one dtype")
-        (ka, ks), (va, vs) = _rows(k, "k", self._index), _rows(v, "v", self._index)
+        (ka, ks), (va, vs) = _rows(k, "k", index, kv_heads, dim), _rows(v, "v", index, kv_heads, dim)
         src_id = torch_dtype_id(kind)
         qa = oa = None
         qs = heads = out_id = 0
         if q is not None:
-            qa, qs = _rows(q, "q", self._index)
-            heads = q.shape[1]
-            if q.shape != (n, heads, row[2]):
+            shape = q.shape
+            if len(shape) != 3 or shape[0] != n or shape[2] != dim:
                 raise ValueError("q must be [n_tokens, n_heads, head_dim]")
+            heads = shape[1]
+            qa, qs = _rows(q, "q", index, heads, dim)
             if q_out is None:
                 q_out = torch.empty_like(q, dtype=q_out_dtype, memory_format=torch.contiguous_format)
                 oa, out_id = q_out.data_ptr(), src_id if q_out_dtype is None else torch_dtype_id(q_out_dtype)
-            elif q_out.shape != q.shape:
+            elif q_out.shape != shape:
                 raise ValueError("q_out must have q's shape")
             else:
-                oa, out_id = _on(q_out, self._index), torch_dtype_id(q_out.dtype)
+                oa, out_id = _on(q_out, index), torch_dtype_id(q_out.dtype)
         elif q_out is not None:
             raise ValueError("q_out without q")
         _check(call.it_kv_append_rotary(self._at, rotary._at, qa, ka, va, src_id, qs, ks, vs, heads,
-                                        _on(slot_mapping, self._index), _on(positions, self._index), n, oa, out_id, _raw_stream(self._index)))
+                                        _on(slot_mapping, index), _on(positions, index), n, oa, out_id, _raw_stream(index)))
         return q_out
 
     def gather(self, block_tables: torch.Tensor, ctx_lens: torch.Tensor, start_pos: Optional[torch.Tensor],
