@@ -56,7 +56,7 @@ constexpr uint32_t kDeadKey = 0x007FFFFFu;  // order_key(-inf)
 struct RowState {
   uint32_t n_gathered, ticket, pad[30];
   uint32_t n_list[kMaxSlices];              // tokens of each slice that are listed, or more than its room
-  uint64_t best[kMaxSlices];               // order of each slice's first token, 0: nothing above -inf
+  uint64_t best[kMaxSlices];               // order of each slice's largest token (the first of equals where the row is greedy), 0: nothing above -inf
   uint32_t group_max[kMaxSlices * kGroups];
   uint32_t count[kBins];
   uint64_t mass[kBins];
@@ -279,6 +279,25 @@ __device__ __forceinline__ uint32_t wave_sums(uint32_t& x) {
   return uint32_t(__builtin_amdgcn_readlane(int(x), 63));
 }
 
+__device__ __forceinline__ float temperature_of(const SampleArgs& a, int row) {
+  return a.temperatures ? a.temperatures[row] : a.temperature;
+}
+// A thread's largest token, and which it is where the row takes the first of the
+// order: the index is three more instructions a token, which took one workgroup 2
+// us of the 4 for 32000.
+template <class W>
+__device__ __forceinline__ void find_top(W& walk, bool greedy, float& top, int& at) {
+  top = -INFINITY;
+  at = 0;
+  if (greedy) {  // uniform
+    walk.each([&](int i, float z) {
+      if (z > top || (z == top && i < at)) top = z, at = i;
+    });
+  } else {
+    walk.each([&](int, float z) { top = fmaxf(top, z); });
+  }
+}
+
 template <int DT>
 __global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
   __shared__ uint64_t best_of[kSliceWaves];
@@ -287,13 +306,11 @@ __global__ __launch_bounds__(kSliceThreads) void sample_maxima(SampleArgs a) {
   if (slice == 0 && threadIdx.x == 0)  // what the second launch adds to
     rs.n_gathered = rs.ticket = 0u;
   for (int b = slice * kSliceThreads + int(threadIdx.x); b < kBins; b += a.slices * kSliceThreads) rs.count[b] = 0u, rs.mass[b] = 0u;
-  float top = -INFINITY;
-  int at = kMaxVocab;
+  float top;
+  int at;
   Walk<DT, kSliceThreads> walk(a.logits + int64_t(blockIdx.y) * a.row_bytes, a.vocab, slice, a.slices);
   walk.start();
-  walk.each([&](int i, float z) {
-    if (z > top || (z == top && i < at)) top = z, at = i;
-  });
+  find_top(walk, !(temperature_of(a, int(blockIdx.y)) > 0.0f), top, at);
   uint64_t best = top > -INFINITY ? order_of(top, at) : 0u;
   const uint32_t group = group_max32(order_key(top), 32);
   if ((lane & 31) == 0) rs.group_max[slice * kGroups + wave * 2 + (lane >> 5)] = group;
@@ -327,9 +344,9 @@ struct Settings {
       group[j] = i < groups ? maxima[i] : 0u;
     }
   }
-  // first: the place of the row's first token, 0 where nothing is above -inf.
+  // first: the place of the row's largest token, 0 where nothing is above -inf.
   __device__ __forceinline__ bool derive(const SampleArgs& a, int row, uint64_t first) {
-    const float temp = a.temperatures ? a.temperatures[row] : a.temperature;
+    const float temp = temperature_of(a, row);
     const float min_p = a.min_ps ? a.min_ps[row] : a.min_p;
     top_k = a.top_ks ? a.top_ks[row] : a.top_k;
     best = lane64(first, 0);
@@ -872,14 +889,12 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   __shared__ uint32_t maxima[kRowGroups];
   const int t = int(threadIdx.x), lane = t & 63, row = int(blockIdx.x);
   const char* const data = a.logits + int64_t(row) * a.row_bytes;
-  float top = -INFINITY;
-  int at = kMaxVocab;
+  float top;
+  int at;
   Walk<DT, kThreads> walk(data, a.vocab, 0, 1);
   walk.start();
   for (int b = t; b < kBins; b += kThreads) s.count[b] = 0u, s.mass[b] = 0u;
-  walk.each([&](int i, float z) {
-    if (z > top || (z == top && i < at)) top = z, at = i;
-  });
+  find_top(walk, !(temperature_of(a, row) > 0.0f), top, at);
   // Groups of eight lanes; of two where threads have no tokens: top-k 50 of 1000
   // would find 31 groups, and take 20.5 us for its long list instead of 9.5
   // (4096: 8.2 with groups of eight, 9.5 of two, a longer floor search).
