@@ -458,7 +458,7 @@ struct Shared {
   uint64_t wave_mass[kWaves];
   uint32_t wave_count[kWaves];
   uint32_t n, base;
-  uint64_t kept;
+  uint64_t kept[2];
   struct Found {
     uint64_t before_mass, mass;
     uint32_t before_count, count, bin;
@@ -566,7 +566,8 @@ struct Questions {
   }
 };
 
-// All answers from the n <= kFew tokens in s.cand, which are all that may be kept.
+// All answers from the n <= kFew tokens in s.cand (a barrier before), which are all
+// that may be kept.
 // Each one's place is found by comparing it with all others, a power of two of
 // threads sharing them: no step waits for the one before, but the work grows with
 // n^2.  1 x 32000 with top-k 100, which lists 129 to 256 tokens, takes 16.9 us, and
@@ -578,7 +579,6 @@ __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const
   int log2_parts = 0;
   while (log2_parts < 4 && uint32_t(kThreads >> (log2_parts + 1)) >= n) ++log2_parts;
   const uint32_t parts = 1u << log2_parts;
-  __syncthreads();
   Shared::Weighed* const all = s.weighed;
   uint64_t own = 0u, w = 0u;
   int bin = 0;
@@ -591,35 +591,32 @@ __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const
   const uint32_t i = uint32_t(t) >> log2_parts, part = uint32_t(t) & (parts - 1);
   own = i < n ? all[i].order : ~0ull;
   uint32_t before_count = 0u;
-  uint64_t before_mass = 0u;
+  uint64_t before_mass = 0u, kept = 0u;
 #pragma unroll 4
   for (uint32_t j = part; j < n; j += parts) {
     const Shared::Weighed x = all[j];
+    kept += x.weight;
     if (x.order > own) before_count += 1u, before_mass += x.weight;
   }
+  kept = group_sum64(kept, parts);
   before_mass = group_sum64(before_mass, parts);
   before_count = uint32_t(group_sum64(before_count, parts));
   w = i < n ? all[i].weight : 0u;
   const bool one = i < n && part == 0;
-  if (one && before_count == n - 1) s.kept = before_mass + w;  // the last of them all knows the total
-  __syncthreads();
-  uint64_t kept = s.kept;
-  __syncthreads();
   // f() for the token at which the count, or the mass, reaches the goal.
   const auto at = [&](bool by_count, uint64_t goal, auto&& f) {
     const uint64_t before = by_count ? uint64_t(before_count) : before_mass, after = before + (by_count ? 1u : w);
     if (one && before < goal && goal <= after) f();
   };
   if (ask.top_k > 0 && ask.top_k < n) {
-    at(true, ask.top_k, [&] { s.kept = before_mass + w; });
+    at(true, ask.top_k, [&] { s.kept[0] = before_mass + w; });
     __syncthreads();
-    kept = s.kept;
-    __syncthreads();
+    kept = s.kept[0];
   }
   if (ask.cuts()) {
-    at(false, ask.cut(kept), [&] { s.kept = before_mass + w; });
+    at(false, ask.cut(kept), [&] { s.kept[1] = before_mass + w; });
     __syncthreads();
-    kept = s.kept;
+    kept = s.kept[1];
   }
   at(false, ask.draw(kept), [&] {
     a.tokens[out] = order_index(own);
@@ -656,11 +653,9 @@ __device__ __forceinline__ void narrow(Shared& s, const Row<DT>& row, const Shar
       row.each(order_value(lo), order_value(hi), member);
     }
   };
-  // Their number; the first 64 of them in s.last.
+  // Their number; the first 64 of them in s.last.  s.n is 0 before, as it is when
+  // narrow() begins, and at the end of each turn below.
   const auto collect = [&] {
-    __syncthreads();
-    if (t == 0) s.n = 0u;
-    __syncthreads();
     each_in([&](uint64_t o, uint64_t w) {
       const uint32_t at = atomicAdd(&s.n, 1u);
       if (at < 64) s.last[at] = {o, w};
@@ -780,11 +775,12 @@ struct Plan {
   __device__ __forceinline__ void answer(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, const SampleArgs& a,
                                          int out) const {
     uint64_t kept = bins.total_mass;
+    __syncthreads();
     for (int question = by_k ? 0 : 1; question < 3; ++question) {
       if (question == 1 && !ask.cuts()) continue;
       const uint64_t goal = question == 0 ? ask.top_k : question == 1 ? ask.cut(kept) : ask.draw(kept);
-      __syncthreads();
       bins.find(s.count, s.mass, s.found[question], question == 0, goal);
+      if (threadIdx.x == 0) s.n = 0u;
       __syncthreads();
       narrow(s, row, s.found[question], question == 0, goal, n);
       if (question < 2) kept = s.mass_to;
@@ -835,6 +831,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw(SampleArgs a) {
   };
   if (from_list && n_listed <= kFew) {
     each_listed([&](uint64_t o, uint32_t at) { s.cand[at] = o; });
+    __syncthreads();
     answer_from(s, r, ask, n_listed, a, row);
     return;
   }
