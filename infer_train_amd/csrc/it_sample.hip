@@ -751,15 +751,18 @@ struct Plan {
       const uint64_t to = s.found[2].before_mass + s.found[2].mass;
       high = to < high ? to : high;
     }
+    // All of this is fp64 and 64-bit work in all waves of the workgroup: what nothing
+    // asks for is left out.
     bins.find(s.count, s.mass, s.found[3], false, ask.draw(low));
-    bins.find(s.count, s.mass, s.found[4], false, ask.draw(high));
+    if (low != high) bins.find(s.count, s.mass, s.found[4], false, ask.draw(high));
     if (threadIdx.x == 0) s.n = 0u;
     __syncthreads();
-    const uint32_t d_first = s.found[3].bin, d_last = s.found[4].bin;
-    row.span(int(d_first), int(d_last), lo[0], hi[0]);
-    row.span(int(ask.cuts() ? p_first : d_first), int(ask.cuts() ? p_last : d_last), lo[1], hi[1]);
-    row.span(int(by_k ? k_bin : d_first), int(by_k ? k_bin : d_last), lo[2], hi[2]);
-    lowest = fminf(fminf(lo[0], lo[1]), lo[2]);
+    row.span(int(s.found[3].bin), int(s.found[low != high ? 4 : 3].bin), lo[0], hi[0]);
+    lo[1] = lo[2] = lowest = lo[0];
+    hi[1] = hi[2] = hi[0];
+    if (ask.cuts()) row.span(int(p_first), int(p_last), lo[1], hi[1]);
+    if (by_k) row.span(int(k_bin), int(k_bin), lo[2], hi[2]);
+    lowest = fminf(fminf(lowest, lo[1]), lo[2]);
   }
   // A token of the row into s.cand, if it is one of them; their number in s.n.
   template <class F>
@@ -779,10 +782,11 @@ struct Plan {
     for (int question = by_k ? 0 : 1; question < 3; ++question) {
       if (question == 1 && !ask.cuts()) continue;
       const uint64_t goal = question == 0 ? ask.top_k : question == 1 ? ask.cut(kept) : ask.draw(kept);
-      bins.find(s.count, s.mass, s.found[question], question == 0, goal);
+      const bool known = question == 2 && !by_k && !ask.cuts();  // the plan's first answer
+      if (!known) bins.find(s.count, s.mass, s.found[question], question == 0, goal);
       if (threadIdx.x == 0) s.n = 0u;
       __syncthreads();
-      narrow(s, row, s.found[question], question == 0, goal, n);
+      narrow(s, row, s.found[known ? 3 : question], question == 0, goal, n);
       if (question < 2) kept = s.mass_to;
     }
     if (threadIdx.x == 0) {
