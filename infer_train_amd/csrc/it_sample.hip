@@ -570,8 +570,8 @@ struct Questions {
 // that may be kept.
 // Each one's place is found by comparing it with all others, a power of two of
 // threads sharing them: no step waits for the one before, but the work grows with
-// n^2.  1 x 32000 with top-k 100, which lists 129 to 256 tokens, takes 16.9 us, and
-// 24.9 by bins; with 120, 257 to 512 tokens, 30.9 all with all and 26.4 by bins.
+// n^2.  1 x 32000 with top-k 100, which lists 129 to 256 tokens, takes 13.4 us, and
+// 20.3 by bins; with 120, 257 to 512 tokens, 24.3 all with all and 21.4 by bins.
 template <int DT>
 __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, const SampleArgs& a,
                                             int out) {
@@ -897,8 +897,8 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   for (int b = t; b < kBins; b += kThreads) s.count[b] = 0u, s.mass[b] = 0u;
   find_top(walk, !(temperature_of(a, row) > 0.0f), top, at);
   // Groups of eight lanes; of two where threads have no tokens: top-k 50 of 1000
-  // would find 31 groups, and take 20.5 us for its long list instead of 9.5
-  // (4096: 8.2 with groups of eight, 9.5 of two, a longer floor search).
+  // would find 31 groups, and take 18.0 us for its long list instead of 9.3
+  // (4096: 7.8 with groups of eight, 9.2 of two, a longer floor search).
   const int log2_lanes = walk.hi - walk.lo >= kThreads ? 3 : 1;
   const uint32_t group = group_max32(order_key(top), 1 << log2_lanes);
   if ((lane & ((1 << log2_lanes) - 1)) == 0) maxima[t >> log2_lanes] = group;
@@ -939,17 +939,17 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
 }
 
 // One launch of a workgroup per row, or three of many per row.  us, f32, T 1 whole / T
-// 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096 11.3 /
-// 8.2 / 13.8 against 16.0 / 21.5 / 18.4; 1 x 32768 20.2 / 11.3 / 23.1 against 18.2 /
-// 14.6 / 20.9; 1 x 50000 27.1 / 13.1 / 29.3 against 18.5 / 14.5 / 21.0; 64 x 65536 40.0
-// / 15.1 / 36.4 against 31.5 / 24.6 / 32.9; 128 x 65536 42.9 / 15.3 / 36.7 against 39.8
-// / 24.8 / 39.8; 128 x 100000 64.0 / 19.7 / 52.2 against 52.2 / 28.7 / 48.5; 256 x
-// 131072, a row for each CU, 85.9 / 32.0 / 79.2 against 95.6 / 55.3 / 86.2.
+// 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096 8.9 /
+// 7.6 / 11.5 against 13.8 / 19.2 / 16.4; 1 x 32768 16.3 / 8.9 / 19.2 against 15.9 /
+// 13.9 / 18.7; 1 x 50000 20.4 / 9.4 / 24.6 against 15.8 / 14.2 / 18.9; 64 x 65536 31.8
+// / 10.5 / 30.4 against 28.6 / 23.6 / 30.8; 128 x 65536 36.5 / 11.2 / 31.0 against 37.0
+// / 23.8 / 37.4; 128 x 100000 53.8 / 17.8 / 49.0 against 49.2 / 27.6 / 46.4; 256 x
+// 131072, a row for each CU, 82.6 / 31.3 / 76.7 against 93.2 / 53.1 / 82.8.
 bool row_per_workgroup(int32_t rows, int32_t vocab) { return vocab <= 32768 || vocab <= 512 * int64_t(rows); }
 
 // Slices of a row in the first two launches: of 2048 tokens or more, as many as
 // are resident at once (four workgroups on each of 256 CUs; with twice as many 64 x
-// 100003 bf16, whole / top-p 0.9, take 41.8 / 43.3 us, instead of 34.8 / 36.0).  The
+// 100003 bf16, whole / top-p 0.9, take 38.9 / 40.6 us, instead of 31.9 / 32.9).  The
 // result does not depend on it, nor on the workgroups that gather in the third.
 int slice_count(int32_t rows, int32_t vocab) {
   int s = (vocab + 2047) / 2048;
@@ -958,7 +958,7 @@ int slice_count(int32_t rows, int32_t vocab) {
   return s < kMaxSlices ? s : kMaxSlices;
 }
 // Workgroups of a row in the third: of 8192 tokens or more, 256 in all (the same
-// calls: 34.8 / 36.0 us; one per row 41.4 / 39.7, 512 in all 43.5 / 48.6).
+// calls: 31.9 / 32.9 us; one per row 41.3 / 36.7, 512 in all 38.9 / 43.6).
 int part_count(int32_t rows, int32_t vocab) {
   const int p = (vocab + 8191) / 8192, fill = 256 / rows > 0 ? 256 / rows : 1;
   return p < fill ? p : fill;

@@ -22,7 +22,9 @@ def sample_workspace(n_rows: int, vocab: int, device) -> torch.Tensor:
 def _per_row(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, index: int) -> int:
     if t.dtype != dtype or t.numel() != n:
         raise TypeError(f"{name} must be {dtype}, one per row")
-    return _on(t, index)
+    if t.get_device() != index or not t.is_contiguous():
+        return _on(t, index)  # which raises
+    return t.data_ptr()
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torch.Tensor] = 1.0,
@@ -52,8 +54,14 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     us = _per_row(u, "u", torch.float32, n, index)
     if tokens is None:
         tokens = torch.empty_like(u, dtype=torch.int32)
+        at_tokens = tokens.data_ptr()
+    else:
+        at_tokens = _per_row(tokens, "tokens", torch.int32, n, index)
     if probs is None:
         probs = torch.empty_like(u)
+        at_probs = probs.data_ptr()
+    else:
+        at_probs = _per_row(probs, "probs", torch.float32, n, index)
     need = 0
     if ws is None:
         need = call.it_sample_workspace(n, vocab)
@@ -62,9 +70,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
     else:
         need = ws.nbytes
     args = (logits.data_ptr(), torch_dtype_id(logits.dtype), logits.stride(0), n, vocab, us, temperatures, top_ks, top_ps, min_ps,
-            float(temperature), int(top_k), float(top_p), float(min_p), _per_row(tokens, "tokens", torch.int32, n, index),
-            _per_row(probs, "probs", torch.float32, n, index), None if ws is None else _on(ws, index), need, _raw_stream(index))
-    if torch.cuda.current_device() == index:
+            float(temperature), int(top_k), float(top_p), float(min_p), at_tokens, at_probs,
+            None if ws is None else _on(ws, index), need, _raw_stream(index))
+    if torch._C._cuda_getDevice() == index:
         _check(call.it_sample(*args))
     else:
         with torch.cuda.device(index):
