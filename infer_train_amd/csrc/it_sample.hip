@@ -939,26 +939,31 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
 }
 
 // One launch of a workgroup per row, or three of many per row.  us, f32, T 1 whole / T
-// 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096 8.9 /
-// 7.6 / 11.5 against 13.8 / 19.2 / 16.4; 1 x 32768 16.3 / 8.9 / 19.2 against 15.9 /
-// 13.9 / 18.7; 1 x 50000 20.4 / 9.4 / 24.6 against 15.8 / 14.2 / 18.9; 64 x 65536 31.8
-// / 10.5 / 30.4 against 28.6 / 23.6 / 30.8; 128 x 65536 36.5 / 11.2 / 31.0 against 37.0
-// / 23.8 / 37.4; 128 x 100000 53.8 / 17.8 / 49.0 against 49.2 / 27.6 / 46.4; 256 x
-// 131072, a row for each CU, 82.6 / 31.3 / 76.7 against 93.2 / 53.1 / 82.8.
+// 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096 9.2 /
+// 7.7 / 11.8 against 14.0 / 18.9 / 16.2; 1 x 32768 16.2 / 9.0 / 19.0 against 16.1 /
+// 13.9 / 18.7; 1 x 50000 20.1 / 9.5 / 23.1 against 15.9 / 14.3 / 18.2; 64 x 65536 38.4
+// / 10.5 / 30.4 against 29.2 / 17.0 / 28.4; 128 x 65536 33.4 / 11.2 / 31.0 against 35.5
+// / 23.5 / 37.2; 128 x 100000 52.1 / 18.2 / 49.6 against 46.5 / 27.4 / 46.3; 256 x
+// 131072, a row for each CU, 81.3 / 31.2 / 76.8 against 91.6 / 52.6 / 82.8.
 bool row_per_workgroup(int32_t rows, int32_t vocab) { return vocab <= 32768 || vocab <= 512 * int64_t(rows); }
 
-// Slices of a row in the first two launches: of 2048 tokens or more, as many as
-// are resident at once (four workgroups on each of 256 CUs; with twice as many 64 x
-// 100003 bf16, whole / top-p 0.9, take 38.9 / 40.6 us, instead of 31.9 / 32.9).  The
-// result does not depend on it, nor on the workgroups that gather in the third.
+// Slices of a row in the first two launches: of 2048 tokens or more; two workgroups
+// on each of 256 CUs, each of which adds its bins to the row's; up to four where a row
+// would have fewer than eight slices, whose maxima bound top-k up to 128.  us with
+// two / three / four workgroups a CU (eight slices a row, twelve, sixteen), 64 x 100003
+// bf16: whole 31.4 / 30.7 / 33.0, T 0.8 with top-k 50 and top-p 0.95 17.8 / 21.5 / 23.9,
+// top-p 0.9 31.0 / 31.0 / 33.0.  The result does not depend on it, nor on the
+// workgroups that gather in the third.
 int slice_count(int32_t rows, int32_t vocab) {
   int s = (vocab + 2047) / 2048;
-  const int fill = 1024 / rows > 0 ? 1024 / rows : 1;
+  const int most = 1024 / rows > 0 ? 1024 / rows : 1, least = most < 8 ? most : 8;
+  const int fill = 512 / rows > least ? 512 / rows : least;
   s = s < fill ? s : fill;
   return s < kMaxSlices ? s : kMaxSlices;
 }
 // Workgroups of a row in the third: of 8192 tokens or more, 256 in all (the same
-// calls: 31.9 / 32.9 us; one per row 41.3 / 36.7, 512 in all 38.9 / 43.6).
+// calls, whole / top-p 0.9: 31.4 / 31.0 us; one per row 42.6 / 34.2, 512 in all 36.2 /
+// 40.9).
 int part_count(int32_t rows, int32_t vocab) {
   const int p = (vocab + 8191) / 8192, fill = 256 / rows > 0 ? 256 / rows : 1;
   return p < fill ? p : fill;
