@@ -333,6 +333,7 @@ struct Settings {
   bool listed;  // few tokens can be kept: they are listed
   static constexpr int kLoads = kMaxSlices * kGroups / 64;
   uint32_t group[kLoads];
+  __device__ __forceinline__ bool plain() const { return !listed && top_k <= 0; }  // uniform
   // The group maxima, 64 to a register, before it is known whether they count.
   __device__ __forceinline__ void load_groups(const SampleArgs& a, const uint32_t* maxima, int n) {
     const int lane = int(threadIdx.x & 63);
@@ -411,6 +412,15 @@ __device__ __forceinline__ void weigh_token(const Settings& set, float z, int in
   }
 }
 
+// The same where no list or count is asked for: one branch a token (256 x 131072 with
+// top-p 76.2 -> 72.4 us, 1 x 32000 whole 15.9 -> 14.5).
+__device__ __forceinline__ void weigh_plain(const Settings& set, float z, uint64_t* mass) {
+  uint64_t w;
+  int b;
+  const int kept = int(set.weigh(z, w, b)) & int(z >= set.weigh.floor);
+  if (kept) atomicAdd(reinterpret_cast<unsigned long long*>(&mass[b]), (unsigned long long)(w));
+}
+
 template <int DT>
 __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
   __shared__ uint64_t mass[kBins], list[kSliceList];
@@ -428,7 +438,8 @@ __global__ __launch_bounds__(kSliceThreads, 8) void sample_weigh(SampleArgs a) {
   if (t == 0) n = 0u;
   __syncthreads();
   const uint32_t room = slice_list(a.slices);
-  walk.each([&](int i, float z) { weigh_token(set, z, i, mass, count, list, &n, room); });
+  if (set.plain()) walk.each([&](int, float z) { weigh_plain(set, z, mass); });
+  else walk.each([&](int i, float z) { weigh_token(set, z, i, mass, count, list, &n, room); });
   __syncthreads();
   if (set.listed) {  // each slice in its own part of the row's list
     if (t == 0) rs.n_list[slice] = n;
@@ -918,8 +929,13 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   const Row<DT> r{data, a.vocab, set.weigh};
   // A thread whose largest token is below the floor has none to weigh: with top-k
   // 50 of 256 x 131072 the call takes 32 us instead of 41.
-  walk.each_wanted(top >= set.weigh.floor, s.fine_count, &s.base,
-                   [&](int i, float z) { weigh_token(set, z, i, s.mass, s.count, s.cand, &s.n, kList); });
+  if (set.plain()) {
+    walk.start();
+    walk.each([&](int, float z) { weigh_plain(set, z, s.mass); });
+  } else {
+    walk.each_wanted(top >= set.weigh.floor, s.fine_count, &s.base,
+                     [&](int i, float z) { weigh_token(set, z, i, s.mass, s.count, s.cand, &s.n, kList); });
+  }
   __syncthreads();
   const uint32_t n_listed = s.n;
   if (set.listed && n_listed <= kFew) {
