@@ -111,9 +111,9 @@ __device__ __forceinline__ double vector(double x) {
 }
 
 // A row's weights, the same in all its threads.  fp64 work bounds them (an fma of
-// every token of 256 x 131072 takes 1.4 us), so whole numbers are taken from the
-// low word of a sum with 1.5 x 2^52 and exponents are added as integers: 35 us,
-// and 38 with fp64's roundings, conversions and ldexp.
+// every token of 256 x 131072 takes 1.4 us of 30), so whole numbers are taken from the
+// low word of a sum with 1.5 x 2^52 and exponents are added as integers: 3 us less
+// than with fp64's roundings, conversions and ldexp.
 struct Weigher {
   float top;      // max z
   float floor;    // tokens below weigh nothing, fail min-p or cannot be among the first k
@@ -581,8 +581,8 @@ struct Questions {
 // that may be kept.
 // Each one's place is found by comparing it with all others, a power of two of
 // threads sharing them: no step waits for the one before, but the work grows with
-// n^2.  1 x 32000 with top-k 100, which lists 129 to 256 tokens, takes 13.4 us, and
-// 20.3 by bins; with 120, 257 to 512 tokens, 24.3 all with all and 21.4 by bins.
+// n^2.  1 x 32000 with top-k 100, which lists 129 to 256 tokens, takes 13.0 us, and
+// 20.0 by bins; with 120, 257 to 512 tokens, 27.4 all with all and 21.6 by bins.
 template <int DT>
 __device__ __forceinline__ void answer_from(Shared& s, const Row<DT>& row, const Questions& ask, uint32_t n, const SampleArgs& a,
                                             int out) {
@@ -908,8 +908,8 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
   for (int b = t; b < kBins; b += kThreads) s.count[b] = 0u, s.mass[b] = 0u;
   find_top(walk, !(temperature_of(a, row) > 0.0f), top, at);
   // Groups of eight lanes; of two where threads have no tokens: top-k 50 of 1000
-  // would find 31 groups, and take 18.0 us for its long list instead of 9.3
-  // (4096: 7.8 with groups of eight, 9.2 of two, a longer floor search).
+  // would find 31 groups, and take 18.1 us for its long list instead of 9.3
+  // (4096: 7.7 with groups of eight, 9.1 of two, a longer floor search).
   const int log2_lanes = walk.hi - walk.lo >= kThreads ? 3 : 1;
   const uint32_t group = group_max32(order_key(top), 1 << log2_lanes);
   if ((lane & ((1 << log2_lanes) - 1)) == 0) maxima[t >> log2_lanes] = group;
@@ -955,20 +955,20 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
 }
 
 // One launch of a workgroup per row, or three of many per row.  us, f32, T 1 whole / T
-// 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096 9.2 /
-// 7.7 / 11.8 against 14.0 / 18.9 / 16.2; 1 x 32768 16.2 / 9.0 / 19.0 against 16.1 /
-// 13.9 / 18.7; 1 x 50000 20.1 / 9.5 / 23.1 against 15.9 / 14.3 / 18.2; 64 x 65536 38.4
-// / 10.5 / 30.4 against 29.2 / 17.0 / 28.4; 128 x 65536 33.4 / 11.2 / 31.0 against 35.5
-// / 23.5 / 37.2; 128 x 100000 52.1 / 18.2 / 49.6 against 46.5 / 27.4 / 46.3; 256 x
-// 131072, a row for each CU, 81.3 / 31.2 / 76.8 against 91.6 / 52.6 / 82.8.
+// 0.8, top-k 50 and top-p 0.95 / top-p 0.9, one launch against three: 1 x 4096 8.3 /
+// 7.8 / 10.8 against 13.7 / 18.4 / 15.9; 1 x 32768 14.6 / 9.1 / 17.1 against 16.0 /
+// 14.4 / 18.2; 1 x 50000 18.3 / 9.3 / 21.7 against 16.1 / 14.3 / 18.3; 64 x 65536 26.4
+// / 10.5 / 26.6 against 25.1 / 17.3 / 27.4; 128 x 65536 27.5 / 11.2 / 27.4 against 34.4
+// / 24.0 / 36.6; 128 x 100000 41.1 / 17.9 / 44.1 against 42.8 / 27.8 / 45.1; 256 x
+// 131072, a row for each CU, 66.1 / 31.3 / 73.5 against 81.3 / 53.1 / 81.9.
 bool row_per_workgroup(int32_t rows, int32_t vocab) { return vocab <= 32768 || vocab <= 512 * int64_t(rows); }
 
 // Slices of a row in the first two launches: of 2048 tokens or more; two workgroups
 // on each of 256 CUs, each of which adds its bins to the row's; up to four where a row
 // would have fewer than eight slices, whose maxima bound top-k up to 128.  us with
 // two / three / four workgroups a CU (eight slices a row, twelve, sixteen), 64 x 100003
-// bf16: whole 31.4 / 30.7 / 33.0, T 0.8 with top-k 50 and top-p 0.95 17.8 / 21.5 / 23.9,
-// top-p 0.9 31.0 / 31.0 / 33.0.  The result does not depend on it, nor on the
+// bf16: whole 27.7 / 28.3 / 29.5, T 0.8 with top-k 50 and top-p 0.95 18.0 / 21.7 / 24.2,
+// top-p 0.9 29.7 / 30.3 / 31.7.  The result does not depend on it, nor on the
 // workgroups that gather in the third.
 int slice_count(int32_t rows, int32_t vocab) {
   int s = (vocab + 2047) / 2048;
@@ -978,8 +978,8 @@ int slice_count(int32_t rows, int32_t vocab) {
   return s < kMaxSlices ? s : kMaxSlices;
 }
 // Workgroups of a row in the third: of 8192 tokens or more, 256 in all (the same
-// calls, whole / top-p 0.9: 31.4 / 31.0 us; one per row 42.6 / 34.2, 512 in all 36.2 /
-// 40.9).
+// calls, whole / top-p 0.9: 27.7 / 29.7 us; one per row 30.2 / 32.2, 512 in all 35.7 /
+// 39.6).
 int part_count(int32_t rows, int32_t vocab) {
   const int p = (vocab + 8191) / 8192, fill = 256 / rows > 0 ? 256 / rows : 1;
   return p < fill ? p : fill;
