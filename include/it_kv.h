@@ -196,7 +196,11 @@ int32_t it_kv_manager_append_cow(it_kv_manager* mgr, const int32_t* seqs, const 
  * keep their positions stay as they are (dropping only a tail, as after a
  * rejected draft, moves nothing); from the first other block on, kept rows go
  * to fresh blocks, so that forks of the sequence are untouched and no row is
- * overwritten before it is read.  The caller then runs, in this order:
+ * overwritten before it is read.  A last block that stays may be a fork's too,
+ * with tokens beyond n_keep that the fork still reads: the next append to the
+ * sequence then has to copy it (it_kv_manager_append_cow, or a step with
+ * cow_src), and one without copy-on-write is IT_INVALID_INPUT before any state
+ * changes (it_kv_manager_needs_cow).  The caller then runs, in this order:
  * it_kv_move(src, dst, delta), it_kv_evict(evicted), it_kv_sync_tables(seq,
  * pos, dst).
  *   src, dst: int64[moves_cap] slots of the moved rows; delta: new - old
@@ -209,6 +213,10 @@ int32_t it_kv_manager_append_cow(it_kv_manager* mgr, const int32_t* seqs, const 
 int32_t it_kv_manager_compact(it_kv_manager* mgr, int32_t seq, const int32_t* keep, int32_t n_keep,
                               int64_t* src, int64_t* dst, int32_t* delta, int32_t* pos, int32_t moves_cap,
                               int32_t* n_moves, int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted);
+/* 1: an append to one of seqs[0..n) needs copy-on-write, because a compaction
+ * set its position back to where another sequence holds a token in the same
+ * block; 0: none does; -1: an argument is invalid. */
+int32_t it_kv_manager_needs_cow(const it_kv_manager* mgr, const int32_t* seqs, int32_t n);
 /* Export tables [max_seqs][max_blocks] (-1 = not held), ctx_lens[max_seqs]
  * (= next position) and start_pos[max_seqs] (window start, else 0).  Any
  * output pointer may be NULL. */

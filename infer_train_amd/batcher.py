@@ -77,6 +77,7 @@ class KvManager:
         h = C.c_void_p()
         check(lib.it_kv_manager_new(pool.handle, block_size, max_seqs, max_blocks_per_seq, window, C.byref(h)))
         self._h = h
+        self._compacted = False  # a sequence was compacted: appends may need copy-on-write
         self._destroy = lib.it_kv_manager_destroy  # bound now: module globals may be gone at exit
         # Reused buffers of it_kv_manager_step (grown on demand), with their
         # addresses cached (ndarray.ctypes.data costs about a microsecond);
@@ -148,9 +149,11 @@ class KvManager:
 
     def compact(self, seq: int, keep: Sequence[int]) -> CompactPlan:
         """Keep only the tokens at these positions (ascending) of `seq`:
-        keep[i] becomes position i (it_kv_manager_compact).  Tokens before the
-        first dropped one stay in their blocks, the others move to fresh ones;
-        dropping a tail moves nothing."""
+        keep[i] becomes position i (it_kv_manager_compact).  Leading blocks
+        whose tokens all keep their positions stay, what is kept of the others
+        moves to fresh ones.  Dropping a tail moves nothing; if a fork still
+        reads dropped tokens in the last block, the next append to `seq` has to
+        be with cow=True (needs_cow), and is refused without."""
         kept = np.asarray(keep)
         if kept.size and kept.dtype.kind not in "iu":
             raise TypeError("keep must hold positions (integers)")
@@ -165,7 +168,20 @@ class KvManager:
         check(lib.it_kv_manager_compact(self._h, seq, pos.ctypes.data, n, src.ctypes.data, dst.ctypes.data, delta.ctypes.data,
                                         new.ctypes.data, n, C.byref(nm), ev.ctypes.data, ev.size, C.byref(nev)))
         m = nm.value
+        self._compacted = True
         return CompactPlan(src[:m], dst[:m], delta[:m], np.full(m, seq, np.int32), new[:m], ev[:nev.value].copy())
+
+    def needs_cow(self, seqs: Sequence[int]) -> bool:
+        """Whether an append to these sequences needs copy-on-write, because a
+        compaction set one back to where a fork holds a token in the same block
+        (it_kv_manager_needs_cow)."""
+        if not self._compacted:
+            return False
+        at = np.ascontiguousarray(seqs, dtype=np.int32)
+        rc = lib.it_kv_manager_needs_cow(self._h, at.ctypes.data, at.size)
+        if rc < 0:
+            raise ValueError("sequence slots outside the manager")
+        return rc == 1
 
     def positions(self) -> np.ndarray:
         """Next position (= context length) of every sequence slot."""
@@ -334,7 +350,11 @@ class ContinuousBatcher:
         return self.manager.append(seqs, lens)
 
     def plan_decode(self) -> StepPlan:
-        return self.manager.append([self.seq_of[r] for r in self.running], 1)
+        """One token for every running request.  After a compaction that
+        dropped a tail which a fork still reads, the plan holds copy-on-write
+        pairs (cow_src, cow_dst), whose pages are copied before the append."""
+        seqs = [self.seq_of[r] for r in self.running]
+        return self.manager.append(seqs, 1, cow=self.manager.needs_cow(seqs))
 
     def sample(self, logits, u) -> List[int]:
         """Draw the running requests' next tokens, each with its own settings,

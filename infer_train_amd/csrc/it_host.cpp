@@ -149,6 +149,7 @@ struct it_kv_manager {
   std::vector<int32_t> table;  // [max_seqs][max_blocks], -1 = not held
   std::vector<int64_t> pos;    // next position of each sequence (= ctx len)
   std::vector<int64_t> first;  // lowest logical block still held
+  std::vector<uint8_t> rewound;  // a compaction set the position back into a block that others hold too
   // Scratch of one step, reused across steps.
   std::vector<int32_t> pending;    // blocks the step returned to the pool, in free order
   std::vector<uint32_t> blk_step;  // [pool capacity] step number of a block's first write...
@@ -176,6 +177,7 @@ extern "C" int32_t it_kv_manager_new(it_block_pool* pool, int32_t block_size, in
   m->table.assign(size_t(max_seqs) * size_t(max_blocks_per_seq), -1);
   m->pos.assign(size_t(max_seqs), 0);
   m->first.assign(size_t(max_seqs), 0);
+  m->rewound.assign(size_t(max_seqs), 0);
   m->old_row.assign(size_t(max_blocks_per_seq), -1);
   m->blk_step.assign(size_t(it_block_pool_capacity(pool)), 0u);
   m->blk_first.assign(size_t(it_block_pool_capacity(pool)), 0);
@@ -198,10 +200,31 @@ extern "C" int32_t it_kv_manager_seed_seq(it_kv_manager* m, int32_t seq, int64_t
   for (int32_t j = 0; j < n_blocks; ++j) row[first_block + j] = blocks[j];
   m->pos[size_t(seq)] = pos;
   m->first[size_t(seq)] = first_block;
+  m->rewound[size_t(seq)] = 0;
   return IT_OK;
 }
 
 namespace {
+// Whether the next token of sequence s, written where it stands, would replace
+// one of another holder of its block: after a compaction that only dropped a
+// tail, the position lies among rows that forks may still read.  Forks whose
+// context ends at or before it do not; holders that this manager does not know
+// are taken to.
+bool overwrites(const it_kv_manager* m, int32_t s) {
+  if (!m->rewound[size_t(s)]) return false;
+  const int64_t p = m->pos[size_t(s)], lb = p / m->bs;
+  if (lb >= m->max_blocks) return false;
+  const int32_t id = m->table[size_t(s) * size_t(m->max_blocks) + size_t(lb)];
+  if (id < 0) return false;
+  int64_t holders = 0;
+  for (int32_t o = 0; o < m->max_seqs; ++o) {
+    if (m->table[size_t(o) * size_t(m->max_blocks) + size_t(lb)] != id) continue;
+    ++holders;
+    if (o != s && m->pos[size_t(o)] > p) return true;
+  }
+  return it_block_pool_ref_count(m->pool, id) > holders;
+}
+
 // Exports ctx_lens / start_pos of every sequence slot (either may be NULL).
 void export_lengths(const it_kv_manager* m, int32_t* ctx_lens, int32_t* start_pos) {
   for (int32_t s = 0; s < m->max_seqs; ++s) {
@@ -267,6 +290,10 @@ int32_t step_impl(it_kv_manager* m, const int32_t* seqs, const int32_t* n_tokens
     return fail(IT_INVALID_INPUT, "%s: %lld tokens exceed tokens_cap %d", who, (long long)total, pl->tokens_cap);
   const bool cow = pl->cow_src != nullptr;
   if (cow && !pl->cow_dst) return fail(IT_INVALID_INPUT, "%s: cow_dst is NULL", who);
+  for (int32_t i = 0; !cow && i < n; ++i)
+    if (n_tokens[i] > 0 && overwrites(m, seqs[i]))
+      return fail(IT_INVALID_INPUT, "%s: seq %d, compacted, would write over a fork's tokens: append with copy-on-write", who,
+                  seqs[i]);
   m->pending.clear();
   if (++m->step == 0) {  // wrapped: no stale stamp may match
     std::fill(m->blk_step.begin(), m->blk_step.end(), 0u);
@@ -340,6 +367,7 @@ int32_t step_impl(it_kv_manager* m, const int32_t* seqs, const int32_t* n_tokens
       if (pl->token_pos) pl->token_pos[t] = int32_t(p);
       ++t;
       m->pos[size_t(s)] = p + 1;
+      m->rewound[size_t(s)] = 0;
     }
   }
   const int32_t ne = int32_t(m->pending.size());
@@ -419,6 +447,7 @@ extern "C" int32_t it_kv_manager_release_seq(it_kv_manager* m, int32_t seq, int3
   }
   m->pos[size_t(seq)] = 0;
   m->first[size_t(seq)] = 0;
+  m->rewound[size_t(seq)] = 0;
   *n_evicted = ne;
   return IT_OK;
 }
@@ -438,7 +467,17 @@ extern "C" int32_t it_kv_manager_fork(it_kv_manager* m, int32_t src, int32_t dst
   }
   m->pos[size_t(dst)] = m->pos[size_t(src)];
   m->first[size_t(dst)] = m->first[size_t(src)];
+  m->rewound[size_t(dst)] = m->rewound[size_t(src)];
   return IT_OK;
+}
+
+extern "C" int32_t it_kv_manager_needs_cow(const it_kv_manager* m, const int32_t* seqs, int32_t n) {
+  if (!m || n < 0 || (n > 0 && !seqs)) return -1;
+  for (int32_t i = 0; i < n; ++i)
+    if (seqs[i] < 0 || seqs[i] >= m->max_seqs) return -1;
+  for (int32_t i = 0; i < n; ++i)
+    if (overwrites(m, seqs[i])) return 1;
+  return 0;
 }
 
 extern "C" int32_t it_kv_manager_compact(it_kv_manager* m, int32_t seq, const int32_t* keep, int32_t n_keep, int64_t* src,
@@ -491,6 +530,10 @@ extern "C" int32_t it_kv_manager_compact(it_kv_manager* m, int32_t seq, const in
     if (it_block_pool_free(m->pool, id) != IT_OK) return IT_INVALID_INPUT;
     if (it_block_pool_ref_count(m->pool, id) == 0) evicted[ne++] = id;
   }
+  // The last block stays where only a tail was dropped: others may hold it, and
+  // rows that this sequence writes next.
+  if (same != n_keep) m->rewound[size_t(seq)] = 0;
+  else if (n_keep != next) m->rewound[size_t(seq)] = n_keep % bs != 0 && it_block_pool_ref_count(m->pool, row[n_keep / bs]) > 1;
   m->pos[size_t(seq)] = n_keep;
   m->first[size_t(seq)] = 0;
   *n_moves = int32_t(moves);
