@@ -202,7 +202,10 @@ int32_t it_kv_manager_append_cow(it_kv_manager* mgr, const int32_t* seqs, const 
  * cow_src), and one without copy-on-write is IT_INVALID_INPUT before any state
  * changes (it_kv_manager_needs_cow).  The caller then runs, in this order:
  * it_kv_move(src, dst, delta), it_kv_evict(evicted), it_kv_sync_tables(seq,
- * pos, dst).
+ * pos, dst), all of it queued before the device work of any later call of the
+ * manager: the returned blocks are the next that the pool hands out, to an
+ * append or to another compaction.  So plans of two calls are not joined into
+ * one move; it_kv_manager_compact_many plans several sequences for one.
  *   src, dst: int64[moves_cap] slots of the moved rows; delta: new - old
  *     position of each (NULL = not wanted); pos: new position (NULL likewise);
  *     *n_moves of them (at most n_keep)
@@ -213,6 +216,17 @@ int32_t it_kv_manager_append_cow(it_kv_manager* mgr, const int32_t* seqs, const 
 int32_t it_kv_manager_compact(it_kv_manager* mgr, int32_t seq, const int32_t* keep, int32_t n_keep,
                               int64_t* src, int64_t* dst, int32_t* delta, int32_t* pos, int32_t moves_cap,
                               int32_t* n_moves, int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted);
+/* it_kv_manager_compact of several sequences as one plan: of seqs[i], keep
+ * [cu_keep[i] .. cu_keep[i + 1]) stays (cu_keep: n_seqs + 1 values from 0; each
+ * sequence once).  No destination is a source, or a returned block, of any of
+ * them, so that one it_kv_move, one it_kv_evict and one it_kv_sync_tables
+ * (token_seq, pos, dst) serve all.  moves_cap, evicted_cap and the free blocks
+ * that are needed are sums over the sequences; token_seq, delta and pos may be
+ * NULL.  IT_INVALID_INPUT and nothing changes, for any of them, as above. */
+int32_t it_kv_manager_compact_many(it_kv_manager* mgr, const int32_t* seqs, int32_t n_seqs, const int32_t* keep,
+                                   const int32_t* cu_keep, int64_t* src, int64_t* dst, int32_t* delta,
+                                   int32_t* token_seq, int32_t* pos, int32_t moves_cap, int32_t* n_moves,
+                                   int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted);
 /* 1: an append to one of seqs[0..n) needs copy-on-write, because a compaction
  * set its position back to where another sequence holds a token in the same
  * block; 0: none does; -1: an argument is invalid. */
@@ -447,7 +461,7 @@ int32_t it_kv_copy_blocks(it_kv_cache* cache, const int32_t* src, const int32_t*
  *     out of range are latched and skipped
  *   rotary: NULL = copy as it is; delta: int32[n], device, NULL only without it
  * dst slots must be distinct and none may be another pair's src (fresh blocks,
- * as it_kv_manager_compact hands out); src[i] == dst[i] is allowed: the row
+ * as one call of it_kv_manager_compact or _compact_many hands out); src[i] == dst[i] is allowed: the row
  * is turned in place (a shift of a sequence's positions).  Takes a multi-layer
  * cache or a layer's view. */
 int32_t it_kv_move(it_kv_cache* cache, const int64_t* src, const int64_t* dst, int32_t n,

@@ -173,6 +173,7 @@ SIGNATURES = {
     "it_kv_append_rotary": (i32, [P, P, P, P, P, i32, i64, i64, i64, i32, P, P, i32, P, i32, P]),
     "it_kv_move": (i32, [P, P, P, i32, P, P, P]),
     "it_kv_manager_compact": (i32, [P, i32, P, i32, P, P, P, P, i32, P, P, i32, P]),
+    "it_kv_manager_compact_many": (i32, [P, P, i32, P, P, P, P, P, P, P, i32, P, P, i32, P]),
     "it_kv_manager_needs_cow": (i32, [P, P, i32]),
     "it_sample_workspace": (sz, [i32, i32]),
     "it_sample": (i32, [P, i32, i64, i32, i32, P, P, P, P, P, f32, i32, f32, f32, P, P, P, sz, P]),

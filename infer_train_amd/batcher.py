@@ -43,10 +43,12 @@ class StepPlan:
 
 @dataclass
 class CompactPlan:
-    """What dropping tokens out of a sequence hands to the device, in this
+    """What dropping tokens out of sequences hands to the device, in this
     order: kv_move (src, dst, and delta for rotated keys), kv_evict of the
     blocks that returned to the pool, kv_sync_tables with (token_seq,
-    token_pos, dst)."""
+    token_pos, dst).  All of it is queued before what any later plan of the
+    manager hands over: that may use the returned blocks.  Two plans are never
+    joined; KvManager.compact_many makes one for several sequences."""
 
     src: np.ndarray
     dst: np.ndarray
@@ -153,23 +155,45 @@ class KvManager:
         whose tokens all keep their positions stay, what is kept of the others
         moves to fresh ones.  Dropping a tail moves nothing; if a fork still
         reads dropped tokens in the last block, the next append to `seq` has to
-        be with cow=True (needs_cow), and is refused without."""
+        be with cow=True (needs_cow), and is refused without.  The plan's device
+        work is queued before that of any later plan; compact_many plans several
+        sequences for one move."""
+        return self.compact_many([seq], [keep])
+
+    def compact_many(self, seqs: Sequence[int], keeps: Sequence[Sequence[int]]) -> CompactPlan:
+        """compact() of several sequences as one plan, whose rows go in one
+        move: no row of it is written before all of them are read
+        (it_kv_manager_compact_many).  All are compacted, or none."""
+        if len(seqs) != len(keeps):
+            raise ValueError("a list of positions per sequence")
+        rows = [self._positions(k) for k in keeps]
+        cu = np.zeros(len(rows) + 1, np.int64)
+        np.cumsum([r.size for r in rows], out=cu[1:])
+        n = int(cu[-1])
+        if n > np.iinfo(np.int32).max:
+            raise ValueError("keep: more than 2^31 - 1 positions")
+        cu = cu.astype(np.int32)
+        at = np.ascontiguousarray(seqs, dtype=np.int32)
+        pos = np.concatenate(rows) if rows else _EMPTY
+        src, dst = np.empty(n, np.int64), np.empty(n, np.int64)
+        delta, of, new = np.empty(n, np.int32), np.empty(n, np.int32), np.empty(n, np.int32)
+        ev = np.empty(min(self.max_blocks * max(at.size, 1), self.pool.capacity()), np.int32)
+        nm, nev = C.c_int32(0), C.c_int32(0)
+        check(lib.it_kv_manager_compact_many(self._h, at.ctypes.data, at.size, pos.ctypes.data, cu.ctypes.data, src.ctypes.data,
+                                             dst.ctypes.data, delta.ctypes.data, of.ctypes.data, new.ctypes.data, n, C.byref(nm),
+                                             ev.ctypes.data, ev.size, C.byref(nev)))
+        m = nm.value
+        self._compacted = True
+        return CompactPlan(src[:m], dst[:m], delta[:m], of[:m], new[:m], ev[:nev.value].copy())
+
+    @staticmethod
+    def _positions(keep: Sequence[int]) -> np.ndarray:
         kept = np.asarray(keep)
         if kept.size and kept.dtype.kind not in "iu":
             raise TypeError("keep must hold positions (integers)")
         if kept.size and (kept.min() < 0 or kept.max() > np.iinfo(np.int32).max):
             raise ValueError("keep: positions outside the sequence")
-        pos = np.ascontiguousarray(kept, dtype=np.int32).reshape(-1)
-        n = pos.size
-        src, dst = np.empty(n, np.int64), np.empty(n, np.int64)
-        delta, new = np.empty(n, np.int32), np.empty(n, np.int32)
-        ev = np.empty(self.max_blocks, np.int32)
-        nm, nev = C.c_int32(0), C.c_int32(0)
-        check(lib.it_kv_manager_compact(self._h, seq, pos.ctypes.data, n, src.ctypes.data, dst.ctypes.data, delta.ctypes.data,
-                                        new.ctypes.data, n, C.byref(nm), ev.ctypes.data, ev.size, C.byref(nev)))
-        m = nm.value
-        self._compacted = True
-        return CompactPlan(src[:m], dst[:m], delta[:m], np.full(m, seq, np.int32), new[:m], ev[:nev.value].copy())
+        return np.ascontiguousarray(kept, dtype=np.int32).reshape(-1)
 
     def needs_cow(self, seqs: Sequence[int]) -> bool:
         """Whether an append to these sequences needs copy-on-write, because a

@@ -151,10 +151,19 @@ struct it_kv_manager {
   std::vector<int64_t> first;  // lowest logical block still held
   std::vector<uint8_t> rewound;  // a compaction set the position back into a block that others hold too
   // Scratch of one step, reused across steps.
-  std::vector<int32_t> pending;    // blocks the step returned to the pool, in free order
+  std::vector<int32_t> pending;    // blocks the step returned to the pool, in free order; those a compaction drops
   std::vector<uint32_t> blk_step;  // [pool capacity] step number of a block's first write...
   std::vector<int32_t> blk_first;  // ...and the output index of that write
-  std::vector<int32_t> old_row;    // [max_blocks] a sequence's blocks before its compaction
+  // Scratch of a compaction.
+  struct Compacted {
+    uint64_t in;          // the compaction that this is of
+    int64_t stay, total;  // blocks that stay; blocks afterwards
+    bool prefix;          // only a tail is dropped
+  };
+  std::vector<Compacted> compacted;  // [max_seqs]
+  std::vector<int32_t> old_row;      // [max_blocks] a sequence's blocks before its compaction
+  std::vector<int32_t> drops;        // [pool capacity] 0 between calls
+  uint64_t compaction = 0;
   uint32_t step = 0;
 };
 
@@ -178,7 +187,9 @@ extern "C" int32_t it_kv_manager_new(it_block_pool* pool, int32_t block_size, in
   m->pos.assign(size_t(max_seqs), 0);
   m->first.assign(size_t(max_seqs), 0);
   m->rewound.assign(size_t(max_seqs), 0);
+  m->compacted.assign(size_t(max_seqs), {});
   m->old_row.assign(size_t(max_blocks_per_seq), -1);
+  m->drops.assign(size_t(it_block_pool_capacity(pool)), 0);
   m->blk_step.assign(size_t(it_block_pool_capacity(pool)), 0u);
   m->blk_first.assign(size_t(it_block_pool_capacity(pool)), 0);
   *out = m;
@@ -480,65 +491,126 @@ extern "C" int32_t it_kv_manager_needs_cow(const it_kv_manager* m, const int32_t
   return 0;
 }
 
-extern "C" int32_t it_kv_manager_compact(it_kv_manager* m, int32_t seq, const int32_t* keep, int32_t n_keep, int64_t* src,
-                                         int64_t* dst, int32_t* delta, int32_t* pos, int32_t moves_cap, int32_t* n_moves,
-                                         int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted) {
-  const char* who = "it_kv_manager_compact";
-  if (!m || !n_moves || !n_evicted || (n_keep > 0 && !keep)) return fail(IT_INVALID_INPUT, "%s: NULL argument", who);
-  if (seq < 0 || seq >= m->max_seqs || n_keep < 0) return fail(IT_INVALID_INPUT, "%s: seq %d, n_keep %d", who, seq, n_keep);
-  if (m->window > 0) return fail(IT_NOT_IMPLEMENTED, "%s: the manager's window drops blocks by position", who);
-  const int64_t bs = m->bs, next = m->pos[size_t(seq)];
-  int32_t* const row = &m->table[size_t(seq) * size_t(m->max_blocks)];
+namespace {
+// Keeps keep[cu[i] .. cu[i + 1]) of seqs[i], for every i.  All fresh blocks are
+// taken before the first is given back, so that no destination is a source, or
+// a block that is listed as returned, of any of the sequences.
+int32_t compact_impl(it_kv_manager* m, const char* who, const int32_t* seqs, int32_t n_seqs, const int32_t* keep, const int32_t* cu,
+                     int64_t* src, int64_t* dst, int32_t* delta, int32_t* token_seq, int32_t* pos, int32_t moves_cap,
+                     int32_t* n_moves, int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted) {
+  const int64_t bs = m->bs;
+  const auto row_of = [&](int32_t s) { return &m->table[size_t(s) * size_t(m->max_blocks)]; };
   // Every check before any change.
-  int64_t same = 0;  // tokens before the first that changes its position
-  for (int32_t i = 0; i < n_keep; ++i) {
-    if (keep[i] < 0 || keep[i] >= next || (i && keep[i] <= keep[i - 1]) || keep[i] / bs >= m->max_blocks || row[keep[i] / bs] < 0)
-      return fail(IT_INVALID_INPUT, "%s: keep[%d] = %d is not held, or not above the one before", who, i, keep[i]);
-    if (keep[i] == i && same == i) same = i + 1;
+  int64_t moves = 0, fresh = 0, held = 0;
+  ++m->compaction;
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    const int32_t s = seqs[i], n_keep = cu[i + 1] - cu[i];
+    if (s < 0 || s >= m->max_seqs || n_keep < 0) return fail(IT_INVALID_INPUT, "%s: seq %d, n_keep %d", who, s, n_keep);
+    if (m->compacted[size_t(s)].in == m->compaction) return fail(IT_INVALID_INPUT, "%s: seq %d is listed twice", who, s);
+    if (m->window > 0) return fail(IT_NOT_IMPLEMENTED, "%s: the manager's window drops blocks by position", who);
+    const int32_t* const k = keep + cu[i];
+    const int32_t* const row = row_of(s);
+    const int64_t next = m->pos[size_t(s)];
+    int64_t same = 0;  // tokens before the first that changes its position
+    for (int32_t j = 0; j < n_keep; ++j) {
+      if (k[j] < 0 || k[j] >= next || (j && k[j] <= k[j - 1]) || k[j] / bs >= m->max_blocks || row[k[j] / bs] < 0)
+        return fail(IT_INVALID_INPUT, "%s: seq %d: keep[%d] = %d is not held, or not above the one before", who, s, j, k[j]);
+      if (k[j] == j && same == j) same = j + 1;
+    }
+    // Blocks that stay: all of what is kept, where no token changes its
+    // position; else the whole ones before the first that does.
+    const int64_t total = (n_keep + bs - 1) / bs, stay = same == n_keep ? total : same / bs;
+    m->compacted[size_t(s)] = {m->compaction, stay, total, same == n_keep};
+    moves += n_keep - stay * bs > 0 ? n_keep - stay * bs : 0;
+    fresh += total - stay;
+    for (int64_t j = stay; j < m->max_blocks; ++j) {
+      if (row[j] < 0) continue;
+      if (it_block_pool_ref_count(m->pool, row[j]) <= 0) return fail(IT_INVALID_INPUT, "%s: block %d is already free", who, row[j]);
+      ++held;
+    }
   }
-  // Blocks that stay: all of what is kept, where no token changes its
-  // position; else the whole ones before the first that does.
-  const int64_t total = (n_keep + bs - 1) / bs, stay = same == n_keep ? total : same / bs;
-  const int64_t moves = n_keep - stay * bs > 0 ? n_keep - stay * bs : 0, fresh = total - stay;
   if (moves > moves_cap || (moves > 0 && (!src || !dst)))
     return fail(IT_INVALID_INPUT, "%s: %lld rows to move, capacity %d", who, (long long)moves, moves_cap);
   if (it_block_pool_num_free(m->pool) < fresh)
     return fail(IT_INVALID_INPUT, "%s: %lld fresh blocks, the pool has %lld", who, (long long)fresh,
                 (long long)it_block_pool_num_free(m->pool));
-  int64_t returned = 0;
-  for (int64_t j = stay; j < m->max_blocks; ++j) {
-    if (row[j] < 0) continue;
-    const int64_t rc = it_block_pool_ref_count(m->pool, row[j]);
-    if (rc <= 0) return fail(IT_INVALID_INPUT, "%s: block %d is already free", who, row[j]);
-    returned += rc == 1;
+  m->pending.clear();
+  try {
+    m->pending.reserve(size_t(held));
+  } catch (const std::bad_alloc&) {
+    return fail(IT_DEVICE_ERROR, "%s: out of host memory", who);
   }
-  if (returned > 0 && (!evicted || returned > evicted_cap))
+  for (int32_t i = 0; i < n_seqs; ++i)
+    for (int64_t j = m->compacted[size_t(seqs[i])].stay; j < m->max_blocks; ++j)
+      if (row_of(seqs[i])[j] >= 0) m->pending.push_back(row_of(seqs[i])[j]);
+  // Blocks whose every holder is among those that drop them (forks that are
+  // compacted together may hold one block) return to the pool.
+  int64_t returned = 0;
+  for (int32_t id : m->pending) returned += ++m->drops[size_t(id)] == it_block_pool_ref_count(m->pool, id);
+  for (int32_t id : m->pending) m->drops[size_t(id)] = 0;
+  if (returned > 0 && (!evicted || returned > evicted_cap)) {
+    m->pending.clear();
     return fail(IT_INVALID_INPUT, "%s: %lld blocks return to the pool, capacity %d", who, (long long)returned, evicted_cap);
-  std::copy(row, row + m->max_blocks, m->old_row.begin());
-  // Fresh blocks first: none of them is one that this call gives back.
-  for (int64_t j = stay; j < m->max_blocks; ++j) row[j] = j < total ? int32_t(it_block_pool_allocate(m->pool)) : -1;
-  for (int64_t i = stay * bs, t = 0; i < n_keep; ++i, ++t) {
-    src[t] = int64_t(m->old_row[size_t(keep[i] / bs)]) * bs + keep[i] % bs;
-    dst[t] = int64_t(row[i / bs]) * bs + i % bs;
-    if (delta) delta[t] = int32_t(i - keep[i]);
-    if (pos) pos[t] = int32_t(i);
+  }
+  int64_t t = 0;
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    const int32_t s = seqs[i], n_keep = cu[i + 1] - cu[i];
+    const int32_t* const k = keep + cu[i];
+    const it_kv_manager::Compacted c = m->compacted[size_t(s)];
+    int32_t* const row = row_of(s);
+    std::copy(row, row + m->max_blocks, m->old_row.begin());
+    for (int64_t j = c.stay; j < m->max_blocks; ++j) row[j] = j < c.total ? int32_t(it_block_pool_allocate(m->pool)) : -1;
+    for (int64_t j = c.stay * bs; j < n_keep; ++j, ++t) {
+      src[t] = int64_t(m->old_row[size_t(k[j] / bs)]) * bs + k[j] % bs;
+      dst[t] = int64_t(row[j / bs]) * bs + j % bs;
+      if (delta) delta[t] = int32_t(j - k[j]);
+      if (token_seq) token_seq[t] = s;
+      if (pos) pos[t] = int32_t(j);
+    }
   }
   int32_t ne = 0;
-  for (int64_t j = stay; j < m->max_blocks; ++j) {
-    const int32_t id = m->old_row[size_t(j)];
-    if (id < 0) continue;
-    if (it_block_pool_free(m->pool, id) != IT_OK) return IT_INVALID_INPUT;
-    if (it_block_pool_ref_count(m->pool, id) == 0) evicted[ne++] = id;
+  for (int32_t id : m->pending) {
+    // A seeded row may name a block more often than it is held; it is freed once.
+    if (it_block_pool_free(m->pool, id) == IT_OK && it_block_pool_ref_count(m->pool, id) == 0) evicted[ne++] = id;
   }
-  // The last block stays where only a tail was dropped: others may hold it, and
-  // rows that this sequence writes next.
-  if (same != n_keep) m->rewound[size_t(seq)] = 0;
-  else if (n_keep != next) m->rewound[size_t(seq)] = n_keep % bs != 0 && it_block_pool_ref_count(m->pool, row[n_keep / bs]) > 1;
-  m->pos[size_t(seq)] = n_keep;
-  m->first[size_t(seq)] = 0;
+  m->pending.clear();
+  for (int32_t i = 0; i < n_seqs; ++i) {
+    const int32_t s = seqs[i], n_keep = cu[i + 1] - cu[i];
+    // The last block stays where only a tail was dropped: others may hold it, and
+    // rows that this sequence writes next.
+    if (!m->compacted[size_t(s)].prefix) m->rewound[size_t(s)] = 0;
+    else if (n_keep != m->pos[size_t(s)])
+      m->rewound[size_t(s)] = n_keep % bs != 0 && it_block_pool_ref_count(m->pool, row_of(s)[n_keep / bs]) > 1;
+    m->pos[size_t(s)] = n_keep;
+    m->first[size_t(s)] = 0;
+  }
   *n_moves = int32_t(moves);
   *n_evicted = ne;
   return IT_OK;
+}
+}  // namespace
+
+extern "C" int32_t it_kv_manager_compact(it_kv_manager* m, int32_t seq, const int32_t* keep, int32_t n_keep, int64_t* src,
+                                         int64_t* dst, int32_t* delta, int32_t* pos, int32_t moves_cap, int32_t* n_moves,
+                                         int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted) {
+  const char* who = "it_kv_manager_compact";
+  if (!m || !n_moves || !n_evicted || (n_keep > 0 && !keep)) return fail(IT_INVALID_INPUT, "%s: NULL argument", who);
+  const int32_t cu[2] = {0, n_keep};
+  return compact_impl(m, who, &seq, 1, keep, cu, src, dst, delta, nullptr, pos, moves_cap, n_moves, evicted, evicted_cap, n_evicted);
+}
+
+extern "C" int32_t it_kv_manager_compact_many(it_kv_manager* m, const int32_t* seqs, int32_t n_seqs, const int32_t* keep,
+                                              const int32_t* cu_keep, int64_t* src, int64_t* dst, int32_t* delta, int32_t* token_seq,
+                                              int32_t* pos, int32_t moves_cap, int32_t* n_moves, int32_t* evicted,
+                                              int32_t evicted_cap, int32_t* n_evicted) {
+  const char* who = "it_kv_manager_compact_many";
+  if (!m || !n_moves || !n_evicted || (n_seqs > 0 && (!seqs || !cu_keep))) return fail(IT_INVALID_INPUT, "%s: NULL argument", who);
+  if (n_seqs < 0 || (n_seqs > 0 && cu_keep[0] != 0)) return fail(IT_INVALID_INPUT, "%s: n_seqs %d, or cu_keep[0] not 0", who, n_seqs);
+  for (int32_t i = 0; i < n_seqs; ++i)
+    if (cu_keep[i + 1] < cu_keep[i]) return fail(IT_INVALID_INPUT, "%s: cu_keep[%d] is below the one before", who, i + 1);
+  if (n_seqs > 0 && cu_keep[n_seqs] > 0 && !keep) return fail(IT_INVALID_INPUT, "%s: NULL argument", who);
+  return compact_impl(m, who, seqs, n_seqs, keep, cu_keep, src, dst, delta, token_seq, pos, moves_cap, n_moves, evicted, evicted_cap,
+                      n_evicted);
 }
 
 extern "C" int32_t it_kv_manager_tables(const it_kv_manager* m, int32_t* tables, int32_t max_blocks,

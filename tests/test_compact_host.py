@@ -1,11 +1,17 @@
 """CPU checks of compaction beside forks, other compactions and the batcher: no
 row that somebody still reads is planned to be overwritten."""
 
+import ctypes as C
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
-from infer_train_amd import BF16, BlockPool, ContinuousBatcher, InvalidInput, KvManager
+from infer_train_amd import BF16, BlockPool, ContinuousBatcher, InvalidInput, KvManager, NotImplementedOp
 from infer_train_amd import _lib as L
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def slots_of(mgr, seq, upto):
@@ -112,3 +118,188 @@ def test_append_in_place_where_nobody_reads_on():
     arr = np.zeros(1, np.int32)
     assert L.lib.it_kv_manager_needs_cow(None, arr.ctypes.data, 1) == -1 == L.lib.it_kv_manager_needs_cow(mgr._h, None, 1)
     assert L.lib.it_kv_manager_needs_cow(mgr._h, None, 0) == 0
+
+
+# ---- several sequences in one plan ---------------------------------------------
+def test_a_plan_of_several_sequences_writes_nothing_that_it_reads():
+    """Planned one after another, the second's fresh blocks are those the first gave back, which its move still reads and
+    its eviction clears; planned together, destinations are apart from every source and returned block."""
+    keep = range(0, 16, 2)
+    pool = BlockPool(16, BF16)
+    mgr = KvManager(pool, 4, 4, 16)
+    mgr.append([0, 1], 16)
+    plan = mgr.compact_many([0, 1], [keep, keep])
+    blocks = lambda x: set((x // 4).tolist())  # noqa: E731
+    assert not blocks(plan.dst) & (blocks(plan.src) | set(plan.evicted.tolist()))
+    assert len(set(plan.dst.tolist())) == 16 == len(set(plan.src.tolist()))
+    assert plan.token_seq.tolist() == [0] * 8 + [1] * 8 and plan.token_pos.tolist() == list(range(8)) * 2
+    assert plan.delta.tolist() == [i - k for i, k in enumerate(keep)] * 2
+    assert mgr.positions().tolist() == [8, 8, 0, 0] and pool.num_free() == 12 and len(plan.evicted) == 8
+
+
+@pytest.mark.parametrize("bs,seed", ((1, 0), (4, 1), (16, 2), (16, 3)))
+def test_compact_many_against_lists(bs, seed):
+    """Random appends, forks, releases and compactions of several sequences, all of a plan's rows read before the first is
+    written and its returned blocks cleared after: every kept token is where the table says."""
+    rng = np.random.default_rng(seed)
+    cap, n_seqs = 900 // bs + 16, 5
+    pool = BlockPool(cap, BF16)
+    mgr, cells, seqs, ident = KvManager(pool, bs, n_seqs, cap), {}, [[] for _ in range(5)], 0
+    together = 0
+    for _ in range(250):
+        op, s = rng.integers(0, 8), int(rng.integers(0, n_seqs))
+        if op <= 3:
+            n = int(rng.integers(1, 40))
+            if pool.num_free() < n // bs + 2:
+                continue
+            plan = mgr.append([s], n, cow=True)
+            for a, b in zip(plan.cow_src, plan.cow_dst):
+                for j in range(bs):
+                    cells[int(b) * bs + j] = cells.get(int(a) * bs + j)
+            for slot in plan.slots:
+                cells[int(slot)] = ident
+                seqs[s].append(ident)
+                ident += 1
+        elif op == 4:
+            d = int(rng.integers(0, n_seqs))
+            if d != s and not seqs[d]:
+                mgr.fork(s, d)
+                seqs[d] = list(seqs[s])
+        elif op == 5 and rng.random() < 0.3:
+            mgr.release(s)
+            seqs[s] = []
+        else:
+            some = rng.permutation(n_seqs)[:int(rng.integers(0, n_seqs + 1))].tolist()
+            keeps = [np.flatnonzero(rng.random(len(seqs[i])) < rng.choice([0.0, 0.3, 0.9, 1.0])) if rng.random() < 0.7
+                     else np.arange(rng.integers(0, len(seqs[i]) + 1)) for i in some]
+            if pool.num_free() < sum(-(-len(k) // bs) for k in keeps):
+                continue
+            held = {b for b in mgr.tables()[0].reshape(-1).tolist() if b >= 0}
+            plan = mgr.compact_many(some, keeps)
+            together += plan.src.size > 0 and len(some) > 1
+            assert not set((plan.dst // bs).tolist()) & held and not set((plan.dst // bs).tolist()) & set(plan.evicted.tolist())
+            assert len(set(plan.dst.tolist())) == plan.dst.size
+            for b, x in [(int(b), cells[int(a)]) for a, b in zip(plan.src, plan.dst)]:
+                cells[b] = x
+            for b in plan.evicted.tolist():
+                assert pool.ref_count(b) == 0 and b in held
+                for j in range(bs):
+                    cells[b * bs + j] = None
+            for i, k in zip(some, keeps):
+                seqs[i] = [seqs[i][t] for t in k]
+        tables, ctx, _ = mgr.tables()
+        users = {}
+        for i, toks in enumerate(seqs):
+            assert ctx[i] == len(toks)
+            assert [cells[x] for x in slots_of(mgr, i, len(toks))] == toks, i
+            for b in tables[i][tables[i] >= 0].tolist():
+                users[b] = users.get(b, 0) + 1
+        assert all(pool.ref_count(b) == users.get(b, 0) for b in range(cap)) and pool.num_free() == cap - len(users)
+    assert together > 5
+
+
+def test_forks_compacted_together_return_their_blocks():
+    pool = BlockPool(12, BF16)
+    mgr = KvManager(pool, 4, 3, 12)
+    mgr.append([0], 12)
+    mgr.fork(0, 1)
+    shared = [int(b) for b in mgr.tables()[0][0][:3]]
+    plan = mgr.compact_many([0, 1], [[1, 5], []])
+    assert sorted(plan.evicted.tolist()) == sorted(shared) and plan.src.tolist() == [shared[0] * 4 + 1, shared[1] * 4 + 1]
+    assert pool.num_free() == 11 and mgr.positions().tolist() == [2, 0, 0]
+
+
+def test_compact_many_refusals_change_nothing():
+    pool = BlockPool(9, BF16)
+    mgr = KvManager(pool, 4, 3, 9)
+    mgr.append([0, 1], [10, 12])  # six blocks, three free
+    before = mgr.tables()[0].copy(), mgr.positions().copy(), pool.num_free()
+
+    def unchanged():
+        return np.array_equal(mgr.tables()[0], before[0]) and np.array_equal(mgr.positions(), before[1]) and pool.num_free() == before[2]
+
+    for seqs, keeps in (([0, 0], [[1], [2]]), ([0, 3], [[1], []]), ([0, -1], [[1], []]), ([0, 1], [[1], [12]]), ([0, 1], [[1], [3, 3]]),
+                        ([0, 1], [[1], [3, 2]]), ([0, 2], [[1], [0]]), ([0, 1], [range(1, 9), range(1, 9)])):  # the last: four fresh
+        with pytest.raises(InvalidInput):
+            mgr.compact_many(seqs, keeps)
+        assert unchanged(), (seqs, keeps)
+    for seqs, keeps, error in (([0, 1], [[1]], ValueError), ([0], [[-1]], ValueError), ([0], [[2 ** 31]], ValueError),
+                               ([0], [[0.5]], TypeError), ([0], [np.ones(10, bool)], TypeError)):
+        with pytest.raises(error):
+            mgr.compact_many(seqs, keeps)
+        assert unchanged()
+    keep, cu, seqs = np.array([1, 2, 5, 6], np.int32), np.array([0, 2, 4], np.int32), np.array([0, 1], np.int32)
+    down, late = np.array([0, 3, 2], np.int32), np.array([1, 2, 4], np.int32)
+    src, dst, ev, n = np.empty(4, np.int64), np.empty(4, np.int64), np.empty(6, np.int32), C.c_int32()
+    call = lambda **kw: L.lib.it_kv_manager_compact_many(*{**dict(  # noqa: E731
+        m=mgr._h, seqs=seqs.ctypes.data, ns=2, keep=keep.ctypes.data, cu=cu.ctypes.data, src=src.ctypes.data, dst=dst.ctypes.data,
+        delta=None, of=None, pos=None, cap=4, nm=C.byref(n), ev=ev.ctypes.data, evc=6, ne=C.byref(n)), **kw}.values())
+    for kw in (dict(m=None), dict(seqs=None), dict(keep=None), dict(cu=None), dict(src=None), dict(dst=None), dict(cap=3), dict(nm=None),
+               dict(ev=None), dict(evc=5), dict(ne=None), dict(ns=-1), dict(cu=down.ctypes.data), dict(cu=late.ctypes.data)):
+        assert call(**kw) == L.INVALID_INPUT and unchanged(), kw
+    assert call(ns=0, seqs=None, cu=None, keep=None, ev=None, evc=0) == L.OK and unchanged()
+    assert mgr.compact_many([], []).src.size == 0 and unchanged()
+    assert call() == L.OK and mgr.positions().tolist() == [2, 2, 0]  # token_seq, delta and pos are optional
+    window = KvManager(BlockPool(8, BF16), 4, 2, 8, window=8)
+    window.append([0], 6)
+    with pytest.raises(NotImplementedOp):
+        window.compact_many([0], [[0, 1]])
+
+
+_DRIVER = r"""
+#include <vector>
+#include "it_kv.h"
+int main() {
+  unsigned r = 1;
+  const auto rnd = [&](int n) { return int((r = r * 1664525u + 1013904223u) >> 8) % n; };
+  it_block_pool* pool; it_kv_manager* m;
+  if (it_block_pool_new(64, 30, &pool) || it_kv_manager_new(pool, 4, 4, 40, 0, &m)) return 1;
+  std::vector<int32_t> ctx(4);
+  for (int step = 0; step < 20000; ++step) {
+    const int32_t s = rnd(4), n = rnd(9);
+    it_kv_manager_tables(m, nullptr, 0, ctx.data(), nullptr);
+    if (rnd(2) && it_block_pool_num_free(pool) > 4 && ctx[s] < 120) {
+      std::vector<int64_t> slots(n + 1); std::vector<int32_t> ev(64), cs(n + 1), cd(n + 1); int32_t ne, nc;
+      if (it_kv_manager_append_cow(m, &s, &n, 1, slots.data(), ev.data(), 64, &ne, cs.data(), cd.data(), n + 1, &nc)) return 2;
+      if (it_kv_manager_needs_cow(m, &s, 1) < 0) return 5;
+    } else {
+      std::vector<int32_t> keep, cu{0}, seqs;
+      for (int32_t i = s; i < 4 && i < s + 1 + n % 3; ++i) {
+        const int drop = rnd(4), tail = rnd(2) ? rnd(ctx[i] + 1) : ctx[i];
+        for (int32_t p = 0; p < tail; ++p) if (rnd(4) >= drop) keep.push_back(p);
+        seqs.push_back(i); cu.push_back(int32_t(keep.size()));
+      }
+      const size_t k = keep.size();
+      std::vector<int64_t> src(k), dst(k); std::vector<int32_t> d(k), of(k), pos(k), ev(64); int32_t nm, ne;
+      const int rc = it_kv_manager_compact_many(m, seqs.data(), int32_t(seqs.size()), keep.data(), cu.data(), src.data(), dst.data(),
+                                                d.data(), of.data(), pos.data(), int32_t(k), &nm, ev.data(), 64, &ne);
+      if (rc && it_block_pool_num_free(pool) >= int64_t(k + 3 * seqs.size()) / 4) return 3;
+      const int32_t t = (s + 1) % 4;
+      if (!rc && rnd(3) == 0) { int32_t n2; if (it_kv_manager_release_seq(m, t, ev.data(), 64, &n2) || it_kv_manager_fork(m, s, t)) return 4; }
+    }
+  }
+  it_kv_manager_destroy(m); it_block_pool_destroy(pool);
+  return 0;
+}
+"""
+
+
+def test_compact_many_under_sanitizers(tmp_path):
+    src, exe = tmp_path / "compact.cpp", str(tmp_path / "compact")
+    src.write_text(_DRIVER)
+    host = os.path.join(ROOT, "infer_train_amd", "csrc", "it_host.cpp")
+    b = subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-I",
+                        os.path.join(ROOT, "include"), "-I", os.path.dirname(host), str(src), host, "-o", exe],
+                       capture_output=True, text=True, timeout=300)
+    assert b.returncode == 0, b.stderr[-2000:]
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, (r.returncode, r.stderr[-2000:])
+
+
+def test_a_seeded_row_that_names_a_block_twice_returns_it_once():
+    pool = BlockPool(6, BF16)
+    mgr = KvManager(pool, 4, 2, 6)
+    block = pool.allocate()
+    mgr.seed_seq(0, 8, 0, [block, block])
+    plan = mgr.compact(0, [])
+    assert plan.evicted.tolist() == [block] and pool.num_free() == 6 and pool.ref_count(block) == 0
