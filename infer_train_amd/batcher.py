@@ -4,6 +4,7 @@ tables and sliding-window eviction it lacks (native: it_kv_manager_*)."""
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 from collections import deque
 from dataclasses import dataclass, field
 from enum import Enum
@@ -80,6 +81,7 @@ class KvManager:
         check(lib.it_kv_manager_new(pool.handle, block_size, max_seqs, max_blocks_per_seq, window, C.byref(h)))
         self._h = h
         self._compacted = False  # a sequence was compacted: appends may need copy-on-write
+        self._watchers: List[weakref.WeakMethod] = []  # called with what a compaction kept
         self._destroy = lib.it_kv_manager_destroy  # bound now: module globals may be gone at exit
         # Reused buffers of it_kv_manager_step (grown on demand), with their
         # addresses cached (ndarray.ctypes.data costs about a microsecond);
@@ -179,11 +181,16 @@ class KvManager:
         delta, of, new = np.empty(n, np.int32), np.empty(n, np.int32), np.empty(n, np.int32)
         ev = np.empty(min(self.max_blocks * max(at.size, 1), self.pool.capacity()), np.int32)
         nm, nev = C.c_int32(0), C.c_int32(0)
+        held = self.positions() if self._watchers else None
         check(lib.it_kv_manager_compact_many(self._h, at.ctypes.data, at.size, pos.ctypes.data, cu.ctypes.data, src.ctypes.data,
                                              dst.ctypes.data, delta.ctypes.data, of.ctypes.data, new.ctypes.data, n, C.byref(nm),
                                              ev.ctypes.data, ev.size, C.byref(nev)))
         m = nm.value
         self._compacted = True
+        for watcher in self._watchers:
+            kept = watcher()
+            for seq, row in zip(at.tolist(), rows) if kept is not None else ():
+                kept(seq, row.tolist(), int(held[seq]))
         return CompactPlan(src[:m], dst[:m], delta[:m], of[:m], new[:m], ev[:nev.value].copy())
 
     @staticmethod
@@ -287,6 +294,11 @@ class ContinuousBatcher:
     requests, in the order they were preempted, before it admits waiting
     ones.  Every choice depends only on the call sequence, so block ids stay
     deterministic.
+
+    A request whose sequence was compacted (KvManager.compact) is prefilled
+    again with what it had kept, at the positions that it had moved to
+    (`context`).  Its generated_tokens are expected to hold the accepted tokens
+    alone when drafts are dropped, or to lack the drafts altogether.
     """
 
     def __init__(self, max_batch_size: int, manager: Optional[KvManager] = None):
@@ -299,11 +311,43 @@ class ContinuousBatcher:
         self._free_seqs: List[int] = list(range(manager.max_seqs - 1, -1, -1)) if manager else []
         self.preempted: deque = deque()  # preemption order
         self.needs_prefill: set = set()  # released by preemption: prefill again on resume
+        # Of compacted requests: which of their tokens (prompt, then generated) the cache
+        # holds, in order, and the first of those that follow them.
+        self._kept: Dict[int, Tuple[List[int], int]] = {}
+        if manager is not None:
+            manager._watchers.append(weakref.WeakMethod(self._note_compaction))
 
     def add_request(self, request_id: int, prompt: Sequence[int], max_tokens: int,
                     sampling: SamplingParams = SamplingParams()) -> None:  # :45-60
         self.requests[request_id] = RequestContext(request_id, RequestState.Waiting, list(prompt), [], max_tokens, sampling)
+        self._kept.pop(request_id, None)
         self.waiting.append(request_id)
+
+    def _note_compaction(self, seq: int, keep: List[int], held: int) -> None:
+        rid = next((r for r, s in self.seq_of.items() if s == seq), None)
+        if rid is None:  # not a request's sequence
+            return
+        ctx = self.requests[rid]
+        n = len(ctx.prompt_tokens) + len(ctx.generated_tokens)
+        base, follow = self._kept.get(rid, ([], 0))
+        token = lambda p: base[p] if p < len(base) else follow + p - len(base)  # noqa: E731
+        kept = [token(p) for p in keep]
+        # Positions past the tokens known are drafts; those kept become the next tokens.
+        follow = max(min(token(max(held, len(base))), n), kept[-1] + 1 if kept else 0)
+        kept += base[held:]
+        if kept == list(range(follow)):
+            self._kept.pop(rid, None)
+        else:
+            self._kept[rid] = kept, follow
+
+    def context(self, request_id: int) -> List[int]:
+        """The tokens of a request's context, in the order of their positions:
+        its prompt and generated tokens, without those that compactions
+        dropped.  What plan_resume prefills."""
+        ctx = self.requests[request_id]
+        tokens = ctx.prompt_tokens + ctx.generated_tokens
+        kept, follow = self._kept.get(request_id, ([], 0))
+        return [tokens[i] for i in kept if i < len(tokens)] + tokens[follow:]
 
     def schedule(self) -> List[int]:  # :62-73
         while len(self.running) < self.max_batch_size:
@@ -361,9 +405,10 @@ class ContinuousBatcher:
 
     def plan_resume(self, request_ids: Sequence[int]) -> StepPlan:
         """Prefill again the requests a releasing preemption emptied: their
-        prompt plus the tokens generated before the preemption."""
+        prompt plus the tokens generated before the preemption, without what
+        compactions had dropped (context)."""
         seqs = [self.seq_of[r] for r in request_ids]
-        lens = [len(self.requests[r].prompt_tokens) + len(self.requests[r].generated_tokens) for r in request_ids]
+        lens = [len(self.context(r)) for r in request_ids]
         for r in request_ids:
             self.needs_prefill.discard(r)
         return self.manager.append(seqs, lens)
@@ -423,6 +468,7 @@ class ContinuousBatcher:
             raise ValueError(f"request {request_id} is {ctx.state.value}")
         ctx.state = RequestState.Finished
         self.needs_prefill.discard(request_id)
+        self._kept.pop(request_id, None)
         freed = np.zeros(0, np.int32)
         if self.manager is not None and request_id in self.seq_of:
             seq = self.seq_of.pop(request_id)

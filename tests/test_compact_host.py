@@ -303,3 +303,91 @@ def test_a_seeded_row_that_names_a_block_twice_returns_it_once():
     mgr.seed_seq(0, 8, 0, [block, block])
     plan = mgr.compact(0, [])
     assert plan.evicted.tolist() == [block] and pool.num_free() == 6 and pool.ref_count(block) == 0
+
+
+# ---- a compacted request that is preempted --------------------------------------
+def test_a_compacted_request_resumes_with_what_it_kept():
+    """Twice compacted, decoded on in between, preempted and resumed: the tokens prefilled again are those that the cache held,
+    in its order, and the one drawn last; a request beside it is prefilled whole."""
+    pool = BlockPool(64, BF16)
+    mgr = KvManager(pool, 4, 4, 32)
+    b = ContinuousBatcher(2, mgr)
+    for rid, n in ((5, 20), (6, 9)):
+        b.add_request(rid, [100 * rid + i for i in range(n)], 50)
+    b.schedule()
+    b.plan_prefill([5, 6])
+    cache, new = {r: list(b.requests[r].prompt_tokens) for r in (5, 6)}, {5: 9000, 6: 9500}
+
+    def draw():
+        for r in (5, 6):
+            b.requests[r].generated_tokens.append(new[r])
+            new[r] += 1
+
+    def step():
+        b.plan_decode()
+        for r in (5, 6):
+            cache[r].append(b.requests[r].generated_tokens[-1])
+        draw()
+
+    draw()
+    for _ in range(3):
+        step()
+    for keep in ([0, 1, 2, 3] + list(range(10, 23)), [0, 2, 5, 6, 7, 8, 12, 13]):
+        mgr.compact(b.seq_of[5], keep)
+        cache[5] = [cache[5][i] for i in keep]
+        step()
+        step()
+        assert len(cache[5]) == mgr.positions()[b.seq_of[5]]
+        for r in (5, 6):
+            assert b.context(r) == cache[r] + b.requests[r].generated_tokens[-1:]
+    b.preempt(5)
+    b.schedule()
+    want = cache[5] + b.requests[5].generated_tokens[-1:]
+    plan = b.plan_resume([5])
+    assert plan.slots.size == len(want) == len(b.context(5)) and b.context(5) == want
+    seq = b.seq_of[5]
+    mgr.compact_many([b.seq_of[6], seq], [list(range(3)), list(range(1, 6))])
+    assert b.context(5) == want[1:6] and b.context(6) == b.requests[6].prompt_tokens[:3] + b.requests[6].generated_tokens[-1:]
+    b.finish(5)
+    b.add_request(5, [1, 2], 4)
+    assert b.context(5) == [1, 2]
+
+
+@pytest.mark.parametrize("appended", (False, True))
+def test_rejected_drafts_leave_the_context_whole(appended):
+    """Drafts are in the cache before they are accepted; dropping the rejected ones takes nothing from the request, whether
+    the accepted ones are already among its tokens or join them afterwards."""
+    mgr = KvManager(BlockPool(32, BF16), 4, 2, 32)
+    b = ContinuousBatcher(1, mgr)
+    b.add_request(0, list(range(10)), 50)
+    b.schedule()
+    b.plan_prefill([0])
+    seq, gen = b.seq_of[0], b.requests[0].generated_tokens
+    for base in (0, 1):  # the second time behind a compaction of the middle
+        gen.append(50)
+        held = int(mgr.positions()[seq])
+        mgr.append([seq], 5)  # 50 and four drafts, two of which are accepted
+        if appended:
+            gen.extend([51, 52])
+        mgr.compact(seq, range(held + 3))
+        if not appended:
+            gen.extend([51, 52])
+        whole = (list(range(10)) if base == 0 else [0, 1, 7, 8, 9, 50, 51, 52])
+        assert b.context(0) == whole + [50, 51, 52] and mgr.positions()[seq] == len(b.context(0))
+        mgr.compact(seq, [0, 1] + list(range(7, held + 3)))
+        assert b.context(0) == [0, 1] + (whole + [50, 51, 52])[7:]
+
+
+def test_compaction_of_sequences_that_are_no_request():
+    mgr = KvManager(BlockPool(32, BF16), 4, 4, 32)
+    gone = ContinuousBatcher(1, mgr)
+    del gone
+    b = ContinuousBatcher(1, mgr)
+    b.add_request(0, [1, 2, 3, 4, 5, 6], 50)
+    b.schedule()
+    b.plan_prefill([0])
+    mgr.fork(b.seq_of[0], 3)
+    mgr.compact(3, [1, 4])
+    assert b.context(0) == [1, 2, 3, 4, 5, 6]
+    mgr.compact(b.seq_of[0], [])
+    assert b.context(0) == []
