@@ -425,24 +425,28 @@ class ContinuousBatcher:
         seqs = [self.seq_of[r] for r in self.running]
         return self.manager.append(seqs, 1, cow=self.manager.needs_cow(seqs))
 
-    def sample(self, logits, u) -> List[int]:
-        """Draw the running requests' next tokens, each with its own settings,
-        from logits [len(running), vocab] in plan_decode's order and uniform
-        numbers u [len(running)] (device tensors, as sampling.sample takes
-        them); they join the requests' generated_tokens, and the caller
+    def sample(self, logits, u, request_ids: Optional[Sequence[int]] = None) -> List[int]:
+        """Draw the next tokens of running requests, each with its own settings,
+        from logits [n, vocab] and uniform numbers u [n] (device tensors, as
+        sampling.sample takes them): a row for each of request_ids (the ones
+        just prefilled or resumed, say), or for all that run, in plan_decode's
+        order.  They join the requests' generated_tokens, and the caller
         finishes those that reached max_tokens.  A row with nothing above -inf
         raises before any request changes."""
         import torch
 
         from .sampling import sample
 
-        n = len(self.running)
+        ids = self.running if request_ids is None else list(request_ids)
+        n = len(ids)
+        if request_ids is not None and (len(set(ids)) != n or not set(ids) <= set(self.running)):
+            raise ValueError("request_ids must be running requests, each listed once")
         if logits.dim() != 2 or logits.shape[0] != n:
-            raise ValueError(f"logits must be [{n}, vocab], a row per running request")
+            raise ValueError(f"logits must be [{n}, vocab], a row per request")
         if n == 0:
             return []
         host = np.empty((4, n), np.float32)  # one copy to the device
-        for i, rid in enumerate(self.running):
+        for i, rid in enumerate(ids):
             p = self.requests[rid].sampling
             host[0, i], host[2, i], host[3, i] = p.temperature, p.top_p, p.min_p
             host[1].view(np.int32)[i] = p.top_k
@@ -450,8 +454,8 @@ class ContinuousBatcher:
         drawn, _ = sample(logits, u, temperature=dev[0], top_k=dev[1].view(torch.int32), top_p=dev[2], min_p=dev[3])
         tokens = drawn.tolist()
         if min(tokens) < 0:
-            raise ValueError(f"request {self.running[tokens.index(-1)]}: no token above -inf")
-        for rid, token in zip(self.running, tokens):
+            raise ValueError(f"request {ids[tokens.index(-1)]}: no token above -inf")
+        for rid, token in zip(ids, tokens):
             self.requests[rid].generated_tokens.append(token)
         return tokens
 

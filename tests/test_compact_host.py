@@ -391,3 +391,32 @@ def test_compaction_of_sequences_that_are_no_request():
     assert b.context(0) == [1, 2, 3, 4, 5, 6]
     mgr.compact(b.seq_of[0], [])
     assert b.context(0) == []
+
+
+# ---- drawing for some of the running requests ------------------------------------
+def test_sample_takes_running_requests_alone(monkeypatch):
+    """The rows' settings and the tokens go to the requests listed; the draw itself is stubbed (it needs a device)."""
+    import torch
+    from infer_train_amd import SamplingParams, sampling
+
+    b = ContinuousBatcher(3)
+    for rid in (4, 5, 6, 7):
+        b.add_request(rid, [1], 9, SamplingParams(temperature=0.25 * rid, top_k=rid))
+    assert b.schedule() == [4, 5, 6]
+    seen = {}
+
+    def draw(logits, u, **kw):
+        seen.update({k: v.tolist() for k, v in kw.items()})
+        return logits.argmax(1).int(), None
+
+    monkeypatch.setattr(sampling, "sample", draw)
+    z, u = torch.eye(3), torch.zeros(3)
+    assert b.sample(z[[2, 0]], u[:2], [6, 4]) == [2, 0]
+    assert seen["temperature"] == [1.5, 1.0] and seen["top_k"] == [6, 4]
+    assert [b.requests[r].generated_tokens for r in (4, 5, 6)] == [[0], [], [2]]
+    assert b.sample(z, u) == [0, 1, 2] and seen["top_k"] == [4, 5, 6]
+    assert b.sample(z[:0], u[:0], []) == []
+    for ids, rows in (([7], 1), ([99], 1), ([4, 4], 2), ([4, 5], 1), ([4], 2), ([], 1)):
+        with pytest.raises(ValueError):
+            b.sample(z[:rows], u[:rows], ids)
+    assert [len(b.requests[r].generated_tokens) for r in (4, 5, 6, 7)] == [2, 1, 2, 0]
