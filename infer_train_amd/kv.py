@@ -97,7 +97,7 @@ def _rows(t: torch.Tensor, name: str, index: int, heads: int, dim: int) -> Tuple
     if t.get_device() != index:
         raise ValueError(f"{name}: tensor on cuda:{index} expected")
     token, head, element = t.stride()
-    if (head != dim and heads != 1) or (element != 1 and dim != 1):
+    if ((head != dim and heads != 1) or (element != 1 and dim != 1)) and t.numel():
         raise ValueError(f"{name}: each token's heads must be contiguous")
     return t.data_ptr(), token
 
