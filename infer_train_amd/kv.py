@@ -137,7 +137,19 @@ class Rotary:
               transpose: bool = False) -> torch.Tensor:
         """x [n_tokens, n_heads, head_dim] (any token stride) rotated to int32
         positions [n_tokens]; transpose: the gradient of that rotation (with
-        magnitude 1 its inverse).  out may be x itself."""
+        magnitude 1 its inverse).  out may be x itself.  Where x requires a
+        gradient the result carries it (the transposed rotation of its own);
+        with out that is refused, as torch's own functions with out do."""
+        if torch.is_grad_enabled() and (x.requires_grad or (out is not None and out.requires_grad)):
+            if out is not None:
+                raise ValueError("out does not go with tensors that require a gradient (use no_grad, or no out)")
+            return _Turn.apply(x, self, positions, bool(transpose))
+        result = self._turn(x, positions, out, transpose)
+        if out is not None and not out.is_inference():
+            torch.autograd.graph.increment_version(out)  # what saved it for a backward pass sees the change
+        return result
+
+    def _turn(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor], transpose: bool) -> torch.Tensor:
         if x.dim() != 3:
             raise ValueError("x must be [tokens, heads, head_dim]")
         n, heads, d = x.shape
@@ -158,6 +170,25 @@ class Rotary:
         if h is not None and h.value:
             self._destroy(h)
             self._h = None
+
+
+class _Turn(torch.autograd.Function):
+    """Rotary.apply, whose gradient is the rotation transposed."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, rotary: Rotary, positions: torch.Tensor, transpose: bool) -> torch.Tensor:
+        ctx.rotary, ctx.transpose = rotary, transpose
+        ctx.save_for_backward(positions)
+        return rotary._turn(x, positions, None, transpose)
+
+    @staticmethod
+    def backward(ctx, grad: torch.Tensor):
+        (positions,) = ctx.saved_tensors
+        _, heads, dim = grad.shape
+        token, head, element = grad.stride()
+        if element != 1 or head != dim or token < heads * dim:  # a broadcast one, say
+            grad = grad.contiguous()
+        return ctx.rotary.apply(grad, positions, transpose=not ctx.transpose), None, None, None
 
 
 class PagedKvCache:
@@ -314,7 +345,8 @@ class PagedKvCache:
         n_heads, D], k, v [n_tokens, n_kv_heads, D] of one float dtype, each
         token contiguous (views of a fused projection's rows too); positions
         int32 [n_tokens].  Returns the rotated q (q's dtype, or q_out_dtype);
-        q None: k and v only."""
+        q None: k and v only.  The cache carries no gradients, nor does this q
+        (Rotary.apply's result does)."""
         if slot_mapping.dtype != torch.int64 or positions.dtype != torch.int32:
             raise TypeError("slot_mapping must be int64 and positions int32")
         n, kind, index = slot_mapping.numel(), k.dtype, self._index
