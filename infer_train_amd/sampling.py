@@ -69,8 +69,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
             ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
     else:
         need = ws.nbytes
+    # No row has more than 2^18 tokens: a count past the parameter's width keeps them all.
+    top_k = min(max(int(top_k), 0), 2 ** 31 - 1)
     args = (logits.data_ptr(), torch_dtype_id(logits.dtype), logits.stride(0), n, vocab, us, temperatures, top_ks, top_ps, min_ps,
-            float(temperature), int(top_k), float(top_p), float(min_p), at_tokens, at_probs,
+            float(temperature), top_k, float(top_p), float(min_p), at_tokens, at_probs,
             None if ws is None else _on(ws, index), need, _raw_stream(index))
     if torch._C._cuda_getDevice() == index:
         _check(call.it_sample(*args))

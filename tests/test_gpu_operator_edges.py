@@ -20,3 +20,16 @@ def test_no_tokens_in_any_layout():
         assert r.apply(x, pos).shape == x.shape and r.apply(x, pos, out=x) is x
         assert cache.append_rotary(r, x, x, x, slots, pos).shape == x.shape
     assert not cache.k_pool.any()
+
+
+def test_counts_past_the_parameter_keep_all():
+    """top_k is 32 bits wide at the library: a larger number is no small one."""
+    import torch
+    from infer_train_amd.sampling import sample
+
+    z = torch.from_numpy(np.random.default_rng(15).standard_normal((4, 5003)).astype(np.float32)).cuda()
+    u = torch.tensor([0.1, 0.6, 0.99, 0.9999]).cuda()
+    want = sample(z, u)
+    for k in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 10 ** 30, -1, -2 ** 32 + 1):
+        got = sample(z, u, top_k=k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
