@@ -368,7 +368,9 @@ int32_t it_kv_append_rope(it_kv_cache* cache, const it_rope_table* rope, const f
 #define IT_ROTARY_SCALE_BASE 2   /* freq_base * factor^(n_dims / (n_dims - 2)) */
 #define IT_ROTARY_SCALE_PARTS 3  /* by parts: with r = original_ctx * f / (2 pi) turns over the trained
                                     context and g = (r - low) / (high - low) clamped to [0, 1],
-                                    f * (g + (1 - g) / factor) */
+                                    f * (g + (1 - g) / factor): the blend is linear in the turns,
+                                    as the YaRN paper has it; checkpoints whose code blends linearly
+                                    in the pair's index p give their own inv_freq */
 typedef struct {
   int32_t n_dims;        /* rotated elements of a head, the first ones: even, 2 .. 1024 */
   int32_t layout;        /* IT_ROTARY_INTERLEAVED, IT_ROTARY_HALF */
@@ -612,7 +614,7 @@ int32_t it_flash_attention(const float* q, const float* k, const float* v, const
  * rounded to nearest once: sums are exact, so a result depends on neither the
  * batch nor the order of the sums.
  *   logits: [n_rows][vocab] of F32, F16 or BF16, row_stride elements between
- *     rows; vocab 1 .. 262144
+ *     rows; n_rows 0 .. 65535, vocab 1 .. 262144
  *   u: float[n_rows], device, in [0, 1) (below 0 and NaN count as 0, 1 and
  *     above as the last kept token)
  *   temperatures, top_ps, min_ps: float[n_rows], top_ks: int32[n_rows], device;

@@ -119,6 +119,13 @@ __global__ __launch_bounds__(kThreads) void rotary_rows(RotaryArgs a) {
 // Any even n_dims, head_dim, alignment and stride: one pair, or one element
 // past n_dims, per lane (quantised k and v: four elements of a 32-group, whose
 // other halves of their pairs are read again).  blockIdx.y: 0 q, 1 k, 2 v.
+// Quantised caches come here where a half of the pairs is no multiple of a 32-group:
+// 32 of 128 elements or a whole head of 96 in halves.  Bound by its fp64 angles, one
+// per element and head: us for 1 / 128 / 4096 tokens of 32 + 2 x 8 bf16 heads of 128,
+// 32 of each rotated: Q8_0 4.1 / 7.2 / 174, Q4_0 4.1 / 8.0 / 188, Q5_1 4.3 / 8.8 / 219
+// (rotary_rows with all 128: 3.1 / 4.0 / 24.1, 3.0 / 3.6 / 23.3, 3.3 / 3.9 / 25.9; into
+// bf16 2.7 / 3.2 / 20.8); 9 + 2 x 3 heads of 96, Q8_0: 3.7 / 4.5 / 35.8.  Rows that are
+// not aligned to their vectors, 128 of 128 into bf16: 2.8 / 4.7 / 87.6.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void rotary_general(RotaryArgs a) {
   const int part = blockIdx.y;

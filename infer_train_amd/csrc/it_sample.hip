@@ -961,6 +961,10 @@ __global__ __launch_bounds__(kThreads) void sample_row(SampleArgs a) {
 // / 10.5 / 26.6 against 25.1 / 17.3 / 27.4; 128 x 65536 27.5 / 11.2 / 27.4 against 34.4
 // / 24.0 / 36.6; 128 x 100000 41.1 / 17.9 / 44.1 against 42.8 / 27.8 / 45.1; 256 x
 // 131072, a row for each CU, 66.1 / 31.3 / 73.5 against 81.3 / 53.1 / 81.9.
+// The limits were set for a slower sample_row and are lower than these figures would
+// put them: a whole row and top-p cross at about 800 to 1000 times the rows, and with
+// top-k one launch is the faster of the two at every size here, so that 128 x 100000
+// takes up to 10 us, 64 x 65536 and 1 x 50000 5 to 7 longer than they might.
 bool row_per_workgroup(int32_t rows, int32_t vocab) { return vocab <= 32768 || vocab <= 512 * int64_t(rows); }
 
 // Slices of a row in the first two launches: of 2048 tokens or more; two workgroups

@@ -109,8 +109,10 @@ class Rotary:
     frequencies for contexts longer than those trained on: "linear" (f /
     factor), "base" (freq_base * factor^(n_dims/(n_dims-2))) or "parts" (pairs
     that turn less than `low` times in original_ctx positions f / factor, those
-    above `high` times f, a blend between); inv_freq gives the f_p themselves.
-    magnitude multiplies the rotated elements (YaRN: 0.1 ln(factor) + 1)."""
+    above `high` times f, between them a blend linear in the turns, as the YaRN
+    paper has it); inv_freq gives the f_p themselves (where a checkpoint's code
+    blends linearly in the pair's index, say).  magnitude multiplies the
+    rotated elements (YaRN: 0.1 ln(factor) + 1)."""
 
     def __init__(self, n_dims: int, layout: str = "half", freq_base: float = 10000.0, scaling: str = "none",
                  factor: float = 1.0, original_ctx: int = 0, low: float = 1.0, high: float = 32.0, magnitude: float = 1.0,

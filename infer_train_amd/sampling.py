@@ -31,7 +31,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
            top_k: Union[int, torch.Tensor] = 0, top_p: Union[float, torch.Tensor] = 1.0,
            min_p: Union[float, torch.Tensor] = 0.0, tokens: Optional[torch.Tensor] = None,
            probs: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """logits [n_rows, vocab] (float32, float16 or bfloat16, any row stride),
+    """logits [n_rows, vocab] (float32, float16 or bfloat16, any row stride; at
+    most 65535 rows of 262144 tokens),
     u float32 [n_rows] in [0, 1); temperature, top_k, top_p and min_p one
     number for all rows or a device tensor with one per row (float32; top_k
     int32).  Returns tokens int32 [n_rows] (-1 where a row holds nothing above
