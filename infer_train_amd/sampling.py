@@ -48,6 +48,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
         temperatures, temperature = _per_row(temperature, "temperature", torch.float32, n, index), 1.0
     if isinstance(top_k, torch.Tensor):
         top_ks, top_k = _per_row(top_k, "top_k", torch.int32, n, index), 0
+    else:  # no row has more than 2^18 tokens: a count past the parameter's width keeps them all
+        top_k = min(max(int(top_k), 0), 2 ** 31 - 1)
     if isinstance(top_p, torch.Tensor):
         top_ps, top_p = _per_row(top_p, "top_p", torch.float32, n, index), 1.0
     if isinstance(min_p, torch.Tensor):
@@ -70,8 +72,6 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: Union[float, torc
             ws = torch.empty(need, dtype=torch.uint8, device=logits.device)
     else:
         need = ws.nbytes
-    # No row has more than 2^18 tokens: a count past the parameter's width keeps them all.
-    top_k = min(max(int(top_k), 0), 2 ** 31 - 1)
     args = (logits.data_ptr(), torch_dtype_id(logits.dtype), logits.stride(0), n, vocab, us, temperatures, top_ks, top_ps, min_ps,
             float(temperature), top_k, float(top_p), float(min_p), at_tokens, at_probs,
             None if ws is None else _on(ws, index), need, _raw_stream(index))
