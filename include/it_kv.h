@@ -70,6 +70,11 @@ extern "C" {
 #define IT_OP_ROTARY 9           /* dtype: the tensor's */
 #define IT_OP_KV_MOVE 10         /* dtype: the cache's */
 #define IT_OP_SAMPLE 11          /* dtype: the logits' */
+#define IT_OP_LATENT_APPEND 12   /* dtype: the latent cache's */
+#define IT_OP_LATENT_DECODE 13   /* dtype: the latent cache's */
+#define IT_OP_LATENT_PREFILL 14  /* dtype: q's, k's and v's */
+#define IT_OP_BEAM_SELECT 15     /* dtype: the logits' */
+#define IT_OP_BEAM_REORDER 16    /* any dtype: whole bytes are moved */
 
 /* Thread-local message for the last non-OK status on this thread. */
 const char* it_last_error(void);
@@ -231,6 +236,19 @@ int32_t it_kv_manager_compact_many(it_kv_manager* mgr, const int32_t* seqs, int3
  * set its position back to where another sequence holds a token in the same
  * block; 0: none does; -1: an argument is invalid. */
 int32_t it_kv_manager_needs_cow(const it_kv_manager* mgr, const int32_t* seqs, int32_t n);
+/* Beams reordered: sequence seqs[i] becomes what seqs[parents[i]] was before
+ * the call (parents[i] an index into the list; below 0, or i itself: it stays),
+ * so that one parent may be continued by several and another by none.  Blocks
+ * are shared, none is copied: the next append to these sequences has to be
+ * copy-on-write, as after it_kv_manager_fork, and a device block table's rows
+ * are put in the same order (it_beam_reorder).  seqs: distinct.
+ *   evicted: blocks that returned to the pool (no sequence continues them), in
+ *     the order of the list and of their positions: the pages to clear with
+ *     it_kv_evict; evicted_cap must cover every block that the sequences hold
+ *     (each once), else IT_INVALID_INPUT
+ * IT_INVALID_INPUT changes nothing. */
+int32_t it_kv_manager_reorder(it_kv_manager* mgr, const int32_t* seqs, const int32_t* parents, int32_t n,
+                              int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted);
 /* Export tables [max_seqs][max_blocks] (-1 = not held), ctx_lens[max_seqs]
  * (= next position) and start_pos[max_seqs] (window start, else 0).  Any
  * output pointer may be NULL. */
@@ -631,6 +649,151 @@ int32_t it_sample(const void* logits, int32_t dtype, int64_t row_stride, int32_t
                   const float* u, const float* temperatures, const int32_t* top_ks, const float* top_ps,
                   const float* min_ps, float temperature, int32_t top_k, float top_p, float min_p,
                   int32_t* tokens, float* probs, void* ws, size_t ws_bytes, void* stream);
+
+/* ======================================================================== */
+/* Device: latent attention.  Keys and values of all heads come from one     */
+/* shared row a token, [c | r]: a latent c of latent_dim elements, from which */
+/* each head's key and value are projected, and a rotated key r of rope_dim   */
+/* elements that all heads share.  Head h's score against token j is          */
+/*   scale * (q_h . k_hj + qr_h . r_j),  k_hj = W_h c_j,  v_hj = U_h c_j.     */
+/* Absorbed (it_latent_decode): (W_h^T q_h) . c_j, the cached rows read as    */
+/* they are, once for all heads, and U_h applied to the result by the caller. */
+/* Expanded (it_latent_prefill): k and v projected up by the caller.  No      */
+/* counterpart in the reference, whose caches are per head (forward.rs:16-19).*/
+/* ======================================================================== */
+/* A cache of such rows: one pool, [n_layers][num_blocks] pages of block_size
+ * rows of latent_dim + rope_dim elements of F32, F16 or BF16.  The pool is
+ * it_kv_cache_desc's k_pool, head_dim a row's elements, n_kv_heads 1, v_pool
+ * NULL.  it_kv_evict, it_kv_copy_blocks, it_kv_sync_tables, it_kv_cache_layer,
+ * _describe, _check and _destroy take it as they take any cache; it_kv_gather
+ * writes its rows to k_out (v_out NULL); it_kv_move turns the rope part alone
+ * (rotary of rope_dim elements).  Entry points for K and V rows refuse it.
+ * latent_dim 8 .. 1024, rope_dim 8 .. 256, both multiples of 8. */
+int32_t it_kv_cache_new_latent(int32_t device, int32_t n_layers, int64_t num_blocks, int32_t block_size,
+                               int32_t latent_dim, int32_t rope_dim, int32_t dtype, it_kv_cache** out);
+/* Wraps a caller-owned pool of n_layers * num_blocks pages (16-byte aligned). */
+int32_t it_kv_cache_wrap_latent(int32_t device, int32_t n_layers, void* pool, int64_t num_blocks,
+                                int32_t block_size, int32_t latent_dim, int32_t rope_dim, int32_t dtype,
+                                it_kv_cache** out);
+/* latent_dim of a latent cache, 0 of any other (and of NULL). */
+int32_t it_kv_cache_latent_dim(const it_kv_cache* cache);
+
+/* Latent rows into the cache, and the rope part of the queries beside them:
+ *   c' = c * rsqrt(mean(c^2) + eps) * weight  (weight NULL: c as it is)
+ *   r' = R(position) r,  q' = R(position) q    (rotary NULL: as they are)
+ * in fp32, each result rounded once.
+ *   kv: [n_tokens][latent_dim + rope_dim] of src_dtype F32, F16 or BF16,
+ *     kv_stride elements between tokens (the down projection's rows)
+ *   weight: [latent_dim] of weight_dtype F32, F16 or BF16
+ *   q: [n_tokens][n_heads][rope_dim] of src_dtype, q_stride elements between
+ *     tokens, q_head_stride between heads (the rope part of a projection's
+ *     heads); n_heads 0: none (q, q_out NULL).  q_out: the same shape, of
+ *     q_out_dtype F32, F16 or BF16, with strides of its own; may be q itself
+ *     (same strides and dtype), and must not overlap it otherwise
+ *   rows_out: NULL, or [n_tokens][latent_dim + rope_dim] of the cache's dtype,
+ *     contiguous: the stored rows, padding tokens' too (what a prompt's
+ *     projection up reads)
+ *   slot_mapping: int64[n_tokens] (slot < 0 = padding: nothing is stored)
+ *   positions: int32[n_tokens], NULL without rotary; a negative one is latched
+ *     (it_kv_cache_check) and its token writes nothing
+ *   rotary: n_dims = rope_dim */
+int32_t it_latent_append(it_kv_cache* cache, const it_rotary* rotary, const void* kv, int32_t src_dtype,
+                         int64_t kv_stride, const void* weight, int32_t weight_dtype, float eps, const void* q,
+                         int64_t q_stride, int64_t q_head_stride, int32_t n_heads, void* q_out,
+                         int32_t q_out_dtype, int64_t out_stride, int64_t out_head_stride, void* rows_out,
+                         const int64_t* slot_mapping, const int32_t* positions, int32_t n_tokens, void* stream);
+
+/* Absorbed latent attention over the cache: q_len new tokens of each sequence
+ * (their rows already appended), the last of its context.  For head h of the
+ * sequence's new token i (position p = ctx - q_len + i)
+ *   out = sum_j softmax_j(scale (q_latent . c_j + q_rope . r_j)) c_j
+ * over the cached tokens start .. p; a row that sees none is 0.
+ *   q_latent: [n_seqs * q_len][n_heads][latent_dim], q_rope: [..][rope_dim],
+ *     each with element strides between tokens and heads (parts of one tensor
+ *     too), of q_dtype: the cache's dtype
+ *   n_heads 1 .. 1024, q_len 1 .. 64; block_tables, ctx_lens, start_pos: as
+ *     it_kv_gather
+ *   max_tokens: upper bound of ctx_b - floor32(start_b) (a longer sequence is
+ *     latched and gives 0, as does one with a negative start)
+ *   ws: it_latent_decode_workspace(...) bytes of device memory, 256-byte
+ *     aligned, for the partial results of sequences that several workgroups
+ *     share; calls that overlap in time need one each
+ *   out: [n_seqs * q_len][n_heads][latent_dim] of out_dtype: F32 or q_dtype,
+ *     16-byte aligned
+ * Sums and the softmax in fp32; for F16 and BF16 caches the probabilities are
+ * rounded to the cache's type for the matrix cores.  How the keys are divided
+ * follows from all sequences of the call, so a row's result may differ between
+ * batches by that rounding. */
+size_t it_latent_decode_workspace(const it_kv_cache* cache, int32_t n_seqs, int32_t q_len, int32_t n_heads,
+                                  int32_t max_tokens);
+int32_t it_latent_decode(const it_kv_cache* cache, const void* q_latent, const void* q_rope, int32_t q_dtype,
+                         int64_t ql_stride, int64_t ql_head_stride, int64_t qr_stride, int64_t qr_head_stride,
+                         int32_t n_heads, int32_t q_len, const int32_t* block_tables, int32_t max_blocks,
+                         const int32_t* ctx_lens, const int32_t* start_pos, int32_t n_seqs, int32_t max_tokens,
+                         float scale, void* ws, size_t ws_bytes, void* out, int32_t out_dtype, void* stream);
+
+/* Expanded latent attention over contiguous keys and values: per head a key
+ * part and a value projected from the latents, and one rope key for all heads.
+ *   q: [total_q][n_heads][nope_dim + rope_dim], k: [total_k][n_heads][nope_dim],
+ *   v: [total_k][n_heads][v_dim], k_rope: [total_k][rope_dim] of dtype F32, F16
+ *     or BF16; element strides between tokens and heads (k and v may be parts
+ *     of one projection, k_rope a part of the gathered rows)
+ *   cu_q, cu_k: int32[n_seqs + 1], device: rows of each sequence, 0 first; with
+ *     causal != 0 query i of a sequence sees its keys 0 .. k_len - q_len + i,
+ *     else all k_len; a query that sees none is 0
+ *   max_q_len, max_k_len: upper bounds; a sequence past them, or outside
+ *     total_q / total_k, is not computed and its rows are left as they are, as
+ *     are rows behind the last sequence
+ *   nope_dim, rope_dim, v_dim: multiples of 8, nope_dim + rope_dim <= 1024,
+ *     v_dim <= 1024; fastest: F16 and BF16 with nope_dim and v_dim 64 or 128,
+ *     rope_dim 32 or 64, and 16-byte aligned rows
+ *   out: [total_q][n_heads][v_dim] contiguous, of out_dtype F32 or dtype
+ * Launched on the current device, to which `stream` must belong. */
+int32_t it_latent_prefill(const void* q, const void* k, const void* v, const void* k_rope, int32_t dtype,
+                          int64_t q_stride, int64_t q_head_stride, int64_t k_stride, int64_t k_head_stride,
+                          int64_t v_stride, int64_t v_head_stride, int64_t rope_stride, int32_t n_heads,
+                          int32_t nope_dim, int32_t rope_dim, int32_t v_dim, const int32_t* cu_q,
+                          const int32_t* cu_k, int32_t n_seqs, int32_t total_q, int32_t total_k,
+                          int32_t max_q_len, int32_t max_k_len, float scale, int32_t causal, void* out,
+                          int32_t out_dtype, void* stream);
+
+/* ======================================================================== */
+/* Device: beam search.  The reference draws one token a step                */
+/* (src/inference/forward.rs:765-796) and carries one hypothesis.            */
+/* ======================================================================== */
+/* The best continuations of each group's beams.  Candidate (b, i), beam b of
+ * the group and token i, has the value
+ *   v = (scores[b] - log sum_j exp(z_bj)) + z_bi        in fp64
+ * and candidates are ordered by v descending, equal v by the lower beam, then
+ * the larger logit (beside a very large one, v does not tell logits apart), then
+ * the lower token.  NaN logits and scores count as -inf; a candidate at -inf is
+ * none; a row whose maximum is +inf weighs its tokens at +inf alone, equally.
+ *   logits: [n_groups * n_beams][vocab] of F32, F16 or BF16, row_stride
+ *     elements between rows; n_beams 1 .. 64, vocab 1 .. 262144
+ *   scores: float[n_groups][n_beams], the beams' log-probabilities so far
+ *     (-inf: the beam is not in use)
+ *   n_out: 1 .. 64 (twice n_beams leaves n_beams of them beside those that end)
+ *   out_scores: float[n_groups][n_out], v rounded; parents: int32 (the beam in
+ *     its group) and tokens: int32 likewise.  Places without a candidate:
+ *     -inf, -1, -1
+ *   ws: it_beam_select_workspace(...) bytes, device, 256-byte aligned; it need
+ *     not be cleared, and calls that overlap in time need one each
+ * A result depends on neither the other groups nor the order of the sums.
+ * Launched on the current device, to which `stream` must belong. */
+size_t it_beam_select_workspace(int32_t n_groups, int32_t n_beams, int32_t vocab, int32_t n_out);
+int32_t it_beam_select(const void* logits, int32_t dtype, int64_t row_stride, int32_t n_groups, int32_t n_beams,
+                       int32_t vocab, const float* scores, int32_t n_out, float* out_scores, int32_t* parents,
+                       int32_t* tokens, void* ws, size_t ws_bytes, void* stream);
+/* Per-beam states put in a new order, in place: in each of n_outer arrays
+ * (outer_stride bytes apart), row g * n_beams + j becomes what row
+ * g * n_beams + parents[g][j] was (parents below 0 or not below n_beams: it
+ * stays).  Block tables, token histories, recurrent states of every layer.
+ *   x: rows of row_bytes bytes, row_stride bytes apart; n_beams 1 .. 64
+ *   parents: int32[n_groups][n_beams], device, not inside x
+ * Rows of 16-byte multiples at aligned addresses run fastest.  Launched on the
+ * current device, to which `stream` must belong. */
+int32_t it_beam_reorder(void* x, int64_t row_bytes, int64_t row_stride, int32_t n_outer, int64_t outer_stride,
+                        int32_t n_groups, int32_t n_beams, const int32_t* parents, void* stream);
 
 #ifdef __cplusplus
 }

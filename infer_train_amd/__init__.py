@@ -3,7 +3,8 @@
 Native library: infer_train_amd/libit_kv.so (C ABI in include/it_kv.h),
 hand-written HIP kernels for slot-mapped append, block-table gather, evict,
 Q8_0 / Q4_0 / Q4_1 / Q5_0 / Q5_1 quantise-append, rotary positions, row moves,
-paged split-K flash-decode, MFMA chunked prefill and token sampling,
+paged split-K flash-decode, MFMA chunked prefill, latent attention, token
+sampling and beam search,
 plus the host-side allocator and slot manager.  Python mirrors the
 reference crate's API surface (memory::paged, batcher, Backend).
 """

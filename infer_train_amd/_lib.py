@@ -29,6 +29,7 @@ BLOCK_Q5_1_BYTES = 24  # ggml block_q5_1 (types.rs:117)
 QUANT_TYPES = (Q8_0, Q4_0, Q4_1, Q5_0, Q5_1)
 OP_KV_APPEND, OP_KV_GATHER, OP_KV_EVICT, OP_PAGED_DECODE, OP_PAGED_PREFILL, OP_FLASH_ATTENTION, OP_KV_COPY_BLOCKS = range(1, 8)
 OP_KV_APPEND_ROTARY, OP_ROTARY, OP_KV_MOVE, OP_SAMPLE = range(8, 12)
+OP_LATENT_APPEND, OP_LATENT_DECODE, OP_LATENT_PREFILL, OP_BEAM_SELECT, OP_BEAM_REORDER = range(12, 17)
 ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
 ROTARY_SCALE_NONE, ROTARY_SCALE_LINEAR, ROTARY_SCALE_BASE, ROTARY_SCALE_PARTS = range(4)
 
@@ -175,6 +176,18 @@ SIGNATURES = {
     "it_kv_manager_compact": (i32, [P, i32, P, i32, P, P, P, P, i32, P, P, i32, P]),
     "it_kv_manager_compact_many": (i32, [P, P, i32, P, P, P, P, P, P, P, i32, P, P, i32, P]),
     "it_kv_manager_needs_cow": (i32, [P, P, i32]),
+    "it_kv_manager_reorder": (i32, [P, P, P, i32, P, i32, P]),
+    "it_kv_cache_new_latent": (i32, [i32, i32, i64, i32, i32, i32, i32, PP]),
+    "it_kv_cache_wrap_latent": (i32, [i32, i32, P, i64, i32, i32, i32, i32, PP]),
+    "it_kv_cache_latent_dim": (i32, [P]),
+    "it_latent_append": (i32, [P, P, P, i32, i64, P, i32, f32, P, i64, i64, i32, P, i32, i64, i64, P, P, P, i32, P]),
+    "it_latent_decode_workspace": (sz, [P, i32, i32, i32, i32]),
+    "it_latent_decode": (i32, [P, P, P, i32, i64, i64, i64, i64, i32, i32, P, i32, P, P, i32, i32, f32, P, sz, P, i32, P]),
+    "it_latent_prefill": (i32, [P, P, P, P, i32, i64, i64, i64, i64, i64, i64, i64, i32, i32, i32, i32, P, P, i32, i32, i32, i32,
+                                i32, f32, i32, P, i32, P]),
+    "it_beam_select_workspace": (sz, [i32, i32, i32, i32]),
+    "it_beam_select": (i32, [P, i32, i64, i32, i32, i32, P, i32, P, P, P, P, sz, P]),
+    "it_beam_reorder": (i32, [P, i64, i64, i32, i64, i32, i32, P, P]),
     "it_sample_workspace": (sz, [i32, i32]),
     "it_sample": (i32, [P, i32, i64, i32, i32, P, P, P, P, P, f32, i32, f32, f32, P, P, P, sz, P]),
 }

@@ -80,7 +80,7 @@ class KvManager:
         h = C.c_void_p()
         check(lib.it_kv_manager_new(pool.handle, block_size, max_seqs, max_blocks_per_seq, window, C.byref(h)))
         self._h = h
-        self._compacted = False  # a sequence was compacted: appends may need copy-on-write
+        self._compacted = False  # a sequence was compacted or reordered: appends may need copy-on-write
         self._watchers: List[weakref.WeakMethod] = []  # called with what a compaction kept
         self._destroy = lib.it_kv_manager_destroy  # bound now: module globals may be gone at exit
         # Reused buffers of it_kv_manager_step (grown on demand), with their
@@ -202,10 +202,26 @@ class KvManager:
             raise ValueError("keep: positions outside the sequence")
         return np.ascontiguousarray(kept, dtype=np.int32).reshape(-1)
 
+    def reorder(self, seqs: Sequence[int], parents: Sequence[int]) -> np.ndarray:
+        """Beams reordered: sequence seqs[i] continues what seqs[parents[i]]
+        held (it_kv_manager_reorder; a parent below 0: it stays).  Nothing is
+        copied: the next append has to be cow=True where beams continue the same
+        partial block (needs_cow), and is refused without.  Returns the blocks
+        that went back to the pool, the pages to clear; the rows of a device
+        block table are put in the same order (beam.beam_reorder)."""
+        if len(seqs) != len(parents):
+            raise ValueError("a parent per sequence")
+        at, of = np.ascontiguousarray(seqs, dtype=np.int32), np.ascontiguousarray(parents, dtype=np.int32)
+        ev = np.empty(min(self.max_blocks * max(at.size, 1), self.pool.capacity()), np.int32)
+        nev = C.c_int32(0)
+        check(lib.it_kv_manager_reorder(self._h, at.ctypes.data, of.ctypes.data, at.size, ev.ctypes.data, ev.size, C.byref(nev)))
+        self._compacted = True
+        return ev[:nev.value].copy()
+
     def needs_cow(self, seqs: Sequence[int]) -> bool:
         """Whether an append to these sequences needs copy-on-write, because a
-        compaction set one back to where a fork holds a token in the same block
-        (it_kv_manager_needs_cow)."""
+        compaction set one back to where a fork holds a token in the same block,
+        or a reordering left several to continue it (it_kv_manager_needs_cow)."""
         if not self._compacted:
             return False
         at = np.ascontiguousarray(seqs, dtype=np.int32)
@@ -420,8 +436,8 @@ class ContinuousBatcher:
 
     def plan_decode(self) -> StepPlan:
         """One token for every running request.  After a compaction that
-        dropped a tail which a fork still reads, the plan holds copy-on-write
-        pairs (cow_src, cow_dst), whose pages are copied before the append."""
+        dropped a tail which a fork still reads, or a reordering after which
+        beams continue the same block, the plan holds copy-on-write pairs (cow_src, cow_dst), whose pages are copied before the append."""
         seqs = [self.seq_of[r] for r in self.running]
         return self.manager.append(seqs, 1, cow=self.manager.needs_cow(seqs))
 
@@ -458,6 +474,31 @@ class ContinuousBatcher:
         for rid, token in zip(ids, tokens):
             self.requests[rid].generated_tokens.append(token)
         return tokens
+
+    def reorder(self, request_ids: Sequence[int], parents: Sequence[int]) -> np.ndarray:
+        """Running requests that are one search's beams put in the selected
+        order: request_ids[i] continues what request_ids[parents[i]] held, its
+        prompt, generated tokens and cached blocks (a parent below 0: it stays).
+        The caller then appends each one's selected token.  Returns the blocks
+        that went back to the pool, the pages to clear."""
+        ids = list(request_ids)
+        if len(set(ids)) != len(ids) or not set(ids) <= set(self.running):
+            raise ValueError("request_ids must be running requests, each listed once")
+        of = [i if p < 0 else p for i, p in enumerate(int(p) for p in parents)]
+        if len(of) != len(ids) or max(of, default=0) >= max(len(ids), 1):
+            raise ValueError("a parent per request, each an index into request_ids")
+        freed = np.zeros(0, np.int32)
+        if self.manager is not None:
+            freed = self.manager.reorder([self.seq_of[r] for r in ids], of)
+        was = [(self.requests[r].prompt_tokens, self.requests[r].generated_tokens, self._kept.get(r)) for r in ids]
+        for rid, p in zip(ids, of):
+            prompt, generated, kept = was[p]
+            self.requests[rid].prompt_tokens, self.requests[rid].generated_tokens = list(prompt), list(generated)
+            if kept is None:
+                self._kept.pop(rid, None)
+            else:
+                self._kept[rid] = (list(kept[0]), kept[1])
+        return freed
 
     def finish(self, request_id: int) -> np.ndarray:
         """Running or Preempted -> Finished; the request's blocks (if it

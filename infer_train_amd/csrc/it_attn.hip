@@ -242,6 +242,7 @@ int32_t paged_decode_phases(const char* who, const it_kv_cache* c, const void* q
                             void* out, int32_t out_dtype, void* stream, int phases) {
   if (!c) return fail(IT_INVALID_INPUT, "%s: cache is NULL", who);
   if (int32_t rc = one_layer(c, who)) return rc;
+  if (int32_t rc = per_head(c, who)) return rc;
   if (!block_tables || !ctx_lens) return fail(IT_INVALID_INPUT, "%s: NULL block_tables/ctx_lens", who);
   if (max_blocks <= 0) return fail(IT_INVALID_INPUT, "%s: max_blocks %d", who, max_blocks);
   if (!(scale == scale)) return fail(IT_INVALID_INPUT, "%s: scale is NaN", who);

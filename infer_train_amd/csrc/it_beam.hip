@@ -1,0 +1,438 @@
+// it_beam.hip -- beam search: the best continuations over a group's beams and
+// the vocabulary, and per-beam states put in the selected order.
+//
+//   v[b, i] = (score_b - log sum_j exp(z_bj)) + z_bi,  the n_out largest of a group.
+//
+// Two launches.  The first cuts each row into slices of 16 tokens a thread, which
+// stay in registers: a slice's maximum, its sum of exponentials against it and its
+// n_out best tokens.  The second joins a group's slices: the rows' logarithms,
+// then the best of all slices' candidates.
+//   The n-th best of a set is bounded from below by the n-th largest of the maxima
+// of 64 groups of it, which one wave finds bit by bit; what is not below it (about
+// n, up to ties) is listed, and a listed entry's place is the number of listed ones
+// before it.  A list that ties overflow is replaced by n rounds of the next best.
+//   Sums are in fp64: the order of two beams' candidates hangs on the difference of
+// their logarithms, whose fp32 error would decide about as many cases as it has
+// units between neighbouring values.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+
+#include "it_internal.hpp"
+#include "it_rows.hpp"
+
+using namespace itkv;
+
+namespace {
+constexpr int kThreads = 512;
+constexpr int kWaves = kThreads / 64;
+constexpr int kPer = 16;                    // tokens a thread holds
+constexpr int kSlice = kThreads * kPer;
+constexpr int kMaxVocab = 1 << 18;
+constexpr int kMaxBeams = 64;
+constexpr int kMaxOut = 64;                 // one wave's lanes bound the last place
+constexpr int kRoom = 1024;                 // listed entries
+constexpr int kIndexBits = 18;
+static_assert(kMaxVocab <= 1 << kIndexBits, "a token's index in its key");
+constexpr int kKeyBits = 32 + kIndexBits;
+constexpr uint64_t kKeyMask = (uint64_t(1) << kKeyBits) - 1;
+
+struct SliceSum {
+  float top;   // -inf: nothing above it
+  float pad;
+  double sum;  // of exp(z - top), exact to fp64's rounding
+};
+struct SelectArgs {
+  const char* logits;
+  int64_t row_bytes;
+  const float* scores;
+  float* out_scores;
+  int32_t* parents;
+  int32_t* tokens;
+  SliceSum* sums;     // [rows][slices]
+  uint64_t* best;     // [rows][slices][n]: keys of the slice's best, descending; 0: none
+  int vocab, slices, n_beams, n_out;
+};
+
+// fp32 values as integers of the same order; NaN as -inf, -0 as +0.
+__device__ __forceinline__ uint32_t order_key(float z) {
+  const uint32_t u = __float_as_uint((z == z ? z : -INFINITY) + 0.0f);
+  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
+// A token's place in its row: larger is earlier, unique, never 0.
+__device__ __forceinline__ uint64_t token_key(float z, int index) {
+  return (uint64_t(order_key(z)) << kIndexBits) | uint32_t(kMaxVocab - 1 - index);
+}
+__device__ __forceinline__ float token_value(uint64_t k) { return key_value(uint32_t(k >> kIndexBits)); }
+__device__ __forceinline__ int token_index(uint64_t k) { return kMaxVocab - 1 - int(k & (kMaxVocab - 1)); }
+// fp64 values likewise.
+__device__ __forceinline__ uint64_t value_key(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
+  return (u >> 63) ? ~u : u | uint64_t(1) << 63;
+}
+__device__ __forceinline__ double key_double(uint64_t k) {
+  return __builtin_bit_cast(double, (k >> 63) ? k & ~(uint64_t(1) << 63) : ~k);
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp64(uint64_t x) {
+  const int hi = __builtin_amdgcn_update_dpp(0, int(x >> 32), CTRL, 0xF, 0xF, true);
+  return uint64_t(uint32_t(hi)) << 32 | uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, 0xF, 0xF, true));
+}
+// The largest of aligned groups of eight lanes, in each of them.
+__device__ __forceinline__ uint64_t eight_max(uint64_t x) {
+  x = max(x, dpp64<kDppQuadXor1>(x));
+  x = max(x, dpp64<kDppQuadXor2>(x));
+  return max(x, dpp64<kDppHalfMirror>(x));
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t x, int lane) {
+  return uint64_t(uint32_t(__builtin_amdgcn_readlane(int(x >> 32), lane))) << 32 | uint32_t(__builtin_amdgcn_readlane(int(x), lane));
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t x) {
+  x = eight_max(x);
+  x = max(x, dpp64<kDppRowRor8>(x));
+  return max(max(lane64(x, 0), lane64(x, 16)), max(lane64(x, 32), lane64(x, 48)));
+}
+// The n-th largest of the wave's values (0 where fewer are above 0), to `bits` bits.
+__device__ __forceinline__ uint64_t wave_nth(uint64_t x, int n, int bits) {
+  uint64_t k = 0u;
+  for (int b = bits - 1; b >= 0; --b) {
+    const uint64_t with = k | uint64_t(1) << b;
+    if (__popcll(__ballot(x >= with)) >= n) k = with;
+  }
+  return k;
+}
+
+// exp(d) for d <= 0: 2^n times the Taylor sum of exp on |x| <= ln(2) / 2, whose
+// next term, x^12 / 12!, is below 2^-47; n ln(2)'s own rounding is below 2^-45.
+__device__ __forceinline__ double exp_below(double d) {
+  if (!(d > -700.0)) return d == d ? 0.0 : d;
+  const double n = __builtin_rint(d * 1.4426950408889634);
+  const double x = fma(n, -0.6931471805599453, d);
+  double p = 1.0 / 39916800.0;
+  p = fma(p, x, 1.0 / 3628800.0);
+  p = fma(p, x, 1.0 / 362880.0);
+  p = fma(p, x, 1.0 / 40320.0);
+  p = fma(p, x, 1.0 / 5040.0);
+  p = fma(p, x, 1.0 / 720.0);
+  p = fma(p, x, 1.0 / 120.0);
+  p = fma(p, x, 1.0 / 24.0);
+  p = fma(p, x, 1.0 / 6.0);
+  p = fma(p, x, 0.5);
+  p = fma(p, x, 1.0);
+  p = fma(p, x, 1.0);
+  return ldexp(p, int(n));
+}
+
+struct Listed {
+  uint64_t key, tie;  // the larger key first, of equal keys the smaller tie
+};
+struct TopShared {
+  uint64_t group[64];
+  Listed list[kRoom];
+  uint64_t round[kWaves];
+  uint64_t round_tie[kWaves];
+  uint32_t n;
+};
+__device__ __forceinline__ bool before(const Listed& a, const Listed& b) { return a.key > b.key || (a.key == b.key && a.tie < b.tie); }
+
+// The n first of the block's entries.  each(f): f(key, tie) for every entry of the
+// thread (key 0: none; no two alike), the same ones each time it is called.
+// put(place, entry): called by one thread for each place that an entry takes.
+template <class Each, class Put>
+__device__ __forceinline__ void top_of_block(TopShared& s, int n, int bits, Each&& each, Put&& put) {
+  const int tid = int(threadIdx.x), lane = tid & 63;
+  uint64_t most = 0u;
+  each([&](uint64_t key, uint64_t) { most = max(most, key); });
+  most = eight_max(most);
+  if ((lane & 7) == 0) s.group[tid >> 3] = most;
+  if (tid == 0) s.n = 0u;
+  __syncthreads();
+  const uint64_t least = max(wave_nth(s.group[lane], n, bits), uint64_t(1));  // every wave for itself
+  each([&](uint64_t key, uint64_t tie) {
+    if (key < least) return;
+    const uint32_t at = atomicAdd(&s.n, 1u);
+    if (at < kRoom) s.list[at] = {key, tie};
+  });
+  __syncthreads();
+  const uint32_t listed = s.n;
+  if (listed <= kRoom) {
+    for (uint32_t i = tid; i < listed; i += kThreads) {
+      const Listed mine = s.list[i];
+      int place = 0;
+      for (uint32_t j = 0; j < listed; ++j) place += before(s.list[j], mine);
+      if (place < n) put(place, mine);
+    }
+    return;
+  }
+  // More than the list holds are as good as the bound: one place after another.
+  Listed last = {~uint64_t(0), 0u};
+  bool first = true;
+  for (int place = 0; place < n; ++place) {
+    Listed mine = {0u, ~uint64_t(0)};
+    each([&](uint64_t key, uint64_t tie) {
+      const Listed x = {key, tie};
+      if (key && (first || before(last, x)) && before(x, mine)) mine = x;
+    });
+    const uint64_t key = wave_max(mine.key), tie = ~wave_max(mine.key == key ? ~mine.tie : uint64_t(0));
+    __syncthreads();  // the round before is read
+    if (lane == 0) s.round[tid >> 6] = key, s.round_tie[tid >> 6] = tie;
+    __syncthreads();
+    Listed best = {0u, ~uint64_t(0)};
+    for (int w = 0; w < kWaves; ++w) {
+      const Listed x = {s.round[w], s.round_tie[w]};
+      if (before(x, best)) best = x;
+    }
+    if (best.key == 0u) return;  // uniform
+    if (mine.key == best.key && mine.tie == best.tie) put(place, mine);
+    last = best;
+    first = false;
+  }
+}
+
+// grid: (slice, row).
+template <int DT>
+__global__ __launch_bounds__(kThreads) void beam_slices(SelectArgs a) {
+  constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es, kVecs = kPer / V;
+  using In = RowVec<DT, V>;
+  __shared__ TopShared top;
+  __shared__ float tops[kWaves];
+  __shared__ double sums[kWaves];
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, slice = int(blockIdx.x);
+  const int64_t row = blockIdx.y;
+  const char* const data = a.logits + row * a.row_bytes;
+  const int lo = slice * kSlice, hi = min(a.vocab, lo + kSlice);
+  // Thread t's tokens: vectors t, t + 512, .. of the slice.
+  float z[kPer];
+  const bool aligned = ((reinterpret_cast<uintptr_t>(data) + size_t(lo) * es) & 15u) == 0;
+#pragma unroll
+  for (int j = 0; j < kVecs; ++j) {
+    const int i = lo + (j * kThreads + tid) * V;
+    float f[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = -INFINITY;
+    if (aligned && i + V <= hi) {
+      In::widen(*reinterpret_cast<const typename In::raw*>(data + int64_t(i) * es), f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (i + e < hi) f[e] = load_element(data, i + e, DT);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) z[j * V + e] = f[e] == f[e] ? f[e] : -INFINITY;
+  }
+  float m = z[0];
+#pragma unroll
+  for (int e = 1; e < kPer; ++e) m = fmaxf(m, z[e]);
+  m = group_max<64>(m);
+  if (lane == 0) tops[wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, tops[w]);
+  double sum = 0.0;
+  if (m > -INFINITY) {  // uniform
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum += z[e] == m ? 1.0 : exp_below(double(z[e]) - double(m));
+  }
+  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  if (lane == 0) sums[wave] = sum;
+  uint64_t* const best = a.best + (row * a.slices + slice) * a.n_out;
+  for (int i = tid; i < a.n_out; i += kThreads) best[i] = 0u;
+  __syncthreads();
+  if (tid == 0) {
+    double total = 0.0;
+    for (int w = 0; w < kWaves; ++w) total += sums[w];
+    a.sums[row * a.slices + slice] = {m, 0.0f, total};
+  }
+  if (m == -INFINITY) return;  // uniform
+  top_of_block(
+      top, a.n_out, kKeyBits,
+      [&](auto&& f) {
+#pragma unroll
+        for (int j = 0; j < kVecs; ++j)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float x = z[j * V + e];
+            f(x > -INFINITY ? token_key(x, lo + (j * kThreads + tid) * V + e) : uint64_t(0), uint64_t(0));
+          }
+      },
+      [&](int place, const Listed& x) { best[place] = x.key; });
+}
+
+// grid: group.
+__global__ __launch_bounds__(kThreads) void beam_join(SelectArgs a) {
+  __shared__ TopShared top;
+  __shared__ double base[kMaxBeams];
+  __shared__ float row_top[kMaxBeams];
+  const int tid = int(threadIdx.x);
+  const int64_t g = blockIdx.x, row0 = g * a.n_beams;
+  for (int b = tid; b < a.n_beams; b += kThreads) {
+    const SliceSum* const s = a.sums + (row0 + b) * a.slices;
+    float m = -INFINITY;
+    for (int i = 0; i < a.slices; ++i) m = fmaxf(m, s[i].top);
+    double sum = 0.0;
+    for (int i = 0; i < a.slices; ++i)
+      if (s[i].top > -INFINITY) sum += s[i].sum * (s[i].top == m ? 1.0 : exp_below(double(s[i].top) - double(m)));
+    const float score = a.scores[g * a.n_beams + b];
+    // A row at +inf: its tokens there share it equally, log 1/count.
+    base[b] = m > -INFINITY && score > -INFINITY ? double(score) - (m < INFINITY ? double(m) + log(sum) : log(sum)) : -INFINITY;
+    row_top[b] = m;
+  }
+  const int64_t out = g * a.n_out;
+  for (int i = tid; i < a.n_out; i += kThreads) {
+    a.out_scores[out + i] = -INFINITY;
+    a.parents[out + i] = a.tokens[out + i] = -1;
+  }
+  __syncthreads();
+  const int per = a.slices * a.n_out, total = a.n_beams * per;
+  const uint64_t* const best = a.best + row0 * per;
+  top_of_block(
+      top, a.n_out, 64,
+      [&](auto&& f) {
+        for (int i = tid; i < total; i += kThreads) {
+          const int b = i / per;
+          const uint64_t k = best[i];
+          if (k == 0u || !(base[b] > -INFINITY)) continue;
+          const float z = token_value(k);
+          if (row_top[b] == INFINITY && z < INFINITY) continue;
+          const double v = base[b] + (z == INFINITY ? 0.0 : double(z));
+          f(value_key(v), uint64_t(b) << kKeyBits | (kKeyMask - k));
+        }
+      },
+      [&](int place, const Listed& x) {
+        a.out_scores[out + place] = float(key_double(x.key));
+        a.parents[out + place] = int32_t(x.tie >> kKeyBits);
+        a.tokens[out + place] = token_index(kKeyMask - (x.tie & kKeyMask));
+      });
+}
+
+// ---- per-beam states -------------------------------------------------------
+// A thread holds one unit of U's size of all of a group's rows: every row that
+// changes is read, then written, so no second buffer and no order is needed.
+// Bound by memory: a changed row is written once, its parent read once (from a
+// cache where several continue it).  grid: (units, group, outer).
+template <class U, int K>
+__global__ __launch_bounds__(256) void beam_rows(char* x, int64_t units, int64_t row_stride, int64_t outer_stride, int n_beams,
+                                                 const int32_t* parents) {
+  const int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (u >= units) return;
+  const int g = int(blockIdx.y);
+  char* const base = x + int64_t(blockIdx.z) * outer_stride + int64_t(g) * n_beams * row_stride + u * int64_t(sizeof(U));
+  const int32_t* const from = parents + int64_t(g) * n_beams;
+  U v[K];
+  int p[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    p[j] = j < n_beams ? from[j] : -1;
+    if (p[j] < 0 || p[j] >= n_beams || p[j] == j) p[j] = -1;  // stays
+  }
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    if (p[j] >= 0) v[j] = *reinterpret_cast<const U*>(base + p[j] * row_stride);
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    if (p[j] >= 0) *reinterpret_cast<U*>(base + j * row_stride) = v[j];
+}
+
+template <class U>
+void launch_rows(char* x, int64_t units, int64_t row_stride, int64_t outer_stride, int n_outer, int n_groups, int n_beams,
+                 const int32_t* parents, hipStream_t s) {
+  const dim3 grid(unsigned((units + 255) / 256), unsigned(n_groups), unsigned(n_outer));
+  auto* const kern = n_beams <= 4 ? beam_rows<U, 4> : n_beams <= 8 ? beam_rows<U, 8> : n_beams <= 16 ? beam_rows<U, 16> : n_beams <= 32 ? beam_rows<U, 32> : beam_rows<U, 64>;
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, s, x, units, row_stride, outer_stride, n_beams, parents);
+}
+
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+int slices_of(int32_t vocab) { return (vocab + kSlice - 1) / kSlice; }
+bool sizes_ok(const char* who, int32_t n_groups, int32_t n_beams, int32_t vocab, int32_t n_out) {
+  if (n_groups < 0 || n_beams < 1 || n_beams > kMaxBeams || int64_t(n_groups) * n_beams > 65535 || vocab < 1 || vocab > kMaxVocab ||
+      n_out < 1 || n_out > kMaxOut) {
+    fail(IT_INVALID_INPUT, "%s: n_groups %d, n_beams %d (1 to %d; to 65535 rows), vocab %d (1 to %d), n_out %d (1 to %d)", who, n_groups,
+         n_beams, kMaxBeams, vocab, kMaxVocab, n_out, kMaxOut);
+    return false;
+  }
+  return true;
+}
+}  // namespace
+
+extern "C" size_t it_beam_select_workspace(int32_t n_groups, int32_t n_beams, int32_t vocab, int32_t n_out) {
+  if (!sizes_ok("it_beam_select_workspace", n_groups, n_beams, vocab, n_out)) return 0;
+  const size_t slices = size_t(n_groups) * size_t(n_beams) * size_t(slices_of(vocab));
+  return align256(slices * sizeof(SliceSum)) + align256(slices * size_t(n_out) * 8);
+}
+
+extern "C" int32_t it_beam_select(const void* logits, int32_t dtype, int64_t row_stride, int32_t n_groups, int32_t n_beams, int32_t vocab,
+                                  const float* scores, int32_t n_out, float* out_scores, int32_t* parents, int32_t* tokens, void* ws,
+                                  size_t ws_bytes, void* stream) {
+  const char* who = "it_beam_select";
+  if (dtype != IT_F32 && dtype != IT_F16 && dtype != IT_BF16) return fail(IT_NOT_IMPLEMENTED, "%s: dtype %d (F32, F16 or BF16)", who, dtype);
+  if (!sizes_ok(who, n_groups, n_beams, vocab, n_out)) return IT_INVALID_INPUT;
+  if (n_groups == 0) return IT_OK;
+  if (int64_t(n_groups) * n_beams > 1 && (row_stride < vocab || row_stride > int64_t(1) << 40))
+    return fail(IT_INVALID_INPUT, "%s: row_stride %lld below vocab %d (or above 2^40)", who, (long long)row_stride, vocab);
+  if (!logits || !scores || !out_scores || !parents || !tokens) return fail(IT_INVALID_INPUT, "%s: NULL tensor", who);
+  const int64_t es = dtype_bytes(dtype);
+  if (reinterpret_cast<uintptr_t>(logits) % uintptr_t(es)) return fail(IT_INVALID_INPUT, "%s: logits must be aligned to their elements", who);
+  const size_t need = it_beam_select_workspace(n_groups, n_beams, vocab, n_out);
+  if (!ws || ws_bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255u))
+    return fail(IT_INVALID_INPUT, "%s: workspace of %zu bytes, %zu needed (256-byte aligned)", who, ws ? ws_bytes : size_t(0), need);
+  SelectArgs a{};
+  a.logits = static_cast<const char*>(logits);
+  a.row_bytes = row_stride * es;
+  a.scores = scores;
+  a.out_scores = out_scores;
+  a.parents = parents;
+  a.tokens = tokens;
+  a.vocab = vocab;
+  a.slices = slices_of(vocab);
+  a.n_beams = n_beams;
+  a.n_out = n_out;
+  a.sums = static_cast<SliceSum*>(ws);
+  a.best = reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + align256(size_t(n_groups) * size_t(n_beams) * size_t(a.slices) * sizeof(SliceSum)));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const dim3 grid(unsigned(a.slices), unsigned(n_groups * n_beams));
+  switch (dtype) {
+    case IT_F32: hipLaunchKernelGGL(beam_slices<IT_F32>, grid, dim3(kThreads), 0, s, a); break;
+    case IT_BF16: hipLaunchKernelGGL(beam_slices<IT_BF16>, grid, dim3(kThreads), 0, s, a); break;
+    default: hipLaunchKernelGGL(beam_slices<IT_F16>, grid, dim3(kThreads), 0, s, a); break;
+  }
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess) {
+    hipLaunchKernelGGL(beam_join, dim3(unsigned(n_groups)), dim3(kThreads), 0, s, a);
+    e = hipGetLastError();
+  }
+  return e == hipSuccess ? IT_OK : fail(IT_DEVICE_ERROR, "%s: launch: %s", who, hipGetErrorString(e));
+}
+
+extern "C" int32_t it_beam_reorder(void* x, int64_t row_bytes, int64_t row_stride, int32_t n_outer, int64_t outer_stride, int32_t n_groups,
+                                   int32_t n_beams, const int32_t* parents, void* stream) {
+  const char* who = "it_beam_reorder";
+  const int64_t kFar = int64_t(1) << 40;
+  if (n_groups < 0 || n_groups > 65535 || n_beams < 1 || n_beams > kMaxBeams || n_outer < 0 || n_outer > 65535 || row_bytes < 0 || row_bytes > kFar)
+    return fail(IT_INVALID_INPUT, "%s: row_bytes %lld, n_outer %d, n_groups %d (to 65535), n_beams %d (1 to %d)", who, (long long)row_bytes,
+                n_outer, n_groups, n_beams, kMaxBeams);
+  const int64_t rows = int64_t(n_groups) * n_beams;
+  if (rows > 1 && (row_stride < row_bytes || row_stride > kFar))
+    return fail(IT_INVALID_INPUT, "%s: row_stride %lld below row_bytes %lld (or above 2^40)", who, (long long)row_stride, (long long)row_bytes);
+  if (n_outer > 1 && (outer_stride < (rows - 1) * row_stride + row_bytes || outer_stride > kFar))
+    return fail(IT_INVALID_INPUT, "%s: outer_stride %lld below an array of %lld rows", who, (long long)outer_stride, (long long)rows);
+  if (rows == 0 || n_outer == 0 || row_bytes == 0) return IT_OK;
+  if (!x || !parents) return fail(IT_INVALID_INPUT, "%s: NULL tensor", who);
+  if (reinterpret_cast<uintptr_t>(parents) & 3u) return fail(IT_INVALID_INPUT, "%s: parents must be aligned to 4 bytes", who);
+  if (rows == 1) row_stride = 0;
+  if (n_outer == 1) outer_stride = 0;
+  const uintptr_t first = reinterpret_cast<uintptr_t>(x), at = reinterpret_cast<uintptr_t>(parents);
+  const int64_t span = (n_outer - 1) * outer_stride + (rows - 1) * row_stride + row_bytes;
+  if (at < first + uintptr_t(span) && first < at + uintptr_t(rows) * 4) return fail(IT_INVALID_INPUT, "%s: parents lie inside x", who);
+  const uintptr_t all = first | uintptr_t(row_bytes) | uintptr_t(row_stride) | uintptr_t(outer_stride);
+  const int unit = (all & 15u) == 0 ? 16 : (all & 3u) == 0 ? 4 : 1;
+  if (row_bytes / unit > int64_t(1) << 31) return fail(IT_INVALID_INPUT, "%s: rows of %lld bytes", who, (long long)row_bytes);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  char* const p = static_cast<char*>(x);
+  if (unit == 16) launch_rows<uint4>(p, row_bytes / 16, row_stride, outer_stride, n_outer, n_groups, n_beams, parents, s);
+  else if (unit == 4) launch_rows<uint32_t>(p, row_bytes / 4, row_stride, outer_stride, n_outer, n_groups, n_beams, parents, s);
+  else launch_rows<uint8_t>(p, row_bytes, row_stride, outer_stride, n_outer, n_groups, n_beams, parents, s);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? IT_OK : fail(IT_DEVICE_ERROR, "%s: launch: %s", who, hipGetErrorString(e));
+}

@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kThreads) void kv_gather_vec(
                       (int64_t(pos & ((1 << log2_bs) - 1)) * row_vecs + c) * 16;
   const int64_t dst = (cu_out[b] * hkv + int64_t(h) * n + i) * row_vecs + c;
   st16(kout + dst, ld16_nt(kpool + src));
-  st16(vout + dst, ld16_nt(vpool + src));
+  if (vout) st16(vout + dst, ld16_nt(vpool + src));  // a latent cache has one pool
 }
 
 // Quantised gather: lane = one 32-element group, written as a packed record:
@@ -554,7 +554,7 @@ __global__ __launch_bounds__(kThreads) void kv_clear_blocks(char* __restrict__ k
                                                             int64_t block_vecs, int64_t num_blocks,
                                                             int64_t layer_bytes, uint32_t* err) {
   kpool += int64_t(blockIdx.z) * layer_bytes;
-  vpool += int64_t(blockIdx.z) * layer_bytes;
+  if (vpool) vpool += int64_t(blockIdx.z) * layer_bytes;  // NULL: a latent cache
   const int blk = blocks[blockIdx.y];
   if (blk < 0 || blk >= num_blocks) {
     if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicOr(err, kErrBlock);
@@ -563,7 +563,7 @@ __global__ __launch_bounds__(kThreads) void kv_clear_blocks(char* __restrict__ k
   const uint4 z = make_uint4(0u, 0u, 0u, 0u);
   for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < block_vecs; i += int64_t(gridDim.x) * kThreads) {
     st16(kpool + (blk * block_vecs + i) * 16, z);
-    st16(vpool + (blk * block_vecs + i) * 16, z);
+    if (vpool) st16(vpool + (blk * block_vecs + i) * 16, z);
   }
 }
 
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(kThreads) void kv_copy_blocks(char* __restrict__ kp
                                                            int64_t block_vecs, int64_t num_blocks,
                                                            int64_t layer_bytes, uint32_t* err) {
   kpool += int64_t(blockIdx.z) * layer_bytes;
-  vpool += int64_t(blockIdx.z) * layer_bytes;
+  if (vpool) vpool += int64_t(blockIdx.z) * layer_bytes;  // NULL: a latent cache
   const int s = src[blockIdx.y], d = dst[blockIdx.y];
   if (s < 0 || s >= num_blocks || d < 0 || d >= num_blocks) {
     if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) atomicOr(err, kErrBlock);
@@ -582,7 +582,7 @@ __global__ __launch_bounds__(kThreads) void kv_copy_blocks(char* __restrict__ kp
   }
   for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < block_vecs; i += int64_t(gridDim.x) * kThreads) {
     st16(kpool + (d * block_vecs + i) * 16, ld16_nt(kpool + (s * block_vecs + i) * 16));
-    st16(vpool + (d * block_vecs + i) * 16, ld16_nt(vpool + (s * block_vecs + i) * 16));
+    if (vpool) st16(vpool + (d * block_vecs + i) * 16, ld16_nt(vpool + (s * block_vecs + i) * 16));
   }
 }
 
@@ -631,7 +631,8 @@ int32_t check_shape(int64_t num_blocks, int32_t block_size, int32_t n_kv_heads, 
 }
 
 int32_t make_cache(int32_t device, void* k, void* v, int32_t n_layers, int64_t num_blocks, int32_t block_size,
-                   int32_t n_kv_heads, int32_t head_dim, int32_t dtype, int32_t owns, it_kv_cache** out) {
+                   int32_t n_kv_heads, int32_t head_dim, int32_t dtype, int32_t owns, it_kv_cache** out,
+                   int32_t latent_dim = 0) {
   auto* c = new (std::nothrow) it_kv_cache;
   if (!c) return fail(IT_DEVICE_ERROR, "kv cache: out of host memory");
   c->k_pool = k;
@@ -648,6 +649,7 @@ int32_t make_cache(int32_t device, void* k, void* v, int32_t n_layers, int64_t n
   c->dtype = dtype;
   c->device = device;
   c->owns_memory = owns;
+  c->latent_dim = latent_dim;
   c->err_flag = nullptr;
   hipError_t e = hipMalloc(&c->err_flag, 256);
   if (e == hipSuccess) e = hipMemset(c->err_flag, 0, 256);
@@ -744,6 +746,49 @@ extern "C" int32_t it_kv_cache_wrap(int32_t device, void* k_pool, void* v_pool, 
                                  out);
 }
 
+// A latent cache: one pool of rows of latent_dim + rope_dim elements.
+namespace {
+int32_t check_latent(const char* who, int32_t n_layers, int64_t num_blocks, int32_t block_size, int32_t latent_dim, int32_t rope_dim,
+                     int32_t dtype, it_kv_cache** out) {
+  if (!out) return fail(IT_INVALID_INPUT, "%s: out is NULL", who);
+  *out = nullptr;
+  if (n_layers <= 0 || n_layers > kMaxLayers) return fail(IT_INVALID_INPUT, "%s: n_layers %d outside [1, %d]", who, n_layers, kMaxLayers);
+  if (latent_dim < 8 || latent_dim > 1024 || latent_dim % 8 || rope_dim < 8 || rope_dim > 256 || rope_dim % 8)
+    return fail(IT_INVALID_INPUT, "%s: latent_dim %d (8 .. 1024) and rope_dim %d (8 .. 256) must be multiples of 8", who, latent_dim, rope_dim);
+  if (is_quant(dtype)) return fail(IT_NOT_IMPLEMENTED, "%s: dtype %d (F32, F16 or BF16)", who, dtype);
+  return check_shape(num_blocks, block_size, 1, latent_dim + rope_dim, dtype);
+}
+}  // namespace
+
+extern "C" int32_t it_kv_cache_new_latent(int32_t device, int32_t n_layers, int64_t num_blocks, int32_t block_size,
+                                          int32_t latent_dim, int32_t rope_dim, int32_t dtype, it_kv_cache** out) {
+  const char* who = "it_kv_cache_new_latent";
+  if (int32_t rc = check_latent(who, n_layers, num_blocks, block_size, latent_dim, rope_dim, dtype, out)) return rc;
+  DeviceGuard g(device);
+  const size_t bytes = size_t(n_layers) * size_t(num_blocks) * size_t(it_kv_page_bytes(block_size, latent_dim + rope_dim, dtype));
+  void* pool = nullptr;
+  hipError_t e = hipMalloc(&pool, bytes);
+  if (e == hipSuccess) e = hipMemset(pool, 0, bytes);
+  if (e != hipSuccess) {
+    if (pool) (void)hipFree(pool);
+    return fail(IT_DEVICE_ERROR, "%s: %zu bytes: %s", who, bytes, hipGetErrorString(e));
+  }
+  const int32_t rc = make_cache(device, pool, nullptr, n_layers, num_blocks, block_size, 1, latent_dim + rope_dim, dtype, 1, out, latent_dim);
+  if (rc) (void)hipFree(pool);
+  return rc;
+}
+
+extern "C" int32_t it_kv_cache_wrap_latent(int32_t device, int32_t n_layers, void* pool, int64_t num_blocks, int32_t block_size,
+                                           int32_t latent_dim, int32_t rope_dim, int32_t dtype, it_kv_cache** out) {
+  const char* who = "it_kv_cache_wrap_latent";
+  if (int32_t rc = check_latent(who, n_layers, num_blocks, block_size, latent_dim, rope_dim, dtype, out)) return rc;
+  if (!pool || !aligned16(pool)) return fail(IT_INVALID_INPUT, "%s: the pool must be given, 16-byte aligned", who);
+  DeviceGuard g(device);
+  return make_cache(device, pool, nullptr, n_layers, num_blocks, block_size, 1, latent_dim + rope_dim, dtype, 0, out, latent_dim);
+}
+
+extern "C" int32_t it_kv_cache_latent_dim(const it_kv_cache* c) { return c ? c->latent_dim : 0; }
+
 extern "C" int32_t it_kv_cache_layer(const it_kv_cache* c, int32_t layer, it_kv_cache** out) {
   if (!out) return fail(IT_INVALID_INPUT, "it_kv_cache_layer: out is NULL");
   *out = nullptr;
@@ -753,7 +798,7 @@ extern "C" int32_t it_kv_cache_layer(const it_kv_cache* c, int32_t layer, it_kv_
   auto* v = new (std::nothrow) it_kv_cache(*c);
   if (!v) return fail(IT_DEVICE_ERROR, "it_kv_cache_layer: out of host memory");
   v->k_pool = static_cast<char*>(c->k_pool) + int64_t(layer) * c->layer_bytes;
-  v->v_pool = static_cast<char*>(c->v_pool) + int64_t(layer) * c->layer_bytes;
+  if (c->v_pool) v->v_pool = static_cast<char*>(c->v_pool) + int64_t(layer) * c->layer_bytes;
   v->n_layers = 1;
   v->owns_memory = 0;
   v->owns_flag = 0;
@@ -766,7 +811,7 @@ extern "C" int32_t it_kv_cache_destroy(it_kv_cache* c) {
   DeviceGuard g(c->device);
   if (c->owns_memory) {
     (void)hipFree(c->k_pool);
-    (void)hipFree(c->v_pool);
+    if (c->v_pool) (void)hipFree(c->v_pool);
   }
   if (c->owns_flag) (void)hipFree(c->err_flag);
   delete c;
@@ -807,6 +852,7 @@ extern "C" int32_t it_kv_append(it_kv_cache* c, const void* k, const void* v, in
                                 const int64_t* slots, int32_t n_tokens, void* stream) {
   if (!c) return fail(IT_INVALID_INPUT, "it_kv_append: cache is NULL");
   if (int32_t rc = one_layer(c, "it_kv_append")) return rc;
+  if (int32_t rc = per_head(c, "it_kv_append")) return rc;
   if (n_tokens < 0) return fail(IT_INVALID_INPUT, "it_kv_append: n_tokens %d < 0", n_tokens);
   if (n_tokens == 0) return IT_OK;
   if (!k || !v || !slots) return fail(IT_INVALID_INPUT, "it_kv_append: NULL tensor");
@@ -887,7 +933,8 @@ extern "C" int32_t it_kv_gather(const it_kv_cache* c, const int32_t* bt, int32_t
   if (n_seqs < 0 || max_tokens < 0 || max_blocks <= 0)
     return fail(IT_INVALID_INPUT, "it_kv_gather: n_seqs=%d max_tokens=%d max_blocks=%d", n_seqs, max_tokens, max_blocks);
   if (n_seqs == 0 || max_tokens == 0) return IT_OK;
-  if (!bt || !ctx_lens || !cu_out || !k_out || !v_out) return fail(IT_INVALID_INPUT, "it_kv_gather: NULL tensor");
+  if (!bt || !ctx_lens || !cu_out || !k_out || (!v_out && !c->latent_dim)) return fail(IT_INVALID_INPUT, "it_kv_gather: NULL tensor");
+  if (v_out && c->latent_dim) return fail(IT_INVALID_INPUT, "it_kv_gather: a latent cache has no V rows (v_out must be NULL)");
   if (n_seqs > 65535) return fail(IT_NOT_IMPLEMENTED, "it_kv_gather: n_seqs %d > 65535", n_seqs);
   DeviceGuard g(c->device);
   hipStream_t s = (hipStream_t)stream;
@@ -977,6 +1024,11 @@ extern "C" int32_t it_supports(int32_t op, int32_t dtype) {
     case IT_OP_SAMPLE: return kv && !is_quant(dtype) ? 1 : 0;
     case IT_OP_PAGED_PREFILL: return (dtype == IT_BF16 || dtype == IT_F16) ? 1 : 0;
     case IT_OP_FLASH_ATTENTION: return dtype == IT_F32 ? 1 : 0;
+    case IT_OP_LATENT_APPEND:
+    case IT_OP_LATENT_DECODE:
+    case IT_OP_LATENT_PREFILL:
+    case IT_OP_BEAM_SELECT: return kv && !is_quant(dtype) ? 1 : 0;
+    case IT_OP_BEAM_REORDER: return 1;
     default: return 0;
   }
 }

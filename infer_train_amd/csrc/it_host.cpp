@@ -149,7 +149,8 @@ struct it_kv_manager {
   std::vector<int32_t> table;  // [max_seqs][max_blocks], -1 = not held
   std::vector<int64_t> pos;    // next position of each sequence (= ctx len)
   std::vector<int64_t> first;  // lowest logical block still held
-  std::vector<uint8_t> rewound;  // a compaction set the position back into a block that others hold too
+  std::vector<uint8_t> rewound;  // kRewound: a compaction set the position back into a block that others hold too;
+                                 // kContinued: a beam among others that continue the same block
   // Scratch of one step, reused across steps.
   std::vector<int32_t> pending;    // blocks the step returned to the pool, in free order; those a compaction drops
   std::vector<uint32_t> blk_step;  // [pool capacity] step number of a block's first write...
@@ -163,7 +164,7 @@ struct it_kv_manager {
   std::vector<Compacted> compacted;  // [max_seqs]
   std::vector<int32_t> old_row;      // [max_blocks] a sequence's blocks before its compaction
   std::vector<int32_t> drops;        // [pool capacity] 0 between calls
-  uint64_t compaction = 0;
+  uint64_t compaction = 0;           // or reordering: which call a sequence was last listed in
   uint32_t step = 0;
 };
 
@@ -216,17 +217,20 @@ extern "C" int32_t it_kv_manager_seed_seq(it_kv_manager* m, int32_t seq, int64_t
 }
 
 namespace {
+enum : uint8_t { kRewound = 1, kContinued = 2 };
+
 // Whether the next token of sequence s, written where it stands, would replace
 // one of another holder of its block: after a compaction that only dropped a
 // tail, the position lies among rows that forks may still read.  Forks whose
 // context ends at or before it do not; holders that this manager does not know
-// are taken to.
+// are taken to.  After a reordering, every holder is about to write there.
 bool overwrites(const it_kv_manager* m, int32_t s) {
   if (!m->rewound[size_t(s)]) return false;
   const int64_t p = m->pos[size_t(s)], lb = p / m->bs;
   if (lb >= m->max_blocks) return false;
   const int32_t id = m->table[size_t(s) * size_t(m->max_blocks) + size_t(lb)];
   if (id < 0) return false;
+  if (m->rewound[size_t(s)] == kContinued) return p % m->bs != 0 && it_block_pool_ref_count(m->pool, id) > 1;
   int64_t holders = 0;
   for (int32_t o = 0; o < m->max_seqs; ++o) {
     if (m->table[size_t(o) * size_t(m->max_blocks) + size_t(lb)] != id) continue;
@@ -303,7 +307,7 @@ int32_t step_impl(it_kv_manager* m, const int32_t* seqs, const int32_t* n_tokens
   if (cow && !pl->cow_dst) return fail(IT_INVALID_INPUT, "%s: cow_dst is NULL", who);
   for (int32_t i = 0; !cow && i < n; ++i)
     if (n_tokens[i] > 0 && overwrites(m, seqs[i]))
-      return fail(IT_INVALID_INPUT, "%s: seq %d, compacted, would write over a fork's tokens: append with copy-on-write", who,
+      return fail(IT_INVALID_INPUT, "%s: seq %d, compacted or reordered, would write over a fork's tokens: append with copy-on-write", who,
                   seqs[i]);
   m->pending.clear();
   if (++m->step == 0) {  // wrapped: no stale stamp may match
@@ -580,7 +584,7 @@ int32_t compact_impl(it_kv_manager* m, const char* who, const int32_t* seqs, int
     // rows that this sequence writes next.
     if (!m->compacted[size_t(s)].prefix) m->rewound[size_t(s)] = 0;
     else if (n_keep != m->pos[size_t(s)])
-      m->rewound[size_t(s)] = n_keep % bs != 0 && it_block_pool_ref_count(m->pool, row_of(s)[n_keep / bs]) > 1;
+      m->rewound[size_t(s)] = n_keep % bs != 0 && it_block_pool_ref_count(m->pool, row_of(s)[n_keep / bs]) > 1 ? kRewound : 0;
     m->pos[size_t(s)] = n_keep;
     m->first[size_t(s)] = 0;
   }
@@ -611,6 +615,90 @@ extern "C" int32_t it_kv_manager_compact_many(it_kv_manager* m, const int32_t* s
   if (n_seqs > 0 && cu_keep[n_seqs] > 0 && !keep) return fail(IT_INVALID_INPUT, "%s: NULL argument", who);
   return compact_impl(m, who, seqs, n_seqs, keep, cu_keep, src, dst, delta, token_seq, pos, moves_cap, n_moves, evicted, evicted_cap,
                       n_evicted);
+}
+
+extern "C" int32_t it_kv_manager_reorder(it_kv_manager* m, const int32_t* seqs, const int32_t* parents, int32_t n,
+                                         int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted) {
+  const char* who = "it_kv_manager_reorder";
+  if (!m || !n_evicted || n < 0 || (n > 0 && (!seqs || !parents))) return fail(IT_INVALID_INPUT, "%s: NULL argument", who);
+  const size_t width = size_t(m->max_blocks);
+  const auto row_of = [&](int32_t i) { return &m->table[size_t(seqs[i]) * width]; };
+  // Every check before any change.
+  ++m->compaction;
+  for (int32_t i = 0; i < n; ++i) {
+    const int32_t s = seqs[i];
+    if (s < 0 || s >= m->max_seqs || parents[i] >= n) return fail(IT_INVALID_INPUT, "%s: seq %d, parent %d of %d", who, s, parents[i], n);
+    if (m->compacted[size_t(s)].in == m->compaction) return fail(IT_INVALID_INPUT, "%s: seq %d is listed twice", who, s);
+    m->compacted[size_t(s)].in = m->compaction;
+  }
+  struct State {
+    int64_t pos, first;
+    uint8_t rewound;
+  };
+  std::vector<int32_t> rows, next;  // what the sequences held; how many continue each
+  std::vector<State> states;
+  m->pending.clear();
+  try {
+    rows.resize(size_t(n) * width);
+    next.assign(size_t(n), 0);
+    states.resize(size_t(n));
+    m->pending.reserve(size_t(n) * width);
+  } catch (const std::bad_alloc&) {
+    return fail(IT_DEVICE_ERROR, "%s: out of host memory", who);
+  }
+  const auto parent_of = [&](int32_t i) { return parents[i] < 0 ? i : parents[i]; };
+  for (int32_t i = 0; i < n; ++i) ++next[size_t(parent_of(i))];
+  for (int32_t i = 0; i < n; ++i)
+    for (size_t j = 0; j < width; ++j) {
+      const int32_t id = row_of(i)[j];
+      if (id < 0) continue;
+      if (it_block_pool_ref_count(m->pool, id) <= 0) {
+        for (int32_t x : m->pending) m->drops[size_t(x)] = 0;
+        m->pending.clear();
+        return fail(IT_INVALID_INPUT, "%s: block %d is already free", who, id);
+      }
+      m->pending.push_back(id);
+      m->drops[size_t(id)] += 1 - next[size_t(i)];
+    }
+  int64_t returned = 0;
+  for (int32_t id : m->pending) {
+    returned += m->drops[size_t(id)] == it_block_pool_ref_count(m->pool, id);
+    m->drops[size_t(id)] = 0;  // counted once
+  }
+  m->pending.clear();
+  if (returned > 0 && (!evicted || returned > evicted_cap))
+    return fail(IT_INVALID_INPUT, "%s: %lld blocks return to the pool, capacity %d", who, (long long)returned, evicted_cap);
+  for (int32_t i = 0; i < n; ++i) {
+    std::copy(row_of(i), row_of(i) + width, &rows[size_t(i) * width]);
+    states[size_t(i)] = {m->pos[size_t(seqs[i])], m->first[size_t(seqs[i])], m->rewound[size_t(seqs[i])]};
+  }
+  for (int32_t i = 0; i < n; ++i) {  // every new reference before the first that goes
+    const int32_t p = parent_of(i);
+    if (p == i) continue;
+    const int32_t* const from = &rows[size_t(p) * width];
+    for (size_t j = 0; j < width; ++j)
+      if (from[j] >= 0) (void)it_block_pool_share(m->pool, from[j]);
+    std::copy(from, from + width, row_of(i));
+    m->pos[size_t(seqs[i])] = states[size_t(p)].pos;
+    m->first[size_t(seqs[i])] = states[size_t(p)].first;
+    m->rewound[size_t(seqs[i])] = states[size_t(p)].rewound;
+  }
+  int32_t ne = 0;
+  for (int32_t i = 0; i < n; ++i) {
+    if (parent_of(i) == i) continue;
+    for (size_t j = 0; j < width; ++j) {
+      const int32_t id = rows[size_t(i) * width + j];
+      if (id >= 0 && it_block_pool_free(m->pool, id) == IT_OK && it_block_pool_ref_count(m->pool, id) == 0 && ne < evicted_cap)
+        evicted[ne++] = id;
+    }
+  }
+  // A block that several now end in is written by each of them next.
+  for (int32_t i = 0; i < n; ++i) {
+    const int64_t p = m->pos[size_t(seqs[i])];
+    if (next[size_t(parent_of(i))] > 1 && p % m->bs != 0) m->rewound[size_t(seqs[i])] = kContinued;
+  }
+  *n_evicted = ne;
+  return IT_OK;
 }
 
 extern "C" int32_t it_kv_manager_tables(const it_kv_manager* m, int32_t* tables, int32_t max_blocks,

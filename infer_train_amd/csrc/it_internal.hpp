@@ -56,6 +56,7 @@ struct it_kv_cache {
   int32_t device;
   int32_t owns_memory;
   int32_t owns_flag;    // 0 for a layer view
+  int32_t latent_dim;   // 0; of a latent cache (v_pool NULL, one row of head_dim elements a token) the latent's elements
 };
 
 namespace itkv {
@@ -65,6 +66,12 @@ inline int32_t one_layer(const it_kv_cache* c, const char* who) {
   if (c && c->n_layers != 1)
     return fail(IT_INVALID_INPUT, "%s: the cache holds %d layers; pass the layer's view (it_kv_cache_layer)", who,
                 c->n_layers);
+  return IT_OK;
+}
+// Entry points for K and V rows do not take a latent cache.
+inline int32_t per_head(const it_kv_cache* c, const char* who) {
+  if (c && c->latent_dim)
+    return fail(IT_INVALID_INPUT, "%s: the cache holds latent rows (it_latent_append, it_latent_decode)", who);
   return IT_OK;
 }
 // Looks up the device address of the no-allocation decode's array on the

@@ -31,7 +31,8 @@ struct MoveArgs {
   uint32_t heads, rows;  // rows of a pair: layers x heads x pools moved
   int log2_bs;
   int main_bytes, side_bytes;  // of a token's row in a page; the side row is quantised formats' (scales, high bits)
-  int pools;                   // 2: K then V; 1: V alone (byte copies), K alone (quantised keys)
+  int pools;                   // 2: K then V; 1: V alone (byte copies), K alone (quantised keys), latent rows
+  int latent;                  // elements of a latent row before its rope part
   RowSplit split;
 };
 
@@ -168,6 +169,35 @@ __global__ __launch_bounds__(kThreads) void kv_move_general(MoveArgs a) {
   store_element(to, e1, DT, y);
 }
 
+// Latent rows, their rope part turned: a wave takes one (pair, layer) row, the
+// latent as 16-byte pieces, a lane per pair of the rope part.  Each lane writes
+// what it has read itself, so a row may be turned in place.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void kv_move_latent(MoveArgs a) {
+  const int lane = int(threadIdx.x & 63);
+  const int64_t i = int64_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  if (i >= a.n) return;
+  int64_t s, d;
+  if (!move_slots(a, i, s, d, blockIdx.y == 0 && lane == 0)) return;
+  const int delta = a.delta[i], half = a.split.n_dims >> 1;
+  const int64_t bs = int64_t(1) << a.log2_bs;
+  if (s == d && delta == 0) return;
+  bool key;
+  const char* const from = move_page(a, blockIdx.y, s, key) + (s & (bs - 1)) * a.main_bytes;
+  char* const to = move_page(a, blockIdx.y, d, key) + (d & (bs - 1)) * a.main_bytes;
+  const bool halves = a.split.layout == IT_ROTARY_HALF;
+  const int pieces = a.latent * (DT == IT_F32 ? 4 : 2) / 16;
+  for (int p = lane; p < half; p += 64) {
+    const int e0 = a.latent + (halves ? p : 2 * p), e1 = a.latent + (halves ? p + half : 2 * p + 1);
+    float x = load_element(from, e0, DT), y = load_element(from, e1, DT);
+    if (delta) LanePairs<4>::pair(rotary_angle(a.turns[p], delta), x, y);
+    store_element(to, e0, DT, x);
+    store_element(to, e1, DT, y);
+  }
+  if (s == d) return;
+  for (int p = lane; p < pieces; p += 64) st16(to + p * 16, ld16(from + p * 16));
+}
+
 // Elements 4 cv .. 4 cv + 3 of a quantised token row.
 template <int DT>
 __device__ __forceinline__ float4 dequant4(const char* page, int64_t off, int64_t bs, int d, int cv) {
@@ -299,6 +329,10 @@ void launch_rows(const MoveArgs& a, bool split, hipStream_t s) {
   else
     hipLaunchKernelGGL((kv_move_rows<DT, 2>), dim3(bx, unsigned(chunks(2))), dim3(kThreads), lds, s, a);
 }
+void launch_latent(const MoveArgs& a, int32_t dtype, hipStream_t s) {
+  auto* const kern = dtype == IT_F32 ? kv_move_latent<IT_F32> : dtype == IT_BF16 ? kv_move_latent<IT_BF16> : kv_move_latent<IT_F16>;
+  hipLaunchKernelGGL(kern, dim3(unsigned((a.n + kWaves - 1) / kWaves), a.rows), dim3(kThreads), 0, s, a);
+}
 template <int DT>
 void launch_quant(MoveArgs a, hipStream_t s) {
   // K alone: its heads are the only ones of a layer (the pool that move_page
@@ -322,6 +356,9 @@ extern "C" int32_t it_kv_move(it_kv_cache* c, const int64_t* src, const int64_t*
   const char* who = "it_kv_move";
   if (!c) return fail(IT_INVALID_INPUT, "%s: cache is NULL", who);
   if (n < 0) return fail(IT_INVALID_INPUT, "%s: n %d < 0", who, n);
+  if (rotary && c->latent_dim && rotary->n_dims != c->head_dim - c->latent_dim)
+    return fail(IT_INVALID_INPUT, "%s: %d rotated elements, a latent row turns its %d rope elements", who, rotary->n_dims,
+                c->head_dim - c->latent_dim);
   if (rotary && rotary->n_dims > c->head_dim)
     return fail(IT_INVALID_INPUT, "%s: %d rotated elements > head_dim %d", who, rotary->n_dims, c->head_dim);
   if (rotary && rotary->device != c->device) return fail(IT_INVALID_INPUT, "%s: rotary and cache on different devices", who);
@@ -330,7 +367,8 @@ extern "C" int32_t it_kv_move(it_kv_cache* c, const int64_t* src, const int64_t*
   if (n == 0) return IT_OK;
   if (!src || !dst) return fail(IT_INVALID_INPUT, "%s: NULL slots", who);
   if (rotary && !delta) return fail(IT_INVALID_INPUT, "%s: delta is NULL", who);
-  const int64_t rows = int64_t(c->n_layers) * c->n_kv_heads * 2, row_items = int64_t(c->head_dim) * 2;
+  const int pools = c->latent_dim ? 1 : 2;
+  const int64_t rows = int64_t(c->n_layers) * c->n_kv_heads * pools, row_items = int64_t(c->head_dim) * 2;
   // A pair's rows are chunks of a grid's second direction (fewer than 65536 at
   // this limit: a chunk is 64 pieces of 16 bytes or 2), pairs its first (2^32 work
   // items).
@@ -338,7 +376,8 @@ extern "C" int32_t it_kv_move(it_kv_cache* c, const int64_t* src, const int64_t*
     return fail(IT_INVALID_INPUT, "%s: %d pairs of %lld rows of %d elements", who, n, (long long)rows, c->head_dim);
   MoveArgs a{};
   a.kpool = static_cast<char*>(c->k_pool);
-  a.vpool = static_cast<char*>(c->v_pool);
+  a.vpool = static_cast<char*>(c->latent_dim ? c->k_pool : c->v_pool);
+  a.latent = c->latent_dim;
   a.src = src;
   a.dst = dst;
   a.delta = rotary ? delta : nullptr;
@@ -354,9 +393,9 @@ extern "C" int32_t it_kv_move(it_kv_cache* c, const int64_t* src, const int64_t*
   const int64_t row_bytes = c->page_bytes / c->block_size;
   a.main_bytes = int(c->dtype == IT_Q8_0 ? c->head_dim : quant ? c->head_dim / 2 : row_bytes);
   a.side_bytes = int(row_bytes - a.main_bytes);
-  a.pools = 2;
+  a.pools = pools;
   bool split = false;
-  if (rotary) {
+  if (rotary && !c->latent_dim) {
     a.split.head_dim = c->head_dim;
     a.split.n_dims = rotary->n_dims;
     a.split.layout = rotary->layout;
@@ -371,6 +410,11 @@ extern "C" int32_t it_kv_move(it_kv_cache* c, const int64_t* src, const int64_t*
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!rotary) {
     launch_bytes(a, s);
+  } else if (c->latent_dim) {
+    a.split.head_dim = c->head_dim;
+    a.split.n_dims = rotary->n_dims;
+    a.split.layout = rotary->layout;
+    launch_latent(a, c->dtype, s);
   } else {
     switch (c->dtype) {
       case IT_F32: launch_rows<IT_F32>(a, split, s); break;

@@ -1042,6 +1042,7 @@ extern "C" int32_t it_paged_prefill_ws(const it_kv_cache* c, const void* q, int3
   const char* who = "it_paged_prefill";
   if (!c) return fail(IT_INVALID_INPUT, "%s: cache is NULL", who);
   if (int32_t rc = one_layer(c, who)) return rc;
+  if (int32_t rc = per_head(c, who)) return rc;
   if (c->dtype != IT_BF16 && c->dtype != IT_F16)
     return fail(IT_NOT_IMPLEMENTED, "%s: cache dtype %d (BF16 or F16 supported)", who, c->dtype);
   if (q_dtype != c->dtype) return fail(IT_NOT_IMPLEMENTED, "%s: q dtype %d must equal the cache dtype", who, q_dtype);

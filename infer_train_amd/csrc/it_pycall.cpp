@@ -100,7 +100,9 @@ struct Call<kHost, R (*)(A...)> {
   X(it_paged_decode_partition, true) X(it_paged_decode, false) X(it_paged_decode_split, false)                           \
   X(it_paged_decode_combine, false) X(it_paged_prefill_workspace, false) X(it_paged_prefill_ws, false)                   \
   X(it_flash_attention_workspace, false) X(it_flash_attention, false) X(it_rotary_apply, false)                          \
-  X(it_kv_append_rotary, false) X(it_kv_move, false) X(it_sample_workspace, false) X(it_sample, false)
+  X(it_kv_append_rotary, false) X(it_kv_move, false) X(it_sample_workspace, false) X(it_sample, false)                   \
+  X(it_latent_append, false) X(it_latent_decode_workspace, false) X(it_latent_decode, false)                             \
+  X(it_latent_prefill, false) X(it_beam_select_workspace, false) X(it_beam_select, false) X(it_beam_reorder, false)
 
 #define IT_WRAP(name, host)                                                         \
   decltype(&name) p_##name = nullptr;                                               \

@@ -438,6 +438,7 @@ extern "C" int32_t it_kv_append_rotary(it_kv_cache* c, const it_rotary* rotary, 
   const char* who = "it_kv_append_rotary";
   if (!c || !rotary) return fail(IT_INVALID_INPUT, "%s: cache or rotary is NULL", who);
   if (int32_t rc = one_layer(c, who)) return rc;
+  if (int32_t rc = per_head(c, who)) return rc;
   if (!is_float(src_dtype)) return fail(IT_NOT_IMPLEMENTED, "%s: src_dtype %d (F32, F16 or BF16)", who, src_dtype);
   if (n_tokens < 0) return fail(IT_INVALID_INPUT, "%s: n_tokens %d < 0", who, n_tokens);
   if (n_heads < 0 || n_heads > 65536 || n_heads % c->n_kv_heads)

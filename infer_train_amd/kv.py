@@ -193,7 +193,87 @@ class _Turn(torch.autograd.Function):
         return ctx.rotary.apply(grad, positions, transpose=not ctx.transpose), None, None, None
 
 
-class PagedKvCache:
+class _Pages:
+    """What every paged cache has: its handle, one layer's view of it, and the
+    moves of whole pages and rows."""
+
+    _LAYER_FIELDS = ("num_blocks", "block_size", "n_kv_heads", "head_dim", "dtype", "page_bytes", "device")
+
+    def _adopt(self, handle: C.c_void_p, index: int) -> None:
+        self._h = handle
+        self._at = handle.value  # the handle as the compiled bindings take it
+        self._index = index
+        # Bound now: at interpreter exit the module global may already be gone.
+        self._destroy = lib.it_kv_cache_destroy
+
+    @property
+    def handle(self) -> C.c_void_p:
+        return self._h
+
+    def layer(self, index: int):
+        """One layer of a multi-layer cache (it_kv_cache_layer): a cache
+        object whose pools are that layer's bytes of this cache's pools."""
+        h = C.c_void_p()
+        check(lib.it_kv_cache_layer(self._h, int(index), C.byref(h)))
+        view = object.__new__(type(self))
+        lb = self.num_blocks * self.n_kv_heads * self.page_bytes
+        view.k_pool = self.k_pool[index * lb:(index + 1) * lb]
+        view.v_pool = None if self.v_pool is None else self.v_pool[index * lb:(index + 1) * lb]
+        view._adopt(h, self._index)
+        for name in self._LAYER_FIELDS:
+            setattr(view, name, getattr(self, name))
+        view.n_layers = 1
+        view._parent = self  # destroyed before the parent
+        return view
+
+    def _one_layer(self) -> None:
+        if self.n_layers != 1:
+            raise TypeError("a multi-layer cache: take one layer's view with layer(l)")
+
+    def describe(self) -> CacheDesc:
+        d = CacheDesc()
+        check(lib.it_kv_cache_describe(self._h, C.byref(d)))
+        return d
+
+    def check(self) -> None:
+        """Raise if a kernel latched a device-side range error (syncs the stream)."""
+        check(lib.it_kv_cache_check(self._h, stream_handle(self.device)))
+
+    def evict(self, blocks: torch.Tensor) -> None:
+        _check(call.it_kv_evict(self._at, _ptr(blocks), blocks.numel(), _raw_stream(self._index)))
+
+    def sync_tables(self, tables: torch.Tensor, seq: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor) -> None:
+        """tables[seq[i], pos[i] // bs] = slots[i] // bs (device int32 table [n_seqs, max_blocks])."""
+        _check(call.it_kv_sync_tables(self._at, _ptr(tables), tables.shape[1], tables.shape[0], _ptr(seq), _ptr(pos),
+                                      _ptr(slots), slots.numel(), _raw_stream(self._index)))
+
+    def copy_blocks(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        _check(call.it_kv_copy_blocks(self._at, _ptr(src), _ptr(dst), src.numel(), _raw_stream(self._index)))
+
+    def move(self, src: torch.Tensor, dst: torch.Tensor, rotary: Optional[Rotary] = None,
+             delta: Optional[torch.Tensor] = None) -> None:
+        """Rows of slots src to slots dst (int64 [n]) in every layer and head
+        (it_kv_move); with rotary, keys are turned by delta positions (int32
+        [n], new - old), as KvManager.compact plans it."""
+        if src.dtype != torch.int64 or dst.dtype != torch.int64 or src.numel() != dst.numel():
+            raise TypeError("src and dst must be int64, one slot each per row")
+        if (rotary is None) != (delta is None):
+            raise TypeError("rotary and delta go together")
+        if delta is not None and (delta.dtype != torch.int32 or delta.numel() != src.numel()):
+            raise TypeError("delta must be int32, one per row")
+        at = self._index
+        _check(call.it_kv_move(self._at, _on(src, at), _on(dst, at), src.numel(), None if rotary is None else rotary._at,
+                               None if delta is None else _on(delta, at), _raw_stream(at)))
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        destroy = getattr(self, "_destroy", None)
+        if h is not None and h.value and destroy is not None:
+            destroy(h)
+            self._h = None
+
+
+class PagedKvCache(_Pages):
     """Paged K/V pools in HBM, [num_blocks][n_kv_heads] pages of block_size
     token rows (Q8_0 pages: int8 rows then fp16 group scales; Q4_0 pages:
     rows of BlockQ4_0 nibble bytes then fp16 group scales; Q4_1 the same
@@ -218,49 +298,13 @@ class PagedKvCache:
         h = C.c_void_p()
         check(lib.it_kv_cache_wrap_layers(device, n_layers, self.k_pool.data_ptr(), self.v_pool.data_ptr(),
                                           num_blocks, block_size, n_kv_heads, head_dim, dtype, C.byref(h)))
-        self._h = h
-        self._at = h.value  # the handle as the compiled bindings take it
-        self._index = device
-        # Bound now: at interpreter exit the module global may already be gone.
-        self._destroy = lib.it_kv_cache_destroy
+        self._adopt(h, device)
         self.num_blocks, self.block_size, self.n_kv_heads, self.head_dim = num_blocks, block_size, n_kv_heads, head_dim
         self.dtype = dtype
         self.page_bytes = page
         self.device = dev
         self.n_layers = n_layers
         self._parent = None
-
-    @property
-    def handle(self) -> C.c_void_p:
-        return self._h
-
-    def layer(self, index: int) -> "PagedKvCache":
-        """One layer of a multi-layer cache (it_kv_cache_layer): a cache
-        object whose pools are that layer's bytes of this cache's pools."""
-        h = C.c_void_p()
-        check(lib.it_kv_cache_layer(self._h, int(index), C.byref(h)))
-        view = object.__new__(PagedKvCache)
-        lb = self.num_blocks * self.n_kv_heads * self.page_bytes
-        view.k_pool = self.k_pool[index * lb:(index + 1) * lb]
-        view.v_pool = self.v_pool[index * lb:(index + 1) * lb]
-        view._h = h
-        view._at = h.value
-        view._index = self._index
-        view._destroy = lib.it_kv_cache_destroy
-        for name in ("num_blocks", "block_size", "n_kv_heads", "head_dim", "dtype", "page_bytes", "device"):
-            setattr(view, name, getattr(self, name))
-        view.n_layers = 1
-        view._parent = self  # destroyed before the parent
-        return view
-
-    def _one_layer(self) -> None:
-        if self.n_layers != 1:
-            raise TypeError("a multi-layer cache: take one layer's view with layer(l)")
-
-    def describe(self) -> CacheDesc:
-        d = CacheDesc()
-        check(lib.it_kv_cache_describe(self._h, C.byref(d)))
-        return d
 
     def view(self, which: str = "k") -> torch.Tensor:
         """Typed view [num_blocks, n_kv_heads, block_size, head_dim] (F32/F16/BF16)."""
@@ -309,10 +353,6 @@ class PagedKvCache:
         shape = (nb, H, bs, ng) + ((2,) if self.dtype == Q5_1 else ())
         d = side[..., 4 * ng:].contiguous().view(torch.int16).reshape(shape)
         return qs, qh, d
-
-    def check(self) -> None:
-        """Raise if a kernel latched a device-side range error (syncs the stream)."""
-        check(lib.it_kv_cache_check(self._h, stream_handle(self.device)))
 
     # ---- data movement ----------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor) -> None:
@@ -386,32 +426,6 @@ class PagedKvCache:
                                  _ptr(cu_out), ctx_lens.numel(), max_tokens, _ptr(k_out), _ptr(v_out),
                                  _raw_stream(self._index)))
 
-    def evict(self, blocks: torch.Tensor) -> None:
-        _check(call.it_kv_evict(self._at, _ptr(blocks), blocks.numel(), _raw_stream(self._index)))
-
-    def sync_tables(self, tables: torch.Tensor, seq: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor) -> None:
-        """tables[seq[i], pos[i] // bs] = slots[i] // bs (device int32 table [n_seqs, max_blocks])."""
-        _check(call.it_kv_sync_tables(self._at, _ptr(tables), tables.shape[1], tables.shape[0], _ptr(seq), _ptr(pos),
-                                      _ptr(slots), slots.numel(), _raw_stream(self._index)))
-
-    def copy_blocks(self, src: torch.Tensor, dst: torch.Tensor) -> None:
-        _check(call.it_kv_copy_blocks(self._at, _ptr(src), _ptr(dst), src.numel(), _raw_stream(self._index)))
-
-    def move(self, src: torch.Tensor, dst: torch.Tensor, rotary: Optional[Rotary] = None,
-             delta: Optional[torch.Tensor] = None) -> None:
-        """Rows of slots src to slots dst (int64 [n]) in every layer and head
-        (it_kv_move); with rotary, keys are turned by delta positions (int32
-        [n], new - old), as KvManager.compact plans it."""
-        if src.dtype != torch.int64 or dst.dtype != torch.int64 or src.numel() != dst.numel():
-            raise TypeError("src and dst must be int64, one slot each per row")
-        if (rotary is None) != (delta is None):
-            raise TypeError("rotary and delta go together")
-        if delta is not None and (delta.dtype != torch.int32 or delta.numel() != src.numel()):
-            raise TypeError("delta must be int32, one per row")
-        at = self._index
-        _check(call.it_kv_move(self._at, _on(src, at), _on(dst, at), src.numel(), None if rotary is None else rotary._at,
-                               None if delta is None else _on(delta, at), _raw_stream(at)))
-
     # ---- attention --------------------------------------------------------
     def decode_workspace(self, n_seqs: int, n_heads: int, max_tokens: int, partition: int = 512) -> torch.Tensor:
         nbytes = call.it_paged_decode_workspace(n_seqs, n_heads, self.head_dim, max_tokens, partition)
@@ -480,13 +494,6 @@ class PagedKvCache:
                                       int(bool(causal)), _ptr(ws), need, _ptr(out), torch_dtype_id(out.dtype),
                                       _raw_stream(self._index)))
         return out
-
-    def __del__(self):
-        h = getattr(self, "_h", None)
-        destroy = getattr(self, "_destroy", None)
-        if h is not None and h.value and destroy is not None:
-            destroy(h)
-            self._h = None
 
 
 def decode_partition(dtype: int, head_dim: int, block_size: int, n_heads: int, n_kv_heads: int, ctx_lens,
