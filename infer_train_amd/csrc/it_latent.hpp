@@ -63,10 +63,24 @@ __device__ __forceinline__ LatentSpan latent_span(const LatentDecodeArgs& a, int
 
 constexpr int kLatentMaxQ = 64;  // new tokens of a sequence
 
+// How an absorbed call's tokens are divided, and where pieces of sequences go.
+struct LatentSplitPlan {
+  int workers;   // runs that the tiles are divided into
+  int row_wgs;   // workgroups that share a run, each with QG * 16 queries of its own
+  float4* o;     // partial O^T: [worker][row wg][2][QG][L / 16][64 lanes]
+  float2* ml;    // and its (maximum, sum): [worker][row wg][2][QG][16]
+};
+
+hipError_t latent_decode_bf16(const LatentDecodeArgs& a, const LatentSplitPlan& p, int qg, hipStream_t s);
+hipError_t latent_decode_f16(const LatentDecodeArgs& a, const LatentSplitPlan& p, int qg, hipStream_t s);
+
 // The matrix-core kernels: false where they do not take the call (its type,
-// widths or pages); else launched, `e` the result.
-inline size_t latent_decode_matrix_ws(int32_t, int, int, int, int, int, int, int) { return 0; }
-inline bool latent_decode_matrix(const LatentDecodeArgs&, int32_t, int, hipStream_t, hipError_t&) { return false; }
+// widths or pages); else launched, `e` the result.  n_cu: the device's compute
+// units (latent_compute_units).
+int latent_compute_units(int device);
+size_t latent_decode_matrix_ws(int32_t dtype, int latent, int rope, int block_size, int n_seqs, int q_len, int n_heads, int max_tokens,
+                               int n_cu);
+bool latent_decode_matrix(const LatentDecodeArgs& a, int32_t dtype, int block_size, int n_cu, hipStream_t s, hipError_t& e);
 inline bool latent_prefill_matrix(const LatentPrefillArgs&, int32_t, hipStream_t, hipError_t&) { return false; }
 
 }  // namespace itkv

@@ -4,6 +4,8 @@
 // (it_latent_decode.hip, it_latent_prefill.hip).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "it_latent.hpp"
@@ -133,9 +135,64 @@ int32_t decode_sizes(const char* who, const it_kv_cache* c, int32_t n_seqs, int3
 }
 }  // namespace
 
+namespace {
+constexpr int kTile = 32;  // of the matrix-core kernels: cached tokens
+// Query groups and token groups of a workgroup by the call's queries.
+struct HostPlan {
+  int qg, kg, workers, row_wgs;
+  size_t o_bytes, ml_bytes;
+};
+HostPlan plan_of(int latent, int n_seqs, int q_len, int n_heads, int max_tokens, int n_cu) {
+  HostPlan p;
+  const int groups = (q_len * n_heads + 15) / 16;  // of 16 queries
+  p.qg = groups <= 1 ? 1 : groups == 2 ? 2 : groups <= 4 ? 4 : 8;
+  p.kg = p.qg == 1 ? 4 : p.qg <= 4 ? 2 : 1;
+  p.row_wgs = (groups + p.qg - 1) / p.qg;
+  const int64_t steps = int64_t(n_seqs) * ((int64_t(max_tokens) + kTile - 1) / kTile / p.kg + 1);
+  p.workers = int(std::max<int64_t>(1, std::min<int64_t>(n_cu / p.row_wgs, steps)));
+  const size_t parts = size_t(p.workers) * size_t(p.row_wgs) * 2 * size_t(p.qg);
+  p.o_bytes = parts * size_t(latent) * 16 * 4;
+  p.ml_bytes = parts * 16 * 8;
+  return p;
+}
+
+bool takes(int32_t dtype, int latent, int rope, int block_size) {
+  if ((dtype != IT_F16 && dtype != IT_BF16) || block_size < 8) return false;
+  return (latent == 512 && rope == 64) || (latent == 256 && (rope == 64 || rope == 32)) || (latent == 128 && rope == 64);
+}
+
+}  // namespace
+
+namespace itkv {
+size_t latent_decode_matrix_ws(int32_t dtype, int latent, int rope, int block_size, int n_seqs, int q_len, int n_heads, int max_tokens,
+                               int n_cu) {
+  if (!takes(dtype, latent, rope, block_size)) return 0;
+  const HostPlan p = plan_of(latent, n_seqs, q_len, n_heads, max_tokens, n_cu);
+  return p.o_bytes + p.ml_bytes;
+}
+
+bool latent_decode_matrix(const LatentDecodeArgs& a, int32_t dtype, int block_size, int n_cu, hipStream_t s, hipError_t& e) {
+  if (!takes(dtype, a.latent, a.rope, block_size)) return false;
+  const HostPlan h = plan_of(a.latent, a.n_seqs, a.q_len, a.n_heads, a.max_tokens, n_cu);
+  const LatentSplitPlan p{h.workers, h.row_wgs, reinterpret_cast<float4*>(a.ws), reinterpret_cast<float2*>(reinterpret_cast<char*>(a.ws) + h.o_bytes)};
+  e = dtype == IT_BF16 ? latent_decode_bf16(a, p, h.qg, s) : latent_decode_f16(a, p, h.qg, s);
+  return true;
+}
+
+int latent_compute_units(int device) {
+  static std::atomic<int> known[64];
+  int n = device >= 0 && device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n <= 0) return 256;
+  if (device >= 0 && device < 64) known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+}  // namespace itkv
+
 extern "C" size_t it_latent_decode_workspace(const it_kv_cache* c, int32_t n_seqs, int32_t q_len, int32_t n_heads, int32_t max_tokens) {
   if (decode_sizes("it_latent_decode_workspace", c, n_seqs, q_len, n_heads, max_tokens)) return 0;
-  return latent_decode_matrix_ws(c->dtype, c->latent_dim, c->head_dim - c->latent_dim, c->block_size, n_seqs, q_len, n_heads, max_tokens);
+  return latent_decode_matrix_ws(c->dtype, c->latent_dim, c->head_dim - c->latent_dim, c->block_size, n_seqs, q_len, n_heads, max_tokens,
+                                 latent_compute_units(c->device));
 }
 
 extern "C" int32_t it_latent_decode(const it_kv_cache* c, const void* q_latent, const void* q_rope, int32_t q_dtype, int64_t ql_stride,
@@ -194,7 +251,7 @@ extern "C" int32_t it_latent_decode(const it_kv_cache* c, const void* q_latent, 
   if (dev != c->device) (void)hipSetDevice(c->device);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   hipError_t e = hipSuccess;
-  if (!latent_decode_matrix(a, c->dtype, c->block_size, s, e)) {
+  if (!latent_decode_matrix(a, c->dtype, c->block_size, latent_compute_units(c->device), s, e)) {
     const dim3 grid(unsigned(q_len * n_heads), unsigned(n_seqs));
     switch (c->dtype) {
       case IT_F32: hipLaunchKernelGGL(latent_decode_general<IT_F32>, grid, dim3(kThreads), 0, s, a); break;

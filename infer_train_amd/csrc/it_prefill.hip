@@ -45,6 +45,7 @@
 
 #include "it_device.hpp"
 #include "it_internal.hpp"
+#include "it_mfma.hpp"
 
 using namespace itkv;
 
@@ -69,7 +70,6 @@ constexpr int kMaxLds = 160 * 1024;                // per workgroup (one per CU)
 constexpr int kMaxGroup = 8;          // query heads per KV head
 
 typedef short v4s __attribute__((ext_vector_type(4)));
-typedef float v16f __attribute__((ext_vector_type(16)));
 
 // Division by a number the host knows: n / d = n inv >> 32 wherever n d < 2^32
 // (inv = 2^32 / d rounded up).
@@ -109,12 +109,6 @@ struct PrefillArgs {
 // Query tiles per workgroup for a GQA group: up to 8 waves of work.
 inline int prefill_q_tiles(int group) { return group >= kMaxGroup ? 1 : kMaxGroup / group; }
 
-__device__ __forceinline__ uint32_t lds_off(const void* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)p));
-}
-__device__ __forceinline__ void dma_b128(const void* g, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(m0), "v"(g) : "memory", "m0");
-}
 // The 16 chunks of row r are XOR-permuted by sw(r) = ((r & 3) << 2) | ((r >> 2) & 3),
 // a bijection of r mod 16: the A-operand reads (16 consecutive rows, one
 // chunk each) hit 16 distinct bank groups, and the transposing V reads (4
@@ -127,50 +121,6 @@ __device__ __forceinline__ int swz(int r, int c) { return r * kRowB + ((c ^ sw(r
 // 32 n + 16 t + 8 (e / 4) + 4 h + e % 4, which sits at position
 // 32 n + 16 t + 8 h + e: one 16-byte read per lane.
 __device__ __forceinline__ int vt_pos(int k) { return (k & ~12) | ((k & 4) << 1) | ((k & 8) >> 1); }
-
-template <bool kBf16>
-__device__ __forceinline__ v16f mfma(const uint4& a, const uint4& b, const v16f& c) {
-  if constexpr (kBf16) {
-    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-  } else {
-    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
-  }
-}
-// Two fp32 -> packed 16-bit pair (lo first), round to nearest even.
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (kBf16) {
-    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-    bf2 p;
-    p[0] = (__bf16)lo;  // v_cvt_pk_bf16_f32
-    p[1] = (__bf16)hi;
-    return __builtin_bit_cast(uint32_t, p);
-  } else {
-    return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16);
-  }
-}
-// acc + lo + hi of a packed bf16 / f16 pair (v_dot2c_f32_*).
-template <bool kBf16>
-__device__ __forceinline__ float dot2_ones(uint32_t w, float acc, uint32_t ones) {
-  if constexpr (kBf16) {
-    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, w), __builtin_bit_cast(bf2, ones), acc, false);
-  } else {
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), __builtin_bit_cast(h2, ones), acc, false);
-  }
-}
-// max / sum of x over this lane and lane ^ 32 (v_permlane32_swap, no LDS).
-__device__ __forceinline__ float max_halves(float x) {
-  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-}
-__device__ __forceinline__ float sum_halves(float x) {
-  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
-}
 
 // Units (sequence, KV head, query block) in longest-first order: by 64-key
 // blocks to read, most first; ties by sequence, query block, KV head.  The
