@@ -81,6 +81,6 @@ int latent_compute_units(int device);
 size_t latent_decode_matrix_ws(int32_t dtype, int latent, int rope, int block_size, int n_seqs, int q_len, int n_heads, int max_tokens,
                                int n_cu);
 bool latent_decode_matrix(const LatentDecodeArgs& a, int32_t dtype, int block_size, int n_cu, hipStream_t s, hipError_t& e);
-inline bool latent_prefill_matrix(const LatentPrefillArgs&, int32_t, hipStream_t, hipError_t&) { return false; }
+bool latent_prefill_matrix(const LatentPrefillArgs& a, int32_t dtype, hipStream_t s, hipError_t& e);
 
 }  // namespace itkv
