@@ -8,7 +8,7 @@
 // n_out best tokens.  The second joins a group's slices: the rows' logarithms,
 // then the best of all slices' candidates.
 //   The n-th best of a set is bounded from below by the n-th largest of the maxima
-// of 64 groups of it, which one wave finds bit by bit; what is not below it (about
+// of 64 groups of it, which a wave finds bit by bit; what is not below it (about
 // n, up to ties) is listed, and a listed entry's place is the number of listed ones
 // before it.  A list that ties overflow is replaced by n rounds of the next best.
 //   Sums are in fp64: the order of two beams' candidates hangs on the difference of
@@ -32,6 +32,7 @@ constexpr int kMaxVocab = 1 << 18;
 constexpr int kMaxBeams = 64;
 constexpr int kMaxOut = 64;                 // one wave's lanes bound the last place
 constexpr int kRoom = 1024;                 // listed entries
+constexpr uint32_t kDeadKey = 0x007FFFFFu;  // order_key(-inf)
 constexpr int kIndexBits = 18;
 static_assert(kMaxVocab <= 1 << kIndexBits, "a token's index in its key");
 constexpr int kKeyBits = 32 + kIndexBits;
@@ -60,7 +61,8 @@ __device__ __forceinline__ uint32_t order_key(float z) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k); }
-// A token's place in its row: larger is earlier, unique, never 0.
+// A token's place in its row: larger is earlier, unique, never 0 (a token that is NaN or
+// -inf has none).
 __device__ __forceinline__ uint64_t token_key(float z, int index) {
   return (uint64_t(order_key(z)) << kIndexBits) | uint32_t(kMaxVocab - 1 - index);
 }
@@ -94,64 +96,71 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t x) {
   x = max(x, dpp64<kDppRowRor8>(x));
   return max(max(lane64(x, 0), lane64(x, 16)), max(lane64(x, 32), lane64(x, 48)));
 }
-// The n-th largest of the wave's values (0 where fewer are above 0), to `bits` bits.
-__device__ __forceinline__ uint64_t wave_nth(uint64_t x, int n, int bits) {
-  uint64_t k = 0u;
-  for (int b = bits - 1; b >= 0; --b) {
-    const uint64_t with = k | uint64_t(1) << b;
+// The first kBoundBits bits of the n-th largest of the wave's values: a lower bound of it
+// (0 where fewer than n are above 0).  Fewer bits let a few more entries through.
+constexpr int kBoundBits = 20;
+__device__ __forceinline__ uint32_t wave_bound(uint32_t x, int n) {
+  uint32_t k = 0u;
+#pragma unroll
+  for (int b = 31; b >= 32 - kBoundBits; --b) {
+    const uint32_t with = k | 1u << b;
     if (__popcll(__ballot(x >= with)) >= n) k = with;
   }
   return k;
 }
+__device__ __forceinline__ uint32_t eight_max(uint32_t x) {
+  x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppQuadXor1, 0xF, 0xF, true)));
+  x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppQuadXor2, 0xF, 0xF, true)));
+  return max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppHalfMirror, 0xF, 0xF, true)));
+}
+// The sum over the wave, the same in all lanes.
+__device__ __forceinline__ double wave_sum(double x) {
+  const auto add = [](double v, auto dpp) { return v + __builtin_bit_cast(double, dpp(__builtin_bit_cast(uint64_t, v))); };
+  x = add(x, [](uint64_t v) { return dpp64<kDppQuadXor1>(v); });
+  x = add(x, [](uint64_t v) { return dpp64<kDppQuadXor2>(v); });
+  x = add(x, [](uint64_t v) { return dpp64<kDppHalfMirror>(v); });
+  x = add(x, [](uint64_t v) { return dpp64<kDppRowRor8>(v); });
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const auto at = [&](int lane) { return __builtin_bit_cast(double, lane64(u, lane)); };
+  return (at(0) + at(16)) + (at(32) + at(48));
+}
 
-// exp(d) for d <= 0: 2^n times the Taylor sum of exp on |x| <= ln(2) / 2, whose
-// next term, x^12 / 12!, is below 2^-47; n ln(2)'s own rounding is below 2^-45.
+// exp(d) for d <= 0 (an fp64 difference; NaN and -inf give next to nothing, 2^-512): 2^n (1 +
+// f h(f)), n the nearest integer to d / ln 2 and h the polynomial through (2^f - 1) / f at
+// the eight Chebyshev nodes of [-1/2, 1/2], off by less than 2^-38 of exp(d), and exactly 1 at
+// d = 0.  Whole numbers from the low word of a sum with 1.5 x 2^52, exponents as integers.
+constexpr double kExp2[8] = {0x1.62e42fef9cc69p-1,  0x1.ebfbdff82a734p-3,  0x1.c6b08da70cce3p-5,  0x1.3b2ab70ad2565p-7,
+                             0x1.5d877598350dep-10, 0x1.4308c7183d6a2p-13, 0x1.00c0e4e15189cp-16, 0x1.63b2d7971923fp-20};
 __device__ __forceinline__ double exp_below(double d) {
-  if (!(d > -700.0)) return d == d ? 0.0 : d;
-  const double n = __builtin_rint(d * 1.4426950408889634);
-  const double x = fma(n, -0.6931471805599453, d);
-  double p = 1.0 / 39916800.0;
-  p = fma(p, x, 1.0 / 3628800.0);
-  p = fma(p, x, 1.0 / 362880.0);
-  p = fma(p, x, 1.0 / 40320.0);
-  p = fma(p, x, 1.0 / 5040.0);
-  p = fma(p, x, 1.0 / 720.0);
-  p = fma(p, x, 1.0 / 120.0);
-  p = fma(p, x, 1.0 / 24.0);
-  p = fma(p, x, 1.0 / 6.0);
-  p = fma(p, x, 0.5);
-  p = fma(p, x, 1.0);
-  p = fma(p, x, 1.0);
-  return ldexp(p, int(n));
+  constexpr double kLog2e = 1.4426950408889634, kWhole = 0x1.8p52;
+  d = fmax(d, -354.0);  // of NaN too
+  const double n = fma(d, kLog2e, kWhole), f = fma(d, kLog2e, kWhole - n);
+  double h = kExp2[7];
+#pragma unroll
+  for (int i = 6; i >= 0; --i) h = fma(h, f, kExp2[i]);
+  const double m = fma(h, f, 1.0);
+  return __hiloint2double(int(uint32_t(__double2hiint(m)) + (uint32_t(__double2loint(n)) << 20)), __double2loint(m));
 }
 
 struct Listed {
   uint64_t key, tie;  // the larger key first, of equal keys the smaller tie
 };
 struct TopShared {
-  uint64_t group[64];
+  uint32_t group[64];  // what bounds the n-th best: the largest first words of 64 groups of entries
   Listed list[kRoom];
-  uint64_t round[kWaves];
-  uint64_t round_tie[kWaves];
+  uint64_t round[kWaves], round_tie[kWaves];
   uint32_t n;
 };
 __device__ __forceinline__ bool before(const Listed& a, const Listed& b) { return a.key > b.key || (a.key == b.key && a.tie < b.tie); }
 
-// The n first of the block's entries.  each(f): f(key, tie) for every entry of the
-// thread (key 0: none; no two alike), the same ones each time it is called.
-// put(place, entry): called by one thread for each place that an entry takes.
-template <class Each, class Put>
-__device__ __forceinline__ void top_of_block(TopShared& s, int n, int bits, Each&& each, Put&& put) {
+// The n first of the block's entries.  pass(add): calls add(key, tie) for the thread's entries
+// that are not below the bound; each(f): f(key, tie) for all of them (key 0: none; no two
+// alike), the same ones each time.  put(place, entry): called by one thread for each place
+// that an entry takes.  s.n is 0 at the start.
+template <class Pass, class Each, class Put>
+__device__ __forceinline__ void top_of_block(TopShared& s, int n, Pass&& pass, Each&& each, Put&& put) {
   const int tid = int(threadIdx.x), lane = tid & 63;
-  uint64_t most = 0u;
-  each([&](uint64_t key, uint64_t) { most = max(most, key); });
-  most = eight_max(most);
-  if ((lane & 7) == 0) s.group[tid >> 3] = most;
-  if (tid == 0) s.n = 0u;
-  __syncthreads();
-  const uint64_t least = max(wave_nth(s.group[lane], n, bits), uint64_t(1));  // every wave for itself
-  each([&](uint64_t key, uint64_t tie) {
-    if (key < least) return;
+  pass([&](uint64_t key, uint64_t tie) {
     const uint32_t at = atomicAdd(&s.n, 1u);
     if (at < kRoom) s.list[at] = {key, tie};
   });
@@ -161,6 +170,7 @@ __device__ __forceinline__ void top_of_block(TopShared& s, int n, int bits, Each
     for (uint32_t i = tid; i < listed; i += kThreads) {
       const Listed mine = s.list[i];
       int place = 0;
+#pragma unroll 4
       for (uint32_t j = 0; j < listed; ++j) place += before(s.list[j], mine);
       if (place < n) put(place, mine);
     }
@@ -191,115 +201,148 @@ __device__ __forceinline__ void top_of_block(TopShared& s, int n, int bits, Each
   }
 }
 
-// grid: (slice, row).
+// grid: (slice, row).  Bound by its fp64 work, about 16 operations a token.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void beam_slices(SelectArgs a) {
+__global__ __launch_bounds__(kThreads, 6) void beam_slices(SelectArgs a) {
   constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es, kVecs = kPer / V;
   using In = RowVec<DT, V>;
   __shared__ TopShared top;
-  __shared__ float tops[kWaves];
   __shared__ double sums[kWaves];
   const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6, slice = int(blockIdx.x);
   const int64_t row = blockIdx.y;
   const char* const data = a.logits + row * a.row_bytes;
   const int lo = slice * kSlice, hi = min(a.vocab, lo + kSlice);
-  // Thread t's tokens: vectors t, t + 512, .. of the slice.
+  // Thread t's tokens: vectors t, t + 512, .. of the slice, -inf past its end.
   float z[kPer];
   const bool aligned = ((reinterpret_cast<uintptr_t>(data) + size_t(lo) * es) & 15u) == 0;
+  if (aligned && hi - lo == kSlice) {  // uniform
+    typename In::raw w[kVecs];
 #pragma unroll
-  for (int j = 0; j < kVecs; ++j) {
-    const int i = lo + (j * kThreads + tid) * V;
-    float f[V];
+    for (int j = 0; j < kVecs; ++j) w[j] = __builtin_nontemporal_load(reinterpret_cast<const typename In::raw*>(data + int64_t(lo + (j * kThreads + tid) * V) * es));
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = -INFINITY;
-    if (aligned && i + V <= hi) {
-      In::widen(*reinterpret_cast<const typename In::raw*>(data + int64_t(i) * es), f);
-    } else {
+    for (int j = 0; j < kVecs; ++j) {
+      float f[V];
+      In::widen(w[j], f);
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (i + e < hi) f[e] = load_element(data, i + e, DT);
+      for (int e = 0; e < V; ++e) z[j * V + e] = f[e];
     }
+  } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) z[j * V + e] = f[e] == f[e] ? f[e] : -INFINITY;
+    for (int j = 0; j < kVecs; ++j) {
+      const int i = lo + (j * kThreads + tid) * V;
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[e] = -INFINITY;
+      if (aligned && i + V <= hi) {
+        In::widen(*reinterpret_cast<const typename In::raw*>(data + int64_t(i) * es), f);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (i + e < hi) f[e] = load_element(data, i + e, DT);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) z[j * V + e] = f[e];
+    }
   }
-  float m = z[0];
+  float m = -INFINITY;  // NaN does not enter
 #pragma unroll
-  for (int e = 1; e < kPer; ++e) m = fmaxf(m, z[e]);
-  m = group_max<64>(m);
-  if (lane == 0) tops[wave] = m;
+  for (int e = 0; e < kPer; ++e) m = fmaxf(m, z[e]);
+  const uint32_t group = eight_max(order_key(m));
+  if ((lane & 7) == 0) top.group[tid >> 3] = group;
+  if (tid == 0) top.n = 0u;
+  uint64_t* const best = a.best + (row * a.slices + slice) * a.n_out;
+  if (tid < a.n_out) best[tid] = 0u;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, tops[w]);
+  const uint32_t groups = top.group[lane];  // every wave for itself
+  m = key_value(uint32_t(wave_max(uint64_t(groups))));
   double sum = 0.0;
   if (m > -INFINITY) {  // uniform
 #pragma unroll
     for (int e = 0; e < kPer; ++e) sum += z[e] == m ? 1.0 : exp_below(double(z[e]) - double(m));
   }
-  for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+  sum = wave_sum(sum);
   if (lane == 0) sums[wave] = sum;
-  uint64_t* const best = a.best + (row * a.slices + slice) * a.n_out;
-  for (int i = tid; i < a.n_out; i += kThreads) best[i] = 0u;
-  __syncthreads();
-  if (tid == 0) {
+  const float least = fmaxf(key_value(max(wave_bound(groups, a.n_out), kDeadKey)), -3.402823466e38f);
+  const auto index = [&](int e) { return lo + (e / V * kThreads + tid) * V + e % V; };
+  top_of_block(
+      top, a.n_out,
+      [&](auto&& add) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          if (z[e] >= least) add(token_key(z[e], index(e)), uint64_t(0));
+      },
+      [&](auto&& f) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) f(z[e] > -INFINITY ? token_key(z[e], index(e)) : uint64_t(0), uint64_t(0));
+      },
+      [&](int place, const Listed& x) { best[place] = x.key; });
+  if (tid == 0) {  // past a barrier
     double total = 0.0;
     for (int w = 0; w < kWaves; ++w) total += sums[w];
     a.sums[row * a.slices + slice] = {m, 0.0f, total};
   }
-  if (m == -INFINITY) return;  // uniform
-  top_of_block(
-      top, a.n_out, kKeyBits,
-      [&](auto&& f) {
-#pragma unroll
-        for (int j = 0; j < kVecs; ++j)
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float x = z[j * V + e];
-            f(x > -INFINITY ? token_key(x, lo + (j * kThreads + tid) * V + e) : uint64_t(0), uint64_t(0));
-          }
-      },
-      [&](int place, const Listed& x) { best[place] = x.key; });
 }
 
-// grid: group.
+// grid: group.  Bound by latency.
 __global__ __launch_bounds__(kThreads) void beam_join(SelectArgs a) {
+  constexpr int kHeld = 4;  // entries that a thread keeps; more are read again
   __shared__ TopShared top;
   __shared__ double base[kMaxBeams];
   __shared__ float row_top[kMaxBeams];
-  const int tid = int(threadIdx.x);
+  const int tid = int(threadIdx.x), lane = tid & 63, wave = tid >> 6;
   const int64_t g = blockIdx.x, row0 = g * a.n_beams;
-  for (int b = tid; b < a.n_beams; b += kThreads) {
-    const SliceSum* const s = a.sums + (row0 + b) * a.slices;
-    float m = -INFINITY;
-    for (int i = 0; i < a.slices; ++i) m = fmaxf(m, s[i].top);
-    double sum = 0.0;
-    for (int i = 0; i < a.slices; ++i)
-      if (s[i].top > -INFINITY) sum += s[i].sum * (s[i].top == m ? 1.0 : exp_below(double(s[i].top) - double(m)));
-    const float score = a.scores[g * a.n_beams + b];
-    // A row at +inf: its tokens there share it equally, log 1/count.
-    base[b] = m > -INFINITY && score > -INFINITY ? double(score) - (m < INFINITY ? double(m) + log(sum) : log(sum)) : -INFINITY;
-    row_top[b] = m;
-  }
-  const int64_t out = g * a.n_out;
-  for (int i = tid; i < a.n_out; i += kThreads) {
-    a.out_scores[out + i] = -INFINITY;
-    a.parents[out + i] = a.tokens[out + i] = -1;
-  }
-  __syncthreads();
   const int per = a.slices * a.n_out, total = a.n_beams * per;
   const uint64_t* const best = a.best + row0 * per;
+  // The entries, on their way while the rows' logarithms are taken.
+  uint64_t held[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) held[j] = j * kThreads + tid < total ? best[j * kThreads + tid] : 0u;
+  static_assert(kMaxVocab / kSlice <= 64, "a row's slices in one wave");
+  for (int b = wave; b < a.n_beams; b += kWaves) {  // a wave per row, a lane per slice
+    SliceSum s = {-INFINITY, 0.0f, 0.0};
+    if (lane < a.slices) s = a.sums[(row0 + b) * a.slices + lane];
+    const float score = a.scores[g * a.n_beams + b];
+    const float m = group_max<64>(s.top);
+    const double sum = wave_sum(s.top > -INFINITY ? s.sum * (s.top == m ? 1.0 : exp_below(double(s.top) - double(m))) : 0.0);
+    if (lane == 0) {
+      // A row at +inf: its tokens there share it equally, log 1/count.
+      base[b] = m > -INFINITY && score > -INFINITY ? double(score) - (m < INFINITY ? double(m) + log(sum) : log(sum)) : -INFINITY;
+      row_top[b] = m;
+    }
+  }
+  const int64_t out = g * a.n_out;
+  if (tid < a.n_out) {
+    a.out_scores[out + tid] = -INFINITY;
+    a.parents[out + tid] = a.tokens[out + tid] = -1;
+  }
+  if (tid == 0) top.n = 0u;
+  __syncthreads();
+  const auto entry = [&](int i, uint64_t k, auto&& f) {
+    if (k == 0u) return;
+    const int b = i / per;
+    const float z = token_value(k);
+    if (!(base[b] > -INFINITY) || (row_top[b] == INFINITY && z < INFINITY)) return;
+    f(value_key(base[b] + (z == INFINITY ? 0.0 : double(z))), uint64_t(b) << kKeyBits | (kKeyMask - k));
+  };
+  const auto each = [&](auto&& f) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) entry(j * kThreads + tid, held[j], f);
+    for (int i = kHeld * kThreads + tid; i < total; i += kThreads) entry(i, best[i], f);
+  };
+  uint32_t most = 0u;
+  each([&](uint64_t key, uint64_t) { most = max(most, uint32_t(key >> 32)); });
+  most = eight_max(most);
+  if ((lane & 7) == 0) top.group[tid >> 3] = most;
+  __syncthreads();
+  const uint32_t least = wave_bound(top.group[lane], a.n_out);
   top_of_block(
-      top, a.n_out, 64,
-      [&](auto&& f) {
-        for (int i = tid; i < total; i += kThreads) {
-          const int b = i / per;
-          const uint64_t k = best[i];
-          if (k == 0u || !(base[b] > -INFINITY)) continue;
-          const float z = token_value(k);
-          if (row_top[b] == INFINITY && z < INFINITY) continue;
-          const double v = base[b] + (z == INFINITY ? 0.0 : double(z));
-          f(value_key(v), uint64_t(b) << kKeyBits | (kKeyMask - k));
-        }
+      top, a.n_out,
+      [&](auto&& add) {
+        each([&](uint64_t key, uint64_t tie) {
+          if (uint32_t(key >> 32) >= least) add(key, tie);
+        });
       },
+      each,
       [&](int place, const Listed& x) {
         a.out_scores[out + place] = float(key_double(x.key));
         a.parents[out + place] = int32_t(x.tie >> kKeyBits);

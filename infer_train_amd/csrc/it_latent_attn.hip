@@ -146,7 +146,7 @@ HostPlan plan_of(int latent, int n_seqs, int q_len, int n_heads, int max_tokens,
   HostPlan p;
   const int groups = (q_len * n_heads + 15) / 16;  // of 16 queries
   p.qg = groups <= 1 ? 1 : groups == 2 ? 2 : groups <= 4 ? 4 : 8;
-  p.kg = p.qg == 1 ? 4 : p.qg <= 4 ? 2 : 1;
+  p.kg = p.qg == 1 ? 4 : p.qg == 2 ? 2 : 1;
   p.row_wgs = (groups + p.qg - 1) / p.qg;
   const int64_t steps = int64_t(n_seqs) * ((int64_t(max_tokens) + kTile - 1) / kTile / p.kg + 1);
   p.workers = int(std::max<int64_t>(1, std::min<int64_t>(n_cu / p.row_wgs, steps)));

@@ -65,7 +65,7 @@ struct Shape {
   static constexpr int kFit = 144 * 1024 / (KG * Tile<L, R>::kBytes);
   static constexpr int kDepth = kFit < 1 ? 1 : kFit > 4 ? 4 : kFit;  // tiles of a token group
   static constexpr int kRing = KG * kDepth * Tile<L, R>::kBytes;
-  static constexpr int kJoin = (KG - 1) * QG * 16 * L * 4;  // O^T of all token groups but the first
+  static constexpr int kJoin = (KG - 1) * QG * 16 * L * 4;  // what token groups hand one another of O^T
   static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
   static_assert(kLds <= 144 * 1024, "one workgroup per CU, and room for what is noted beside");
   // The loads of a tile, shared by QG waves: whole units, or parts of one (the last
@@ -82,6 +82,11 @@ __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlan
 // A uniform element of a read-only array by a scalar load, which does not count among the vector loads.
 __device__ __forceinline__ int scalar_at(const int32_t* p, int i) {
   return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+// The same address in all lanes, so that it is kept in scalar registers.
+__device__ __forceinline__ const char* uni(const char* p) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const char*>(uint64_t(uint32_t(uni(int(x >> 32)))) << 32 | uint32_t(uni(int(x))));
 }
 template <bool kNt>
 __device__ __forceinline__ void load_lds(const char* base, uint32_t off, uint32_t m0) {
@@ -143,7 +148,7 @@ __device__ __forceinline__ float sum_quarters(float x) {
 
 // What of a sequence a run covers.
 struct Piece {
-  int b;            // sequence; n_seqs: none
+  int b;            // sequence
   int start, ctx;   // its visible tokens
   int begin;        // steps of all sequences before it
   int steps;        // of it
@@ -152,38 +157,50 @@ template <int KG>
 __device__ __forceinline__ int steps_of(const LatentSpan& s) {
   return s.ctx > s.start ? ((s.ctx + kTile - 1) / kTile - s.start / kTile + KG - 1) / KG : 0;
 }
-// The sequence in which step t of all lies, and the number of all steps.  Every
-// wave for itself: lane i holds sequence i of 64.
+// The sequences in chunks of 64, lane i of a wave sequence i of the chunk.  What the first
+// chunk's lanes found stays in LDS, for all waves and pieces; further ones are read again.
 template <int KG>
-__device__ __forceinline__ int total_steps(const LatentDecodeArgs& a, bool latch) {
-  int total = 0;
-  for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
-    const int b = b0 + int(threadIdx.x & 63);
-    total += b < a.n_seqs ? steps_of<KG>(latent_span(a, b, latch)) : 0;
+struct Spans {
+  struct Lane {
+    int start, ctx, mine, upto;  // steps of the sequence, and with those before it in the chunk
+  };
+  const LatentDecodeArgs& a;
+  Lane* kept;                 // [64] in LDS
+  int first, before, all;     // the chunk, the steps before it, its steps
+  __device__ __forceinline__ Lane read(int c, bool latch) const {
+    const int b = c + int(threadIdx.x & 63);
+    const LatentSpan s = b < a.n_seqs ? latent_span(a, b, latch) : LatentSpan{0, 0};
+    const int mine = steps_of<KG>(s);
+    return {s.start, s.ctx, mine, wave_inclusive_sum(mine)};
   }
-  return uni(__builtin_amdgcn_readlane(wave_inclusive_sum(total), 63));
-}
-template <int KG>
-__device__ __forceinline__ Piece piece_at(const LatentDecodeArgs& a, int t) {
-  int before = 0;
-  for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
-    const int b = b0 + int(threadIdx.x & 63);
-    LatentSpan s{0, 0};
-    if (b < a.n_seqs) s = latent_span(a, b, false);
-    const int mine = steps_of<KG>(s), incl = wave_inclusive_sum(mine);
-    const int all = __builtin_amdgcn_readlane(incl, 63);
-    if (t < before + all) {
-      const int i = __builtin_ctzll(__ballot(t < before + incl));
-      return {uni(b0 + i), __builtin_amdgcn_readlane(s.start, i), __builtin_amdgcn_readlane(s.ctx, i),
-              uni(before + __builtin_amdgcn_readlane(incl - mine, i)), __builtin_amdgcn_readlane(mine, i)};
+  static __device__ __forceinline__ int last(const Lane& x) { return __builtin_amdgcn_readlane(x.upto, 63); }
+  __device__ __forceinline__ Spans(const LatentDecodeArgs& args, Lane* lds) : a(args), kept(lds), first(0), before(0) {}
+  // The steps of all sequences; a barrier for the workgroup.
+  __device__ __forceinline__ int total(bool latch) {
+    const Lane x = read(0, latch);
+    if (threadIdx.x < 64) kept[threadIdx.x] = x;
+    int t = all = last(x);
+    for (int c = 64; c < a.n_seqs; c += 64) t = uni(t + last(read(c, latch)));
+    __syncthreads();
+    return t;
+  }
+  // The sequence in which step t of all lies, below the total; t does not decrease from call to call.
+  __device__ __forceinline__ Piece at(int t) {
+    Lane x = first ? read(first, false) : kept[threadIdx.x & 63];
+    while (t >= before + all) {
+      before = uni(before + all);
+      first += 64;
+      x = read(first, false);
+      all = last(x);
     }
-    before = uni(before + all);
+    const int i = __builtin_ctzll(__ballot(t < before + x.upto));
+    return {uni(first + i), __builtin_amdgcn_readlane(x.start, i), __builtin_amdgcn_readlane(x.ctx, i),
+            uni(before + __builtin_amdgcn_readlane(x.upto - x.mine, i)), __builtin_amdgcn_readlane(x.mine, i)};
   }
-  return {a.n_seqs, 0, 0, before, 0};
-}
+};
 
 template <bool kBf16, int L, int R, int QG, int KG, bool kNt>
-__global__ __launch_bounds__(64 * QG * KG, QG * KG / 4) void latent_decode_split(LatentDecodeArgs a, LatentSplitPlan plan) {
+__global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_decode_split(LatentDecodeArgs a, LatentSplitPlan plan) {
   using T = Tile<L, R>;
   using S = Shape<L, R, QG, KG>;
   constexpr int kDepth = S::kDepth, ND = L / 16, NQ = (L + R) / 32;
@@ -195,7 +212,9 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG / 4) void latent_decode_split
   // The workgroups that share a run's tiles on one XCD, next to one another.
   const int id = int(blockIdx.x), slot = id >> 3, worker = slot / plan.row_wgs * 8 + (id & 7), rw = slot % plan.row_wgs;
   if (worker >= plan.workers) return;
-  const int total = total_steps<KG>(a, id == 0 && wave == 0);
+  __shared__ typename Spans<KG>::Lane kept[64];
+  Spans<KG> spans(a, kept);
+  const int total = spans.total(id == 0 && wave == 0);
   const int per = max(1, (total + plan.workers - 1) / plan.workers);
   int t = uni(worker * per);
   const int t_end = uni(min(total, t + per));
@@ -224,7 +243,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG / 4) void latent_decode_split
   const int load0 = S::kParts > 1 ? min(qg % S::kParts * S::kPart, T::kUnitLoads - S::kPart) : 0;
 
   while (t < t_end) {
-    const Piece found = piece_at<KG>(a, t);
+    const Piece found = spans.at(t);
     const Piece pc = {uni(found.b), uni(found.start), uni(found.ctx), uni(found.begin), uni(found.steps)};
     const int s0 = uni(t - pc.begin), n_steps = uni(min(t_end - t, pc.steps - s0));
     t = uni(t + n_steps);
@@ -232,20 +251,33 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG / 4) void latent_decode_split
     const int tile0 = pc.start / kTile + s0 * KG + kg;  // this wave's first tile
     const int tiles = max(0, min(n_steps, ((pc.ctx + kTile - 1) / kTile - tile0 + KG - 1) / KG));
 
+    // The pages of tile i's eight-token runs that this wave loads, read a tile ahead by
+    // scalar loads that wait for one another no longer than for one.  Tokens outside
+    // [start, ctx) are read from the nearest page that is held, and masked.
+    constexpr int kRuns = S::kUnitsOwn * T::kUnit / 8;
+    const auto key_of = [&](int i, int run) __attribute__((always_inline)) {
+      const int key = (tile0 + i * KG) * kTile + unit0 * T::kUnit + 8 * run;
+      return uni(min(max(key, pc.start & ~7), (pc.ctx - 1) & ~7));
+    };
+    int ids[kRuns];
+    const auto read_ids = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) ids[r] = scalar_at(bt, key_of(i, r) >> a.log2_bs);
+    };
     // Tile i of this wave into ring slot i % kDepth: this wave's share of its loads.
-    // Tokens outside [start, ctx) are read from the nearest page that is held, and masked.
     const auto issue = [&](int i) __attribute__((always_inline)) {
-      const int key0 = (tile0 + i * KG) * kTile;
       const uint32_t m0 = ring + uint32_t((kDepth == 1 ? 0 : i % kDepth) * T::kBytes);
-      const auto page = [&](int key) __attribute__((always_inline)) {  // of eight tokens from `key`
-        const int k = uni(min(max(key, pc.start & ~7), (pc.ctx - 1) & ~7));
-        int blk = scalar_at(bt, k >> a.log2_bs);
-        if (blk < 0 || blk >= a.num_blocks) {  // uniform
-          if (lane == 0) atomicOr(a.err, kErrBlock);
-          blk = 0;
-        }
-        return a.pool + int64_t(uni(blk)) * a.page_bytes + (k & ((1 << a.log2_bs) - 1)) * T::kRow;
-      };
+      const char* pages[kRuns];
+      bool bad = false;
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) {
+        const int k = key_of(i, r), id = uni(ids[r]);
+        const bool off = id < 0 || id >= a.num_blocks;  // uniform
+        bad |= off;
+        pages[r] = uni(a.pool + int64_t(off ? 0 : id) * a.page_bytes + (k & ((1 << a.log2_bs) - 1)) * T::kRow);
+      }
+      if (bad && lane == 0) atomicOr(a.err, kErrBlock);
+      read_ids(i + 1);  // past the last tile: the last page again
       // This lane's chunks of a unit's rows, as the loads place them: where registers are short,
       // computed for each tile.
       int ln = lane;
@@ -261,13 +293,13 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG / 4) void latent_decode_split
         const int unit = unit0 + u;
         const uint32_t to = m0 + uint32_t((unit * T::kUnitLoads + load0) * 1024);
         if constexpr (T::kLines) {
-          const char* const base = page(key0 + 8 * unit);
+          const char* const base = pages[u];
           const uint32_t flip = (unit & 1) << 4;  // the rows' key has bit 0 of the unit's number
 #pragma unroll
           for (int j = 0; j < S::kPart; ++j) load_lds<kNt>(base, from[j] ^ flip, uni(to + uint32_t(j * 1024)));
         } else {  // sixteen rows are two runs of eight; the load in the middle has rows of both
-          const char* const first = page(key0 + 16 * unit);
-          const char* const second = page(key0 + 16 * unit + 8) - 8 * T::kRow;
+          const char* const first = pages[2 * u];
+          const char* const second = pages[2 * u + 1] - 8 * T::kRow;
 #pragma unroll
           for (int j = 0; j < S::kPart; ++j) {
             const int at = load0 + j;  // uniform
@@ -277,6 +309,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG / 4) void latent_decode_split
         }
       }
     };
+    read_ids(0);
     if constexpr (kDepth > 1)
       for (int i = 0; i < kDepth - 1 && i < tiles; ++i) issue(i);
 
@@ -461,7 +494,9 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG / 4) void latent_decode_split
       }
     }
 
-    // The token groups joined: the first adds the others' sums to its own.
+    // The token groups joined, each for a part of the values.
+    constexpr int kOwn = ND / KG;
+    v4f own[kOwn];
     if constexpr (KG > 1) {
       if (quarter == 0) ml_of[wave][col] = make_float2(m_run, l);
       __syncthreads();  // all tiles are read too
@@ -475,40 +510,56 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG / 4) void latent_decode_split
         l = fmaf(__builtin_amdgcn_exp2f(x.x - use), x.y, l);
       }
       const float mine = __builtin_amdgcn_exp2f(m_run - use);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] *= mine;
+      // Token group kg keeps d-tiles kg ND / KG ..: it writes the others' and reads theirs.
       v4f* const join = reinterpret_cast<v4f*>(lds);
-      if (kg > 0) {
+      const auto place = [&](int from, int to, int d) { return (((from * (KG - 1) + to - (to > from)) * QG + qg) * kOwn + d) * 64 + lane; };
+      if constexpr (KG == 2) {
 #pragma unroll
-        for (int d = 0; d < ND; ++d) join[((wave - QG) * ND + d) * 64 + lane] = o[d];
+        for (int d = 0; d < kOwn; ++d) {
+          const v4f x = o[d] * mine, y = o[kOwn + d] * mine;
+          join[place(kg, 1 - kg, d)] = kg ? x : y;
+          own[d] = kg ? y : x;
+        }
+      } else {
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          if (g == kg) continue;  // uniform
+#pragma unroll
+          for (int d = 0; d < kOwn; ++d) join[place(kg, g, d)] = o[g * kOwn + d] * mine;
+        }
+#pragma unroll
+        for (int g = 0; g < KG; ++g)
+          if (g == kg) {
+#pragma unroll
+            for (int d = 0; d < kOwn; ++d) own[d] = o[g * kOwn + d] * mine;
+          }
       }
       __syncthreads();
-      if (kg == 0) {
 #pragma unroll
-        for (int g = 1; g < KG; ++g)
+      for (int g = 1; g < KG; ++g)
 #pragma unroll
-          for (int d = 0; d < ND; ++d) o[d] += join[((wave + (g - 1) * QG) * ND + d) * 64 + lane];
-      }
+        for (int d = 0; d < kOwn; ++d) own[d] += join[place((kg + g) % KG, kg, d)];
+    } else {
+#pragma unroll
+      for (int d = 0; d < kOwn; ++d) own[d] = o[d];
     }
-    if (kg == 0) {
-      if (n_steps == pc.steps) {  // the whole sequence: done
-        if (live) {
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-          const int64_t out = ((int64_t(pc.b) * a.q_len + tok) * a.n_heads + head) * L + 4 * quarter;
+    if (n_steps == pc.steps) {  // the whole sequence: done
+      if (live) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t out = ((int64_t(pc.b) * a.q_len + tok) * a.n_heads + head) * L + 16 * kOwn * kg + 4 * quarter;
 #pragma unroll
-          for (int d = 0; d < ND; ++d) {
-            const v4f x = o[d] * inv;
-            if (a.out_dtype == IT_F32) *reinterpret_cast<v4f*>(static_cast<float*>(a.out) + out + 16 * d) = x;
-            else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out + 16 * d) = make_uint2(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]));
-          }
+        for (int d = 0; d < kOwn; ++d) {
+          const v4f x = own[d] * inv;
+          if (a.out_dtype == IT_F32) *reinterpret_cast<v4f*>(static_cast<float*>(a.out) + out + 16 * d) = x;
+          else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out + 16 * d) = make_uint2(pack2<kBf16>(x[0], x[1]), pack2<kBf16>(x[2], x[3]));
         }
-      } else {  // slot 1: the piece that begins its sequence; 0: one that continues it
-        const int64_t part = ((int64_t(worker) * plan.row_wgs + rw) * 2 + (s0 == 0)) * QG + qg;
-        v4f* const to = reinterpret_cast<v4f*>(plan.o) + part * (ND * 64) + lane;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) to[d * 64] = o[d];
-        if (quarter == 0) plan.ml[part * 16 + col] = make_float2(M, l);
       }
+    } else {  // slot 1: the piece that begins its sequence; 0: one that continues it
+      const int64_t part = ((int64_t(worker) * plan.row_wgs + rw) * 2 + (s0 == 0)) * QG + qg;
+      v4f* const to = reinterpret_cast<v4f*>(plan.o) + part * (ND * 64) + kOwn * kg * 64 + lane;
+#pragma unroll
+      for (int d = 0; d < kOwn; ++d) to[d * 64] = own[d];
+      if (kg == 0 && quarter == 0) plan.ml[part * 16 + col] = make_float2(M, l);
     }
     __syncthreads();  // before the next piece's loads into the ring, and ml_of
   }
@@ -541,17 +592,33 @@ __global__ __launch_bounds__(256) void latent_decode_join(LatentDecodeArgs a, La
   if (steps > 0) {
     const auto part = [&](int w) { return ((int64_t(w) * plan.row_wgs + rw) * 2 + (w == w0)) * QG + qg; };
     float M = -INFINITY, l = 0.0f;
-#pragma unroll 4
-    for (int w = w0; w <= w1; ++w) M = fmaxf(M, plan.ml[part(w) * 16 + col].x);
-    const float use = M == -INFINITY ? 0.0f : M;
-#pragma unroll 4
-    for (int w = w0; w <= w1; ++w) {
-      const float2 ml = plan.ml[part(w) * 16 + col];
-      const v4f x = reinterpret_cast<const v4f*>(plan.o)[(part(w) * nd + dt) * 64 + lane];
-      const float f = __builtin_amdgcn_exp2f(ml.x - use);
-      l = fmaf(f, ml.y, l);
+    // Pieces eight at a time, their maxima, sums and values loaded together.
+    constexpr int kAtOnce = 8;
+#pragma unroll 1
+    for (int w = w0; w <= w1; w += kAtOnce) {
+      float2 ml[kAtOnce];
+      v4f x[kAtOnce];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, x[e], sum[e]);
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int64_t from = part(min(w + i, w1));
+        ml[i] = plan.ml[from * 16 + col];
+        x[i] = reinterpret_cast<const v4f*>(plan.o)[(from * nd + dt) * 64 + lane];
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, ml[i].x);
+      const float use = top == -INFINITY ? 0.0f : top, old = __builtin_amdgcn_exp2f(M - use);
+      l *= old;
+      sum *= old;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const float f = __builtin_amdgcn_exp2f(ml[i].x - use);
+        if (w + i > w1) continue;  // uniform
+        l = fmaf(f, ml[i].y, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = fmaf(f, x[i][e], sum[e]);
+      }
+      M = top;
     }
     inv = l == 0.0f ? 0.0f : 1.0f / l;
   }
@@ -580,7 +647,7 @@ hipError_t launch(const LatentDecodeArgs& a, const LatentSplitPlan& p, int qg, h
   switch (qg) {
     case 1: return launch_split<kBf16, L, R, 1, 4, true>(a, p, s);
     case 2: return launch_split<kBf16, L, R, 2, 2, true>(a, p, s);
-    case 4: return launch_split<kBf16, L, R, 4, 2, true>(a, p, s);
+    case 4: return launch_split<kBf16, L, R, 4, 1, true>(a, p, s);
     default:  // where several workgroups read a tile, the later ones find it in their XCD's L2
       return p.row_wgs == 1 ? launch_split<kBf16, L, R, 8, 1, true>(a, p, s) : launch_split<kBf16, L, R, 8, 1, false>(a, p, s);
   }
