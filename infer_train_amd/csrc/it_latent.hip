@@ -78,13 +78,12 @@ __global__ __launch_bounds__(kThreads) void latent_append_rows(LatentAppendArgs 
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = int(threadIdx.x & 63);
   const int task = int(blockIdx.x) * kWaves + wave, t = task / a.parts, part = task - t * a.parts;
   if (t >= a.n_tokens) return;  // uniform
-  int pos;
-  int64_t slot;
-  if (!token_of(a, t, part == 0 && lane == 0, pos, slot)) return;  // uniform
   const RowSplit& s = a.split;
   float2* const own = angles + wave * angle_room<V>(a.rope);
   const int sub = int((uint32_t(lane) * s.inv) >> 16), c = lane - sub * s.lanes;
   LanePairs<V> lp(s, c);
+  int pos;
+  int64_t slot;
   if (part > 0) {  // the rope part of kHeadSteps * s.rows heads
     typename In::raw xa[kHeadSteps], xb[kHeadSteps];
     const int h0 = (part - 1) * (s.rows * kHeadSteps) + sub;
@@ -95,6 +94,7 @@ __global__ __launch_bounds__(kThreads) void latent_append_rows(LatentAppendArgs 
       xa[j] = *reinterpret_cast<const typename In::raw*>(src + lp.ea * es);
       xb[j] = *reinterpret_cast<const typename In::raw*>(src + lp.eb * es);
     }
+    if (!token_of(a, t, false, pos, slot)) return;  // uniform; the elements are on their way
     if (a.turns) {
       wave_angles(own, a.turns, a.rope >> 1, pos, a.magnitude, false, lane);
       lp.load(s, own);
@@ -124,6 +124,7 @@ __global__ __launch_bounds__(kThreads) void latent_append_rows(LatentAppendArgs 
     ra = *reinterpret_cast<const typename In::raw*>(src + (a.latent + lp.ea) * es);
     rb = *reinterpret_cast<const typename In::raw*>(src + (a.latent + lp.eb) * es);
   }
+  if (!token_of(a, t, lane == 0, pos, slot)) return;  // uniform
   float weight[V], norm = 1.0f;
   if (a.weight) {
     load_weight(a, min(lane, vecs - 1) * V, weight);  // the first vector's, in the shadow of the sum

@@ -69,6 +69,7 @@ struct LatentSplitPlan {
   int row_wgs;   // workgroups that share a run, each with QG * 16 queries of its own
   float4* o;     // partial O^T: [worker][row wg][2][QG][L / 16][64 lanes]
   float2* ml;    // and its (maximum, sum): [worker][row wg][2][QG][16]
+  int2* shares;  // of each sequence that holds something: its first worker and how many share it
 };
 
 hipError_t latent_decode_bf16(const LatentDecodeArgs& a, const LatentSplitPlan& p, int qg, hipStream_t s);

@@ -140,7 +140,7 @@ constexpr int kTile = 32;  // of the matrix-core kernels: cached tokens
 // Query groups and token groups of a workgroup by the call's queries.
 struct HostPlan {
   int qg, kg, workers, row_wgs;
-  size_t o_bytes, ml_bytes;
+  size_t o_bytes, ml_bytes, share_bytes;
 };
 HostPlan plan_of(int latent, int n_seqs, int q_len, int n_heads, int max_tokens, int n_cu) {
   HostPlan p;
@@ -153,6 +153,7 @@ HostPlan plan_of(int latent, int n_seqs, int q_len, int n_heads, int max_tokens,
   const size_t parts = size_t(p.workers) * size_t(p.row_wgs) * 2 * size_t(p.qg);
   p.o_bytes = parts * size_t(latent) * 16 * 4;
   p.ml_bytes = parts * 16 * 8;
+  p.share_bytes = size_t(n_seqs) * 8;
   return p;
 }
 
@@ -168,13 +169,15 @@ size_t latent_decode_matrix_ws(int32_t dtype, int latent, int rope, int block_si
                                int n_cu) {
   if (!takes(dtype, latent, rope, block_size)) return 0;
   const HostPlan p = plan_of(latent, n_seqs, q_len, n_heads, max_tokens, n_cu);
-  return p.o_bytes + p.ml_bytes;
+  return p.o_bytes + p.ml_bytes + p.share_bytes;
 }
 
 bool latent_decode_matrix(const LatentDecodeArgs& a, int32_t dtype, int block_size, int n_cu, hipStream_t s, hipError_t& e) {
   if (!takes(dtype, a.latent, a.rope, block_size)) return false;
   const HostPlan h = plan_of(a.latent, a.n_seqs, a.q_len, a.n_heads, a.max_tokens, n_cu);
-  const LatentSplitPlan p{h.workers, h.row_wgs, reinterpret_cast<float4*>(a.ws), reinterpret_cast<float2*>(reinterpret_cast<char*>(a.ws) + h.o_bytes)};
+  char* const ws = reinterpret_cast<char*>(a.ws);
+  const LatentSplitPlan p{h.workers, h.row_wgs, reinterpret_cast<float4*>(ws), reinterpret_cast<float2*>(ws + h.o_bytes),
+                          reinterpret_cast<int2*>(ws + h.o_bytes + h.ml_bytes)};
   e = dtype == IT_BF16 ? latent_decode_bf16(a, p, h.qg, s) : latent_decode_f16(a, p, h.qg, s);
   return true;
 }

@@ -146,56 +146,89 @@ __device__ __forceinline__ float sum_quarters(float x) {
   return sum_halves(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
-// What of a sequence a run covers.
+// What of a sequence a workgroup takes at a time.
 struct Piece {
   int b;            // sequence
   int start, ctx;   // its visible tokens
-  int begin;        // steps of all sequences before it
-  int steps;        // of it
+  int steps;        // of KG tiles, of it
+  int s0, n;        // the piece: steps s0 .. s0 + n
+  int shared;       // workers from this one on that share the sequence
 };
+// x / d and x / d rounded up, 0 <= x < 2^21: the quotient of x + 1/2 is further from a whole
+// number than its rounding reaches.
+__device__ __forceinline__ int quotient(int x, int d) { return int((float(x) + 0.5f) * __builtin_amdgcn_rcpf(float(d))); }
+__device__ __forceinline__ int over(int x, int d) { return quotient(x + d - 1, d); }
+
+// How the steps of all sequences are divided among the workers; every wave finds it for
+// itself from the lengths, sequences in chunks of 64, one a lane.
+//   Runs: each worker takes `per` steps of all, which may begin and end inside sequences.
+// Most workers then have two pieces, and a piece costs about as much as four steps beside
+// its own: pages, queries and the first tile are waited for one after another, then sums are
+// joined and stored.
+//   Whole numbers of workers: sequences are divided, one piece a worker, where the longest
+// piece is not four steps longer than a run.
 template <int KG>
-__device__ __forceinline__ int steps_of(const LatentSpan& s) {
-  return s.ctx > s.start ? ((s.ctx + kTile - 1) / kTile - s.start / kTile + KG - 1) / KG : 0;
-}
-// The sequences in chunks of 64, lane i of a wave sequence i of the chunk.  What the first
-// chunk's lanes found stays in LDS, for all waves and pieces; further ones are read again.
-template <int KG>
-struct Spans {
-  struct Lane {
-    int start, ctx, mine, upto;  // steps of the sequence, and with those before it in the chunk
+struct Division {
+  static constexpr int kPieceCost = 4;
+  struct Span {
+    int start, ctx, steps;
   };
   const LatentDecodeArgs& a;
-  Lane* kept;                 // [64] in LDS
-  int first, before, all;     // the chunk, the steps before it, its steps
-  __device__ __forceinline__ Lane read(int c, bool latch) const {
+  int per, total;
+  bool whole;
+  Span lanes;                 // of the chunk
+  int chunk = 0, before = 0;  // and the steps before it
+
+  __device__ __forceinline__ Span read(int c, bool latch) const {
     const int b = c + int(threadIdx.x & 63);
     const LatentSpan s = b < a.n_seqs ? latent_span(a, b, latch) : LatentSpan{0, 0};
-    const int mine = steps_of<KG>(s);
-    return {s.start, s.ctx, mine, wave_inclusive_sum(mine)};
+    return {s.start, s.ctx, s.ctx > s.start ? ((s.ctx + kTile - 1) / kTile - s.start / kTile + KG - 1) / KG : 0};
   }
-  static __device__ __forceinline__ int last(const Lane& x) { return __builtin_amdgcn_readlane(x.upto, 63); }
-  __device__ __forceinline__ Spans(const LatentDecodeArgs& args, Lane* lds) : a(args), kept(lds), first(0), before(0) {}
-  // The steps of all sequences; a barrier for the workgroup.
-  __device__ __forceinline__ int total(bool latch) {
-    const Lane x = read(0, latch);
-    if (threadIdx.x < 64) kept[threadIdx.x] = x;
-    int t = all = last(x);
-    for (int c = 64; c < a.n_seqs; c += 64) t = uni(t + last(read(c, latch)));
-    __syncthreads();
-    return t;
+  static __device__ __forceinline__ int sum(int x) { return uni(__builtin_amdgcn_readlane(wave_inclusive_sum(x), 63)); }
+
+  __device__ __forceinline__ Division(const LatentDecodeArgs& args, int workers, bool latch) : a(args) {
+    lanes = read(0, latch);
+    int mine = lanes.steps;
+    for (int c = 64; c < a.n_seqs; c += 64) mine += read(c, latch).steps;
+    total = sum(mine);
+    per = max(1, (total + workers - 1) / workers);
+    whole = false;
+    if (a.n_seqs > 64 || total >= 1 << 20) return;
+    const int busy = __popcll(__ballot(lanes.steps > 0));
+    if (busy == 0 || busy >= workers) return;
+    int length = per;  // of a piece at most; sum over(steps, length) <= total / length + busy
+    if (sum(over(lanes.steps, length)) > workers) length = max(length, over(total, workers - busy));
+    if (length - per > kPieceCost) return;
+    per = length;
+    whole = true;
   }
-  // The sequence in which step t of all lies, below the total; t does not decrease from call to call.
-  __device__ __forceinline__ Piece at(int t) {
-    Lane x = first ? read(first, false) : kept[threadIdx.x & 63];
-    while (t >= before + all) {
-      before = uni(before + all);
-      first += 64;
-      x = read(first, false);
-      all = last(x);
+  // The piece that worker w takes of a division into whole numbers; n 0: none.
+  __device__ __forceinline__ Piece of(int w) const {
+    const int mine = over(lanes.steps, per), upto = wave_inclusive_sum(mine);
+    const uint64_t past = __ballot(w < upto);
+    if (past == 0) return {};
+    const int i = __builtin_ctzll(past), steps = __builtin_amdgcn_readlane(lanes.steps, i), n = __builtin_amdgcn_readlane(mine, i);
+    const int first = __builtin_amdgcn_readlane(upto, i) - n, j = w - first;
+    const int each = uni(quotient(steps, n)), more = steps - each * n;
+    return {uni(i), __builtin_amdgcn_readlane(lanes.start, i), __builtin_amdgcn_readlane(lanes.ctx, i), steps,
+            uni(j * each + min(j, more)), uni(each + (j < more)), uni(n)};
+  }
+  // The piece that begins at step t of all, in worker w's run, which ends at `end`; t does not
+  // decrease from call to call.
+  __device__ __forceinline__ Piece at(int t, int end, int w) {
+    for (;;) {  // ends: t is below the total
+      const int upto = before + wave_inclusive_sum(lanes.steps), all = __builtin_amdgcn_readlane(upto, 63);
+      if (t >= all) {
+        before = uni(all);
+        chunk += 64;
+        lanes = read(chunk, false);
+        continue;
+      }
+      const int i = __builtin_ctzll(__ballot(t < upto)), steps = __builtin_amdgcn_readlane(lanes.steps, i);
+      const int last = __builtin_amdgcn_readlane(upto, i), s0 = t - (last - steps);
+      return {uni(chunk + i), __builtin_amdgcn_readlane(lanes.start, i), __builtin_amdgcn_readlane(lanes.ctx, i), steps,
+              uni(s0), uni(min(end - t, steps - s0)), uni((last - 1) / per - w + 1)};
     }
-    const int i = __builtin_ctzll(__ballot(t < before + x.upto));
-    return {uni(first + i), __builtin_amdgcn_readlane(x.start, i), __builtin_amdgcn_readlane(x.ctx, i),
-            uni(before + __builtin_amdgcn_readlane(x.upto - x.mine, i)), __builtin_amdgcn_readlane(x.mine, i)};
   }
 };
 
@@ -212,13 +245,10 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
   // The workgroups that share a run's tiles on one XCD, next to one another.
   const int id = int(blockIdx.x), slot = id >> 3, worker = slot / plan.row_wgs * 8 + (id & 7), rw = slot % plan.row_wgs;
   if (worker >= plan.workers) return;
-  __shared__ typename Spans<KG>::Lane kept[64];
-  Spans<KG> spans(a, kept);
-  const int total = spans.total(id == 0 && wave == 0);
-  const int per = max(1, (total + plan.workers - 1) / plan.workers);
-  int t = uni(worker * per);
-  const int t_end = uni(min(total, t + per));
-  if (t >= t_end) return;
+  Division<KG> division(a, plan.workers, id == 0 && wave == 0);
+  int t = uni(worker * division.per);
+  const int t_end = division.whole ? t + 1 : uni(min(division.total, t + division.per));
+  if (!division.whole && t >= t_end) return;
 
   // This lane's query.
   const int rows = a.q_len * a.n_heads, row = (rw * QG + qg) * 16 + col;
@@ -243,10 +273,12 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
   const int load0 = S::kParts > 1 ? min(qg % S::kParts * S::kPart, T::kUnitLoads - S::kPart) : 0;
 
   while (t < t_end) {
-    const Piece found = spans.at(t);
-    const Piece pc = {uni(found.b), uni(found.start), uni(found.ctx), uni(found.begin), uni(found.steps)};
-    const int s0 = uni(t - pc.begin), n_steps = uni(min(t_end - t, pc.steps - s0));
-    t = uni(t + n_steps);
+    const Piece found = division.whole ? division.of(worker) : division.at(t, t_end, worker);
+    const Piece pc = {uni(found.b), uni(found.start), uni(found.ctx), uni(found.steps), uni(found.s0), uni(found.n), uni(found.shared)};
+    const int s0 = pc.s0, n_steps = pc.n;
+    if (n_steps == 0) return;
+    t = division.whole ? t_end : uni(t + n_steps);
+    if (s0 == 0 && rw == 0 && threadIdx.x == 0) plan.shares[pc.b] = make_int2(worker, pc.shared);
     const int32_t* const bt = a.bt + int64_t(pc.b) * a.max_blocks;
     const int tile0 = pc.start / kTile + s0 * KG + kg;  // this wave's first tile
     const int tiles = max(0, min(n_steps, ((pc.ctx + kTile - 1) / kTile - tile0 + KG - 1) / KG));
@@ -259,13 +291,16 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
       const int key = (tile0 + i * KG) * kTile + unit0 * T::kUnit + 8 * run;
       return uni(min(max(key, pc.start & ~7), (pc.ctx - 1) & ~7));
     };
-    int ids[kRuns];
-    const auto read_ids = [&](int i) __attribute__((always_inline)) {
+    constexpr int kFirst = kDepth > 1 ? kDepth - 1 : 1;  // tiles whose pages are read together at first
+    int ids[kRuns], first_ids[kFirst][kRuns];
+    const auto read_ids = [&](int i, int (&to)[kRuns]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int r = 0; r < kRuns; ++r) ids[r] = scalar_at(bt, key_of(i, r) >> a.log2_bs);
+      for (int r = 0; r < kRuns; ++r) to[r] = scalar_at(bt, key_of(i, r) >> a.log2_bs);
     };
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) read_ids(i, first_ids[i]);
     // Tile i of this wave into ring slot i % kDepth: this wave's share of its loads.
-    const auto issue = [&](int i) __attribute__((always_inline)) {
+    const auto issue = [&](int i, const int (&ids)[kRuns]) __attribute__((always_inline)) {
       const uint32_t m0 = ring + uint32_t((kDepth == 1 ? 0 : i % kDepth) * T::kBytes);
       const char* pages[kRuns];
       bool bad = false;
@@ -277,11 +312,10 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
         pages[r] = uni(a.pool + int64_t(off ? 0 : id) * a.page_bytes + (k & ((1 << a.log2_bs) - 1)) * T::kRow);
       }
       if (bad && lane == 0) atomicOr(a.err, kErrBlock);
-      read_ids(i + 1);  // past the last tile: the last page again
       // This lane's chunks of a unit's rows, as the loads place them: where registers are short,
       // computed for each tile.
       int ln = lane;
-      if constexpr (S::kWaves > 4) asm volatile("" : "+v"(ln));
+      if constexpr (L > 256 && S::kWaves > 4) asm volatile("" : "+v"(ln));
       uint32_t from[S::kPart];
 #pragma unroll
       for (int j = 0; j < S::kPart; ++j) {
@@ -309,9 +343,18 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
         }
       }
     };
-    read_ids(0);
-    if constexpr (kDepth > 1)
-      for (int i = 0; i < kDepth - 1 && i < tiles; ++i) issue(i);
+    if constexpr (kDepth > 1) {
+#pragma unroll 1
+      for (int i = 0; i < kDepth - 1 && i < tiles; ++i) {
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r) ids[r] = i == 0 ? first_ids[0][r] : i == 1 ? first_ids[kFirst > 1 ? 1 : 0][r] : first_ids[kFirst > 2 ? 2 : 0][r];
+        issue(i, ids);
+      }
+      read_ids(kDepth - 1, ids);  // past the last tile: the last page again
+    } else {
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) ids[r] = first_ids[0][r];
+    }
 
     uint4 q[NQ];
     {
@@ -349,7 +392,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
       }
       // The operands of kAhead steps are on their way while one is multiplied; the
       // scheduler, left to itself, loads so far ahead that it runs out of registers.
-      constexpr int kAhead = S::kWaves > 4 ? 1 : 2;
+      constexpr int kAhead = L > 256 && S::kWaves > 4 ? 1 : 4;
       v4f s[2] = {v4f{}, v4f{}};
       uint4 key_rows[kAhead + 1][2];
       const auto load_rows = [&](int k) __attribute__((always_inline)) {
@@ -448,7 +491,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
         }
       }
       {
-        constexpr int kNext = S::kWaves > 4 ? 3 : 4;  // d-tiles ahead
+        constexpr int kNext = L > 256 && S::kWaves > 4 ? 3 : ND < 8 ? ND : 8;  // d-tiles ahead
         uint2 v[kNext + 1][2];
 #pragma unroll
         for (int d = 0; d < kNext; ++d) v[d][0] = values(d, 0), v[d][1] = values(d, 1);
@@ -465,7 +508,8 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
     if constexpr (kDepth == 1) {
       for (int i = 0; i < tiles; ++i) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile before is read
-        issue(i);
+        issue(i, ids);
+        read_ids(i + 1, ids);
         wait_loads<0>();
         compute(i);
       }
@@ -479,7 +523,8 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
         else wait_loads<0>();
         if constexpr (QG == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (i + kDepth - 1 < tiles) issue(i + kDepth - 1);  // where tile i - 1 was
+        if (i + kDepth - 1 < tiles) issue(i + kDepth - 1, ids);  // where tile i - 1 was
+        read_ids(i + kDepth, ids);
         if (i < tiles) compute(i);
         else if (QG > 1 && a.q_len > 1 && step_end(i) > pc.ctx - a.q_len + 1) asm volatile("s_barrier" ::: "memory");  // compute()'s
       }
@@ -558,7 +603,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
       const int64_t part = ((int64_t(worker) * plan.row_wgs + rw) * 2 + (s0 == 0)) * QG + qg;
       v4f* const to = reinterpret_cast<v4f*>(plan.o) + part * (ND * 64) + kOwn * kg * 64 + lane;
 #pragma unroll
-      for (int d = 0; d < kOwn; ++d) to[d * 64] = own[d];
+      for (int d = 0; d < kOwn; ++d) __builtin_nontemporal_store(own[d], to + d * 64);  // on its way at once, not at the kernel's end
       if (kg == 0 && quarter == 0) plan.ml[part * 16 + col] = make_float2(M, l);
     }
     __syncthreads();  // before the next piece's loads into the ring, and ml_of
@@ -572,24 +617,16 @@ __global__ __launch_bounds__(256) void latent_decode_join(LatentDecodeArgs a, La
   const int lane = int(threadIdx.x & 63), quarter = lane >> 4, col = lane & 15;
   const int nd = int(gridDim.x) * 4, dt = int(blockIdx.x) * 4 + int(threadIdx.x >> 6), group = int(blockIdx.y), b = int(blockIdx.z);
   const int rw = group / QG, qg = group - rw * QG;
-  // Steps before this sequence, and of all.
-  int before = 0, total = 0;
-  for (int b0 = 0; b0 < a.n_seqs; b0 += 64) {
-    const int x = b0 + lane;
-    const int n = x < a.n_seqs ? steps_of<KG>(latent_span(a, x, false)) : 0;
-    total += n;
-    before += x < b ? n : 0;
-  }
-  total = uni(__builtin_amdgcn_readlane(wave_inclusive_sum(total), 63));
-  before = uni(__builtin_amdgcn_readlane(wave_inclusive_sum(before), 63));
-  const int steps = steps_of<KG>(latent_span(a, b, false));
-  const int per = max(1, (total + plan.workers - 1) / plan.workers);
-  const int w0 = before / per, w1 = (before + steps - 1) / per;
-  if (steps > 0 && w0 == w1) return;  // one workgroup wrote it
+  // A sequence that holds something has been given its first worker; what others hold is of an earlier call.
+  const LatentSpan span = latent_span(a, b, false);
+  const int2 share = plan.shares[b];
+  const bool some = uni(span.ctx) > uni(span.start);
+  const int w0 = uni(share.x), w1 = w0 + uni(share.y) - 1;
+  if (some && w0 == w1) return;  // one workgroup wrote it
   const int rows = a.q_len * a.n_heads, row = group * 16 + col;
   v4f sum = v4f{};
   float inv = 0.0f;
-  if (steps > 0) {
+  if (some) {
     const auto part = [&](int w) { return ((int64_t(w) * plan.row_wgs + rw) * 2 + (w == w0)) * QG + qg; };
     float M = -INFINITY, l = 0.0f;
     // Pieces eight at a time, their maxima, sums and values loaded together.
