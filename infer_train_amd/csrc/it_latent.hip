@@ -6,9 +6,9 @@
 //
 // Bound by memory, and by latency for single tokens: each row is read and
 // written once, whole 16-byte vectors per lane.  A wave takes one token's row
-// (its sum of squares is a sum over the wave's lanes, no LDS), or the rope part
-// of a run of its heads; both compute the token's angles for themselves, a pair
-// per lane, as the rotation of K and V rows does.
+// (its sum of squares is a sum over the wave's lanes, no LDS), the rope part of a run
+// of its heads, or both; it computes the token's angles for itself, a pair per lane, as
+// the rotation of K and V rows does.
 #include <hip/hip_runtime.h>
 
 #include "it_latent.hpp"
@@ -19,7 +19,6 @@ using namespace itkv;
 namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kMaxVecs = 4;  // a lane's vectors of a latent: 1024 elements of four bytes
 constexpr int kHeadSteps = 2;  // rows of heads that a lane takes
 
 struct LatentAppendArgs {
@@ -37,6 +36,7 @@ struct LatentAppendArgs {
   float eps, magnitude;
   int n_tokens, n_heads, latent, rope, layout, cache_dtype, weight_dtype, out_dtype;
   int parts;  // waves of a token: its row's, then its heads'
+  int apart;  // 1: the row has a wave of its own
   RowSplit split;
 };
 
@@ -54,10 +54,8 @@ __device__ __forceinline__ void load_weight(const LatentAppendArgs& a, int e, fl
     RowVec<IT_F16, V>::widen(*reinterpret_cast<const typename RowVec<IT_F16, V>::raw*>(static_cast<const uint16_t*>(a.weight) + e), w);
 }
 
-// A token's slot and whether it is written at all; false: a bad position.
-__device__ __forceinline__ bool token_of(const LatentAppendArgs& a, int t, bool latch, int& pos, int64_t& slot) {
-  pos = a.turns ? a.positions[t] : 0;
-  slot = a.slots[t];
+// Whether a token is written at all (false: a bad position), and its slot, -1 where it is not one.
+__device__ __forceinline__ bool token_ok(const LatentAppendArgs& a, bool latch, int pos, int64_t& slot) {
   if (pos < 0) {
     if (latch) atomicOr(a.err, kErrPos);
     return false;
@@ -69,24 +67,52 @@ __device__ __forceinline__ bool token_of(const LatentAppendArgs& a, int t, bool 
   return true;
 }
 
-// Vectors of V elements of SRC (16 bytes), aligned.
-template <int SRC>
+// V elements to `dtype`, which is SRC where kSame: chosen when the kernel was, and converted
+// without a branch (its own NaN for fp16's).
+template <int SRC, bool kSame, int V>
+__device__ __forceinline__ void put_vec(void* base, int64_t element, int dtype, const float (&x)[V]) {
+  if constexpr (kSame && SRC == IT_F16) {
+    typedef uint32_t words __attribute__((ext_vector_type(V / 2)));
+    words w;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) w[i] = f32_to_f16_bits(x[2 * i]) | f32_to_f16_bits(x[2 * i + 1]) << 16;
+    *reinterpret_cast<words*>(static_cast<uint16_t*>(base) + element) = w;
+  } else {
+    store_row_vec<V>(base, element, kSame ? SRC : dtype, x);
+  }
+}
+
+// Vectors of V elements of SRC (16 bytes), aligned.  kSame: the cache's and q_out's type is SRC.
+template <int SRC, bool kSame>
 __global__ __launch_bounds__(kThreads) void latent_append_rows(LatentAppendArgs a) {
   constexpr int es = SRC == IT_F32 ? 4 : 2, V = 16 / es;
+  constexpr int kMaxVecs = 1024 / (64 * V);  // a lane's vectors of a latent
+  constexpr int kMaxTurns = 2;               // and pairs of a rope part: 256 elements
   using In = RowVec<SRC, V>;
   extern __shared__ __attribute__((aligned(16))) float2 angles[];
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = int(threadIdx.x & 63);
   const int task = int(blockIdx.x) * kWaves + wave, t = task / a.parts, part = task - t * a.parts;
   if (t >= a.n_tokens) return;  // uniform
+  // The token's row is its first wave's; the heads begin with that or with the next.
+  const bool with_row = part == 0;
+  const int head_part = part - a.apart;
   const RowSplit& s = a.split;
   float2* const own = angles + wave * angle_room<V>(a.rope);
   const int sub = int((uint32_t(lane) * s.inv) >> 16), c = lane - sub * s.lanes;
+  const int h0 = head_part * (s.rows * kHeadSteps) + sub;
   LanePairs<V> lp(s, c);
-  int pos;
-  int64_t slot;
-  if (part > 0) {  // the rope part of kHeadSteps * s.rows heads
-    typename In::raw xa[kHeadSteps], xb[kHeadSteps];
-    const int h0 = (part - 1) * (s.rows * kHeadSteps) + sub;
+  // All loads before the first of what follows from the token's position.
+  const int pos = a.turns ? a.positions[t] : 0;
+  int64_t slot = a.slots[t];
+  double turns[kMaxTurns];
+  if (a.turns) {
+#pragma unroll
+    for (int j = 0; j < kMaxTurns; ++j)
+      if (j * 128 < a.rope) turns[j] = a.turns[min(j * 64 + lane, (a.rope >> 1) - 1)];
+  }
+  typename In::raw xa[kHeadSteps], xb[kHeadSteps];
+  const bool heads = head_part >= 0 && a.n_heads > 0;  // uniform
+  if (heads) {
 #pragma unroll
     for (int j = 0; j < kHeadSteps; ++j) {  // past the last head a lane reads it again; only the stores are predicated
       const int h = min(h0 + j * s.rows, a.n_heads - 1);
@@ -94,11 +120,34 @@ __global__ __launch_bounds__(kThreads) void latent_append_rows(LatentAppendArgs 
       xa[j] = *reinterpret_cast<const typename In::raw*>(src + lp.ea * es);
       xb[j] = *reinterpret_cast<const typename In::raw*>(src + lp.eb * es);
     }
-    if (!token_of(a, t, false, pos, slot)) return;  // uniform; the elements are on their way
-    if (a.turns) {
-      wave_angles(own, a.turns, a.rope >> 1, pos, a.magnitude, false, lane);
-      lp.load(s, own);
+  }
+  const char* const src = a.kv + t * a.kv_stride * es;
+  const int vecs = a.latent / V;
+  const bool turner = lane < s.lanes;
+  typename In::raw x[kMaxVecs], ra, rb;
+  float weight[V];
+  if (with_row) {
+#pragma unroll
+    for (int j = 0; j < kMaxVecs; ++j)
+      if (j * 64 < vecs) x[j] = *reinterpret_cast<const typename In::raw*>(src + min(j * 64 + lane, vecs - 1) * 16);
+    if (turner) {
+      ra = *reinterpret_cast<const typename In::raw*>(src + (a.latent + lp.ea) * es);
+      rb = *reinterpret_cast<const typename In::raw*>(src + (a.latent + lp.eb) * es);
     }
+    if (a.weight) load_weight(a, min(lane, vecs - 1) * V, weight);  // the first vector's
+  }
+  if (!token_ok(a, with_row && lane == 0, pos, slot)) return;  // uniform
+  if (a.turns) {
+#pragma unroll
+    for (int j = 0; j < kMaxTurns; ++j) {
+      if (j * 128 >= a.rope) continue;  // uniform
+      const float2 cs = rotary_angle(turns[j], pos);
+      if (j * 128 + 2 * lane < a.rope) own[j * 64 + lane] = make_float2(cs.x * a.magnitude, cs.y * a.magnitude);
+    }
+    wave_lds_fence();
+    lp.load(s, own);
+  }
+  if (heads) {
 #pragma unroll
     for (int j = 0; j < kHeadSteps; ++j) {
       const int h = h0 + j * s.rows;
@@ -108,26 +157,13 @@ __global__ __launch_bounds__(kThreads) void latent_append_rows(LatentAppendArgs 
       In::widen(xb[j], fb);
       if (a.turns) lp.turn(s, fa, fb);
       const int64_t at = t * a.out_stride + h * a.out_head;
-      store_row_vec<V>(a.q_out, at + lp.ea, a.out_dtype, fa);
-      store_row_vec<V>(a.q_out, at + lp.eb, a.out_dtype, fb);
+      put_vec<SRC, kSame, V>(a.q_out, at + lp.ea, a.out_dtype, fa);
+      put_vec<SRC, kSame, V>(a.q_out, at + lp.eb, a.out_dtype, fb);
     }
-    return;
   }
-  const char* const src = a.kv + t * a.kv_stride * es;
-  const int vecs = a.latent / V;
-  typename In::raw x[kMaxVecs], ra, rb;
-#pragma unroll
-  for (int j = 0; j < kMaxVecs; ++j)
-    if (j * 64 < vecs) x[j] = *reinterpret_cast<const typename In::raw*>(src + min(j * 64 + lane, vecs - 1) * 16);
-  const bool turner = lane < s.lanes;
-  if (turner) {
-    ra = *reinterpret_cast<const typename In::raw*>(src + (a.latent + lp.ea) * es);
-    rb = *reinterpret_cast<const typename In::raw*>(src + (a.latent + lp.eb) * es);
-  }
-  if (!token_of(a, t, lane == 0, pos, slot)) return;  // uniform
-  float weight[V], norm = 1.0f;
+  if (!with_row) return;  // uniform
+  float norm = 1.0f;
   if (a.weight) {
-    load_weight(a, min(lane, vecs - 1) * V, weight);  // the first vector's, in the shadow of the sum
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < kMaxVecs; ++j) {
@@ -139,15 +175,11 @@ __global__ __launch_bounds__(kThreads) void latent_append_rows(LatentAppendArgs 
     }
     norm = 1.0f / sqrtf(group_sum<64>(sum) / float(a.latent) + a.eps);
   }
-  if (a.turns) {
-    wave_angles(own, a.turns, a.rope >> 1, pos, a.magnitude, false, lane);
-    lp.load(s, own);
-  }
   const int64_t row = int64_t(a.latent + a.rope);
   char* const to = slot >= 0 ? row_of(a, slot) : nullptr;
   const auto put = [&](int e, const float(&f)[V]) {
-    if (to) store_row_vec<V>(to, e, a.cache_dtype, f);
-    if (a.rows_out) store_row_vec<V>(a.rows_out, t * row + e, a.cache_dtype, f);
+    if (to) put_vec<SRC, kSame, V>(to, e, a.cache_dtype, f);
+    if (a.rows_out) put_vec<SRC, kSame, V>(a.rows_out, t * row + e, a.cache_dtype, f);
   };
 #pragma unroll
   for (int j = 0; j < kMaxVecs; ++j) {
@@ -180,9 +212,9 @@ __global__ __launch_bounds__(kThreads) void latent_append_general(LatentAppendAr
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = int(threadIdx.x & 63);
   const int task = int(blockIdx.x) * kWaves + wave, t = task / a.parts, part = task - t * a.parts;
   if (t >= a.n_tokens) return;
-  int pos;
-  int64_t slot;
-  if (!token_of(a, t, part == 0 && lane == 0, pos, slot)) return;
+  const int pos = a.turns ? a.positions[t] : 0;
+  int64_t slot = a.slots[t];
+  if (!token_ok(a, part == 0 && lane == 0, pos, slot)) return;
   const int half = a.rope >> 1, es_out = a.out_dtype == IT_F32 ? 4 : 2;
   const bool halves = a.layout == IT_ROTARY_HALF;
   const int64_t row = int64_t(a.latent + a.rope);
@@ -332,7 +364,11 @@ extern "C" int32_t it_latent_append(it_kv_cache* c, const it_rotary* rotary, con
     a.split.rows = 16;  // heads of a wave in the general kernel
     a.parts = 1 + (n_heads + 15) / 16;
   } else {
-    a.parts = 1 + (n_heads + a.split.rows * kHeadSteps - 1) / (a.split.rows * kHeadSteps);
+    // A wave of its own for the row while all waves are resident at once, which is what one
+    // token waits for; beyond, the row and the first heads share a wave, and its angles.
+    const int head_waves = (n_heads + a.split.rows * kHeadSteps - 1) / (a.split.rows * kHeadSteps);
+    a.apart = head_waves > 0 && int64_t(n_tokens) * (1 + head_waves) <= 256 * 32;
+    a.parts = a.apart + (head_waves > 1 ? head_waves : 1);
   }
   if (int64_t(n_tokens) * a.parts > int64_t(1) << 30) return fail(IT_INVALID_INPUT, "%s: %d tokens of %d heads", who, n_tokens, n_heads);
   int dev = -1;
@@ -341,19 +377,12 @@ extern "C" int32_t it_latent_append(it_kv_cache* c, const it_rotary* rotary, con
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 grid(unsigned((n_tokens * a.parts + kWaves - 1) / kWaves));
   const size_t lds = size_t(kWaves) * (v == 4 ? angle_room<4>(rope) : angle_room<8>(rope)) * sizeof(float2);
+  const bool same = c->dtype == src_dtype && (!n_heads || q_out_dtype == src_dtype);
+  const auto launch = [&](auto* kern) { hipLaunchKernelGGL(kern, grid, dim3(kThreads), fast ? lds : 0, s, a); };
   switch (src_dtype) {
-    case IT_F32:
-      if (fast) hipLaunchKernelGGL(latent_append_rows<IT_F32>, grid, dim3(kThreads), lds, s, a);
-      else hipLaunchKernelGGL(latent_append_general<IT_F32>, grid, dim3(kThreads), 0, s, a);
-      break;
-    case IT_BF16:
-      if (fast) hipLaunchKernelGGL(latent_append_rows<IT_BF16>, grid, dim3(kThreads), lds, s, a);
-      else hipLaunchKernelGGL(latent_append_general<IT_BF16>, grid, dim3(kThreads), 0, s, a);
-      break;
-    default:
-      if (fast) hipLaunchKernelGGL(latent_append_rows<IT_F16>, grid, dim3(kThreads), lds, s, a);
-      else hipLaunchKernelGGL(latent_append_general<IT_F16>, grid, dim3(kThreads), 0, s, a);
-      break;
+    case IT_F32: launch(!fast ? latent_append_general<IT_F32> : same ? latent_append_rows<IT_F32, true> : latent_append_rows<IT_F32, false>); break;
+    case IT_BF16: launch(!fast ? latent_append_general<IT_BF16> : same ? latent_append_rows<IT_BF16, true> : latent_append_rows<IT_BF16, false>); break;
+    default: launch(!fast ? latent_append_general<IT_F16> : same ? latent_append_rows<IT_F16, true> : latent_append_rows<IT_F16, false>); break;
   }
   const hipError_t e = hipGetLastError();
   if (dev >= 0 && dev != c->device) (void)hipSetDevice(dev);
