@@ -113,6 +113,12 @@ __device__ __forceinline__ uint32_t eight_max(uint32_t x) {
   x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppQuadXor2, 0xF, 0xF, true)));
   return max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppHalfMirror, 0xF, 0xF, true)));
 }
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = eight_max(x);
+  x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), kDppRowRor8, 0xF, 0xF, true)));
+  const auto at = [&](int lane) { return uint32_t(__builtin_amdgcn_readlane(int(x), lane)); };
+  return max(max(at(0), at(16)), max(at(32), at(48)));
+}
 // The sum over the wave, the same in all lanes.
 __device__ __forceinline__ double wave_sum(double x) {
   const auto add = [](double v, auto dpp) { return v + __builtin_bit_cast(double, dpp(__builtin_bit_cast(uint64_t, v))); };
@@ -131,16 +137,27 @@ __device__ __forceinline__ double wave_sum(double x) {
 // d = 0.  Whole numbers from the low word of a sum with 1.5 x 2^52, exponents as integers.
 constexpr double kExp2[8] = {0x1.62e42fef9cc69p-1,  0x1.ebfbdff82a734p-3,  0x1.c6b08da70cce3p-5,  0x1.3b2ab70ad2565p-7,
                              0x1.5d877598350dep-10, 0x1.4308c7183d6a2p-13, 0x1.00c0e4e15189cp-16, 0x1.63b2d7971923fp-20};
-__device__ __forceinline__ double exp_below(double d) {
-  constexpr double kLog2e = 1.4426950408889634, kWhole = 0x1.8p52;
-  d = fmax(d, -354.0);  // of NaN too
-  const double n = fma(d, kLog2e, kWhole), f = fma(d, kLog2e, kWhole - n);
-  double h = kExp2[7];
+// The coefficients stay in scalar registers: as literals each would be moved to a vector
+// register again for every token, a third of the work.
+struct ExpBelow {
+  double c[8], log2e = 1.4426950408889634, least = -354.0, whole = 0x1.8p52;
+  __device__ __forceinline__ ExpBelow() {
 #pragma unroll
-  for (int i = 6; i >= 0; --i) h = fma(h, f, kExp2[i]);
-  const double m = fma(h, f, 1.0);
-  return __hiloint2double(int(uint32_t(__double2hiint(m)) + (uint32_t(__double2loint(n)) << 20)), __double2loint(m));
-}
+    for (int i = 0; i < 8; ++i) c[i] = kExp2[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) asm("" : "+s"(c[i]));
+    asm("" : "+s"(log2e), "+s"(least), "+v"(whole));
+  }
+  __device__ __forceinline__ double operator()(double d) const {
+    d = fmax(d, least);  // of NaN too
+    const double n = fma(d, log2e, whole), f = fma(d, log2e, whole - n);
+    double h = c[7];
+#pragma unroll
+    for (int i = 6; i >= 0; --i) h = fma(h, f, c[i]);
+    const double m = fma(h, f, 1.0);
+    return __hiloint2double(int(uint32_t(__double2hiint(m)) + (uint32_t(__double2loint(n)) << 20)), __double2loint(m));
+  }
+};
 
 struct Listed {
   uint64_t key, tie;  // the larger key first, of equal keys the smaller tie
@@ -201,9 +218,10 @@ __device__ __forceinline__ void top_of_block(TopShared& s, int n, Pass&& pass, E
   }
 }
 
-// grid: (slice, row).  Bound by its fp64 work, about 16 operations a token.
+// grid: (slice, row).  Bound by the vector units: about 29 operations a token, 16 of them in
+// fp64 (32 groups x 8 beams x 100003 bf16 31 us, of which the logits' 51 MB take 8).
 template <int DT>
-__global__ __launch_bounds__(kThreads, 6) void beam_slices(SelectArgs a) {
+__global__ __launch_bounds__(kThreads, 8) void beam_slices(SelectArgs a) {
   constexpr int es = DT == IT_F32 ? 4 : 2, V = 16 / es, kVecs = kPer / V;
   using In = RowVec<DT, V>;
   __shared__ TopShared top;
@@ -214,11 +232,13 @@ __global__ __launch_bounds__(kThreads, 6) void beam_slices(SelectArgs a) {
   const int lo = slice * kSlice, hi = min(a.vocab, lo + kSlice);
   // Thread t's tokens: vectors t, t + 512, .. of the slice, -inf past its end.
   float z[kPer];
-  const bool aligned = ((reinterpret_cast<uintptr_t>(data) + size_t(lo) * es) & 15u) == 0;
-  if (aligned && hi - lo == kSlice) {  // uniform
+  // Rows of an odd vocabulary start anywhere: loads of 16 bytes at an element's alignment.
+  typedef typename In::raw Any __attribute__((aligned(es)));
+  const Any* const vecs = reinterpret_cast<const Any*>(data + int64_t(lo) * es) + tid;
+  if (hi - lo == kSlice) {  // uniform
     typename In::raw w[kVecs];
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) w[j] = __builtin_nontemporal_load(reinterpret_cast<const typename In::raw*>(data + int64_t(lo + (j * kThreads + tid) * V) * es));
+    for (int j = 0; j < kVecs; ++j) w[j] = __builtin_nontemporal_load(vecs + j * kThreads);
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
       float f[V];
@@ -233,8 +253,8 @@ __global__ __launch_bounds__(kThreads, 6) void beam_slices(SelectArgs a) {
       float f[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) f[e] = -INFINITY;
-      if (aligned && i + V <= hi) {
-        In::widen(*reinterpret_cast<const typename In::raw*>(data + int64_t(i) * es), f);
+      if (i + V <= hi) {
+        In::widen(vecs[j * kThreads], f);
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -254,11 +274,16 @@ __global__ __launch_bounds__(kThreads, 6) void beam_slices(SelectArgs a) {
   if (tid < a.n_out) best[tid] = 0u;
   __syncthreads();
   const uint32_t groups = top.group[lane];  // every wave for itself
-  m = key_value(uint32_t(wave_max(uint64_t(groups))));
+  m = key_value(wave_max(groups));
   double sum = 0.0;
-  if (m > -INFINITY) {  // uniform
+  if (m == INFINITY) {  // uniform, as is the other: the tokens there share the row
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) sum += z[e] == m ? 1.0 : exp_below(double(z[e]) - double(m));
+    for (int e = 0; e < kPer; ++e) sum += z[e] == m ? 1.0 : 0.0;
+  } else if (m > -INFINITY) {
+    const ExpBelow exp_below;
+    const double top_value = double(m);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) sum += exp_below(double(z[e]) - top_value);
   }
   sum = wave_sum(sum);
   if (lane == 0) sums[wave] = sum;
@@ -298,6 +323,7 @@ __global__ __launch_bounds__(kThreads) void beam_join(SelectArgs a) {
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) held[j] = j * kThreads + tid < total ? best[j * kThreads + tid] : 0u;
   static_assert(kMaxVocab / kSlice <= 64, "a row's slices in one wave");
+  const ExpBelow exp_below;
   for (int b = wave; b < a.n_beams; b += kWaves) {  // a wave per row, a lane per slice
     SliceSum s = {-INFINITY, 0.0f, 0.0};
     if (lane < a.slices) s = a.sums[(row0 + b) * a.slices + lane];
