@@ -78,6 +78,12 @@ struct Shape {
   static_assert(kDepth > 1 || QG == 1, "one slot is one wave's own");
 };
 
+// The same value, of which nothing is known: what follows from it is computed where it is used,
+// not kept in registers from loop turn to loop turn.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 // A uniform element of a read-only array by a scalar load, which does not count among the vector loads.
 __device__ __forceinline__ int scalar_at(const int32_t* p, int i) {
@@ -314,8 +320,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
       if (bad && lane == 0) atomicOr(a.err, kErrBlock);
       // This lane's chunks of a unit's rows, as the loads place them: where registers are short,
       // computed for each tile.
-      int ln = lane;
-      if constexpr (L > 256 && S::kWaves > 4) asm volatile("" : "+v"(ln));
+      const int ln = L > 256 && S::kWaves > 4 ? fresh(lane) : lane;
       uint32_t from[S::kPart];
 #pragma unroll
       for (int j = 0; j < S::kPart; ++j) {
@@ -365,6 +370,16 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
       for (int i = 0; i < L / 32; ++i) q[i] = ld16_any(ql + 32 * i);
 #pragma unroll
       for (int i = 0; i < R / 32; ++i) q[L / 32 + i] = ld16_any(qr + 32 * i);
+      // Waited for here: at their first use, inside the loop, every turn would wait again, for
+      // the tiles in flight too.
+      if constexpr (S::kWaves > 4) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+          u32x4 x = __builtin_bit_cast(u32x4, q[i]);
+          asm volatile("" : "+v"(x));
+          q[i] = __builtin_bit_cast(uint4, x);
+        }
+      }
     }
     v4f o[ND];
 #pragma unroll
@@ -416,10 +431,10 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
       for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * a.scale_log2;
       const bool edge = key0 < pc.start || key0 + kTile > pc.ctx - a.q_len + 1;  // uniform
       if (edge) {
-        const int lo = pc.start - key0, hi = pc.ctx - a.q_len + 1 + tok - key0;
+        const int lo = pc.start - key0, hi = pc.ctx - a.q_len + 1 + tok - key0, first = fresh(lane) >> 4 << 2;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int r = 16 * (e >> 2) + 4 * quarter + (e & 3);
+          const int r = 16 * (e >> 2) + first + (e & 3);
           x[e] = r >= lo && r < hi ? x[e] : -INFINITY;
         }
       }
@@ -458,7 +473,7 @@ __global__ __launch_bounds__(64 * QG * KG, QG * KG > 4 ? 2 : 1) void latent_deco
       const bool drafted = a.q_len > 1 && step_end(i) > pc.ctx - a.q_len + 1;  // the same in all waves
       const int lo = max(pc.start - key0, 0), hi = min(pc.ctx - key0, kTile), late = max(lo, pc.ctx - a.q_len + 1 - key0);
       const auto chunk = [&](int r) __attribute__((always_inline)) {  // a row's values, 16 bytes a lane
-        return reinterpret_cast<__attribute__((address_space(3))) u32x4*>(uintptr_t(ring + at + uint32_t(r * T::kRow + lane * 16)));
+        return reinterpret_cast<__attribute__((address_space(3))) u32x4*>(uintptr_t(ring + at + uint32_t(r * T::kRow + fresh(lane) * 16)));
       };
       if (drafted) {
         const int seen = pc.ctx - a.q_len + 1 + tok - key0;
