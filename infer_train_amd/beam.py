@@ -49,12 +49,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: Optional[int]
     device = logits.device
     if ws is None:
         ws = beam_select_workspace(groups, beams, vocab, n, device)
-    best = torch.empty((groups, n), dtype=torch.float32, device=device)
-    chosen = torch.empty((2, groups, n), dtype=torch.int32, device=device)
-    parents, tokens = chosen[0], chosen[1]
+    best = torch.empty((3, groups, n), dtype=torch.int32, device=device)
+    at, part = best.data_ptr(), 4 * groups * n
     _launch(index, call.it_beam_select, logits.data_ptr(), torch_dtype_id(logits.dtype), logits.stride(0), groups, beams, vocab,
-            at_scores, n, best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _on(ws, index), ws.nbytes, _raw_stream(index))
-    return best, parents, tokens
+            at_scores, n, at, at + part, at + 2 * part, _on(ws, index), ws.nbytes, _raw_stream(index))
+    best_scores, parents, tokens = best.unbind()
+    return best_scores.view(torch.float32), parents, tokens
 
 
 def beam_reorder(x: torch.Tensor, parents: torch.Tensor, dim: int = 0) -> torch.Tensor:
