@@ -719,7 +719,8 @@ int32_t it_latent_append(it_kv_cache* cache, const it_rotary* rotary, const void
  *     aligned, for the partial results of sequences that several workgroups
  *     share; calls that overlap in time need one each
  *   out: [n_seqs * q_len][n_heads][latent_dim] of out_dtype: F32 or q_dtype,
- *     16-byte aligned
+ *     16-byte aligned, apart from the inputs
+ *   n_seqs * max_tokens (or what max_blocks hold) at most about 2^35
  * Sums and the softmax in fp32; for F16 and BF16 caches the probabilities are
  * rounded to the cache's type for the matrix cores.  How the keys are divided
  * follows from all sequences of the call, so a row's result may differ between
@@ -747,7 +748,8 @@ int32_t it_latent_decode(const it_kv_cache* cache, const void* q_latent, const v
  *   nope_dim, rope_dim, v_dim: multiples of 8, nope_dim + rope_dim <= 1024,
  *     v_dim <= 1024; fastest: F16 and BF16 with nope_dim and v_dim 64 or 128,
  *     rope_dim 32 or 64, and 16-byte aligned rows
- *   out: [total_q][n_heads][v_dim] contiguous, of out_dtype F32 or dtype
+ *   out: [total_q][n_heads][v_dim] contiguous, of out_dtype F32 or dtype,
+ *     16-byte aligned, apart from the inputs
  * Launched on the current device, to which `stream` must belong. */
 int32_t it_latent_prefill(const void* q, const void* k, const void* v, const void* k_rope, int32_t dtype,
                           int64_t q_stride, int64_t q_head_stride, int64_t k_stride, int64_t k_head_stride,

@@ -137,7 +137,13 @@ int32_t decode_sizes(const char* who, const it_kv_cache* c, int32_t n_seqs, int3
 
 namespace {
 constexpr int kTile = 32;  // of the matrix-core kernels: cached tokens
-// Query groups and token groups of a workgroup by the call's queries.
+// Query groups and token groups of a workgroup by the call's queries.  Token groups join in
+// LDS at each piece's end, which few queries pay for by more waves (64 heads: four query
+// groups 52 us, with two token groups 65).  Past 64 queries eight groups share a tile where
+// pieces are long; short ones are mostly the partial results' way out and in, which is half
+// as long where two workgroups of four groups halve the workers (128 heads in bf16, two
+// workgroups against one: 64 x 1000 tokens 56 us against 64, 16 x 2048 36 against 51, 16 x
+// 12288 equal, 16 of 8192 to 16384 123 against 112).
 struct HostPlan {
   int qg, kg, workers, row_wgs;
   size_t o_bytes, ml_bytes, share_bytes;
@@ -145,7 +151,8 @@ struct HostPlan {
 HostPlan plan_of(int latent, int n_seqs, int q_len, int n_heads, int max_tokens, int n_cu) {
   HostPlan p;
   const int groups = (q_len * n_heads + 15) / 16;  // of 16 queries
-  p.qg = groups <= 1 ? 1 : groups == 2 ? 2 : groups <= 4 ? 4 : 8;
+  const int64_t tiles = int64_t(n_seqs) * ((int64_t(max_tokens) + kTile - 1) / kTile);
+  p.qg = groups <= 1 ? 1 : groups == 2 ? 2 : groups <= 4 || tiles < 16 * std::max<int64_t>(1, n_cu / ((groups + 7) / 8)) ? 4 : 8;
   p.kg = p.qg == 1 ? 4 : p.qg == 2 ? 2 : 1;
   p.row_wgs = (groups + p.qg - 1) / p.qg;
   const int64_t steps = int64_t(n_seqs) * ((int64_t(max_tokens) + kTile - 1) / kTile / p.kg + 1);
@@ -215,6 +222,9 @@ extern "C" int32_t it_latent_decode(const it_kv_cache* c, const void* q_latent, 
   if (n_heads == 1) ql_head_stride = qr_head_stride = 0;
   for (int64_t s : {ql_stride, ql_head_stride, qr_stride, qr_head_stride})
     if (s < 0 || s > kFar) return fail(IT_INVALID_INPUT, "%s: stride %lld", who, (long long)s);
+  // All sequences' tiles are numbered in 32 bits.
+  if (int64_t(n_seqs) * (std::min<int64_t>(max_tokens, int64_t(max_blocks) << c->log2_bs) / kTile + 2) > int64_t(1) << 30)
+    return fail(IT_INVALID_INPUT, "%s: %d sequences of up to %d tokens: more than 2^30 runs of %d", who, n_seqs, max_tokens, kTile);
   if (n_seqs == 0) return IT_OK;
   if (!q_latent || !q_rope || !block_tables || !ctx_lens || !out) return fail(IT_INVALID_INPUT, "%s: NULL tensor", who);
   const int64_t es = dtype_bytes(q_dtype);

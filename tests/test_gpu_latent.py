@@ -220,7 +220,7 @@ def exact_decode(q, flat, slots, seen, latent, scale):
 
 
 def decode_case(dtype, latent, rope, heads, lens, q_len=1, bs=16, start=None, seed=0, poison=False, split_q=False, out_dtype=None,
-                spread=1.0):
+                spread=1.0, bound=0):
     g = gen(seed + heads + sum(lens))
     held = [-(-n // bs) for n in lens]
     blocks = sum(held) + 3
@@ -253,7 +253,7 @@ def decode_case(dtype, latent, rope, heads, lens, q_len=1, bs=16, start=None, se
     ql, qr = qd[..., :latent], qd[..., latent:]
     if split_q:
         ql, qr = ql.contiguous(), qr.contiguous()
-    longest = max([m - (0 if start is None else start[i] & ~31) for i, m in enumerate(lens)] + [0])
+    longest = max([m - (0 if start is None else start[i] & ~31) for i, m in enumerate(lens)] + [bound])
     out = c.decode(ql, qr, tables.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), longest, scale,
                    start_pos=None if start is None else torch.tensor(start, dtype=torch.int32, device=DEV), q_len=q_len,
                    out_dtype=out_dtype)
@@ -281,6 +281,13 @@ def test_decode(dtype, latent, rope, heads, q_len):
 @pytest.mark.parametrize("dtype,latent,rope", [(torch.bfloat16, 512, 64), (torch.float16, 256, 32)])
 def test_decode_many_heads(dtype, latent, rope, heads):
     decode_case(dtype, latent, rope, heads, [700, 0, 45, 1025], poison=True)
+
+
+@pytest.mark.parametrize("heads,q_len", [(80, 1), (128, 1), (40, 3), (24, 6)])
+@pytest.mark.parametrize("dtype,latent,rope", [(torch.bfloat16, 512, 64), (torch.float16, 256, 32), (torch.bfloat16, 128, 64)])
+def test_decode_many_heads_under_a_bound_far_above(dtype, latent, rope, heads, q_len):
+    """The bound, not the lengths, chooses how many queries share a workgroup."""
+    decode_case(dtype, latent, rope, heads, [700, 0, 45, 1025, 31], q_len=q_len, poison=True, bound=1 << 17, start=[3, 0, 40, 900, 0])
 
 
 @pytest.mark.parametrize("bs", [1, 4, 8, 16, 64, 256])
@@ -322,7 +329,7 @@ def test_decode_more_new_tokens_than_context():
 def test_decode_values_that_later_tokens_bring():
     """A drafted token's infinities and NaN do not reach the tokens before it, and
     reach those that see it as a sum would."""
-    for heads in (2, 12, 32, 48):
+    for heads, bound in ((2, 0), (12, 0), (32, 0), (48, 0), (32, 1 << 20), (48, 1 << 20)):
         g, latent, rope, bs, n, t = gen(heads), 256, 32, 16, 70, 4
         c = LatentKvCache(8, bs, latent, rope, BF16)
         flat = normal(g, 8 * bs, latent + rope).to(torch.bfloat16)
@@ -332,8 +339,8 @@ def test_decode_values_that_later_tokens_bring():
         q = normal(g, t, heads, latent + rope).to(torch.bfloat16)
         q[..., 3] = -q[..., 3].abs() - 0.5  # an infinite latent element scores -inf: its weight is 0, and 0 * inf NaN
         tables = torch.arange(8, dtype=torch.int32, device=DEV)[None]
-        out = c.decode(q.to(DEV)[..., :latent], q.to(DEV)[..., latent:], tables, torch.tensor([n], dtype=torch.int32, device=DEV), n, 0.1,
-                       q_len=t)
+        out = c.decode(q.to(DEV)[..., :latent], q.to(DEV)[..., latent:], tables, torch.tensor([n], dtype=torch.int32, device=DEV),
+                       max(n, bound), 0.1, q_len=t)
         for j in range(2):
             want, mag, terms = exact_decode(q[j], flat, torch.arange(n), torch.arange(n) < n - t + 1 + j, latent, 0.1)
             within(out[j], want, u(torch.bfloat16) * (want.abs() + 2 * mag) + 2 * 160 * 2.0 ** -24 * terms * mag + 1e-5 * mag, f"token {j}")
@@ -634,6 +641,10 @@ def test_refusals_on_the_device():
         c.decode(ql, qr, tables, lens, 16, 0.1, q_len=2)
     with pytest.raises(InvalidInput):
         c.decode(ql.expand(3, 4, 256).repeat(65, 1, 1)[:65 * 3], qr.repeat(65, 1, 1), tables, lens, 16, 0.1, q_len=65)
+    with pytest.raises(InvalidInput):  # 2^31 runs of 32 tokens
+        many = LatentKvCache(2, 1024, 8, 8, BF16)
+        z = torch.zeros(65535, 1, 8, dtype=torch.bfloat16, device=DEV)
+        many.decode(z, z, torch.zeros(65535, 1024, dtype=torch.int32, device=DEV), torch.zeros(65535, dtype=torch.int32, device=DEV), 1 << 20, 0.1)
     with pytest.raises(InvalidInput):
         c.move(slots, slots + 8, Rotary(64), pos)
     k = torch.zeros(5, 4, 64, dtype=torch.bfloat16, device=DEV)
