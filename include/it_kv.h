@@ -234,7 +234,7 @@ int32_t it_kv_manager_compact_many(it_kv_manager* mgr, const int32_t* seqs, int3
                                    int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted);
 /* 1: an append to one of seqs[0..n) needs copy-on-write, because a compaction
  * set its position back to where another sequence holds a token in the same
- * block; 0: none does; -1: an argument is invalid. */
+ * block, or a reordering left several to continue it; 0: none does; -1: an argument is invalid. */
 int32_t it_kv_manager_needs_cow(const it_kv_manager* mgr, const int32_t* seqs, int32_t n);
 /* Beams reordered: sequence seqs[i] becomes what seqs[parents[i]] was before
  * the call (parents[i] an index into the list; below 0, or i itself: it stays),

@@ -490,9 +490,10 @@ class ContinuousBatcher:
         freed = np.zeros(0, np.int32)
         if self.manager is not None:
             freed = self.manager.reorder([self.seq_of[r] for r in ids], of)
-        was = [(self.requests[r].prompt_tokens, self.requests[r].generated_tokens, self._kept.get(r)) for r in ids]
+        was = [(self.requests[r].prompt_tokens, self.requests[r].generated_tokens, self._kept.get(r), r in self.needs_prefill) for r in ids]
         for rid, p in zip(ids, of):
-            prompt, generated, kept = was[p]
+            prompt, generated, kept, empty = was[p]
+            (self.needs_prefill.add if empty else self.needs_prefill.discard)(rid)
             self.requests[rid].prompt_tokens, self.requests[rid].generated_tokens = list(prompt), list(generated)
             if kept is None:
                 self._kept.pop(rid, None)

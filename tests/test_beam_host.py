@@ -165,6 +165,14 @@ def test_batcher_reorders_requests():
     b.preempt(10)
     b.schedule()
     assert b.plan_resume([10]).slots.size == len(b.context(10))
+    b.preempt(12)  # what has to be prefilled again goes with what the cache holds
+    b.schedule()
+    assert b.needs_prefill == {12}
+    b.reorder([10, 11, 12], [2, 1, 2])
+    assert b.needs_prefill == {10, 12} and mgr.positions()[b.seq_of[10]] == 0
+    b.reorder([10, 11, 12], [1, 1, 0])
+    assert b.needs_prefill == {12} and mgr.positions()[b.seq_of[10]] > 0
+    assert b.plan_resume([12]).slots.size == len(b.context(12))
     for r in (10, 11, 12):
         b.finish(r)
     assert pool.num_free() == 40
