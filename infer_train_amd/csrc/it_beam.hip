@@ -254,7 +254,8 @@ __global__ __launch_bounds__(kThreads, 8) void beam_slices(SelectArgs a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) f[e] = -INFINITY;
       if (i + V <= hi) {
-        In::widen(vecs[j * kThreads], f);
+        const typename In::raw w = vecs[j * kThreads];
+        In::widen(w, f);
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
