@@ -11,6 +11,9 @@
 // of 64 groups of it, which a wave finds bit by bit; what is not below it (about
 // n, up to ties) is listed, and a listed entry's place is the number of listed ones
 // before it.  A list that ties overflow is replaced by n rounds of the next best.
+//   Times, both launches: four beams of 32000 fp32 logits 10.5 us, 32 groups of eight of
+// 100003 bf16 39 (104 and 105 as first written: fp64 throughout, unaligned rows by elements,
+// coefficients moved for every token).
 //   Sums are in fp64: the order of two beams' candidates hangs on the difference of
 // their logarithms, whose fp32 error would decide about as many cases as it has
 // units between neighbouring values.

@@ -119,6 +119,12 @@ def test_append(src, cache, latent, rope, heads, layout, odd, n):
     assert torch.equal(proj[..., :40].cpu(), proj.cpu()[..., :40])
 
 
+@pytest.mark.parametrize("src,cache,heads,layout", [(torch.bfloat16, torch.bfloat16, 3, "interleaved"), (torch.float16, torch.float16, 8, "half"),
+                                                    (torch.float32, torch.bfloat16, 1, "half")])
+def test_append_many_tokens_of_few_heads(src, cache, heads, layout):
+    test_append(src, cache, 256, 64, heads, layout, False, 4500)
+
+
 def test_append_without_norm_rotation_or_queries():
     g = gen(3)
     c = LatentKvCache(4, 8, 128, 32, BF16)
