@@ -210,11 +210,12 @@ struct Division {
     if (a.n_seqs > 64 || total >= 1 << 20) return;
     const int busy = __popcll(__ballot(lanes.steps > 0));
     if (busy == 0 || busy >= workers) return;
-    int length = per;  // of a piece at most; sum over(steps, length) <= total / length + busy
-    if (sum(over(lanes.steps, length)) > workers) length = max(length, over(total, workers - busy));
-    if (length - per > kPieceCost) return;
-    per = length;
-    whole = true;
+    for (int length = per; length <= per + kPieceCost; ++length) {  // of a piece at most
+      if (sum(over(lanes.steps, length)) > workers) continue;
+      per = length;
+      whole = true;
+      return;
+    }
   }
   // The piece that worker w takes of a division into whole numbers; n 0: none.
   __device__ __forceinline__ Piece of(int w) const {
