@@ -61,6 +61,7 @@ __device__ __forceinline__ LatentSpan latent_span(const LatentDecodeArgs& a, int
   return {st, ctx};
 }
 
+constexpr int kLatentNarrow = 288;  // elements of a row of which LDS holds two tiles for each of four token groups
 constexpr int kLatentMaxQ = 64;  // new tokens of a sequence
 
 // How an absorbed call's tokens are divided, and where pieces of sequences go.

@@ -137,26 +137,32 @@ int32_t decode_sizes(const char* who, const it_kv_cache* c, int32_t n_seqs, int3
 
 namespace {
 constexpr int kTile = 32;  // of the matrix-core kernels: cached tokens
-// Query groups and token groups of a workgroup by the call's queries.  Token groups join in
-// LDS at each piece's end, which few queries pay for by more waves (64 heads: four query
-// groups 52 us, with two token groups 65).  Past 64 queries eight groups share a tile where
-// pieces are long; short ones are mostly the partial results' way out and in, which is half
-// as long where two workgroups of four groups halve the workers (128 heads in bf16, two
-// workgroups against one: 64 x 1000 tokens 56 us against 64, 16 x 2048 36 against 51, 16 x
-// 12288 equal, 16 of 8192 to 16384 123 against 112).
+// Query groups and token groups of a workgroup, by the call's groups of 16 queries and the
+// tiles that a CU gets of it (by max_tokens).  Many query groups read a tile from LDS and from
+// memory once for all; few have partial results that are as much smaller, and more waves on a
+// piece's own latency.
+//   Rows of up to 288 elements, of which LDS holds two tiles for each of four token groups: two
+// query groups or, of one and below 6 tiles, one (L = 256, 64 heads, 16 x 12288 tokens: two
+// 32 us, four with one token group 42, eight 51; 128 heads 49, 64, 54; 32 heads, 16 x 1024: one
+// 12.4, two 13.4; 28 heads, 24 x 4000: 22.3, 21.3).
+//   Wider ones (L = 512, one, two, four and eight groups): below 10 tiles 28 heads over 1 x 1023
+// tokens 15.0, 16.0, 17.6, 22.0 us, 32 over 32 x 512 18, 24, 27, 34, 64 over 16 x 2048 28, 24,
+// 35, 44, 128 over 64 x 1000 67, 49, 55, 62; from there 32 over 32 x 4096 46, 40, 46, 66, 64 over
+// 24 x 4096 54, 46, 43, 61, 128 over 16 x 8192 87, 85, 73, 77; from 24 on 128 over 16 x 12288
+// 149, 119, 97, 96, over 16 of 8192 to 16384 the last two 123, 107.
 struct HostPlan {
-  int qg, kg, workers, row_wgs;
+  int qg, workers, row_wgs;
   size_t o_bytes, ml_bytes, share_bytes;
 };
-HostPlan plan_of(int latent, int n_seqs, int q_len, int n_heads, int max_tokens, int n_cu) {
+HostPlan plan_of(int latent, int rope, int n_seqs, int q_len, int n_heads, int max_tokens, int n_cu) {
   HostPlan p;
   const int groups = (q_len * n_heads + 15) / 16;  // of 16 queries
-  const int64_t tiles = int64_t(n_seqs) * ((int64_t(max_tokens) + kTile - 1) / kTile);
-  p.qg = groups <= 1 ? 1 : groups == 2 ? 2 : groups <= 4 || tiles < 16 * std::max<int64_t>(1, n_cu / ((groups + 7) / 8)) ? 4 : 8;
-  p.kg = p.qg == 1 ? 4 : p.qg == 2 ? 2 : 1;
+  const int64_t all = int64_t(n_seqs) * ((int64_t(max_tokens) + kTile - 1) / kTile), tiles = all / n_cu;
+  if (latent + rope <= kLatentNarrow) p.qg = groups == 1 || tiles < 6 ? 1 : 2;
+  else if (tiles < 10) p.qg = groups <= 2 ? 1 : 2;
+  else p.qg = groups <= 1 ? 1 : groups == 2 ? 2 : groups <= 4 || tiles < 24 ? 4 : 8;
   p.row_wgs = (groups + p.qg - 1) / p.qg;
-  const int64_t steps = int64_t(n_seqs) * ((int64_t(max_tokens) + kTile - 1) / kTile / p.kg + 1);
-  p.workers = int(std::max<int64_t>(1, std::min<int64_t>(n_cu / p.row_wgs, steps)));
+  p.workers = int(std::max<int64_t>(1, std::min<int64_t>(n_cu / p.row_wgs, all + n_seqs)));
   const size_t parts = size_t(p.workers) * size_t(p.row_wgs) * 2 * size_t(p.qg);
   p.o_bytes = parts * size_t(latent) * 16 * 4;
   p.ml_bytes = parts * 16 * 8;
@@ -175,13 +181,13 @@ namespace itkv {
 size_t latent_decode_matrix_ws(int32_t dtype, int latent, int rope, int block_size, int n_seqs, int q_len, int n_heads, int max_tokens,
                                int n_cu) {
   if (!takes(dtype, latent, rope, block_size)) return 0;
-  const HostPlan p = plan_of(latent, n_seqs, q_len, n_heads, max_tokens, n_cu);
+  const HostPlan p = plan_of(latent, rope, n_seqs, q_len, n_heads, max_tokens, n_cu);
   return p.o_bytes + p.ml_bytes + p.share_bytes;
 }
 
 bool latent_decode_matrix(const LatentDecodeArgs& a, int32_t dtype, int block_size, int n_cu, hipStream_t s, hipError_t& e) {
   if (!takes(dtype, a.latent, a.rope, block_size)) return false;
-  const HostPlan h = plan_of(a.latent, a.n_seqs, a.q_len, a.n_heads, a.max_tokens, n_cu);
+  const HostPlan h = plan_of(a.latent, a.rope, a.n_seqs, a.q_len, a.n_heads, a.max_tokens, n_cu);
   char* const ws = reinterpret_cast<char*>(a.ws);
   const LatentSplitPlan p{h.workers, h.row_wgs, reinterpret_cast<float4*>(ws), reinterpret_cast<float2*>(ws + h.o_bytes),
                           reinterpret_cast<int2*>(ws + h.o_bytes + h.ml_bytes)};

@@ -15,7 +15,7 @@
 // 72, two waves a SIMD.  (32 queries a wave halve the LDS reads, but O^T then is
 // 256 registers, which the compiler does not keep in place.)  A workgroup has QG
 // query groups that share each 32-token tile and KG token groups, joined in LDS at
-// the end: few queries split the tokens among waves, many share them.
+// the end.
 // Tiles come by direct loads into LDS, as many ahead as fit in 144 KB: at L = 512 three
 // where all waves share a tile, one where two do, none where each has tiles of its own.
 // Work is divided by tiles over all sequences of the call (Division, below); pieces of
@@ -703,15 +703,19 @@ hipError_t launch_split(const LatentDecodeArgs& a, const LatentSplitPlan& p, hip
   hipLaunchKernelGGL((latent_decode_join<kBf16, QG, KG>), grid, dim3(256), 0, s, a, p);
   return hipGetLastError();
 }
+// Where several workgroups read a tile, the later ones find it in their XCD's L2 (128 heads over
+// 64 x 1000 tokens 49 us, 53 past it); else tiles go past it.
+template <bool kBf16, int L, int R, int QG, int KG>
+hipError_t launch_groups(const LatentDecodeArgs& a, const LatentSplitPlan& p, hipStream_t s) {
+  return p.row_wgs == 1 ? launch_split<kBf16, L, R, QG, KG, true>(a, p, s) : launch_split<kBf16, L, R, QG, KG, false>(a, p, s);
+}
 template <bool kBf16, int L, int R>
 hipError_t launch(const LatentDecodeArgs& a, const LatentSplitPlan& p, int qg, hipStream_t s) {
-  switch (qg) {
-    case 1: return launch_split<kBf16, L, R, 1, 4, true>(a, p, s);
-    case 2: return launch_split<kBf16, L, R, 2, 2, true>(a, p, s);
-    case 4: return launch_split<kBf16, L, R, 4, 1, true>(a, p, s);
-    default:  // where several workgroups read a tile, the later ones find it in their XCD's L2 (512 rows over 4 x 8192 tokens 76 us, 80 with nt)
-      return p.row_wgs == 1 ? launch_split<kBf16, L, R, 8, 1, true>(a, p, s) : launch_split<kBf16, L, R, 8, 1, false>(a, p, s);
-  }
+  if (qg == 1) return launch_groups<kBf16, L, R, 1, 4>(a, p, s);
+  if constexpr (L + R <= kLatentNarrow) return launch_groups<kBf16, L, R, 2, 4>(a, p, s);
+  else if (qg == 2) return launch_groups<kBf16, L, R, 2, 2>(a, p, s);
+  else if (qg == 4) return launch_groups<kBf16, L, R, 4, 1>(a, p, s);
+  else return launch_groups<kBf16, L, R, 8, 1>(a, p, s);
 }
 template <bool kBf16>
 hipError_t launch_latent_decode(const LatentDecodeArgs& a, const LatentSplitPlan& p, int qg, hipStream_t s) {

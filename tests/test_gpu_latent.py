@@ -289,11 +289,13 @@ def test_decode_many_heads(dtype, latent, rope, heads):
     decode_case(dtype, latent, rope, heads, [700, 0, 45, 1025], poison=True)
 
 
-@pytest.mark.parametrize("heads,q_len", [(80, 1), (128, 1), (40, 3), (24, 6)])
-@pytest.mark.parametrize("dtype,latent,rope", [(torch.bfloat16, 512, 64), (torch.float16, 256, 32), (torch.bfloat16, 128, 64)])
-def test_decode_many_heads_under_a_bound_far_above(dtype, latent, rope, heads, q_len):
+@pytest.mark.parametrize("bound", [1 << 15, 1 << 17])
+@pytest.mark.parametrize("heads,q_len", [(28, 1), (64, 1), (80, 1), (128, 1), (40, 3), (24, 6)])
+@pytest.mark.parametrize("dtype,latent,rope", [(torch.bfloat16, 512, 64), (torch.float16, 256, 32), (torch.bfloat16, 128, 64),
+                                               (torch.float16, 256, 64)])
+def test_decode_under_a_bound_far_above(dtype, latent, rope, heads, q_len, bound):
     """The bound, not the lengths, chooses how many queries share a workgroup."""
-    decode_case(dtype, latent, rope, heads, [700, 0, 45, 1025, 31], q_len=q_len, poison=True, bound=1 << 17, start=[3, 0, 40, 900, 0])
+    decode_case(dtype, latent, rope, heads, [700, 0, 45, 1025, 31], q_len=q_len, poison=True, bound=bound, start=[3, 0, 40, 900, 0])
 
 
 @pytest.mark.parametrize("bs", [1, 4, 8, 16, 64, 256])
@@ -335,8 +337,9 @@ def test_decode_more_new_tokens_than_context():
 def test_decode_values_that_later_tokens_bring():
     """A drafted token's infinities and NaN do not reach the tokens before it, and
     reach those that see it as a sum would."""
-    for heads, bound in ((2, 0), (12, 0), (32, 0), (48, 0), (32, 1 << 20), (48, 1 << 20)):
-        g, latent, rope, bs, n, t = gen(heads), 256, 32, 16, 70, 4
+    wide = [(h, b, 512, 64) for h in (12, 32, 48) for b in (0, 1 << 17, 1 << 20)]
+    for heads, bound, latent, rope in [(2, 0, 256, 32), (12, 0, 256, 32), (32, 0, 256, 32), (48, 0, 256, 32), (48, 1 << 20, 256, 32)] + wide:
+        g, bs, n, t = gen(heads), 16, 70, 4
         c = LatentKvCache(8, bs, latent, rope, BF16)
         flat = normal(g, 8 * bs, latent + rope).to(torch.bfloat16)
         flat[n - 2, 3] = INF  # token 2 of the four
