@@ -17,7 +17,7 @@
 // query groups that share each 32-token tile and KG token groups, joined in LDS at
 // the end.
 // Tiles come by direct loads into LDS, as many ahead as fit in 144 KB: at L = 512 three
-// where all waves share a tile, one where two do, none where each has tiles of its own.
+// where there is one token group, one where there are two, none where there are four.
 // Work is divided by tiles over all sequences of the call (Division, below); pieces of
 // sequences go through the workspace, at most two of a workgroup, and a second kernel
 // joins them.
@@ -25,9 +25,9 @@
 // token), by LDS reads and products in turn beyond.  With the join, L = 512 in bf16: 32
 // sequences of 256 to 8192 tokens, 32 heads, 41 us (151 MB at 3.7 TB/s; a copy reaches
 // 6.65); 16 of 8192 to 16384, 128 heads, 100 us (226 MB; 16 us of them the join of 64 MB of
-// partial results); one of 1023, 28 heads, 16 us, all latency (launches, lengths, pages,
+// partial results); one of 1023, 28 heads, 15 us, all latency (launches, lengths, pages,
 // tile, join, one after another).  L = 256 in f16: 24 of 100 to 4096, four drafted tokens
-// of 12 heads, 27 us (33 MB).  On the vector units the 32, the 16 and the 24 took 15.8, 47
+// of 12 heads, 24 us (33 MB).  On the vector units the 32, the 16 and the 24 took 15.8, 47
 // and 3.6 ms.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -180,7 +180,7 @@ __device__ __forceinline__ int over(int x, int d) { return quotient(x + d - 1, d
 //   Whole numbers of workers: sequences are divided, one piece a worker, where the longest
 // piece is not four steps longer than a run.
 // Measured: 32 sequences of 256 to 8192 tokens, 32 heads, 41 us against 47 by runs; 24 of 100
-// to 4096 with four drafted tokens of 12 heads 27 against 37.
+// to 4096 with four drafted tokens of 12 heads, in workgroups of 64 queries, 27 against 37.
 template <int KG>
 struct Division {
   static constexpr int kPieceCost = 4;
