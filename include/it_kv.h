@@ -232,9 +232,11 @@ int32_t it_kv_manager_compact_many(it_kv_manager* mgr, const int32_t* seqs, int3
                                    const int32_t* cu_keep, int64_t* src, int64_t* dst, int32_t* delta,
                                    int32_t* token_seq, int32_t* pos, int32_t moves_cap, int32_t* n_moves,
                                    int32_t* evicted, int32_t evicted_cap, int32_t* n_evicted);
-/* 1: an append to one of seqs[0..n) needs copy-on-write, because a compaction
- * set its position back to where another sequence holds a token in the same
- * block, or a reordering left several to continue it; 0: none does; -1: an argument is invalid. */
+/* 1: one append of tokens to each of seqs[0..n) needs copy-on-write, because a
+ * compaction set the position of one back to where another sequence holds a
+ * token in the same block, or where another of seqs would write one, or a
+ * reordering left several to continue a block; 0: it does not; -1: an argument
+ * is invalid. */
 int32_t it_kv_manager_needs_cow(const it_kv_manager* mgr, const int32_t* seqs, int32_t n);
 /* Beams reordered: sequence seqs[i] becomes what seqs[parents[i]] was before
  * the call (parents[i] an index into the list; below 0, or i itself: it stays),

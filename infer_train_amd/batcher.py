@@ -219,9 +219,10 @@ class KvManager:
         return ev[:nev.value].copy()
 
     def needs_cow(self, seqs: Sequence[int]) -> bool:
-        """Whether an append to these sequences needs copy-on-write, because a
-        compaction set one back to where a fork holds a token in the same block,
-        or a reordering left several to continue it (it_kv_manager_needs_cow)."""
+        """Whether one append to these sequences needs copy-on-write, because a
+        compaction set one back to where a fork holds a token in the same block
+        or another of them would write one, or a reordering left several to
+        continue it (it_kv_manager_needs_cow)."""
         if not self._compacted:
             return False
         at = np.ascontiguousarray(seqs, dtype=np.int32)

@@ -222,9 +222,11 @@ enum : uint8_t { kRewound = 1, kContinued = 2 };
 // Whether the next token of sequence s, written where it stands, would replace
 // one of another holder of its block: after a compaction that only dropped a
 // tail, the position lies among rows that forks may still read.  Forks whose
-// context ends at or before it do not; holders that this manager does not know
-// are taken to.  After a reordering, every holder is about to write there.
-bool overwrites(const it_kv_manager* m, int32_t s) {
+// context ends at or before it do not, but one that ends there and is in the
+// same step (seqs[0 .. n), n_tokens NULL: a token each) is about to write there
+// too; holders that this manager does not know are taken to read on.  After a
+// reordering, every holder is about to write there.
+bool overwrites(const it_kv_manager* m, int32_t s, const int32_t* seqs, const int32_t* n_tokens, int32_t n) {
   if (!m->rewound[size_t(s)]) return false;
   const int64_t p = m->pos[size_t(s)], lb = p / m->bs;
   if (lb >= m->max_blocks) return false;
@@ -235,7 +237,10 @@ bool overwrites(const it_kv_manager* m, int32_t s) {
   for (int32_t o = 0; o < m->max_seqs; ++o) {
     if (m->table[size_t(o) * size_t(m->max_blocks) + size_t(lb)] != id) continue;
     ++holders;
-    if (o != s && m->pos[size_t(o)] > p) return true;
+    if (o == s || m->pos[size_t(o)] < p) continue;
+    if (m->pos[size_t(o)] > p) return true;
+    for (int32_t i = 0; i < n; ++i)
+      if (seqs[i] == o && (!n_tokens || n_tokens[i] > 0)) return true;
   }
   return it_block_pool_ref_count(m->pool, id) > holders;
 }
@@ -306,7 +311,7 @@ int32_t step_impl(it_kv_manager* m, const int32_t* seqs, const int32_t* n_tokens
   const bool cow = pl->cow_src != nullptr;
   if (cow && !pl->cow_dst) return fail(IT_INVALID_INPUT, "%s: cow_dst is NULL", who);
   for (int32_t i = 0; !cow && i < n; ++i)
-    if (n_tokens[i] > 0 && overwrites(m, seqs[i]))
+    if (n_tokens[i] > 0 && overwrites(m, seqs[i], seqs, n_tokens, n))
       return fail(IT_INVALID_INPUT, "%s: seq %d, compacted or reordered, would write over a fork's tokens: append with copy-on-write", who,
                   seqs[i]);
   m->pending.clear();
@@ -491,7 +496,7 @@ extern "C" int32_t it_kv_manager_needs_cow(const it_kv_manager* m, const int32_t
   for (int32_t i = 0; i < n; ++i)
     if (seqs[i] < 0 || seqs[i] >= m->max_seqs) return -1;
   for (int32_t i = 0; i < n; ++i)
-    if (overwrites(m, seqs[i])) return 1;
+    if (overwrites(m, seqs[i], seqs, nullptr, n)) return 1;
   return 0;
 }
 
