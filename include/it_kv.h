@@ -767,10 +767,11 @@ int32_t it_latent_prefill(const void* q, const void* k, const void* v, const voi
 /* ======================================================================== */
 /* The best continuations of each group's beams.  Candidate (b, i), beam b of
  * the group and token i, has the value
- *   v = (scores[b] - log sum_j exp(z_bj)) + z_bi        in fp64
- * and candidates are ordered by v descending, equal v by the lower beam, then
- * the larger logit (beside a very large one, v does not tell logits apart), then
- * the lower token.  NaN logits and scores count as -inf; a candidate at -inf is
+ *   v = scores[b] + log_softmax(z_b)_i
+ *     = (scores[b] - log sum_j exp(z_bj - m_b)) + (z_bi - m_b), m_b = max_j z_bj
+ * in fp64, and candidates are ordered by v descending, equal v by the lower
+ * beam, then the larger logit (far enough below the row's maximum, v does not
+ * tell logits apart), then the lower token.  NaN logits and scores count as -inf; a candidate at -inf is
  * none; a row whose maximum is +inf weighs its tokens at +inf alone, equally.
  *   logits: [n_groups * n_beams][vocab] of F32, F16 or BF16, row_stride
  *     elements between rows; n_beams 1 .. 64, vocab 1 .. 262144

@@ -1,7 +1,11 @@
 // it_beam.hip -- beam search: the best continuations over a group's beams and
 // the vocabulary, and per-beam states put in the selected order.
 //
-//   v[b, i] = (score_b - log sum_j exp(z_bj)) + z_bi,  the n_out largest of a group.
+//   v[b, i] = score_b + log_softmax(z_b)_i = (score_b - log sum_j exp(z_bj - m_b)) + (z_bi - m_b),
+//
+// m_b the row's maximum, the n_out largest of a group.  The sum of exponentials is between 1 and
+// the vocabulary, so its logarithm is added to the score; added to a maximum near the type's
+// largest or lowest value it would vanish, and the score with it.
 //
 // Two launches.  The first cuts each row into slices of 16 tokens a thread, which
 // stay in registers: a slice's maximum, its sum of exponentials against it and its
@@ -336,7 +340,7 @@ __global__ __launch_bounds__(kThreads) void beam_join(SelectArgs a) {
     const double sum = wave_sum(s.top > -INFINITY ? s.sum * (s.top == m ? 1.0 : exp_below(double(s.top) - double(m))) : 0.0);
     if (lane == 0) {
       // A row at +inf: its tokens there share it equally, log 1/count.
-      base[b] = m > -INFINITY && score > -INFINITY ? double(score) - (m < INFINITY ? double(m) + log(sum) : log(sum)) : -INFINITY;
+      base[b] = m > -INFINITY && score > -INFINITY ? double(score) - log(sum) : -INFINITY;
       row_top[b] = m;
     }
   }
@@ -352,7 +356,7 @@ __global__ __launch_bounds__(kThreads) void beam_join(SelectArgs a) {
     const int b = i / per;
     const float z = token_value(k);
     if (!(base[b] > -INFINITY) || (row_top[b] == INFINITY && z < INFINITY)) return;
-    f(value_key(base[b] + (z == INFINITY ? 0.0 : double(z))), uint64_t(b) << kKeyBits | (kKeyMask - k));
+    f(value_key(base[b] + (z == INFINITY ? 0.0 : double(z) - double(row_top[b]))), uint64_t(b) << kKeyBits | (kKeyMask - k));
   };
   const auto each = [&](auto&& f) {
 #pragma unroll
