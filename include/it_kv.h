@@ -691,7 +691,10 @@ int32_t it_kv_cache_latent_dim(const it_kv_cache* cache);
  *     tokens, q_head_stride between heads (the rope part of a projection's
  *     heads); n_heads 0: none (q, q_out NULL).  q_out: the same shape, of
  *     q_out_dtype F32, F16 or BF16, with strides of its own; may be q itself
- *     (same strides and dtype), and must not overlap it otherwise
+ *     (same strides and dtype)
+ *   Otherwise q_out and rows_out lie on no other tensor; between its rows they
+ *     may, where both are equally many bytes apart from token to token (q, q_out
+ *     and kv as parts of one projection)
  *   rows_out: NULL, or [n_tokens][latent_dim + rope_dim] of the cache's dtype,
  *     contiguous: the stored rows, padding tokens' too (what a prompt's
  *     projection up reads)

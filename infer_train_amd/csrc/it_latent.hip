@@ -16,6 +16,7 @@
 
 #include "it_latent.hpp"
 #include "it_rotary.hpp"
+#include "it_strided.hpp"
 
 using namespace itkv;
 
@@ -266,11 +267,6 @@ __global__ __launch_bounds__(kThreads) void latent_append_general(LatentAppendAr
 
 inline bool is_float(int32_t dt) { return dt == IT_F32 || dt == IT_F16 || dt == IT_BF16; }
 inline bool aligned(const void* p, int64_t to) { return reinterpret_cast<uintptr_t>(p) % uintptr_t(to) == 0; }
-struct Range {
-  uintptr_t lo, hi;
-  Range(const void* p, int64_t bytes) : lo(reinterpret_cast<uintptr_t>(p)), hi(lo + uintptr_t(bytes)) {}
-  bool overlaps(const Range& o) const { return lo < o.hi && o.lo < hi; }
-};
 }  // namespace
 
 extern "C" int32_t it_latent_append(it_kv_cache* c, const it_rotary* rotary, const void* kv, int32_t src_dtype, int64_t kv_stride,
@@ -311,20 +307,22 @@ extern "C" int32_t it_latent_append(it_kv_cache* c, const it_rotary* rotary, con
   if (!aligned(kv, es) || (weight && !aligned(weight, dtype_bytes(weight_dtype))) || (n_heads && (!aligned(q, es) || !aligned(q_out, os))) ||
       (rows_out && !aligned(rows_out, dtype_bytes(c->dtype))))
     return fail(IT_INVALID_INPUT, "%s: tensors must be aligned to their elements", who);
-  const Range r_kv(kv, ((n_tokens - 1) * kv_stride + row) * es);
+  // What is written may lie between the rows of what is read (parts of one projection), not on them.
+  const int64_t cs = dtype_bytes(c->dtype);
+  const auto rows_at = [](const void* p, int64_t token, int64_t head, int64_t elements, int64_t size, int64_t tokens, int64_t heads) {
+    return StridedRows{reinterpret_cast<uintptr_t>(p), token * size, head * size, elements * size, tokens, heads};
+  };
+  const StridedRows r_kv = rows_at(kv, kv_stride, 0, row, es, n_tokens, 1), r_rows = rows_at(rows_out, row, 0, row, cs, n_tokens, 1);
   if (n_heads) {
-    const Range r_q(q, ((n_tokens - 1) * q_stride + (n_heads - 1) * q_head_stride + rope) * es);
-    const Range r_out(q_out, ((n_tokens - 1) * out_stride + (n_heads - 1) * out_head_stride + rope) * os);
+    const StridedRows r_q = rows_at(q, q_stride, q_head_stride, rope, es, n_tokens, n_heads);
+    const StridedRows r_out = rows_at(q_out, out_stride, out_head_stride, rope, os, n_tokens, n_heads);
     const bool same = q == q_out && src_dtype == q_out_dtype && q_stride == out_stride && q_head_stride == out_head_stride;
-    if ((!same && r_out.overlaps(r_q)) || r_out.overlaps(r_kv))
+    if ((!same && share_memory(r_out, r_q)) || share_memory(r_out, r_kv))
       return fail(IT_INVALID_INPUT, "%s: q_out overlaps q or kv (it may be q itself, with its strides and dtype)", who);
-    if (rows_out && r_out.overlaps(Range(rows_out, n_tokens * row * dtype_bytes(c->dtype))))
-      return fail(IT_INVALID_INPUT, "%s: q_out overlaps rows_out", who);
-    if (rows_out && r_q.overlaps(Range(rows_out, n_tokens * row * dtype_bytes(c->dtype))))
-      return fail(IT_INVALID_INPUT, "%s: rows_out overlaps q", who);
+    if (rows_out && share_memory(r_out, r_rows)) return fail(IT_INVALID_INPUT, "%s: q_out overlaps rows_out", who);
+    if (rows_out && share_memory(r_q, r_rows)) return fail(IT_INVALID_INPUT, "%s: rows_out overlaps q", who);
   }
-  if (rows_out && r_kv.overlaps(Range(rows_out, n_tokens * row * dtype_bytes(c->dtype))))
-    return fail(IT_INVALID_INPUT, "%s: rows_out overlaps kv", who);
+  if (rows_out && share_memory(r_kv, r_rows)) return fail(IT_INVALID_INPUT, "%s: rows_out overlaps kv", who);
   LatentAppendArgs a{};
   a.kv = static_cast<const char*>(kv);
   a.q = static_cast<const char*>(n_heads ? q : nullptr);

@@ -76,8 +76,9 @@ class LatentKvCache(_Pages):
         [latent_dim] (None: as it is), its rope part turned to int32 positions
         by rotary (None: as it is).  q_rope [n_tokens, n_heads, rope_dim] (any
         token and head strides: the rope part of the heads' projection) is
-        turned with it: returned as q_out (q_rope itself is allowed), or a new
-        tensor of q's dtype or q_out_dtype.  rows_out [n_tokens, latent_dim +
+        turned with it: returned as q_out (q_rope itself is allowed, inside a
+        projection that holds kv too), or a new tensor of q's dtype or
+        q_out_dtype.  rows_out [n_tokens, latent_dim +
         rope_dim] of the cache's dtype gets the stored rows too.  No gradients."""
         if slot_mapping.dtype != torch.int64:
             raise TypeError("slot_mapping must be int64")
