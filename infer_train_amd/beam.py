@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._lib import call
-from .kv import _check, _on, _raw_stream, torch_dtype_id
+from .kv import _check, _on, _raw_stream, _refuse_gradient, torch_dtype_id
 
 __all__ = ["beam_select", "beam_select_workspace", "beam_reorder"]
 
@@ -36,7 +36,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: Optional[int]
     as many leave enough beside those that end) their scores float32, parents
     int32 (the beam in its group) and tokens int32, [n_groups, n_out] each, best
     first, equal ones by the lower beam, larger logit and lower token; -inf, -1,
-    -1 where there are no more."""
+    -1 where there are no more.  The scores carry no gradient: logits and scores
+    that require one are refused, unless gradients are off."""
+    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+        _refuse_gradient("beam_select")
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] != 1):
         raise ValueError("logits must be [n_groups * n_beams, vocab] with contiguous rows")
     if not logits.is_cuda:
@@ -66,7 +69,7 @@ def beam_reorder(x: torch.Tensor, parents: torch.Tensor, dim: int = 0) -> torch.
     if parents.dtype != torch.int32 or parents.dim() != 2:
         raise TypeError("parents must be int32 [n_groups, n_beams]")
     if x.requires_grad and torch.is_grad_enabled():
-        raise ValueError("beam_reorder works in place and carries no gradient")
+        _refuse_gradient("beam_reorder")
     if not -x.dim() <= dim < x.dim():
         raise ValueError(f"dim {dim} of a tensor of {x.dim()} dimensions")
     dim %= x.dim()

@@ -55,6 +55,10 @@ def _check(rc: int) -> None:
         check(rc)
 
 
+def _refuse_gradient(who: str) -> None:
+    raise ValueError(f"{who} carries no gradient: call it under torch.no_grad(), or with detached tensors")
+
+
 _DECODE = {"both": call.it_paged_decode, "split": call.it_paged_decode_split, "combine": call.it_paged_decode_combine}
 
 

@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._lib import BF16, call, check, lib
-from .kv import _check, _ID_TORCH, _on, _Pages, _raw_stream, Rotary, torch_dtype_id
+from .kv import _check, _ID_TORCH, _on, _Pages, _raw_stream, _refuse_gradient, Rotary, torch_dtype_id
 
 __all__ = ["LatentKvCache", "latent_prefill"]
 
@@ -78,8 +78,13 @@ class LatentKvCache(_Pages):
         token and head strides: the rope part of the heads' projection) is
         turned with it: returned as q_out (q_rope itself is allowed, inside a
         projection that holds kv too), or a new tensor of q's dtype or
-        q_out_dtype.  rows_out [n_tokens, latent_dim +
-        rope_dim] of the cache's dtype gets the stored rows too.  No gradients."""
+        q_out_dtype.  rows_out [n_tokens, latent_dim + rope_dim] of the cache's
+        dtype gets the stored rows too.  Carries no gradient: tensors that
+        require one are refused, unless gradients are off."""
+        if torch.is_grad_enabled() and (kv.requires_grad or (weight is not None and weight.requires_grad) or
+                                        (q_rope is not None and q_rope.requires_grad) or (q_out is not None and q_out.requires_grad) or
+                                        (rows_out is not None and rows_out.requires_grad)):
+            _refuse_gradient("append")
         if slot_mapping.dtype != torch.int64:
             raise TypeError("slot_mapping must be int64")
         n, index = slot_mapping.numel(), self._index
@@ -154,7 +159,10 @@ class LatentKvCache(_Pages):
         one tensor or of two; scale the expanded form's, 1 / sqrt(its key
         width).  max_tokens bounds the contexts (with start_pos: what is seen of
         them and up to 31 more).  Returns [n_seqs * q_len, n_heads, latent_dim], which the
-        caller projects up to each head's value."""
+        caller projects up to each head's value, without a gradient: queries
+        that require one are refused, unless gradients are off."""
+        if torch.is_grad_enabled() and (q_latent.requires_grad or q_rope.requires_grad or (out is not None and out.requires_grad)):
+            _refuse_gradient("decode")
         index, n_seqs = self._index, ctx_lens.numel()
         if q_latent.dim() != 3 or q_latent.dtype != q_rope.dtype:
             raise ValueError("q_latent and q_rope must be [n_seqs * q_len, n_heads, ..] of one dtype")
@@ -187,7 +195,11 @@ def latent_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_rope: to
     k_rope [total_k, rope] shared by all heads (a part of the gathered rows);
     int32 cu_q, cu_k [n_seqs + 1], and bounds of the sequences' lengths, past
     which a sequence is not computed.  With causal, query i of a sequence sees
-    its keys 0 .. k_len - q_len + i.  Returns [total_q, n_heads, v_dim]."""
+    its keys 0 .. k_len - q_len + i.  Returns [total_q, n_heads, v_dim], without
+    a gradient: tensors that require one are refused, unless gradients are off."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_rope.requires_grad or
+                                    (out is not None and out.requires_grad)):
+        _refuse_gradient("latent_prefill")
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k_rope.dim() != 2:
         raise ValueError("q, k, v must be [tokens, n_heads, dim], k_rope [tokens, rope_dim]")
     if not q.is_cuda:
