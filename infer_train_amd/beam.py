@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._lib import call
-from .kv import _check, _on, _raw_stream, _refuse_gradient, torch_dtype_id
+from .kv import _check, _on, _raw_stream, _refuse_gradient, _written, torch_dtype_id
 
 __all__ = ["beam_select", "beam_select_workspace", "beam_reorder"]
 
@@ -85,6 +85,5 @@ def beam_reorder(x: torch.Tensor, parents: torch.Tensor, dim: int = 0) -> torch.
     row = x.element_size() * (x.numel() // (outer * rows) if outer * rows else 0)
     _launch(index, call.it_beam_reorder, at, row, row, outer, row * rows, parents.shape[0], parents.shape[1], _on(parents, index),
             _raw_stream(index))
-    if not x.is_inference():
-        torch.autograd.graph.increment_version(x)
+    _written(x)
     return x

@@ -59,6 +59,12 @@ def _refuse_gradient(who: str) -> None:
     raise ValueError(f"{who} carries no gradient: call it under torch.no_grad(), or with detached tensors")
 
 
+def _written(t: torch.Tensor) -> None:
+    """A tensor of the caller's was written: what saved it for a backward pass sees the change."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 _DECODE = {"both": call.it_paged_decode, "split": call.it_paged_decode_split, "combine": call.it_paged_decode_combine}
 
 
@@ -151,8 +157,8 @@ class Rotary:
                 raise ValueError("out does not go with tensors that require a gradient (use no_grad, or no out)")
             return _Turn.apply(x, self, positions, bool(transpose))
         result = self._turn(x, positions, out, transpose)
-        if out is not None and not out.is_inference():
-            torch.autograd.graph.increment_version(out)  # what saved it for a backward pass sees the change
+        if out is not None:
+            _written(out)
         return result
 
     def _turn(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor], transpose: bool) -> torch.Tensor:

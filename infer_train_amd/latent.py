@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._lib import BF16, call, check, lib
-from .kv import _check, _ID_TORCH, _on, _Pages, _raw_stream, _refuse_gradient, Rotary, torch_dtype_id
+from .kv import _check, _ID_TORCH, _on, _Pages, _raw_stream, _refuse_gradient, _written, Rotary, torch_dtype_id
 
 __all__ = ["LatentKvCache", "latent_prefill"]
 
@@ -96,7 +96,7 @@ class LatentKvCache(_Pages):
             raise ValueError("kv: rows must be contiguous")
         if (rotary is None) != (positions is None):
             raise TypeError("rotary and positions go together")
-        pa = wa = qa = oa = ra = None
+        pa = wa = qa = oa = ra = given = None
         qs = qh = os = oh = heads = out_id = weight_id = 0
         if positions is not None:
             if positions.dtype != torch.int32 or positions.numel() != n:
@@ -111,6 +111,7 @@ class LatentKvCache(_Pages):
                 raise TypeError("q_rope and kv must have one dtype")
             heads = q_rope.shape[1] if q_rope.dim() == 3 else 0
             qa, qs, qh = _heads(q_rope, "q_rope", index, n, heads, self.rope_dim)
+            given = q_out
             if q_out is None:
                 q_out = torch.empty((n, heads, self.rope_dim), dtype=q_out_dtype or q_rope.dtype, device=self.device)
             oa, os, oh = _heads(q_out, "q_out", index, n, heads, self.rope_dim)
@@ -124,6 +125,10 @@ class LatentKvCache(_Pages):
         _check(call.it_latent_append(self._at, None if rotary is None else rotary._at, kv.data_ptr(), torch_dtype_id(kv.dtype),
                                      kv.stride(0), wa, weight_id, float(eps), qa, qs, qh, heads, oa, out_id, os, oh, ra,
                                      _on(slot_mapping, index), pa, n, _raw_stream(index)))
+        if given is not None:
+            _written(given)
+        if rows_out is not None:
+            _written(rows_out)
         return q_out
 
     def gather(self, block_tables: torch.Tensor, ctx_lens: torch.Tensor, start_pos: Optional[torch.Tensor], cu_out: torch.Tensor,
@@ -173,6 +178,7 @@ class LatentKvCache(_Pages):
             raise TypeError("block_tables must be int32 [n_seqs, max_blocks], ctx_lens int32 [n_seqs]")
         if start_pos is not None and (start_pos.dtype != torch.int32 or start_pos.numel() != n_seqs):
             raise TypeError("start_pos must be int32 [n_seqs]")
+        given = out
         if out is None:
             out = torch.empty((n, heads, self.latent_dim), dtype=out_dtype or q_latent.dtype, device=self.device)
         elif out.shape != q_latent.shape:
@@ -183,6 +189,8 @@ class LatentKvCache(_Pages):
                                      _on(block_tables, index), block_tables.shape[1], _on(ctx_lens, index),
                                      None if start_pos is None else _on(start_pos, index), n_seqs, max_tokens, float(scale),
                                      _on(ws, index), ws.nbytes, _on(out, index), torch_dtype_id(out.dtype), _raw_stream(index)))
+        if given is not None:
+            _written(given)
         return out
 
 
@@ -217,7 +225,7 @@ def latent_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_rope: to
     va, vs, vh = _heads(v, "v", index, total_k, heads, v.shape[2])
     if k_rope.shape[0] != total_k or k_rope.get_device() != index or (k_rope.stride(1) != 1 and rope != 1 and k_rope.numel()):
         raise ValueError(f"k_rope must be [{total_k}, rope_dim] on cuda:{index}, rows contiguous")
-    shape = (total_q, heads, v.shape[2])
+    shape, given = (total_q, heads, v.shape[2]), out
     if out is None:
         out = torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
     elif out.shape != shape:
@@ -230,4 +238,6 @@ def latent_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_rope: to
     else:
         with torch.cuda.device(index):
             _check(call.it_latent_prefill(*args))
+    if given is not None:
+        _written(given)
     return out

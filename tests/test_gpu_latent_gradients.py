@@ -34,3 +34,27 @@ def test_inputs_that_require_gradients_are_refused():
                 fn(*leaf)
             with torch.inference_mode():
                 fn(*leaf)
+
+
+def test_outputs_given_by_the_caller_show_that_they_changed():
+    """A tensor saved for a backward pass and then written here is found out."""
+    g, n = gen(24), 3
+    z = lambda *s: normal(g, *s).to(DEV)  # noqa: E731
+    c = LatentKvCache(4, 16, 64, 32, F32)
+    slots = torch.arange(n, device=DEV)
+    tables, lens = torch.zeros(n, 1, dtype=torch.int32, device=DEV), torch.ones(n, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    q = z(n, 2, 32)
+    rows, out, pre = z(n, 96), z(n, 2, 64), z(n, 2, 64)
+    for t, fn in ((q, lambda: c.append(z(n, 96), slots, q_rope=q, q_out=q)), (rows, lambda: c.append(z(n, 96), slots, rows_out=rows)),
+                  (out, lambda: c.decode(z(n, 2, 64), z(n, 2, 32), tables, lens, 16, 0.1, out=out)),
+                  (pre, lambda: latent_prefill(z(n, 2, 96), z(n, 2, 64), z(n, 2, 64), z(n, 32), cu, cu, n, n, 0.1, out=pre))):
+        w = torch.ones_like(t, requires_grad=True)
+        loss = (w * t).sum()
+        version = t._version
+        fn()
+        assert t._version > version
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with torch.inference_mode():
+            fn()
