@@ -746,7 +746,9 @@ int32_t it_latent_decode(const it_kv_cache* cache, const void* q_latent, const v
  *     of one projection, k_rope a part of the gathered rows)
  *   cu_q, cu_k: int32[n_seqs + 1], device: rows of each sequence, 0 first; with
  *     causal != 0 query i of a sequence sees its keys 0 .. k_len - q_len + i,
- *     else all k_len; a query that sees none is 0
+ *     else all k_len; a query that sees none is 0.  An infinite value is in the
+ *     sums of the queries that see it: infinite, or NaN beside one of the other
+ *     sign, or where its weight is 0 (F16, BF16: rounds to 0)
  *   max_q_len, max_k_len: upper bounds; a sequence past them, or outside
  *     total_q / total_k, is not computed and its rows are left as they are, as
  *     are rows behind the last sequence

@@ -77,6 +77,13 @@ __device__ __forceinline__ uint32_t wild_halves(uint32_t x) {  // which of a pai
   return uint32_t((x & kExp) == kExp) | uint32_t((x >> 16 & kExp) == kExp) << 1;
 }
 
+// Half f of it as fp32.
+template <bool kBf16>
+__device__ __forceinline__ float half_value(uint32_t x, int f) {
+  const uint32_t bits = f ? x >> 16 : x & 0xFFFFu;
+  return kBf16 ? __uint_as_float(bits << 16) : float(__builtin_bit_cast(_Float16, uint16_t(bits)));
+}
+
 template <bool kBf16, int DN, int R, int DV>
 __global__ __launch_bounds__(kThreads, 2) void latent_prefill(LatentPrefillArgs a, int n_qb) {
   using K = Part<DN>;
@@ -125,7 +132,6 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill(LatentPrefillArgs 
 #pragma unroll
   for (int d = 0; d < ND; ++d) o[d] = v16f{};
   float m_run = -INFINITY, l_run = 0.0f;
-  uint32_t wild[ND / 2] = {};  // results that infinities and NaN of late keys reach (below)
 
   // LDS addresses of the operands: chunk 2 k + h of key row `col`; of the values rows 4 h +
   // j / 4 (+ 8 g + 16 t), columns 16 (lane / 16 % 2) + 4 (j % 4) of a d-tile, j = lane % 16.
@@ -139,12 +145,14 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill(LatentPrefillArgs 
     if (i + 1 < blocks) issue(i + 1);
     const int key0 = i * kKeys;
     const uint32_t stage = ring + uint32_t((i & 1) * kStage), v_stage = stage + K::kBytes + KR::kBytes;
-    if (key0 + kKeys > lo) {  // uniform: keys that not every query of the workgroup sees, or past the last
-      // A weight of 0 does not silence an infinity: values of rows past the last key are cleared;
-      // infinities and NaN of others are noted for the queries that see them, then cleared.  Each
-      // wave looks at all rows for itself: two workgroups leave no LDS for a word between them.
+    // Values of rows past the last key are cleared, since a weight of 0 does not silence an
+    // infinity.  Infinities and NaN of others that not every query of the workgroup sees are added
+    // to the results of the queries that do, then cleared.  Each wave looks at all rows for itself:
+    // two workgroups leave no LDS for a word between them.
+    const int end = min(n - key0, kKeys), late = max(0, lo - key0);
+    bool wild = false;  // uniform, the same in all waves, and nearly never
+    if (key0 + kKeys > lo) {  // uniform
       bool any = false;
-      const int end = min(n - key0, kKeys), late = max(0, lo - key0);
       for (int c = lane; c < kKeys * V::kChunks; c += 64) {
         const int r = c / V::kChunks;
         lds_u32x4* const at = reinterpret_cast<lds_u32x4*>(uintptr_t(v_stage + uint32_t(c * 16)));
@@ -155,79 +163,108 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill(LatentPrefillArgs 
           any |= (wild_halves<kBf16>(x[0]) | wild_halves<kBf16>(x[1]) | wild_halves<kBf16>(x[2]) | wild_halves<kBf16>(x[3])) != 0u;
         }
       }
-      if (__ballot(any) != 0) {  // the same in all waves, nearly never
-#pragma unroll 1
-        for (int r = late; r < end; ++r)
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {  // columns 32 d + 8 e + 4 h ..: half h of chunk 4 d + e
-              typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-              const u32x2 x = *reinterpret_cast<const __attribute__((address_space(3))) u32x2*>(
-                  uintptr_t(v_stage + uint32_t(r * V::kRow + (((4 * d + e) ^ V::key(r)) << 4) + 8 * h)));
-              const uint32_t bits = wild_halves<kBf16>(x[0]) | wild_halves<kBf16>(x[1]) << 2;
-              if (key0 + r < mine) wild[d / 2] |= bits << (d % 2 * 16 + 4 * e);
-            }
-        __syncthreads();
-        for (int c = int(threadIdx.x); c < kKeys * V::kChunks; c += kThreads) {
-          if (c / V::kChunks < late) continue;
-          lds_u32x4* const at = reinterpret_cast<lds_u32x4*>(uintptr_t(v_stage + uint32_t(c * 16)));
-          u32x4 x = *at;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t w = wild_halves<kBf16>(x[e]);
-            x[e] &= ~((w & 1u ? 0xFFFFu : 0u) | (w & 2u ? 0xFFFF0000u : 0u));
-          }
-          *at = x;
-        }
-        __syncthreads();
-      }
+      wild = __ballot(any) != 0;
     }
-    if (key0 >= wave_hi) continue;  // uniform: nothing here for this wave's queries
-
-    uint32_t k_base = stage + uint32_t(col * K::kRow), r_base = stage + uint32_t(K::kBytes + col * KR::kRow);
-    asm volatile("" : "+v"(k_base), "+v"(r_base));
-    v16f s[2] = {v16f{}, v16f{}};
+    const auto clean = [&]() __attribute__((always_inline)) {  // once all waves have read them
+      __syncthreads();
+      for (int c = int(threadIdx.x); c < kKeys * V::kChunks; c += kThreads) {
+        if (c / V::kChunks < late) continue;
+        lds_u32x4* const at = reinterpret_cast<lds_u32x4*>(uintptr_t(v_stage + uint32_t(c * 16)));
+        u32x4 x = *at;
 #pragma unroll
-    for (int k = 0; k < DN / 16; ++k)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {  // keys 32 t ..: their swizzle is that of row `col`
-        const lds_char* const p = reinterpret_cast<const lds_char*>(uintptr_t(k_base + ((uint32_t(2 * k + h) ^ k_key) << 4))) + t * 32 * K::kRow;
-        s[t] = mfma<kBf16>(__builtin_bit_cast(uint4, *reinterpret_cast<const lds_u32x4*>(p)), q[k], s[t]);
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t w = wild_halves<kBf16>(x[e]);
+          x[e] &= ~((w & 1u ? 0xFFFFu : 0u) | (w & 2u ? 0xFFFF0000u : 0u));
+        }
+        *at = x;
       }
+      __syncthreads();
+    };
+    const bool idle = key0 >= wave_hi;  // uniform: nothing here for this wave's queries
+    // The block's scores of this lane's query, and the largest of all of them.
+    const auto score = [&](float (&x)[2][16]) __attribute__((always_inline)) {
+      uint32_t k_base = stage + uint32_t(col * K::kRow), r_base = stage + uint32_t(K::kBytes + col * KR::kRow);
+      asm volatile("" : "+v"(k_base), "+v"(r_base));
+      v16f s[2] = {v16f{}, v16f{}};
 #pragma unroll
-    for (int k = 0; k < R / 16; ++k)
+      for (int k = 0; k < DN / 16; ++k)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const lds_char* const p = reinterpret_cast<const lds_char*>(uintptr_t(r_base + ((uint32_t(2 * k + h) ^ r_key) << 4))) + t * 32 * KR::kRow;
-        s[t] = mfma<kBf16>(__builtin_bit_cast(uint4, *reinterpret_cast<const lds_u32x4*>(p)), q[DN / 16 + k], s[t]);
-      }
-    float x[2][16];
+        for (int t = 0; t < 2; ++t) {  // keys 32 t ..: their swizzle is that of row `col`
+          const lds_char* const p = reinterpret_cast<const lds_char*>(uintptr_t(k_base + ((uint32_t(2 * k + h) ^ k_key) << 4))) + t * 32 * K::kRow;
+          s[t] = mfma<kBf16>(__builtin_bit_cast(uint4, *reinterpret_cast<const lds_u32x4*>(p)), q[k], s[t]);
+        }
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int k = 0; k < R / 16; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[t][e] = s[t][e] * a.scale_log2;
-    if (key0 + kKeys > wave_lo) {  // uniform
-      const int seen = mine - key0;
+        for (int t = 0; t < 2; ++t) {
+          const lds_char* const p = reinterpret_cast<const lds_char*>(uintptr_t(r_base + ((uint32_t(2 * k + h) ^ r_key) << 4))) + t * 32 * KR::kRow;
+          s[t] = mfma<kBf16>(__builtin_bit_cast(uint4, *reinterpret_cast<const lds_u32x4*>(p)), q[DN / 16 + k], s[t]);
+        }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] = 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) < seen ? x[t][e] : -INFINITY;
-    }
-    float top = x[0][0];
+        for (int e = 0; e < 16; ++e) x[t][e] = s[t][e] * a.scale_log2;
+      if (key0 + kKeys > wave_lo) {  // uniform
+        const int seen = mine - key0;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) top = fmaxf(top, x[t][e]);
-    top = max_halves(top);
-    if (__ballot(top > m_run + kLazy) != 0) {  // uniform, rare after the first block
+          for (int e = 0; e < 16; ++e) x[t][e] = 32 * t + 8 * (e >> 2) + 4 * h + (e & 3) < seen ? x[t][e] : -INFINITY;
+      }
+      float top = x[0][0];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, x[t][e]);
+      return max_halves(top);
+    };
+    // Raises the running maximum where a score is far above it.
+    const auto raise = [&](float top) __attribute__((always_inline)) {
+      if (__ballot(top > m_run + kLazy) == 0) return;  // uniform, and mostly so after the first block
       const float m_new = fmaxf(m_run, top);
       const float alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
       l_run *= alpha;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] *= alpha;
       m_run = m_new;
+    };
+    if (wild && !idle) {
+      // Which weights of this lane's query are not 0: bit 16 t + e of its half's word is key 32 t + 8 (e / 4) +
+      // 4 half + e % 4.  A weight of 0 makes NaN of an infinity, as it does in the products.
+      float x[2][16];
+      raise(score(x));
+      const float use = m_run == -INFINITY ? 0.0f : m_run;
+      uint32_t some = 0u;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float* const y = &x[e >> 3][2 * (e & 7)];
+        const uint32_t p = pack2<kBf16>(__builtin_amdgcn_exp2f(y[0] - use), __builtin_amdgcn_exp2f(y[1] - use));
+        some |= (uint32_t((p & 0xFFFFu) != 0u) | uint32_t(p >> 16 != 0u) << 1) << (2 * e);
+      }
+      const auto halves = __builtin_amdgcn_permlane32_swap(some, some, false, false);
+#pragma unroll 1
+      for (int r = late; r < end; ++r) {
+        if (key0 + r >= mine) break;
+        const uint32_t bit = uint32_t(r >> 5 << 4 | (r >> 3 & 3) << 2 | (r & 3)), weighs = (r >> 2 & 1 ? halves[1] : halves[0]) >> bit & 1u;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {  // columns 32 d + 8 e + 4 h ..: half h of chunk 4 d + e
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            const u32x2 v = *reinterpret_cast<const __attribute__((address_space(3))) u32x2*>(
+                uintptr_t(v_stage + uint32_t(r * V::kRow + (((4 * d + e) ^ V::key(r)) << 4) + 8 * h)));
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+              if (wild_halves<kBf16>(v[f >> 1]) >> (f & 1) & 1u) o[d][4 * e + f] += weighs ? half_value<kBf16>(v[f >> 1], f & 1) : NAN;
+            __builtin_amdgcn_sched_barrier(0);  // one load at a time: registers are short
+          }
+      }
     }
+    if (wild) clean();
+    if (idle) continue;
+
+    float x[2][16];
+    raise(score(x));
     const float use = m_run == -INFINITY ? 0.0f : m_run;
     // P rounded to the values' type, and summed as rounded: numerator and denominator hold the same weights.
     uint32_t p[16];
@@ -266,7 +303,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_prefill(LatentPrefillArgs 
     for (int e = 0; e < 4; ++e) {
       float y[4];
 #pragma unroll
-      for (int f = 0; f < 4; ++f) y[f] = wild[d / 2] >> (d % 2 * 16 + 4 * e + f) & 1u ? NAN : o[d][4 * e + f] * inv;
+      for (int f = 0; f < 4; ++f) y[f] = o[d][4 * e + f] * inv;
       const int64_t at = out + 32 * d + 8 * e;
       if (a.out_dtype == IT_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(y[0], y[1], y[2], y[3]);
       else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = make_uint2(pack2<kBf16>(y[0], y[1]), pack2<kBf16>(y[2], y[3]));
