@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._lib import call
-from .kv import _check, _on, _raw_stream, _refuse_gradient, _written, torch_dtype_id
+from .kv import _check, _grad_on, _on, _raw_stream, _refuse_gradient, _written, torch_dtype_id
 
 __all__ = ["beam_select", "beam_select_workspace", "beam_reorder"]
 
@@ -38,15 +38,17 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: Optional[int]
     first, equal ones by the lower beam, larger logit and lower token; -inf, -1,
     -1 where there are no more.  The scores carry no gradient: logits and scores
     that require one are refused, unless gradients are off."""
-    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+    if _grad_on() and (logits.requires_grad or scores.requires_grad):
         _refuse_gradient("beam_select")
-    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] != 1):
+    strides, index = logits.stride(), logits.get_device()
+    if len(strides) != 2 or (strides[1] != 1 and logits.shape[1] != 1):
         raise ValueError("logits must be [n_groups * n_beams, vocab] with contiguous rows")
-    if not logits.is_cuda:
+    if index < 0:
         raise ValueError("device tensor expected")
-    if scores.dtype != torch.float32 or scores.dim() != 2 or scores.numel() != logits.shape[0]:
+    rows, vocab = logits.shape
+    if scores.dtype != torch.float32 or scores.dim() != 2 or scores.numel() != rows:
         raise TypeError("scores must be float32 [n_groups, n_beams], one per row of logits")
-    index, (groups, beams), vocab = logits.get_device(), scores.shape, logits.shape[1]
+    groups, beams = scores.shape
     n = beams if n_out is None else int(n_out)
     at_scores = _on(scores, index)
     device = logits.device
@@ -54,7 +56,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n_out: Optional[int]
         ws = beam_select_workspace(groups, beams, vocab, n, device)
     best = torch.empty((3, groups, n), dtype=torch.int32, device=device)
     at, part = best.data_ptr(), 4 * groups * n
-    _launch(index, call.it_beam_select, logits.data_ptr(), torch_dtype_id(logits.dtype), logits.stride(0), groups, beams, vocab,
+    _launch(index, call.it_beam_select, logits.data_ptr(), torch_dtype_id(logits.dtype), strides[0], groups, beams, vocab,
             at_scores, n, at, at + part, at + 2 * part, _on(ws, index), ws.nbytes, _raw_stream(index))
     best_scores, parents, tokens = best.unbind()
     return best_scores.view(torch.float32), parents, tokens
@@ -68,7 +70,7 @@ def beam_reorder(x: torch.Tensor, parents: torch.Tensor, dim: int = 0) -> torch.
     Returns x."""
     if parents.dtype != torch.int32 or parents.dim() != 2:
         raise TypeError("parents must be int32 [n_groups, n_beams]")
-    if x.requires_grad and torch.is_grad_enabled():
+    if x.requires_grad and _grad_on():
         _refuse_gradient("beam_reorder")
     if not -x.dim() <= dim < x.dim():
         raise ValueError(f"dim {dim} of a tensor of {x.dim()} dimensions")

@@ -34,6 +34,7 @@ def stream_handle(device: Optional[torch.device] = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_grad_on = torch.is_grad_enabled  # looked up once
 # The current stream's handle of a device index, without building a Stream
 # object (1.5 us of each call).
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (

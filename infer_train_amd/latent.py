@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from ._lib import BF16, call, check, lib
-from .kv import _check, _ID_TORCH, _on, _Pages, _raw_stream, _refuse_gradient, _written, Rotary, torch_dtype_id
+from .kv import _check, _grad_on, _ID_TORCH, _on, _Pages, _raw_stream, _refuse_gradient, _written, Rotary, torch_dtype_id
 
 __all__ = ["LatentKvCache", "latent_prefill"]
 
@@ -81,9 +81,9 @@ class LatentKvCache(_Pages):
         q_out_dtype.  rows_out [n_tokens, latent_dim + rope_dim] of the cache's
         dtype gets the stored rows too.  Carries no gradient: tensors that
         require one are refused, unless gradients are off."""
-        if torch.is_grad_enabled() and (kv.requires_grad or (weight is not None and weight.requires_grad) or
-                                        (q_rope is not None and q_rope.requires_grad) or (q_out is not None and q_out.requires_grad) or
-                                        (rows_out is not None and rows_out.requires_grad)):
+        if _grad_on() and (kv.requires_grad or (weight is not None and weight.requires_grad) or
+                           (q_rope is not None and q_rope.requires_grad) or (q_out is not None and q_out.requires_grad) or
+                           (rows_out is not None and rows_out.requires_grad)):
             _refuse_gradient("append")
         if slot_mapping.dtype != torch.int64:
             raise TypeError("slot_mapping must be int64")
@@ -92,7 +92,8 @@ class LatentKvCache(_Pages):
             raise ValueError(f"kv must be [n_tokens, {self.head_dim}], with a slot per token")
         if kv.get_device() != index:
             raise ValueError(f"kv: tensor on cuda:{index} expected")
-        if kv.stride(1) != 1 and kv.numel():
+        token, element = kv.stride()
+        if element != 1 and kv.numel():
             raise ValueError("kv: rows must be contiguous")
         if (rotary is None) != (positions is None):
             raise TypeError("rotary and positions go together")
@@ -123,7 +124,7 @@ class LatentKvCache(_Pages):
                 raise TypeError("rows_out must have kv's shape and the cache's dtype")
             ra = _on(rows_out, index)
         _check(call.it_latent_append(self._at, None if rotary is None else rotary._at, kv.data_ptr(), torch_dtype_id(kv.dtype),
-                                     kv.stride(0), wa, weight_id, float(eps), qa, qs, qh, heads, oa, out_id, os, oh, ra,
+                                     token, wa, weight_id, float(eps), qa, qs, qh, heads, oa, out_id, os, oh, ra,
                                      _on(slot_mapping, index), pa, n, _raw_stream(index)))
         if given is not None:
             _written(given)
@@ -166,7 +167,7 @@ class LatentKvCache(_Pages):
         them and up to 31 more).  Returns [n_seqs * q_len, n_heads, latent_dim], which the
         caller projects up to each head's value, without a gradient: queries
         that require one are refused, unless gradients are off."""
-        if torch.is_grad_enabled() and (q_latent.requires_grad or q_rope.requires_grad or (out is not None and out.requires_grad)):
+        if _grad_on() and (q_latent.requires_grad or q_rope.requires_grad or (out is not None and out.requires_grad)):
             _refuse_gradient("decode")
         index, n_seqs = self._index, ctx_lens.numel()
         if q_latent.dim() != 3 or q_latent.dtype != q_rope.dtype:
@@ -205,15 +206,15 @@ def latent_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_rope: to
     which a sequence is not computed.  With causal, query i of a sequence sees
     its keys 0 .. k_len - q_len + i.  Returns [total_q, n_heads, v_dim], without
     a gradient: tensors that require one are refused, unless gradients are off."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_rope.requires_grad or
-                                    (out is not None and out.requires_grad)):
+    if _grad_on() and (q.requires_grad or k.requires_grad or v.requires_grad or k_rope.requires_grad or
+                       (out is not None and out.requires_grad)):
         _refuse_gradient("latent_prefill")
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3 or k_rope.dim() != 2:
         raise ValueError("q, k, v must be [tokens, n_heads, dim], k_rope [tokens, rope_dim]")
-    if not q.is_cuda:
+    index = q.get_device()
+    if index < 0:
         raise ValueError("device tensor expected")
-    index, total_q, heads, width = q.get_device(), q.shape[0], q.shape[1], q.shape[2]
-    total_k, nope, rope = k.shape[0], k.shape[2], k_rope.shape[1]
+    (total_q, heads, width), (total_k, _, nope), rope = q.shape, k.shape, k_rope.shape[1]
     if nope + rope != width:
         raise ValueError(f"q holds {width} elements a head, k and k_rope {nope} + {rope}")
     if k.dtype != q.dtype or v.dtype != q.dtype or k_rope.dtype != q.dtype:
