@@ -1,7 +1,10 @@
 // it_latent_attn.hip -- latent attention: the C ABI of its absorbed and expanded
 // forms, and the kernels for every type and width, in fp32 on the vector units.
 // 16-bit rows of the usual widths run on the matrix cores instead
-// (it_latent_decode.hip, it_latent_prefill.hip).
+// (it_latent_decode.hpp, it_latent_prefill.hip).  A query row a workgroup, so that every
+// head reads a sequence's rows again: F32 rows of 512 + 64 elements, 32 sequences of 256 to
+// 8192 tokens, 32 heads, 15.9 ms; prompt chunks of 512 over 1536 to 2560 keys, 8 x 32 heads,
+// 116 ms.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -18,7 +18,7 @@
 // bytes a clock and 16 KB of values at 64, 450 clocks of the CU, 8 waves 3600, where
 // their 320 products take 2560 of the four matrix cores, and the two overlap by half.
 // Eight chunks of 512 queries over 1536 to 2560 keys, 32 heads of 192 and 128 elements in
-// bf16: 195 us, 766 TFLOP/s of the 1317 that an 8192^3 product reaches (on the vector
+// bf16: 196 us (192 to 201 from run to run), 761 TFLOP/s of the 1317 that an 8192^3 product reaches (on the vector
 // units 113 ms).  Blocks of 32 keys take 4% longer, and where they let three waves on a SIMD
 // (25 registers spilled) 90%; the scale in the exponent's fma, the reads ordered ahead of
 // the products, and wave priorities are all within 2%.
