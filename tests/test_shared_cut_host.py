@@ -99,3 +99,47 @@ def test_a_search_that_drops_its_drafts(together):
     cut(mgr, [b.seq_of[1], b.seq_of[2]], 11, together)
     plan = b.plan_decode()
     assert len(set(plan.slots.tolist())) == 2 and plan.cow_src.size == 1
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_random_searches_with_cuts(seed):
+    """Appends with copy-on-write only where it is asked for, reorderings, cuts and compactions of any of the sequences:
+    each one's tokens are found through its table."""
+    for sub in range(25):
+        rng = np.random.default_rng([seed, sub])
+        bs, n, tok = int(rng.choice([4, 8])), int(rng.integers(2, 6)), 0
+        pool = BlockPool(400, BF16)
+        mgr = KvManager(pool, bs, n, 32)
+        pages, model = np.full((400, bs), -1, np.int64), {s: [] for s in range(n)}
+        for _ in range(60):
+            seqs = [int(x) for x in rng.permutation(n)[:rng.integers(1, n + 1)]]
+            op = rng.integers(0, 6)
+            if op < 3:
+                counts = [int(x) for x in rng.integers(0, 4, len(seqs))]
+                if max(len(model[s]) for s in seqs) + 4 > 32 * bs:
+                    continue
+                plan = mgr.append(seqs, counts, cow=mgr.needs_cow(seqs))
+                for a, b in zip(plan.cow_src, plan.cow_dst):
+                    pages[b] = pages[a]
+                for slot, s in zip(plan.slots, plan.token_seq):
+                    model[int(s)] = model[int(s)] + [tok]
+                    pages[slot // bs, slot % bs] = tok
+                    tok += 1
+            elif op == 3:
+                parents = [int(x) for x in rng.integers(-1, len(seqs), len(seqs))]
+                pages[mgr.reorder(seqs, parents)] = -1
+                was = {s: model[s] for s in seqs}
+                model.update({s: was[seqs[p]] for s, p in zip(seqs, parents) if p >= 0})
+            else:
+                most = int(rng.integers(0, 40))
+                keeps = [list(range(min(len(model[s]), most))) if rng.random() < 0.75 else
+                         sorted(rng.permutation(len(model[s]))[:most].tolist()) for s in seqs]
+                plan = mgr.compact_many(seqs, keeps)
+                moved = pages[plan.src // bs, plan.src % bs].copy()
+                pages[plan.dst // bs, plan.dst % bs] = moved
+                pages[plan.evicted] = -1
+                model.update({s: [model[s][j] for j in k] for s, k in zip(seqs, keeps)})
+            tables, ctx, _ = mgr.tables()
+            for s, tokens in model.items():
+                p = np.arange(len(tokens))
+                assert ctx[s] == len(tokens) and pages[tables[s, p // bs], p % bs].tolist() == tokens, (sub, s)
